@@ -216,6 +216,35 @@ enum {
      *
      * LINEAR_HEADS_GROUP: the projections of a multi-head attention layer as one call, each as LINEAR_FWD with T and heads:
      *   l{count (2 or 3), N, K, heads, then M, T, hX, hWeight, hBias (0 = none), hY of each}
+     *
+     * QK_NORM_ROPE_FWD / QK_NORM_ROPE_BWD: RMS norm of every head of queries (batch, heads, T, hs) and keys (batch, kvHeads, T, hs)
+     * and the rotation of its position, 0 .. T - 1, in one pass: y = R(t) (w x / sqrt(mean(x^2) + eps)), w of hs values.  The
+     * rotation is that of a CREATE_ROPE handle of this head size and at least T positions, its angles taken in 64 bits (ROPE_FWD's
+     * tables hold the reference's, taken in fp32).  hs even, 2 .. 256.
+     *   f{eps}  l{batch, T, heads, kvHeads, hs, hQ, hK, hWq (0 = ones), hWk (0 = ones), hRope (0 = none), hYq, hYk}
+     * hYq may be hQ, hYk hK.  Backward, from hQ and hK as the forward call had them:
+     *   f{eps}  l{batch, T, heads, kvHeads, hs, hQ, hK, hWq, hWk, hRope, hdYq, hdYk, hdQ, hdK, hdWq (0 = not computed), hdWk (0) [, accumW]}
+     * hdQ may be hQ or hdYq, hdK hK or hdYk; the weights' gradients are overwritten (accumW 1: added to).
+     *
+     * Paged caches.  hKpages and hVpages hold `pages` pages of pageSize positions; value i of key head h at position p of a page lies
+     * at page * stridePage + h * strideHead + p * stridePos + i.  Position t of sequence b is in page table[b * maxPages + t / pageSize];
+     * an entry that is no page (below 0, from `pages` on, not a number) means that those positions are not there.  hTable (batch,
+     * maxPages), hStarts (batch + 1) and hLens (batch) are fp32 tensors of whole numbers: sequence b has the rows hStarts[b] ..
+     * hStarts[b + 1] - 1 of the tokens of a call (never decreasing; rows from hStarts[batch] on are left alone), and hLens[b] positions with
+     * these tokens, which are its last ones.  Numbers outside of their range count as its nearest end.  tokens, pages and maxPages *
+     * pageSize are at most 2^24, hs even, 2 .. 256.  Rows and output of one type, both caches of one type, the rows' or, under fp32 rows, 16 bits.
+     * PAGED_APPEND: of every token a row q | k | v ((heads + 2 kvHeads) hs values, as a projection writes it): queries to hQ (tokens,
+     * heads, hs), keys and values to the token's position; norm 1: queries and keys with the norm above first, hRope: turned to that
+     * position.  A token before position 0 (hLens below the new tokens) is not stored and turned as position 0 is.
+     *   f{eps}  l{batch, tokens, heads, kvHeads, hs, pages, pageSize, maxPages, hQKV, hKpages, hVpages, hTable, hStarts, hLens, hQ,
+     *             stridePage, strideHead, stridePos, hRope (0 = none), norm, hWq (0 = ones), hWk (0 = ones)}
+     * New tokens of one call must have places of their own (a page that is written belongs to one sequence).  Places may not overlap: strides are
+     * refused if they do.  hRope's handle has at least maxPages * pageSize positions.
+     * ATTN_PAGED_FWD: attention of queries (tokens, heads, hs), every token over the positions of its sequence up to its own, to
+     * hY (tokens, heads, hs); a token with none gets zeros.
+     *   f{scale (0 = 1/sqrt(hs))}  l{batch, tokens, heads, kvHeads, hs, pages, pageSize, maxPages, hQ, hKpages, hVpages, hTable, hStarts,
+     *             hLens, hY, stridePage, strideHead, stridePos [, maxNew]}
+     * maxNew: no sequence has more new tokens than this (0: not known); only the choice of kernels follows from it.
      */
     MCH_FN_ATTN_DECODE_FWD = 2001,
     MCH_FN_RMSNORM_FWD = 2002,
@@ -228,7 +257,11 @@ enum {
     MCH_FN_SWIGLU_BWD = 2009,
     MCH_FN_NORM_ADD_FWD = 2010,
     MCH_FN_NORM_ADD_BWD = 2011,
-    MCH_FN_LINEAR_HEADS_GROUP = 2012
+    MCH_FN_LINEAR_HEADS_GROUP = 2012,
+    MCH_FN_QK_NORM_ROPE_FWD = 2013,
+    MCH_FN_QK_NORM_ROPE_BWD = 2014,
+    MCH_FN_PAGED_APPEND = 2015,
+    MCH_FN_ATTN_PAGED_FWD = 2016
 };
 
 /* DEVINIT flags (CudaDnnDLL/Cuda Files/device.h:18-22) */

@@ -253,4 +253,32 @@ hipError_t k_rope_append(hipStream_t s, DType dt, void* q, void* knew, const voi
                          int H, int kvH, int hs, int pos, long long strideB, long long strideH, long long strideT,
                          const float* fcos, const float* fsin);
 
+// ---- norms of heads with their rotation, paged caches (head_norm.hip, attn_paged.hip) -----------------------------------------
+// cosines and sines of every position, {cos, sin} [seq][hs / 2], angles pos theta^(-2 i / hs) taken in 64 bits
+hipError_t k_rope_turns(hipStream_t s, int seq, int hs, float theta, float* turns);
+// y = rotation(position) of w x / sqrt(mean(x^2) + eps) for every row of hs values of q (B,H,T,hs) and k (B,kvH,T,hs); wq, wk, turns may be
+// null; y may be x
+hipError_t k_qk_norm_rope(hipStream_t s, DType dt, int B, int T, int H, int kvH, int hs, const void* q, const void* k, const void* wq, const void* wk,
+                          const float* turns, void* yq, void* yk, float eps);
+// its gradient; dwq, dwk (may be null) are overwritten, with `accum` added to.  dx may be x or dy.
+size_t k_qk_norm_rope_bwd_workspace_bytes(int hs);
+hipError_t k_qk_norm_rope_bwd(hipStream_t s, DType dt, int B, int T, int H, int kvH, int hs, const void* q, const void* k, const void* wq, const void* wk,
+                              const float* turns, const void* dyq, const void* dyk, void* dxq, void* dxk, void* dwq, void* dwk, bool accum, float eps,
+                              void* workspace);
+// A paged cache and the sequences of a launch (csrc/paged.h): position p of sequence b, key head h lies at
+// page * sP + h * sH + (p % pageSize) * sT of k and v (type ct), page = table[b * maxPages + p / pageSize]
+struct PagedCache {
+    void *k, *v;
+    DType ct;
+    const float *table, *starts, *lens;
+    int batch, tokens, H, kvH, hs, pages, pageSize, maxPages;
+    long long sP, sH, sT;
+};
+// rows of qkv ((H + 2 kvH) hs values a token): queries and keys normalised (norm; wq, wk may be null) and rotated (turns may be null), queries
+// to q (tokens, H, hs), keys and values to their pages
+hipError_t k_paged_append(hipStream_t s, DType dt, const PagedCache& c, const void* qkv, void* q, const void* wq, const void* wk, bool norm, float eps,
+                          const float* turns);
+// y (tokens, H, hs) = attention of q (tokens, H, hs) over the pages, every token over the positions up to its own
+hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale);
+
 }  // namespace mch

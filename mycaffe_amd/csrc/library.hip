@@ -20,6 +20,7 @@
 #include <algorithm>
 #include <climits>
 
+#include "paged.h"
 #include "runtime.h"
 
 namespace mch {
@@ -2336,6 +2337,11 @@ long Kernel::run(long fn, float* pf, long lf, MCH_LONGLONG* pl, long ll, float**
         return 0;
     }
 
+    case MCH_FN_QK_NORM_ROPE_FWD: return qk_norm_rope(pf, lf, pl, ll, false);
+    case MCH_FN_QK_NORM_ROPE_BWD: return qk_norm_rope(pf, lf, pl, ll, true);
+    case MCH_FN_PAGED_APPEND: return paged_append(pf, lf, pl, ll);
+    case MCH_FN_ATTN_PAGED_FWD: return attn_paged_fwd(pf, lf, pl, ll);
+
     // ---- RoPE ------------------------------------------------------------------
     case MCH_FN_CREATE_ROPE: {
         // f{theta}, l{sharedIdx,gpuId,count,batch,seqLen,heads,hs} (device.h:4201-4229, rope.cu:502-607)
@@ -2644,6 +2650,212 @@ long Kernel::attn_decode_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool
     return 0;
 }
 
+// whether n values of x and m of y share memory
+static bool overlap(const MemItem* x, long long n, const MemItem* y, long long m)
+{
+    const char *a = (const char*)x->ptr, *b = (const char*)y->ptr;
+    return a < b + (size_t)m * y->esize() && b < a + (size_t)n * x->esize();
+}
+static bool same(const MemItem* x, const MemItem* y) { return x->ptr == y->ptr; }
+
+// {cos, sin} of the positions of a rope handle, null for handle 0
+long Kernel::rope_turns(long hRope, long long hs, long long positions, const float** turns)
+{
+    *turns = nullptr;
+    if (!hRope) return 0;
+    RopeState* r = m_rope.get(hRope);
+    if (!r || !r->set) return MCH_ERROR_ROPE_NOT_INITIALIZED;
+    if (r->hs != hs || r->seq < positions) {
+        last_detail = "the rope handle was created for another head size or for fewer positions";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    if (!r->turns) {
+        void* p = nullptr;
+        HIPCHK(hipMalloc(&p, (size_t)r->seq * r->hs * sizeof(float)));
+        r->turns = std::shared_ptr<void>(p, [](void* q) { (void)hipFree(q); });
+        const hipError_t e = k_rope_turns(m_stream, r->seq, r->hs, r->theta, (float*)p);
+        if (e != hipSuccess) { r->turns.reset(); return (long)e; }
+    }
+    *turns = (const float*)r->turns.get();
+    return 0;
+}
+
+// QK_NORM_ROPE_FWD: f{eps}, l{batch,T,heads,kvHeads,hs,hQ,hK,hWq,hWk,hRope,hYq,hYk}
+// QK_NORM_ROPE_BWD: f{eps}, l{batch,T,heads,kvHeads,hs,hQ,hK,hWq,hWk,hRope,hdYq,hdYk,hdQ,hdK,hdWq,hdWk[,accumW]}
+long Kernel::qk_norm_rope(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool backward)
+{
+    NEED_F(1, 1);
+    NEED_L(backward ? 16 : 12, backward ? 17 : 12);
+    const long long B = pl[0], T = pl[1], H = pl[2], KVH = pl[3], hs = pl[4];
+    if (B < 1 || T < 1 || H < 1 || KVH < 1 || H > 65535 || KVH > 65535 || hs < 2 || hs > 256 || (hs & 1) || B > INT_MAX || T > INT_MAX || B * T > INT_MAX || !(pf[0] >= 0.f))
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const long long n[2] = {B * H * T * hs, B * KVH * T * hs};
+    MemItem *X[2], *W[2] = {}, *dY[2], *Y[2], *dW[2] = {};
+    for (int i = 0; i < 2; i++) {
+        ERRCHK(mem((long)pl[5 + i], &X[i]));
+        if (pl[7 + i]) ERRCHK(mem((long)pl[7 + i], &W[i]));
+        if (backward) ERRCHK(mem((long)pl[10 + i], &dY[i]));
+        ERRCHK(mem((long)pl[(backward ? 12 : 10) + i], &Y[i]));
+        if (backward && pl[14 + i]) ERRCHK(mem((long)pl[14 + i], &dW[i]));
+    }
+    for (int i = 0; i < 2; i++) {
+        const bool half = X[0]->half;
+        if (X[i]->half != half || Y[i]->half != half || (W[i] && W[i]->half != half) || (backward && dY[i]->half != half) || (dW[i] && dW[i]->half != half))
+            return MCH_ERROR_MEMORY_MIXED_HALF_TYPES;
+        RANGE(X[i], 0, n[i]);
+        RANGE(Y[i], 0, n[i]);
+        if (W[i]) RANGE(W[i], 0, hs);
+        if (backward) RANGE(dY[i], 0, n[i]);
+        if (dW[i]) RANGE(dW[i], 0, hs);
+    }
+    // a row is read before it is written: an output may be its own input, and share memory with nothing else
+    bool clash = overlap(Y[0], n[0], Y[1], n[1]) || (dW[0] && dW[1] && overlap(dW[0], hs, dW[1], hs));
+    for (int i = 0; i < 2; i++)
+        for (int j = 0; j < 2; j++) {
+            clash = clash || (overlap(Y[i], n[i], X[j], n[j]) && !(i == j && same(Y[i], X[j])));
+            if (backward) clash = clash || (overlap(Y[i], n[i], dY[j], n[j]) && !(i == j && same(Y[i], dY[j])));
+            if (W[j]) clash = clash || overlap(Y[i], n[i], W[j], hs);
+            if (dW[j]) clash = clash || overlap(Y[i], n[i], dW[j], hs) || overlap(dW[j], hs, X[i], n[i]) || overlap(dW[j], hs, dY[i], n[i]) || (W[i] && overlap(dW[j], hs, W[i], hs));
+        }
+    if (clash) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    const float* turns;
+    ERRCHK(rope_turns((long)pl[9], hs, T, &turns));
+    auto at = [](MemItem* m) -> void* { return m ? m->ptr : nullptr; };
+    if (!backward) {
+        HIPCHK(k_qk_norm_rope(m_stream, X[0]->dt(), (int)B, (int)T, (int)H, (int)KVH, (int)hs, X[0]->ptr, X[1]->ptr, at(W[0]), at(W[1]), turns, Y[0]->ptr, Y[1]->ptr, pf[0]));
+    } else {
+        void* ws = nullptr;
+        if (dW[0] || dW[1]) ERRCHK(workspace(k_qk_norm_rope_bwd_workspace_bytes((int)hs), &ws));
+        HIPCHK(k_qk_norm_rope_bwd(m_stream, X[0]->dt(), (int)B, (int)T, (int)H, (int)KVH, (int)hs, X[0]->ptr, X[1]->ptr, at(W[0]), at(W[1]), turns, dY[0]->ptr, dY[1]->ptr,
+                                  Y[0]->ptr, Y[1]->ptr, at(dW[0]), at(dW[1]), ll > 16 && pl[16] != 0, pf[0], ws));
+    }
+    for (int i = 0; i < 2; i++) {
+        m_mem.touch((long)pl[(backward ? 12 : 10) + i]);
+        if (dW[i]) m_mem.touch((long)pl[14 + i]);
+    }
+    return 0;
+}
+
+// What PAGED_APPEND and ATTN_PAGED_FWD have in common: l{batch,tokens,heads,kvHeads,hs,pages,pageSize,maxPages,hRows,hKpages,hVpages,
+// hTable,hStarts,hLens,hOut,stridePage,strideHead,stridePos}, rows of rowHeads heads, output of `heads`
+long Kernel::paged_operands(const MCH_LONGLONG* pl, long long rowHeads, PagedCache* c, MemItem** rows, MemItem** out)
+{
+    const long long B = pl[0], N = pl[1], H = pl[2], KVH = pl[3], hs = pl[4], pages = pl[5], ps = pl[6], width = pl[7];
+    if (B < 1 || N < 1 || H < 1 || KVH < 1 || pages < 1 || ps < 1 || width < 1 || hs < 2 || (hs & 1) || hs > 256 || H > 65535 || KVH > H || H % KVH || B > PAGED_EXACT ||
+        N > PAGED_EXACT || pages > PAGED_EXACT || ps > PAGED_EXACT || width > PAGED_EXACT || ps * width > PAGED_EXACT)
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemItem *K, *V, *table, *starts, *lens;
+    ERRCHK(mem((long)pl[8], rows));
+    ERRCHK(mem((long)pl[9], &K));
+    ERRCHK(mem((long)pl[10], &V));
+    ERRCHK(mem((long)pl[11], &table));
+    ERRCHK(mem((long)pl[12], &starts));
+    ERRCHK(mem((long)pl[13], &lens));
+    ERRCHK(mem((long)pl[14], out));
+    if (table->half || starts->half || lens->half) {
+        last_detail = "block table, starts and lengths are fp32 tensors";
+        return MCH_ERROR_MEMORY_HALF_TYPE_NOT_SUPPORTED;
+    }
+    if ((*rows)->half != (*out)->half || K->half != V->half || ((*rows)->half && !K->half)) return MCH_ERROR_MEMORY_MIXED_HALF_TYPES;
+    RANGE(*rows, 0, N * rowHeads * hs);
+    RANGE(*out, 0, N * H * hs);
+    RANGE(table, 0, B * width);
+    RANGE(starts, 0, B + 1);
+    RANGE(lens, 0, B);
+    const long long sP = pl[15], sH = pl[16], sT = pl[17];
+    const long long most = (long long)std::min(K->count, V->count);
+    if (sP < 0 || sH < 0 || sT < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    if ((pages > 1 && sP > most) || (KVH > 1 && sH > most) || (ps > 1 && sT > most)) {
+        last_detail = "range exceeds the allocation behind the memory handle";
+        return MCH_ERROR_MEMORY_RANGE_EXCEEDED;
+    }
+    const long long need = (pages > 1 ? (pages - 1) * sP : 0) + (KVH > 1 ? (KVH - 1) * sH : 0) + (ps > 1 ? (ps - 1) * sT : 0) + hs;
+    RANGE(K, 0, need);
+    RANGE(V, 0, need);
+    if (overlap(*out, N * H * hs, *rows, N * rowHeads * hs) || overlap(*out, N * H * hs, K, need) || overlap(*out, N * H * hs, V, need) || overlap(*out, N * H * hs, table, B * width) ||
+        overlap(*out, N * H * hs, starts, B + 1) || overlap(*out, N * H * hs, lens, B)) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    *c = PagedCache{K->ptr, V->ptr, K->dt(), (const float*)table->ptr, (const float*)starts->ptr, (const float*)lens->ptr, (int)B, (int)N, (int)H, (int)KVH, (int)hs,
+                    (int)pages, (int)ps, (int)width, sP, sH, sT};
+    return 0;
+}
+
+// PAGED_APPEND: f{eps}, l{..., hRope, norm, hWq, hWk} behind what paged_operands reads
+long Kernel::paged_append(float* pf, long lf, MCH_LONGLONG* pl, long ll)
+{
+    NEED_F(1, 1);
+    NEED_L(22, 22);
+    PagedCache c;
+    MemItem *X, *Q, *K, *V, *W[2] = {}, *meta;
+    if (!(pf[0] >= 0.f) || pl[2] > 65535 || pl[3] > 65535) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    ERRCHK(paged_operands(pl, pl[2] + 2 * pl[3], &c, &X, &Q));
+    ERRCHK(mem((long)pl[9], &K));
+    ERRCHK(mem((long)pl[10], &V));
+    // every place of its own: each stride reaches past what the smaller ones span, the distance between keys and values in one piece of memory
+    // (rows k | v, say) among them
+    const long long apart = std::llabs((const char*)V->ptr - (const char*)K->ptr) / (long long)K->esize();
+    const long long reach = (c.pages - 1) * (c.pages > 1 ? c.sP : 0) + (c.kvH - 1) * (c.kvH > 1 ? c.sH : 0) + (c.pageSize - 1) * (c.pageSize > 1 ? c.sT : 0) + c.hs;
+    std::pair<long long, int> dims[4] = {{c.sP, c.pages}, {c.sH, c.kvH}, {c.sT, c.pageSize}, {apart, apart < reach ? 2 : 1}};
+    std::sort(dims, dims + 4);
+    long long span = c.hs;
+    for (const auto& d : dims) {
+        if (d.second == 1) continue;
+        if (d.first < span) {
+            last_detail = "the strides of the pages let positions overlap";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+        span += (d.second - 1) * d.first;
+    }
+    const long long rows = (long long)c.tokens * (c.H + 2 * c.kvH) * c.hs;
+    bool clash = false;
+    MemItem* in[] = {X, nullptr, nullptr, nullptr, nullptr, nullptr};
+    long long count[] = {rows, (long long)c.batch * c.maxPages, c.batch + 1, c.batch, c.hs, c.hs};
+    for (int i = 0; i < 3; i++) {
+        ERRCHK(mem((long)pl[11 + i], &meta));
+        in[1 + i] = meta;
+    }
+    for (int i = 0; i < 2; i++)
+        if (pl[20 + i]) {
+            ERRCHK(mem((long)pl[20 + i], &W[i]));
+            if (W[i]->half != X->half) return MCH_ERROR_MEMORY_MIXED_HALF_TYPES;
+            RANGE(W[i], 0, c.hs);
+            in[4 + i] = W[i];
+        }
+    for (int i = 0; i < 6; i++)
+        if (in[i]) clash = clash || overlap(K, reach, in[i], count[i]) || overlap(V, reach, in[i], count[i]) || (i > 3 && overlap(Q, (long long)c.tokens * c.H * c.hs, in[i], count[i]));
+    if (clash) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    const float* turns;
+    ERRCHK(rope_turns((long)pl[18], c.hs, (long long)c.maxPages * c.pageSize, &turns));
+    HIPCHK(k_paged_append(m_stream, X->dt(), c, X->ptr, Q->ptr, W[0] ? W[0]->ptr : nullptr, W[1] ? W[1]->ptr : nullptr, pl[19] != 0, pf[0], turns));
+    m_mem.touch((long)pl[9]);
+    m_mem.touch((long)pl[10]);
+    m_mem.touch((long)pl[14]);
+    return 0;
+}
+
+// ATTN_PAGED_FWD: f{scale}, l{...[, maxNew]} behind what paged_operands reads
+long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll)
+{
+    NEED_F(1, 1);
+    NEED_L(18, 19);
+    if (ll > 18 && pl[18] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    PagedCache c;
+    MemItem *Q, *Y;
+    ERRCHK(paged_operands(pl, pl[2], &c, &Q, &Y));
+    const float scale = pf[0] != 0.f ? pf[0] : (float)(1.0 / sqrt((double)c.hs));
+    HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale));
+    m_mem.touch((long)pl[14]);
+    return 0;
+}
+
 // the same call through the entry point that allocates nothing
 long Kernel::attn_decode_no_alloc(float* pf, long lf, MCH_LONGLONG* pl, long ll)
 {
@@ -2753,7 +2965,7 @@ static const char* api_name(long fn)
 #define N(x) {MCH_FN_##x, "CUDA_FN_" #x}
     static const struct { long id; const char* name; } table[] = {
         {MCH_DLL_FREEMEM, "CUDA_DLL_FREEMEM"}, {MCH_DLL_INITIALIZE, "CUDA_DLL_INITIALIZE"}, {MCH_DLL_CLEANUP, "CUDA_DLL_CLEANUP"},
-        N(SETDEVICE), N(GETDEVICE), N(SYNCHRONIZEDEVICE), N(CREATE_MEMORYPOINTER), N(FREE_MEMORYPOINTER), N(ALLOCMEM_HALF), N(ALLOCMEM), N(FREEMEM), N(GETMEM), N(SETMEM), N(CREATE_CUDNN), N(FREE_CUDNN), N(CREATE_TENSORDESC), N(FREE_TENSORDESC), N(SET_TENSORDESC), N(CREATE_EXTENSION), N(FREE_EXTENSION), N(EXTENSION_RUN), N(SOFTMAX_FWD), N(SOFTMAX_BWD), N(ATTN_CREATE), N(ATTN_FREE), N(ATTN_SET), N(ATTN_FWD), N(ATTN_BWD), N(SET), N(COPY), N(GEMM2), N(GEMM), N(GEMV), N(AXPY), N(SCAL), N(SCALE), N(ADD_SCALAR), N(ADD), N(SUB), N(MUL), N(DIV), N(EXP), N(LOG), N(POWX), N(SQRT), N(TRANSPOSE), N(MASK), N(MASK_BATCH), N(TRANSPOSE_HW), N(INVERT), N(CHANNEL_MEAN), N(CHANNEL_MAX), N(CHANNEL_SUB), N(CHANNEL_SUM), N(CHANNEL_DIV), N(CHANNEL_DOT), N(CHANNEL_COPY), N(CHANNEL_FILLFROM), N(CHANNEL_COPYALL), N(CHANNEL_DUP), N(CHANNEL_SUM2), N(EMBED_FWD), N(RELU_FWD), N(RELU_BWD), N(GELU_FWD), N(GELU_BWD), N(SILU_FWD), N(SILU_BWD), N(CREATE_LAYERNORM), N(FREE_LAYERNORM), N(LAYERNORM_FWD), N(LAYERNORM_BWD), N(CREATE_ROPE), N(FREE_ROPE), N(ROPE_FWD), N(ROPE_BWD), N(CREATE_BLOBLOADER), N(FREE_BLOBLOADER), N(BLOBLOADER_LOAD), N(BLOBLOADER_RESETOFFSET), N(BLOBLOADER_ADDTOOFFSET), N(ATTN_DECODE_FWD), N(RMSNORM_FWD), N(SWIGLU_FWD), N(QKV_PROJ_HEADS), N(LINEAR_FWD), N(LINEAR_BWD), N(QKV_HEADS_GRAD), N(RMSNORM_BWD), N(SWIGLU_BWD), N(NORM_ADD_FWD), N(NORM_ADD_BWD), N(LINEAR_HEADS_GROUP)};
+        N(SETDEVICE), N(GETDEVICE), N(SYNCHRONIZEDEVICE), N(CREATE_MEMORYPOINTER), N(FREE_MEMORYPOINTER), N(ALLOCMEM_HALF), N(ALLOCMEM), N(FREEMEM), N(GETMEM), N(SETMEM), N(CREATE_CUDNN), N(FREE_CUDNN), N(CREATE_TENSORDESC), N(FREE_TENSORDESC), N(SET_TENSORDESC), N(CREATE_EXTENSION), N(FREE_EXTENSION), N(EXTENSION_RUN), N(SOFTMAX_FWD), N(SOFTMAX_BWD), N(ATTN_CREATE), N(ATTN_FREE), N(ATTN_SET), N(ATTN_FWD), N(ATTN_BWD), N(SET), N(COPY), N(GEMM2), N(GEMM), N(GEMV), N(AXPY), N(SCAL), N(SCALE), N(ADD_SCALAR), N(ADD), N(SUB), N(MUL), N(DIV), N(EXP), N(LOG), N(POWX), N(SQRT), N(TRANSPOSE), N(MASK), N(MASK_BATCH), N(TRANSPOSE_HW), N(INVERT), N(CHANNEL_MEAN), N(CHANNEL_MAX), N(CHANNEL_SUB), N(CHANNEL_SUM), N(CHANNEL_DIV), N(CHANNEL_DOT), N(CHANNEL_COPY), N(CHANNEL_FILLFROM), N(CHANNEL_COPYALL), N(CHANNEL_DUP), N(CHANNEL_SUM2), N(EMBED_FWD), N(RELU_FWD), N(RELU_BWD), N(GELU_FWD), N(GELU_BWD), N(SILU_FWD), N(SILU_BWD), N(CREATE_LAYERNORM), N(FREE_LAYERNORM), N(LAYERNORM_FWD), N(LAYERNORM_BWD), N(CREATE_ROPE), N(FREE_ROPE), N(ROPE_FWD), N(ROPE_BWD), N(CREATE_BLOBLOADER), N(FREE_BLOBLOADER), N(BLOBLOADER_LOAD), N(BLOBLOADER_RESETOFFSET), N(BLOBLOADER_ADDTOOFFSET), N(ATTN_DECODE_FWD), N(RMSNORM_FWD), N(SWIGLU_FWD), N(QKV_PROJ_HEADS), N(LINEAR_FWD), N(LINEAR_BWD), N(QKV_HEADS_GRAD), N(RMSNORM_BWD), N(SWIGLU_BWD), N(NORM_ADD_FWD), N(NORM_ADD_BWD), N(LINEAR_HEADS_GROUP), N(QK_NORM_ROPE_FWD), N(QK_NORM_ROPE_BWD), N(PAGED_APPEND), N(ATTN_PAGED_FWD)};
 #undef N
     for (const auto& t : table)
         if (t.id == fn) return t.name;

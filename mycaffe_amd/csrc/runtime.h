@@ -100,6 +100,9 @@ struct RopeState {
     int sharedIdx = 0, count = 0, batch = 0, seq = 0, heads = 0, hs = 0;
     float theta = 10000.f;
     std::shared_ptr<void> dcos, dsin;  // device tables [seq, hs/2] fp32, shared by sharedIdx
+    // {cos, sin} of angles taken in 64 bits, made when a call that uses them first comes (the tables above follow the reference, whose
+    // fp32 angles are off by up to half a step of the position)
+    std::shared_ptr<void> turns;
 };
 struct LayerNormState {
     bool set = false;
@@ -176,6 +179,11 @@ public:
     std::string last_detail;  // human-readable detail of the last failure
 
 private:
+    long rope_turns(long hRope, long long hs, long long positions, const float** turns);
+    long paged_operands(const MCH_LONGLONG* pl, long long rowHeads, PagedCache* c, MemItem** rows, MemItem** out);
+    long paged_append(float* pf, long lf, MCH_LONGLONG* pl, long ll);
+    long attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll);
+    long qk_norm_rope(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool backward);
     long attn_decode_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool staticScratch);
     long workspace(size_t bytes, void** p);
     void workspace_or_none(size_t* bytes, void** p);

@@ -126,6 +126,10 @@ class CUDAFN:
     NORM_ADD_FWD = 2010
     NORM_ADD_BWD = 2011
     LINEAR_HEADS_GROUP = 2012
+    QK_NORM_ROPE_FWD = 2013
+    QK_NORM_ROPE_BWD = 2014
+    PAGED_APPEND = 2015
+    ATTN_PAGED_FWD = 2016
 
 
 class CUDAQRY:
@@ -828,6 +832,37 @@ class CudaDnn:
     def SwigluBackward(self, n, hA, hB, hdY, hdA, hdB):
         """Gradients of y = silu(a) * b in one pass."""
         self._ex2(CUDAFN.SWIGLU_BWD, None, [n, hA, hB, hdY, hdA, hdB])
+
+    # ---- norms of heads, paged caches -----------------------------------------------------------
+    def QkNormRopeForward(self, nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hYq, hYk, hRope=0, fEps=1e-5):
+        """RMS norm of every head of q (B,H,T,hs) and k (B,kvH,T,hs), with weights of hs values (0: ones), and the rotation of its position
+        (hRope 0: none) in one pass; hYq may be hQ, hYk hK."""
+        self._ex2(CUDAFN.QK_NORM_ROPE_FWD, [fEps], [nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hRope, hYq, hYk])
+
+    def QkNormRopeBackward(self, nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hdYq, hdYk, hdQ, hdK, hdWq, hdWk, hRope=0, fEps=1e-5,
+                           bAccumulate=False):
+        """Gradient of QkNormRopeForward from q and k as that had them.  hdWq, hdWk (0: not computed) are overwritten, with bAccumulate added to."""
+        self._ex2(CUDAFN.QK_NORM_ROPE_BWD, [fEps], [nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hRope, hdYq, hdYk, hdQ, hdK, hdWq, hdWk,
+                                                    1 if bAccumulate else 0])
+
+    def PagedAppend(self, nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQKV, hQ, hKPages, hVPages, hTable, hStarts, hLens,
+                    nStridePage, nStrideHead, nStridePos, hRope=0, bNorm=False, hWq=0, hWk=0, fEps=1e-5):
+        """New tokens of many sequences into a paged cache: rows q | k | v of hQKV, queries and keys with the norm of QkNormRopeForward (bNorm) and
+        the rotation of their position (hRope), queries to hQ (tokens, heads, hs), keys and values to the pages that hTable (batch, nMaxPages) names.
+        Sequence b has the rows hStarts[b] .. hStarts[b + 1] - 1 and hLens[b] positions, these tokens the last of them (all three fp32)."""
+        self._ex2(CUDAFN.PAGED_APPEND, [fEps], [nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQKV, hKPages, hVPages, hTable,
+                                                hStarts, hLens, hQ, nStridePage, nStrideHead, nStridePos, hRope, 1 if bNorm else 0, hWq, hWk])
+
+    def AttnPagedForward(self, nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQ, hKPages, hVPages, hTable, hStarts, hLens, hY,
+                         nStridePage, nStrideHead, nStridePos, fScale=0.0, nMaxNew=0):
+        """Attention of the new tokens of many sequences (hQ as PagedAppend writes it), each over the positions of its sequence up to its own, to hY
+        (tokens, heads, hs).  Positions whose table entry names no page are left out; a token with none gets zeros.  nMaxNew: no sequence has
+        more new tokens (0: not known)."""
+        rgl = [nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQ, hKPages, hVPages, hTable, hStarts, hLens, hY, nStridePage,
+               nStrideHead, nStridePos]
+        if nMaxNew:
+            rgl.append(nMaxNew)
+        self._ex2(CUDAFN.ATTN_PAGED_FWD, [fScale], rgl)
 
     # ---- RoPE ---------------------------------------------------------------------------------
     def CreateRope(self, nSharedIndex, nGpuID, nCount, nBatch, nSeqLen, nHeads, nDim, fTheta=10000.0):

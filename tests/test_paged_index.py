@@ -1,0 +1,67 @@
+"""What the paged kernels take from device memory (csrc/paged.h), on the host: every number ends inside its range, whatever it is."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PROGRAM = """
+#include <cstdio>
+#include <cstring>
+#include "paged.h"
+static float bits(unsigned u) { float f; memcpy(&f, &u, 4); return f; }
+int main()
+{
+    char what;
+    unsigned u, v, w;
+    int a, b;
+    while (scanf(" %c", &what) == 1) {
+        if (what == 'i') { scanf("%x %d %d", &u, &a, &b); printf("%d\\n", mch::paged_int(bits(u), a, b)); }
+        else if (what == 'p') { scanf("%x %d", &u, &a); printf("%d\\n", mch::paged_page(bits(u), a)); }
+        else {
+            scanf("%x %x %x %d %d", &u, &v, &w, &a, &b);
+            const mch::PagedSpan s = mch::paged_span(bits(u), bits(v), bits(w), a, b);
+            printf("%d %d %d\\n", s.first, s.count, s.len);
+        }
+    }
+}
+"""
+BAD = [np.nan, -np.nan, np.inf, -np.inf, -1.0, -0.0, -0.5, 0.0, 0.99, 1.0, 1e-45, 3.0, 4.0, 4.5, 16777215.0, 16777216.0, 2147483648.0, 4294967296.0, 1e38, -1e38]
+
+
+def hexof(v):
+    return "%08x" % int(np.float32(v).view(np.uint32))
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    d = tmp_path_factory.mktemp("paged_index")
+    (d / "main.cpp").write_text(PROGRAM)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(ROOT, "mycaffe_amd", "csrc"), str(d / "main.cpp"), "-o", str(d / "main")], check=True)
+
+    def run(lines):
+        out = subprocess.run([str(d / "main")], input="\n".join(lines) + "\n", capture_output=True, text=True, check=True).stdout
+        return [tuple(int(x) for x in line.split()) for line in out.splitlines()]
+    return run
+
+
+def test_whole_numbers(ask):
+    for hi in (0, 1, 5, 1 << 24):
+        got = ask(["i %s 0 %d" % (hexof(v), hi) for v in BAD])
+        want = [0 if np.isnan(v) else int(min(max(np.trunc(np.float64(np.float32(v))), 0), hi)) for v in BAD]
+        assert [g[0] for g in got] == want
+
+
+def test_pages(ask):
+    for pages in (1, 4, 1 << 24):
+        got = ask(["p %s %d" % (hexof(v), pages) for v in BAD])
+        want = [int(v) if v >= 0 and v < pages else -1 for v in BAD]
+        assert [g[0] for g in got] == want
+
+
+def test_spans_stay_inside(ask):
+    triples = [(a, b, c) for a in BAD for b in BAD for c in BAD[:14]]
+    for (a, b, c), (first, count, length) in zip(triples, ask(["s %s %s %s 7 40" % (hexof(a), hexof(b), hexof(c)) for a, b, c in triples])):
+        assert 0 <= first and 0 <= count and first + count <= 7 and 0 <= length <= 40, (a, b, c)
+    assert ask(["s %s %s %s 7 40" % (hexof(2), hexof(5), hexof(9))]) == [(2, 3, 9)]
