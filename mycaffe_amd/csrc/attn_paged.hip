@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "flash_traits.h"
 #include "kernels.h"
 #include "lane_ops.h"
 #include "paged.h"
@@ -103,15 +104,517 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a)
     }
 }
 
+
+// ---- few rows a sequence: the positions are what is split --------------------------------------------------------------------------
+// 16 rows - tokens times the heads that share a key head - make the columns of one 16 x 16 matrix product, so every key and value is read once
+// for all of them: what bounds this kernel is reading the cache.  All positions of all sequences, in units of four tiles of KT positions, are
+// one list that is dealt to the workgroups in equal runs, whatever the lengths: a run ends inside an item (a sequence's key head and row
+// tile), which the last workgroup to finish puts together.  A wavefront has every fourth tile, with statistics of its own; tiles of the wavefronts
+// meet in LDS at the end of an item.
+//
+// Scores are S^T = K Q^T, so that a lane has one row: register v of a tile holds key 4 (lane / 16) + v of row lane % 16, which is the operand
+// layout that O^T = V^T P^T wants of P (which slot of the contraction is which key only has to agree between the two).  Keys go from memory to the
+// operand registers as they are.  16-bit values take the way through LDS, where the transposing read makes columns of them; fp32 sums (rows in
+// fp32) contract four keys at a time, one a lane group, and take values, of either type, as they come.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+struct SplitArgs {
+    float* part;      // partial results, [workgroup][2][16 {maximum, sum} | 16 rows of HSP]
+    int* tickets;     // one a workgroup; zero between launches
+    int few;          // sequences of more rows a key head than this are another kernel's (0: all are this one's)
+    int shift;        // log2 of the page size, or -1
+    int perTile;      // tokens a row tile
+    int tileHeads;    // heads a row tile, of G
+    int headTiles;    // row tiles that the G heads of a key head take
+};
+
+// of a maximum over scores that a row sees: what tells "all of them -inf" from "none"
+constexpr float SCORE_FLOOR = -3.0e38f;
+
+__device__ __forceinline__ void put2(float* p, float a, float b)
+{
+    union { float f[2]; uint64_t u; } x = {{a, b}};
+    __hip_atomic_store((uint64_t*)p, x.u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p)
+{
+    union { uint64_t u; float2 f; } x;
+    x.u = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return x.f;
+}
+// weight of sums with maximum m beside others whose maximum is M (sums without a score are zero or not a number)
+__device__ __forceinline__ float weight_of(float m, float M) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - M) : 1.f; }
+
+template <typename T> __device__ __forceinline__ bool not_finite(u32x4 x)
+{
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : 0x7f807f80u;
+    bool r = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) r = r || (x[i] & E) == E;
+        else r = r || (x[i] & 0x7f80u) == 0x7f80u || (x[i] & 0x7f800000u) == 0x7f800000u;
+    }
+    return r;
+}
+
+template <typename TQ, typename TC, int HSP>
+__global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs a, SplitArgs w)
+{
+    constexpr bool B16 = sizeof(TQ) == 2;
+    constexpr int EPL = 16 / (int)sizeof(TC), NF = HSP / (4 * EPL);            // values a piece, pieces a lane and key
+    constexpr int KG = sizeof(TC) == 4 ? 1 : 2, KT = 16 * KG, UNIT = 4 * KT;   // groups of 16 keys a tile
+    constexpr int VE = sizeof(TC) == 4 ? 4 : HSP / 16 < 8 ? HSP / 16 : 8, NH = HSP / (16 * VE), NO = HSP / 16;
+    constexpr int ROWB = HSP * 2, STAGE = B16 ? KT * ROWB : 0;
+    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2);
+    constexpr int SHARED = 4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4;
+    static_assert(HSP == 64 || HSP == 128, "tile");
+    __shared__ __attribute__((aligned(16))) unsigned char smem[SHARED];
+    __shared__ float sM[4][16], sL[4][16];
+    __shared__ uint64_t sScan[4], sFound[2];
+    __shared__ int sSeq, sBad, sTicket;
+    float* sO = (float*)smem;                                                   // [wavefront][row][LDO], once the stages are done with
+
+    const PagedCache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int G = c.H / c.kvH, positions = c.maxPages * c.pageSize;
+
+    // units of a sequence; a row tile without positions is one all the same (its rows are zeros)
+    auto span_of = [&](int b) { return paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions); };
+    auto units_of = [&](const PagedSpan& s) { return max(1, (s.len + UNIT - 1) / UNIT); };
+    auto tiles_of = [&](const PagedSpan& s) -> int { return w.few && (long long)s.count * G > w.few ? 0 : (s.count + w.perTile - 1) / w.perTile * w.headTiles; };
+    auto work_of = [&](int b) -> uint64_t {
+        if (b >= c.batch) return 0;
+        const PagedSpan s = span_of(b);
+        return (uint64_t)tiles_of(s) * c.kvH * units_of(s);
+    };
+    // sums of 256 sequences at a time: the exclusive one of the thread's own, and all of them
+    auto scan = [&](uint64_t v, uint64_t* all) -> uint64_t {
+        uint64_t x = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t y = __shfl_up(x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) sScan[wave] = x;
+        __syncthreads();
+        uint64_t before = 0, sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            before += i < wave ? sScan[i] : 0;
+            sum += sScan[i];
+        }
+        *all = sum;
+        return before + x - v;
+    };
+    uint64_t mine = work_of(tid), total, at = scan(mine, &total);
+    for (int b0 = 256; b0 < c.batch; b0 += 256) {
+        uint64_t all;
+        scan(work_of(b0 + tid), &all);
+        total += all;
+    }
+    const uint64_t W = total < gridDim.x ? total : gridDim.x;
+    if (blockIdx.x >= W) return;
+    const uint64_t lo = total * blockIdx.x / W, hi = total * (blockIdx.x + 1) / W;
+    // the sequence that has unit `lo`
+    {
+        uint64_t all, base = 0;
+        for (int b0 = 0;; b0 += 256) {
+            if (b0) { mine = work_of(b0 + tid); at = base + scan(mine, &all); }
+            else if (c.batch > 256) scan(mine, &all);
+            else all = total;
+            if (at <= lo && lo < at + mine) { sSeq = b0 + tid; sFound[0] = at; }
+            base += all;
+            if (lo < base) break;
+        }
+        __syncthreads();
+    }
+    int b = sSeq;
+    uint64_t local = lo - sFound[0];
+    PagedSpan sp = span_of(b);
+
+    const TC *kp = (const TC*)c.k, *vp = (const TC*)c.v;
+    for (uint64_t u = lo; u < hi;) {
+        // ---- the item and the piece of it that is this workgroup's ----
+        const int units = units_of(sp);
+        const uint64_t item = local / units;
+        const int unit0 = (int)(local - item * units), count = (int)min((uint64_t)(units - unit0), hi - u);
+        const int kh = (int)(item % c.kvH), tile = (int)(item / c.kvH), ht = tile % w.headTiles, j0 = tile / w.headTiles * w.perTile;
+        const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads), nt = min(w.perTile, sp.count - j0);
+        const int base = sp.len - sp.count + j0;                                 // position of the tile's first token
+        const int p0 = unit0 * UNIT, p1 = min(min((unit0 + count) * UNIT, sp.len), base + nt);
+        const int token = r16 / w.tileHeads, head = r16 - token * w.tileHeads;   // of the lane's row
+        const bool rowLive = token < nt && head < nh;
+        const int last = base + token;
+        auto row_at = [&](int t, int h) { return ((size_t)(sp.first + j0 + t) * c.H + h0 + h) * c.hs; };
+
+        // ---- the row's queries, in the operand layout ----
+        u32x4 qb[B16 ? NF : 1];
+        float qf[B16 ? 1 : NF * EPL];
+        {
+            const TQ* q = (const TQ*)a.q + (rowLive ? row_at(token, head) : 0);
+#pragma unroll
+            for (int f = 0; f < NF; f++) {
+                const int d = (4 * f + g) * EPL;
+                if constexpr (B16) qb[f] = rowLive && d < c.hs ? *(const u32x4*)(q + d) : u32x4{0u, 0u, 0u, 0u};
+                else
+#pragma unroll
+                    for (int e = 0; e < EPL; e += 4) {
+                        const float4 x = rowLive && d < c.hs ? *(const float4*)(q + d + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        qf[f * EPL + e] = x.x; qf[f * EPL + e + 1] = x.y; qf[f * EPL + e + 2] = x.z; qf[f * EPL + e + 3] = x.w;
+                    }
+            }
+        }
+        // ---- where keys lie: the lane's keys r16 and 16 + r16 of a tile ----
+        const float* table = c.table + (size_t)b * c.maxPages;
+        auto entry_of = [&](int t, float (&e)[KG]) {
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                const int p = t + 16 * k + r16;
+                e[k] = p < p1 ? table[w.shift >= 0 ? p >> w.shift : p / c.pageSize] : -1.f;
+            }
+        };
+        auto places = [&](int t, const float (&e)[KG], long long (&off)[KG]) {
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                const int p = t + 16 * k + r16, page = p < p1 ? paged_page(e[k], c.pages) : -1;
+                const int slot = w.shift >= 0 ? p & (c.pageSize - 1) : p % c.pageSize;
+                off[k] = page >= 0 ? page * c.sP + slot * c.sT + kh * c.sH : -1;
+            }
+        };
+        const u32x4 zero4 = {0u, 0u, 0u, 0u};
+        auto piece_of = [&](const TC* p, long long off, int d) -> u32x4 { return off >= 0 && d < c.hs ? *(const u32x4*)(p + off + d) : zero4; };
+        u32x4 kf[KG][NF], vf[B16 ? KG : 1][B16 ? NF : 1], vd[B16 ? 1 : KG][4][NH];
+        auto load_k = [&](const long long (&off)[KG]) {
+#pragma unroll
+            for (int k = 0; k < KG; k++)
+#pragma unroll
+                for (int f = 0; f < NF; f++) kf[k][f] = piece_of(kp, off[k], (4 * f + g) * EPL);
+        };
+        auto load_v = [&](const long long (&off)[KG]) {
+            if constexpr (B16) {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int f = 0; f < NF; f++) vf[k][f] = piece_of(vp, off[k], (4 * f + g) * EPL);
+            } else {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const long long o = __shfl(off[k], 4 * g + v);
+#pragma unroll
+                        for (int h = 0; h < NH; h++) {
+                            const int d = 16 * VE * h + VE * r16;
+                            if constexpr (sizeof(TC) * VE == 16) vd[k][v][h] = piece_of(vp, o, d);
+                            else {
+                                const uint2 x = o >= 0 && d < c.hs ? *(const uint2*)(vp + o + d) : make_uint2(0u, 0u);
+                                vd[k][v][h] = u32x4{x.x, x.y, 0u, 0u};
+                            }
+                        }
+                    }
+            }
+        };
+        // ---- the wavefront's tiles ----
+        floatx4 o[NO];
+        float m = -INFINITY, l = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NO; i++) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+        unsigned char* stage = smem + wave * STAGE;
+        long long off[KG], next[KG];
+        float entry[KG];
+        int t = p0 + wave * KT;
+        if (tid == 0) sBad = 0;
+        if (t < p1) {
+            entry_of(t, entry);
+            places(t, entry, off);
+            load_k(off);
+            load_v(off);
+            entry_of(t + UNIT, entry);
+        }
+        for (; t < p1; t += UNIT) {
+            floatx4 s[KG];
+#pragma unroll
+            for (int k = 0; k < KG; k++) {
+                s[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < NF; f++) {
+                    if constexpr (B16) s[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(bf16x8*)&kf[k][f], *(bf16x8*)&qb[f], s[k], 0, 0, 0);
+                    else
+#pragma unroll
+                        for (int e = 0; e < EPL; e++) {
+                            float x;
+                            if constexpr (EPL == 4) x = __uint_as_float(kf[k][f][e]);
+                            else x = __uint_as_float(e & 1 ? kf[k][f][e >> 1] & 0xffff0000u : kf[k][f][e >> 1] << 16);
+                            s[k] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, qf[f * EPL + e], s[k], 0, 0, 0);
+                        }
+                }
+            }
+            uint32_t given = 0;                                                  // keys of the tile that lie in a page
+#pragma unroll
+            for (int k = 0; k < KG; k++) given |= (uint32_t)(__ballot(off[k] >= 0) & 0xffffu) << (16 * k);
+            // the next tile's keys, and the entries of the one behind it
+            places(t + UNIT, entry, next);
+            load_k(next);
+            entry_of(t + 2 * UNIT, entry);
+
+            const bool open = t + KT <= base + 1;                                // every row sees all of it
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < KG; k++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) s[k][v] *= a.c2;
+            if (open && given == (KG == 2 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) mx = fmaxf(mx, s[k][v]);
+                mx = fmaxf(mx, SCORE_FLOOR);
+            } else {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const int key = 16 * k + 4 * g + v;
+                        const bool sees = (given >> key & 1) && t + key <= last;
+                        mx = fmaxf(mx, sees ? fmaxf(s[k][v], SCORE_FLOOR) : -INFINITY);
+                        s[k][v] = sees ? s[k][v] : -INFINITY;
+                    }
+            }
+            mx = max_lane_xor<16>(mx);
+            mx = fmaxf(max_lane_xor<32>(mx), m);
+            const float ref = mx > -INFINITY ? mx : 0.f, alpha = __builtin_amdgcn_exp2f(m - ref);
+            const bool moved = __any(mx != m);
+            m = mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < KG; k++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    s[k][v] = __builtin_amdgcn_exp2f(s[k][v] - ref);
+                    sum += s[k][v];
+                }
+            l = l * alpha + sum;
+            if (moved)
+#pragma unroll
+                for (int i = 0; i < NO; i++) o[i] *= alpha;
+            if constexpr (B16) {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int f = 0; f < NF; f++) {
+                        const int row = 16 * k + r16, sw = HSP == 64 ? (row >> 1) & 7 : row & 15;
+                        *(u32x4*)(stage + row * ROWB + (((4 * f + g) ^ sw) << 4)) = vf[k][f];
+                        if (!open) bad = bad || not_finite<TC>(vf[k][f]);
+                    }
+                load_v(next);
+                wave_lds_fence();
+                // weights rounded to 16 bits, their sum not: the roundings of many weights even out
+                const u32x4 p = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]), pack_bf16x2(s[KG - 1][0], s[KG - 1][1]), pack_bf16x2(s[KG - 1][2], s[KG - 1][3])};
+#pragma unroll
+                for (int i = 0; i < NO; i++) {
+                    uint2 half[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int row = 16 * k + 4 * g + (r16 >> 2), sw = HSP == 64 ? (row >> 1) & 7 : row & 15, piece = 2 * i + ((r16 & 3) >> 1);
+                        half[k] = lds_read_tr16((const bf16_t*)(stage + row * ROWB + ((piece ^ sw) << 4) + (r16 & 1) * 8));
+                    }
+                    u32x4 vt = {half[0].x, half[0].y, half[1].x, half[1].y};
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(bf16x8*)&vt, *(const bf16x8*)&p, o[i], 0, 0, 0);
+                }
+                wave_lds_fence();
+            } else {
+#pragma unroll
+                for (int k = 0; k < KG; k++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++)
+#pragma unroll
+                        for (int h = 0; h < NH; h++) {
+                            if (!open) bad = bad || not_finite<TC>(vd[k][v][h]);
+#pragma unroll
+                            for (int e = 0; e < VE; e++) {
+                                float x;
+                                if constexpr (sizeof(TC) == 4) x = __uint_as_float(vd[k][v][h][e]);
+                                else x = __uint_as_float(e & 1 ? vd[k][v][h][e >> 1] & 0xffff0000u : vd[k][v][h][e >> 1] << 16);
+                                o[h * VE + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, s[k][v], o[h * VE + e], 0, 0, 0);
+                            }
+                        }
+                load_v(next);
+            }
+#pragma unroll
+            for (int k = 0; k < KG; k++) off[k] = next[k];
+        }
+        // ---- the wavefronts meet ----
+        l = add_lane_xor<32>(add_lane_xor<16>(l));
+        __syncthreads();                                                         // the stages are done with
+        if (g == 0) { sM[wave][r16] = m; sL[wave][r16] = l; }
+#pragma unroll
+        for (int i = 0; i < NO; i++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                const int d = B16 ? 16 * i + 4 * g + v : 16 * VE * (i / VE) + VE * (4 * g + v) + i % VE;
+                sO[(wave * 16 + r16) * LDO + d] = o[i][v];
+            }
+        if (__any(bad) && lane == 0) sBad = 1;
+        __syncthreads();
+        if (sBad) {
+            // A value that is not finite lies where only some of the rows look: weights of zero would not keep it from the others.  Row by row, then.
+            __syncthreads();
+            for (int r = wave; r < nt * w.tileHeads; r += 4) {
+                const int tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+                if (hd >= nh) continue;
+                const TQ* q = (const TQ*)a.q + row_at(tk, hd);
+                float qv[2], acc[2] = {0.f, 0.f}, mr = -INFINITY, lr = 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; i++) qv[i] = lane + 64 * i < c.hs ? value_of<TQ>(q[lane + 64 * i]) : 0.f;
+                for (int p = p0; p < p1 && p <= base + tk; p++) {
+                    const int e = p / c.pageSize, page = paged_page(table[e], c.pages);
+                    if (page < 0) continue;
+                    const long long at = page * c.sP + (p - e * c.pageSize) * c.sT + kh * c.sH;
+                    float x = 0.f, val[2];
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int d = lane + 64 * i;
+                        x += d < c.hs ? qv[i] * value_of<TC>(kp[at + d]) : 0.f;
+                        val[i] = d < c.hs ? value_of<TC>(vp[at + d]) : 0.f;
+                    }
+                    x = group_sum<64>(x) * a.c2;
+                    const float mn = fmaxf(mr, fmaxf(x, SCORE_FLOOR)), f = __builtin_amdgcn_exp2f(mr - mn), wt = __builtin_amdgcn_exp2f(x - mn);
+                    mr = mn;
+                    lr = lr * f + wt;
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc[i] = acc[i] * f + wt * val[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (lane == 0) { sM[i][r] = i ? -INFINITY : mr; sL[i][r] = i ? 0.f : lr; }
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        if (lane + 64 * j < HSP) sO[(i * 16 + r) * LDO + lane + 64 * j] = i ? 0.f : acc[j];
+                }
+            }
+            __syncthreads();
+        }
+        const bool whole = count == units;
+        const int rows = nt * w.tileHeads, pairs = c.hs >> 1;
+        float* part = w.part + ((size_t)blockIdx.x * 2 + (unit0 == 0 ? 1 : 0)) * PART;
+        for (int e = tid; e < rows * pairs; e += 256) {
+            const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+            if (hd >= nh) continue;
+            float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) M = fmaxf(M, sM[i][r]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float f = weight_of(sM[i][r], M);
+                const float2 v = *(const float2*)(sO + (i * 16 + r) * LDO + d);
+                L += sL[i][r] * f;
+                x += v.x * f;
+                y += v.y * f;
+            }
+            if (whole) {
+                TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
+                const float xs = M > -INFINITY ? x / L : 0.f, ys = M > -INFINITY ? y / L : 0.f;
+                if constexpr (B16) *(uint32_t*)out = pack_bf16x2(xs, ys);
+                else *(float2*)out = make_float2(xs, ys);
+            } else {
+                put2(part + 32 + r * HSP + d, x, y);
+                if (d == 0) put2(part + 2 * r, M, L);
+            }
+        }
+        if (!whole) {
+            // Who comes last puts the item together; its workgroups follow from the list alone.  Partial results go to the level that all XCDs
+            // share, and are there before the ticket is taken.
+            const uint64_t first = u - unit0, end = first + units - 1;
+            const int wf = (int)(((first + 1) * W - 1) / total), we = (int)(((end + 1) * W - 1) / total);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) sTicket = __hip_atomic_fetch_add(w.tickets + wf, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __syncthreads();
+            if (sTicket == we - wf) {
+                for (int e = tid; e < rows * pairs; e += 256) {
+                    const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+                    if (hd >= nh) continue;
+                    float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+                    for (int i = wf; i <= we; i += 8) {
+                        float2 ml[8], v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float* from = w.part + ((size_t)min(i + j, we) * 2 + (i + j == wf ? 1 : 0)) * PART;
+                            ml[j] = get2(from + 2 * r);
+                            v[j] = get2(from + 32 + r * HSP + d);
+                        }
+                        float Mn = M;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) Mn = i + j <= we ? fmaxf(Mn, ml[j].x) : Mn;
+                        const float f0 = weight_of(M, Mn);
+                        L *= f0; x *= f0; y *= f0;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float f = weight_of(ml[j].x, Mn);
+                            L += i + j <= we ? ml[j].y * f : 0.f;
+                            x += i + j <= we ? v[j].x * f : 0.f;
+                            y += i + j <= we ? v[j].y * f : 0.f;
+                        }
+                        M = Mn;
+                    }
+                    TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
+                    const float xs = M > -INFINITY ? x / L : 0.f, ys = M > -INFINITY ? y / L : 0.f;
+                    if constexpr (B16) *(uint32_t*)out = pack_bf16x2(xs, ys);
+                    else *(float2*)out = make_float2(xs, ys);
+                }
+                if (tid == 0) __hip_atomic_store(w.tickets + wf, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+            }
+        }
+        // ---- the next item ----
+        u += count;
+        local += count;
+        if (u < hi) {
+            if (local == (uint64_t)tiles_of(sp) * c.kvH * units) {
+                local = 0;
+                do sp = span_of(++b); while (tiles_of(sp) == 0);
+            }
+            __syncthreads();                                                     // LDS is read no more
+        }
+    }
+}
+
+constexpr int SPLIT_GRID = 512;   // two workgroups a CU
+
+inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// rows and cache in pieces of 16 bytes
+inline bool in_pieces(const PagedCache& c, DType dt, const void* q, const void* y)
+{
+    const int e = dt == BF16 || c.ct == BF16 ? 8 : 4;
+    return c.hs <= 128 && c.hs % e == 0 && c.sP % e == 0 && c.sH % e == 0 && c.sT % e == 0 && at16(c.k) && at16(c.v) && at16(q) && at16(y);
+}
+
 }  // namespace
 
-hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale)
+size_t attn_paged_workspace_bytes(const PagedCache& c) { return (size_t)SPLIT_GRID * 2 * 16 * ((c.hs <= 64 ? 64 : 128) + 2) * sizeof(float); }
+size_t attn_paged_tickets(const PagedCache& c) { return SPLIT_GRID; }
+
+hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets)
 {
     PagedAttnArgs a = {};
     a.c = c; a.q = q; a.y = y; a.c2 = scale * 1.44269504088896340736f;
     auto go = [&](auto type, auto ctype) {
         typedef decltype(type) T_;
         typedef decltype(ctype) TC_;
+        if (in_pieces(c, dt, q, y)) {
+            const int G = c.H / c.kvH;
+            SplitArgs w = {};
+            w.part = (float*)workspace;
+            w.tickets = tickets;
+            w.shift = (c.pageSize & (c.pageSize - 1)) == 0 ? __builtin_ctz(c.pageSize) : -1;
+            w.headTiles = (G + 15) / 16;
+            w.tileHeads = (G + w.headTiles - 1) / w.headTiles;
+            w.perTile = 16 / w.tileHeads;
+            if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 64>), SPLIT_GRID, 256, 0, s, a, w);
+            else hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
+            return hipGetLastError();
+        }
         const dim3 grid(c.tokens, (c.H + 3) / 4);
         if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 16>), grid, 256, 0, s, a);
         else if (c.hs <= 128) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 32>), grid, 256, 0, s, a);
