@@ -580,6 +580,337 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
     }
 }
 
+// ---- chunks: rows by the hundred ----------------------------------------------------------------------------------------------------
+// A workgroup has 128 rows of one key head (tokens times the heads that share it), 32 a wavefront, and stages blocks of KB keys and values in LDS for
+// all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
+// follow each other by key head), whose L2 then holds that head's keys and values.  Where tiles are few their blocks are split among
+// workgroups, and the last one puts a tile together.
+struct ChunkArgs {
+    float* part;      // [split][tile][key head x head tile][128 {maximum, sum} | 128 rows of HSP]
+    int* tickets;     // [tile][key head x head tile]; zero between launches
+    int few;          // sequences of at most this many rows a key head are another kernel's
+    int shift, perTile, tileHeads, headTiles, splits;
+};
+
+// the block_scan of 256 threads: the exclusive sum of the thread's own number, and all of them
+__device__ __forceinline__ int block_scan(int v, int* sums, int* all)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    int before = 0, sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        before += i < wave ? sums[i] : 0;
+        sum += sums[i];
+    }
+    *all = sum;
+    return before + x - v;
+}
+
+template <typename TQ, typename TC, int HSP>
+__global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs a, ChunkArgs w)
+{
+    typedef FlashTraits<TQ> TR;
+    constexpr bool B16 = sizeof(TQ) == 2;
+    constexpr int KB = B16 ? 64 : 32, KF = HSP / TR::CPF, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
+    constexpr int LDK = B16 ? HSP + 8 : HSP + 4, LDV = B16 ? HSP + 8 : HSP;                       // values a row in LDS
+    constexpr int PART = 128 * (HSP + 2);
+    __shared__ __attribute__((aligned(16))) TQ sK[KB * LDK];
+    __shared__ __attribute__((aligned(16))) TQ sV[KB * LDV];
+    __shared__ long long sPlace[2][KB];
+    __shared__ uint64_t sGiven[2];
+    __shared__ int sSum[4], sSeq, sTile, sBad, sTicket, sFront;
+
+    const PagedCache& c = a.c;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
+    const int G = c.H / c.kvH, positions = c.maxPages * c.pageSize;
+    const int groups = c.kvH * w.headTiles, want = blockIdx.x / groups, group = blockIdx.x - want * groups, kh = group / w.headTiles, ht = group - kh * w.headTiles;
+
+    // ---- the sequence and its tile ----
+    auto span_of = [&](int b) { return paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions); };
+    if (tid == 0) { sSeq = -1; sBad = 0; }
+    for (int b0 = 0, base = 0; b0 < c.batch && base <= want; b0 += 256) {
+        int tiles = 0, all;
+        if (b0 + tid < c.batch) {
+            const PagedSpan s = span_of(b0 + tid);
+            if ((long long)s.count * G > w.few) tiles = (s.count + w.perTile - 1) / w.perTile;
+        }
+        const int at = base + block_scan(tiles, sSum, &all);
+        if (at <= want && want < at + tiles) { sSeq = b0 + tid; sTile = tiles - 1 - (want - at); }   // those that see most come first
+        base += all;
+    }
+    __syncthreads();
+    const int b = sSeq;
+    if (b < 0) return;
+    const PagedSpan sp = span_of(b);
+    const int j0 = sTile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
+    const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads);
+    const int end = min(sp.len, base + nt);                                                       // positions that some row sees
+    const float* table = c.table + (size_t)b * c.maxPages;
+    const TC *kp = (const TC*)c.k + kh * c.sH, *vp = (const TC*)c.v + kh * c.sH;
+    auto page_at = [&](int p) -> float { return table[w.shift >= 0 ? p >> w.shift : p / c.pageSize]; };
+    auto place_of = [&](int p, float e) -> long long {
+        const int page = p < end ? paged_page(e, c.pages) : -1;
+        return page >= 0 ? page * c.sP + (w.shift >= 0 ? p & (c.pageSize - 1) : p % c.pageSize) * c.sT : -1;
+    };
+    // pages given up at the front are passed over
+    if (wave == 0) {
+        int front = 0;
+        const int entries = end > 0 ? (end - 1) / c.pageSize + 1 : 0;
+        for (; front < entries; front += 64) {
+            const uint64_t some = __ballot(front + lane < entries && paged_page(table[min(front + lane, entries - 1)], c.pages) >= 0);
+            if (some) { front += __ffsll((unsigned long long)some) - 1; break; }
+        }
+        if (lane == 0) sFront = min(front, entries) * c.pageSize;
+    }
+    __syncthreads();
+    const int kb0 = min(sFront, max(end, 0)) / KB, nkb = (max(end, 0) + KB - 1) / KB;
+    const int first = kb0 + (int)((long long)(nkb - kb0) * blockIdx.y / w.splits), stop = kb0 + (int)((long long)(nkb - kb0) * (blockIdx.y + 1) / w.splits);
+
+    // ---- the lane's row ----
+    const int row = 32 * wave + l32, token = row / w.tileHeads, head = row - token * w.tileHeads;
+    const bool live = token < nt && head < nh;
+    const int last = live ? base + token : -1;
+    const int waveEnd = min(end, base + min((32 * wave + 31) / w.tileHeads, nt - 1) + 1), waveOpen = base + 32 * wave / w.tileHeads + 1;   // past what any, and what every row sees
+    auto row_at = [&](int t, int h) { return ((size_t)(sp.first + j0 + t) * c.H + h0 + h) * c.hs; };
+    const u32x4 zero4 = {0u, 0u, 0u, 0u};
+    u32x4 qf[KF];
+    {
+        const TQ* q = (const TQ*)a.q + (live ? row_at(token, head) : 0);
+#pragma unroll
+        for (int f = 0; f < KF; f++) {
+            const int d = f * TR::CPF + half * TR::EPC;
+            qf[f] = live && d < c.hs ? *(const u32x4*)(q + d) : zero4;
+        }
+    }
+    floatx16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; i++)
+#pragma unroll
+        for (int v = 0; v < 16; v++) o[i][v] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    bool bad = false;
+
+    // ---- staging: places two blocks ahead, values one ----
+    u32x4 rk[NP], rv[NP];
+    auto load = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int r = tid / CPR + RPP * i, d = (tid % CPR) * EPL;
+            const long long at = sPlace[slot][r];
+            const bool there = at >= 0 && d < c.hs;
+            rk[i] = there ? *(const u32x4*)(kp + at + d) : zero4;
+            rv[i] = there ? *(const u32x4*)(vp + at + d) : zero4;
+        }
+    };
+    auto publish = [&](int kb, float e) {   // wavefront 0
+        const int p = kb * KB + lane;
+        const long long at = lane < KB ? place_of(p, e) : -1;
+        if (lane < KB) sPlace[kb & 1][lane] = at;
+        const uint64_t given = __ballot(at >= 0);
+        if (lane == 0) sGiven[kb & 1] = given;
+    };
+    auto entry = [&](int kb) -> float { const int p = kb * KB + lane; return lane < KB && p < end ? page_at(p) : -1.f; };
+    float ahead = -1.f;
+    if (wave == 0 && first < stop) {
+        publish(first, entry(first));
+        publish(first + 1, entry(first + 1));
+        ahead = entry(first + 2);
+    }
+    __syncthreads();
+    if (first < stop) load(first & 1);
+    for (int kb = first; kb < stop; kb++) {
+        const uint64_t given = sGiven[kb & 1];
+        __syncthreads();                                                         // everybody has left the previous block
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int r = tid / CPR + RPP * i, d = (tid % CPR) * EPL;
+            if constexpr (sizeof(TQ) == sizeof(TC)) {
+                *(u32x4*)(sK + r * LDK + d) = rk[i];
+                *(u32x4*)(sV + r * LDV + d) = rv[i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const u32x4 x = {rk[i][2 * e] << 16, rk[i][2 * e] & 0xffff0000u, rk[i][2 * e + 1] << 16, rk[i][2 * e + 1] & 0xffff0000u};
+                    const u32x4 y = {rv[i][2 * e] << 16, rv[i][2 * e] & 0xffff0000u, rv[i][2 * e + 1] << 16, rv[i][2 * e + 1] & 0xffff0000u};
+                    *(u32x4*)(sK + r * LDK + d + 4 * e) = x;
+                    *(u32x4*)(sV + r * LDV + d + 4 * e) = y;
+                }
+            }
+            if (kb * KB + KB > base + 1) bad = bad || not_finite<TC>(rv[i]);
+        }
+        if (wave == 0 && kb + 2 < stop) publish(kb + 2, ahead);
+        __syncthreads();
+        if (kb + 1 < stop) load((kb + 1) & 1);
+        if (wave == 0) ahead = entry(kb + 3);
+#pragma unroll 1
+        for (int j = 0; j < KB / 32; j++) {
+            const int t = kb * KB + 32 * j;
+            const uint32_t there = (uint32_t)(given >> (32 * j));
+            if (t >= waveEnd || !there) continue;
+            floatx16 s;
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[v] = 0.f;
+            const TQ* k = sK + (32 * j + l32) * LDK + half * TR::EPC;
+#pragma unroll
+            for (int f = 0; f < KF; f++) s = TR::mma(*(const u32x4*)(k + f * TR::CPF), qf[f], s);
+            float mx = -INFINITY;
+            if (t + 32 <= waveOpen && there == 0xffffffffu) {
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    s[v] *= a.c2;
+                    mx = fmaxf(mx, s[v]);
+                }
+                mx = fmaxf(mx, SCORE_FLOOR);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; v++) {
+                    const int key = 8 * (v >> 2) + 4 * half + (v & 3);
+                    const bool sees = (there >> key & 1) && t + key <= last;
+                    const float x = s[v] * a.c2;
+                    mx = fmaxf(mx, sees ? fmaxf(x, SCORE_FLOOR) : -INFINITY);
+                    s[v] = sees ? x : -INFINITY;
+                }
+            }
+            mx = fmaxf(max_lane_xor<32>(mx), m);
+            const float ref = mx > -INFINITY ? mx : 0.f, alpha = __builtin_amdgcn_exp2f(m - ref);
+            const bool moved = __any(mx != m);
+            m = mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                s[v] = __builtin_amdgcn_exp2f(s[v] - ref);
+                sum += s[v];
+            }
+            l = l * alpha + sum;
+            if (moved)
+#pragma unroll
+                for (int i = 0; i < DT; i++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++) o[i][v] *= alpha;
+            if constexpr (B16) {
+                const u32x4 w0 = TR::pack_p(s, 0), w1 = TR::pack_p(s, 1);
+#pragma unroll
+                for (int i = 0; i < DT; i++) {
+                    const TQ* tile = sV + 32 * j * LDV + 32 * i;
+                    o[i] = TR::mma(TR::load_vt_rowmajor(tile, LDV, 0, lane), w0, o[i]);
+                    o[i] = TR::mma(TR::load_vt_rowmajor(tile, LDV, 1, lane), w1, o[i]);
+                }
+            } else {
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    const u32x4 wt = TR::pack_p(s, f);
+#pragma unroll
+                    for (int i = 0; i < DT; i++) {
+                        const TQ* v = sV + (32 * j + 8 * f + 4 * half) * LDV + 32 * i + l32;
+                        const u32x4 x = {__float_as_uint((float)v[0]), __float_as_uint((float)v[LDV]), __float_as_uint((float)v[2 * LDV]), __float_as_uint((float)v[3 * LDV])};
+                        o[i] = TR::mma(x, wt, o[i]);
+                    }
+                }
+            }
+        }
+    }
+    l = add_lane_xor<32>(l);
+    if (__any(bad) && lane == 0) sBad = 1;
+    __syncthreads();
+
+    const size_t place = blockIdx.x, part0 = gridDim.x;
+    float* part = w.part + (blockIdx.y * part0 + place) * PART;
+    if (!sBad) {
+        if (live) {
+            TQ* y = (TQ*)a.y + row_at(token, head);
+            const float inv = 1.f / l;
+            if (w.splits > 1 && half == 0) put2(part + 2 * row, m, l);
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    const int d = 32 * i + 8 * v + 4 * half;
+                    if (d >= c.hs) continue;
+                    float x[4] = {o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]};
+                    if (w.splits > 1) {
+                        put2(part + 256 + row * HSP + d, x[0], x[1]);
+                        put2(part + 256 + row * HSP + d + 2, x[2], x[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = m > -INFINITY ? x[e] * inv : 0.f;
+                        TR::store4(y + d, x[0], x[1], x[2], x[3]);
+                    }
+                }
+        }
+    } else {
+        // A value that is not finite lies where only some of the rows look: weights of zero would not keep it from the others.  Row by row, then.
+        for (int r = wave; r < nt * w.tileHeads; r += 4) {
+            const int tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+            if (hd >= nh) continue;
+            const TQ* q = (const TQ*)a.q + row_at(tk, hd);
+            float qv[2], acc[2] = {0.f, 0.f}, mr = -INFINITY, lr = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; i++) qv[i] = 2 * lane + i < c.hs ? value_of<TQ>(q[2 * lane + i]) : 0.f;
+            for (int p = first * KB; p < stop * KB && p <= base + tk; p++) {
+                const long long at = place_of(p, p < end ? page_at(p) : -1.f);
+                if (at < 0) continue;
+                float x = 0.f, val[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int d = 2 * lane + i;
+                    x += d < c.hs ? qv[i] * value_of<TC>(kp[at + d]) : 0.f;
+                    val[i] = d < c.hs ? value_of<TC>(vp[at + d]) : 0.f;
+                }
+                x = group_sum<64>(x) * a.c2;
+                const float mn = fmaxf(mr, fmaxf(x, SCORE_FLOOR)), f = __builtin_amdgcn_exp2f(mr - mn), wt = __builtin_amdgcn_exp2f(x - mn);
+                mr = mn;
+                lr = lr * f + wt;
+#pragma unroll
+                for (int i = 0; i < 2; i++) acc[i] = acc[i] * f + wt * val[i];
+            }
+            if (2 * lane < c.hs) {
+                if (w.splits > 1) put2(part + 256 + r * HSP + 2 * lane, acc[0], acc[1]);
+                else {
+                    TQ* y = (TQ*)a.y + row_at(tk, hd) + 2 * lane;
+                    y[0] = stored<TQ>(mr > -INFINITY ? acc[0] / lr : 0.f);
+                    y[1] = stored<TQ>(mr > -INFINITY ? acc[1] / lr : 0.f);
+                }
+            }
+            if (w.splits > 1 && lane == 0) put2(part + 2 * r, mr, lr);
+        }
+    }
+    if (w.splits == 1) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) sTicket = __hip_atomic_fetch_add(w.tickets + place, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (sTicket != w.splits - 1) return;
+    const int pairs = c.hs >> 1, rows = nt * w.tileHeads;
+    for (int e = tid; e < rows * pairs; e += 256) {
+        const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+        if (hd >= nh) continue;
+        float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+        for (int z = 0; z < w.splits; z++) {
+            const float* from = w.part + (z * part0 + place) * PART;
+            const float2 ml = get2(from + 2 * r), v = get2(from + 256 + r * HSP + d);
+            const float Mn = fmaxf(M, ml.x), f0 = weight_of(M, Mn), f1 = weight_of(ml.x, Mn);
+            L = L * f0 + ml.y * f1;
+            x = x * f0 + v.x * f1;
+            y = y * f0 + v.y * f1;
+            M = Mn;
+        }
+        TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
+        out[0] = stored<TQ>(M > -INFINITY ? x / L : 0.f);
+        out[1] = stored<TQ>(M > -INFINITY ? y / L : 0.f);
+    }
+    if (tid == 0) __hip_atomic_store(w.tickets + place, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+}
+
 constexpr int SPLIT_GRID = 512;   // two workgroups a CU
 
 inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -592,8 +923,40 @@ inline bool in_pieces(const PagedCache& c, DType dt, const void* q, const void* 
 
 }  // namespace
 
-size_t attn_paged_workspace_bytes(const PagedCache& c) { return (size_t)SPLIT_GRID * 2 * 16 * ((c.hs <= 64 ? 64 : 128) + 2) * sizeof(float); }
-size_t attn_paged_tickets(const PagedCache& c) { return SPLIT_GRID; }
+// Rows of a key head up to which a sequence's positions are what is split (16-row tiles read the cache once each), beyond which its rows are
+constexpr int FEW_ROWS = 64;
+constexpr int CHUNK_ROWS = 128, CHUNK_GRID = 512;
+
+// how a launch of the chunk kernel looks: what it takes from the host are the numbers of tokens and sequences alone
+struct ChunkPlan { int headTiles, tileHeads, perTile, tiles, splits; };
+static ChunkPlan chunk_plan(const PagedCache& c)
+{
+    const int G = c.H / c.kvH;
+    ChunkPlan p;
+    p.headTiles = (G + CHUNK_ROWS - 1) / CHUNK_ROWS;
+    p.tileHeads = (G + p.headTiles - 1) / p.headTiles;
+    p.perTile = CHUNK_ROWS / p.tileHeads;
+    // every sequence may end inside a tile; those that have tiles have more than FEW_ROWS rows
+    const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1));
+    p.tiles = (int)(c.tokens / p.perTile + having);
+    const long long groups = (long long)p.tiles * c.kvH * p.headTiles;
+    p.splits = (int)std::max<long long>(1, std::min<long long>(16, CHUNK_GRID / std::max<long long>(1, groups)));
+    return p;
+}
+static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : 128; }
+
+size_t attn_paged_workspace_bytes(const PagedCache& c)
+{
+    const ChunkPlan p = chunk_plan(c);
+    const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
+    const size_t chunk = p.splits > 1 ? (size_t)p.splits * p.tiles * c.kvH * p.headTiles * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) : 0;
+    return std::max(split, chunk);
+}
+size_t attn_paged_tickets(const PagedCache& c)
+{
+    const ChunkPlan p = chunk_plan(c);
+    return std::max<size_t>(SPLIT_GRID, p.splits > 1 ? (size_t)p.tiles * c.kvH * p.headTiles : 0);
+}
 
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets)
 {
@@ -611,6 +974,20 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
             w.headTiles = (G + 15) / 16;
             w.tileHeads = (G + w.headTiles - 1) / w.headTiles;
             w.perTile = 16 / w.tileHeads;
+            const int most = maxNew > 0 ? std::min(maxNew, c.tokens) : c.tokens;
+            const bool chunks = (long long)most * G > FEW_ROWS;
+            w.few = chunks ? FEW_ROWS : 0;
+            if (chunks) {
+                const ChunkPlan p = chunk_plan(c);
+                ChunkArgs g = {(float*)workspace, tickets, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits};
+                const long long blocks = (long long)c.kvH * p.headTiles * p.tiles;
+                if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+                const dim3 grid((unsigned)blocks, p.splits);
+                if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid, 256, 0, s, a, g);
+                else hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 128>), grid, 256, 0, s, a, g);
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) return e;
+            }
             if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 64>), SPLIT_GRID, 256, 0, s, a, w);
             else hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
             return hipGetLastError();

@@ -135,6 +135,8 @@ SHAPES = [
     ("many", 2, 1, 32, 8, "head", [(1 + b % 3, 3 + 7 * b % 61, 0) for b in range(200)], 0),
     ("more_than_a_scan", 1, 1, 32, 16, "pos", [(b % 3, (b % 3) + 11 * b % 40, 0) for b in range(600)], 1),
     ("heads_of_two_tiles", 20, 1, 64, 16, "head", [(1, 200, 0), (2, 30, 0), (40, 60, 0)], 0),
+    ("more_tiles_than_workgroups_at_once", 8, 8, 64, 16, "head", [(65 + b % 3, 65 + b % 3 + 5 * b % 30, 0) for b in range(70)], 4),
+    ("a_prompt", 4, 1, 128, 16, "pos", [(400, 400, 0), (90, 700, 48)], 0),
     ("long_and_short", 4, 1, 128, 32, "pos", [(1, 3000, 0), (1, 1, 0), (2, 700, 0), (0, 500, 0), (1, 64, 0)], 0),
 ]
 
