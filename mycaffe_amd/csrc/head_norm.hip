@@ -28,8 +28,9 @@ template <typename T> __device__ __forceinline__ T of_f(float v);
 template <> __device__ __forceinline__ float of_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16_t of_f<bf16_t>(float v) { return f32_to_bf16(v); }
 
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 template <typename T, int V> struct alignas(16) Piece { T e[V]; };
-template <typename T, int V, bool VEC> __device__ __forceinline__ Piece<T, V> piece_load(const T* p, int d0, int hs)
+template <typename T, int V, bool VEC, bool ONCE = false> __device__ __forceinline__ Piece<T, V> piece_load(const T* p, int d0, int hs)
 {
     Piece<T, V> r;
     if constexpr (VEC) {
@@ -37,7 +38,10 @@ template <typename T, int V, bool VEC> __device__ __forceinline__ Piece<T, V> pi
         uint32_t* w = (uint32_t*)&r;
         if (d0 < hs) {
 #pragma unroll
-            for (int i = 0; i < W; i += 4) *(uint4*)(w + i) = *(const uint4*)((const uint32_t*)(p + d0) + i);
+            for (int i = 0; i < W; i += 4) {
+                const u4* from = (const u4*)((const uint32_t*)(p + d0) + i);
+                *(u4*)(w + i) = ONCE ? __builtin_nontemporal_load(from) : *from;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < W; i++) w[i] = 0u;
@@ -48,7 +52,7 @@ template <typename T, int V, bool VEC> __device__ __forceinline__ Piece<T, V> pi
     }
     return r;
 }
-template <typename T, int V, bool VEC> __device__ __forceinline__ void piece_store(T* p, int d0, int hs, const float (&v)[V])
+template <typename T, int V, bool VEC, bool AWAY = false> __device__ __forceinline__ void piece_store(T* p, int d0, int hs, const float (&v)[V])
 {
     if constexpr (VEC) {
         Piece<T, V> r;
@@ -59,7 +63,11 @@ template <typename T, int V, bool VEC> __device__ __forceinline__ void piece_sto
         if (d0 < hs) {
             if constexpr (W >= 4) {
 #pragma unroll
-                for (int i = 0; i < W; i += 4) *(uint4*)((uint32_t*)(p + d0) + i) = *(const uint4*)(w + i);
+                for (int i = 0; i < W; i += 4) {
+                    u4* to = (u4*)((uint32_t*)(p + d0) + i);
+                    if (AWAY) __builtin_nontemporal_store(*(const u4*)(w + i), to);
+                    else *to = *(const u4*)(w + i);
+                }
             } else *(uint2*)(p + d0) = *(const uint2*)w;
         }
     } else {
@@ -74,10 +82,12 @@ template <typename T, int V> __device__ __forceinline__ void piece_floats(const 
     for (int i = 0; i < V; i++) v[i] = to_f<T>(p.e[i]);
 }
 // the weights of a lane's values (1 without weights, 0 past the head's end) and the cosines and sines of its pairs
-template <typename T, int V> __device__ __forceinline__ void weights_of(const T* w, int d0, int hs, float (&v)[V])
+template <typename T, int V, bool VEC> __device__ __forceinline__ void weights_of(const T* w, int d0, int hs, float (&v)[V])
 {
+    if (w && VEC) piece_floats<T, V>(piece_load<T, V, VEC>(w, d0, hs), v);
+    else
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = d0 + i >= hs ? 0.f : w ? to_f<T>(w[d0 + i]) : 1.f;
+        for (int i = 0; i < V; i++) v[i] = d0 + i >= hs ? 0.f : w ? to_f<T>(w[d0 + i]) : 1.f;
 }
 template <int V> __device__ __forceinline__ void turns_of(const float* turns, int pos, int d0, int hs, float (&c)[V / 2], float (&s)[V / 2])
 {
@@ -126,7 +136,11 @@ struct HeadNormArgs {
     int B, T, H, kvH, hs;
     float eps, inv_hs;
 };
-constexpr int AHEAD = 4;      // heads a lane group has in flight
+// Heads a lane group has in flight, and how the values that pass through once go by the caches: stores that are not kept there (forward, append),
+// loads that are not (backward, whose two inputs are twice its output).  us for 8 x 1024 positions of 24 heads of 64, the gradient at 4 x 2048 of 40
+// of 128, 8192 tokens of 48 of 128 appended, 16-bit storage:
+//   plain, 4 heads 13.8 | 64 | 63     stores 11.5 (3 heads 10.7) | 60 | 47 (48)     loads 14.0 | 58 (2 heads 53.6) | 48     both 12.9 | 58 | 49
+constexpr int AHEAD = 3, AHEAD_BWD = 2;      // heads a lane group has in flight
 
 // A lane group keeps one position and walks the heads of its part, so that cosines, sines and weights are read once for all of them.
 // grid: (groups of positions, parts of the heads)
@@ -140,18 +154,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadNormArgs a)
     const int b = live ? (int)(at / a.T) : 0, t = live ? (int)(at - (long long)b * a.T) : 0;
     float c[V / 2], s[V / 2], w[2][V];
     turns_of<V>(a.turns, t, d0, a.hs, c, s);
-    weights_of<T, V>((const T*)a.wq, d0, a.hs, w[0]);
-    weights_of<T, V>((const T*)a.wk, d0, a.hs, w[1]);
+    weights_of<T, V, VEC>((const T*)a.wq, d0, a.hs, w[0]);
+    weights_of<T, V, VEC>((const T*)a.wk, d0, a.hs, w[1]);
     const int heads = a.H + a.kvH;
     // head h of all: where its row starts in its tensor
-    auto row = [&](int h) { return h < a.H ? (((size_t)b * a.H + h) * a.T + t) * a.hs : (((size_t)b * a.kvH + (h - a.H)) * a.T + t) * a.hs; };
+    const size_t step = (size_t)a.T * a.hs, inq = ((size_t)b * a.H * a.T + t) * a.hs, ink = ((size_t)b * a.kvH * a.T + t) * a.hs;
+    auto row = [&](int h) { return h < a.H ? inq + h * step : ink + (h - a.H) * step; };
+    Piece<T, V> x[AHEAD];
+    auto request = [&](int i, int h) {
+        if (h < heads) x[i] = piece_load<T, V, VEC>((h < a.H ? (const T*)a.q : (const T*)a.k) + row(h), live ? d0 : a.hs, a.hs);
+    };
     for (int h0 = blockIdx.y; h0 < heads; h0 += AHEAD * gridDim.y) {
-        Piece<T, V> x[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            const int h = h0 + i * gridDim.y;
-            if (h < heads) x[i] = piece_load<T, V, VEC>((h < a.H ? (const T*)a.q : (const T*)a.k) + row(h), live ? d0 : a.hs, a.hs);
-        }
+        for (int i = 0; i < AHEAD; i++) request(i, h0 + i * gridDim.y);
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int h = h0 + i * gridDim.y;
@@ -162,23 +177,23 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadNormArgs a)
 #pragma unroll
             for (int e = 0; e < V; e++) v[e] = v[e] * r * (h < a.H ? w[0][e] : w[1][e]);
             turn<V>(v, c, s);
-            if (live) piece_store<T, V, VEC>((h < a.H ? (T*)a.yq : (T*)a.yk) + row(h), d0, a.hs, v);
+            if (live) piece_store<T, V, VEC, true>((h < a.H ? (T*)a.yq : (T*)a.yk) + row(h), d0, a.hs, v);
         }
     }
 }
 
-// The gradient, with the same walk; a workgroup takes every gridDim.x-th group of positions and every gridDim.y-th head.  The weights' gradients stay in registers, meet in
-// LDS group by group in order, and leave as one row of sums a workgroup, which head_norm_dw_kernel adds in order: no sum depends on timing.
+// The gradient, with the same walk; a workgroup takes every gridDim.x-th group of positions and every gridDim.y-th head.  The weights' gradients stay in registers, meet
+// in a fixed order, and leave as one row of sums a workgroup, which head_norm_dw_kernel adds in order: no sum depends on timing.
 template <typename T, int V, bool VEC, int LPH>
 __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(HeadNormArgs a)
 {
     constexpr int GROUPS = 256 / LPH;
-    __shared__ float red[GROUPS][LPH * V + 1];
+    __shared__ float red[4][2][LPH * V + 1];
     const int d0 = (threadIdx.x % LPH) * V, group = threadIdx.x / LPH;
     const int heads = a.H + a.kvH;
     float w[2][V], dw[2][V];
-    weights_of<T, V>((const T*)a.wq, d0, a.hs, w[0]);
-    weights_of<T, V>((const T*)a.wk, d0, a.hs, w[1]);
+    weights_of<T, V, VEC>((const T*)a.wq, d0, a.hs, w[0]);
+    weights_of<T, V, VEC>((const T*)a.wk, d0, a.hs, w[1]);
 #pragma unroll
     for (int e = 0; e < V; e++) dw[0][e] = dw[1][e] = 0.f;
     const long long positions = (long long)a.B * a.T;
@@ -191,19 +206,19 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(HeadNormArgs a)
 #pragma unroll
         for (int i = 0; i < V / 2; i++) s[i] = -s[i];
         const int dl = live ? d0 : a.hs;
-        auto row = [&](int h) { return h < a.H ? (((size_t)b * a.H + h) * a.T + t) * a.hs : (((size_t)b * a.kvH + (h - a.H)) * a.T + t) * a.hs; };
-        for (int h0 = blockIdx.y; h0 < heads; h0 += AHEAD * gridDim.y) {
-            Piece<T, V> x[AHEAD], g[AHEAD];
+        const size_t step = (size_t)a.T * a.hs, inq = ((size_t)b * a.H * a.T + t) * a.hs, ink = ((size_t)b * a.kvH * a.T + t) * a.hs;
+        auto row = [&](int h) { return h < a.H ? inq + h * step : ink + (h - a.H) * step; };
+        Piece<T, V> x[AHEAD_BWD], g[AHEAD_BWD];
+        auto request = [&](int i, int h) {
+            if (h >= heads) return;
+            x[i] = piece_load<T, V, VEC, true>((h < a.H ? (const T*)a.q : (const T*)a.k) + row(h), dl, a.hs);
+            g[i] = piece_load<T, V, VEC, true>((h < a.H ? (const T*)a.dyq : (const T*)a.dyk) + row(h), dl, a.hs);
+        };
+        for (int h0 = blockIdx.y; h0 < heads; h0 += AHEAD_BWD * gridDim.y) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const int h = h0 + i * gridDim.y;
-                if (h < heads) {
-                    x[i] = piece_load<T, V, VEC>((h < a.H ? (const T*)a.q : (const T*)a.k) + row(h), dl, a.hs);
-                    g[i] = piece_load<T, V, VEC>((h < a.H ? (const T*)a.dyq : (const T*)a.dyk) + row(h), dl, a.hs);
-                }
-            }
+            for (int i = 0; i < AHEAD_BWD; i++) request(i, h0 + i * gridDim.y);
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
+            for (int i = 0; i < AHEAD_BWD; i++) {
                 const int h = h0 + i * gridDim.y;
                 if (h >= heads) break;
                 const bool isq = h < a.H;
@@ -229,34 +244,44 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(HeadNormArgs a)
         }
     }
     if (!a.part) return;
+    // the lane groups of a wavefront, then the wavefronts
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        if (x) __syncthreads();
+    for (int x = 0; x < 2; x++)
 #pragma unroll
-        for (int e = 0; e < V; e++) red[group][d0 + e] = dw[x][e];
-        __syncthreads();
-        for (int d = threadIdx.x; d < a.hs; d += 256) {
-            float sum = 0.f;
-            for (int i = 0; i < GROUPS; i++) sum += red[i][d];
-            a.part[(((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + x) * a.hs + d] = sum;
+        for (int e = 0; e < V; e++) {
+            float v = dw[x][e];
+            if constexpr (LPH <= 8) v = add_lane_xor<8>(v);
+            if constexpr (LPH <= 16) v = add_lane_xor<16>(v);
+            if constexpr (LPH <= 32) v = add_lane_xor<32>(v);
+            if ((threadIdx.x & 63) < LPH) red[threadIdx.x >> 6][x][d0 + e] = v;
         }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * a.hs; i += 256) {
+        const int x = i / a.hs, d = i - x * a.hs;
+        a.part[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * a.hs + i] = (red[0][x][d] + red[1][x][d]) + (red[2][x][d] + red[3][x][d]);
     }
 }
-// 16 columns by 16 lanes of workgroups; the lanes' sums are added in order
+// 16 columns by 64 lanes of workgroups; the lanes' sums are added in order
 template <typename T>
-__global__ __launch_bounds__(256) void head_norm_dw_kernel(const float* part, int rows, int hs, T* dwq, T* dwk, int accum)
+__global__ __launch_bounds__(1024) void head_norm_dw_kernel(const float* part, int rows, int hs, T* dwq, T* dwk, int accum)
 {
-    __shared__ float red[16][17];
+    __shared__ float red[64][17];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
     float acc = 0.f;
     if (j < 2 * hs)
-#pragma unroll 4
-        for (int i = r; i < rows; i += 16) acc += part[(size_t)i * 2 * hs + j];
+#pragma unroll 8
+        for (int i = r; i < rows; i += 64) acc += part[(size_t)i * 2 * hs + j];
     red[r][c] = acc;
     __syncthreads();
-    if (r == 0 && j < 2 * hs) {
+    if (r < 4) {
         float t = 0.f;
-        for (int q = 0; q < 16; q++) t += red[q][c];
+#pragma unroll
+        for (int q = 0; q < 16; q++) t += red[16 * r + q][c];
+        red[16 * r][c] = t;
+    }
+    __syncthreads();
+    if (r == 0 && j < 2 * hs) {
+        const float t = (red[0][c] + red[16][c]) + (red[32][c] + red[48][c]);
         T* dw = j < hs ? dwq : dwk;
         if (dw) {
             T* p = dw + (j < hs ? j : j - hs);
@@ -302,14 +327,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
     const T* row = (const T*)a.qkv + (size_t)token * heads * c.hs;
     int h0 = blockIdx.y * HPW + lane / LPH;
     Piece<T, V> x[AHEAD];
-    auto request = [&]() {
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            const int h = h0 + i * stride;
-            if (h < heads) x[i] = piece_load<T, V, VEC>(row + (size_t)h * c.hs, d0, c.hs);
-        }
+    auto request = [&](int i, int h) {
+        if (h < heads) x[i] = piece_load<T, V, VEC>(row + (size_t)h * c.hs, d0, c.hs);
     };
-    request();
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) request(i, h0 + i * stride);
     const int b = sequence_of(c.starts, c.batch, c.tokens, token);
     if (b < 0) return;
     const int positions = c.maxPages * c.pageSize;
@@ -321,8 +343,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
     const long long at = page * c.sP + (max(pos, 0) - entry * c.pageSize) * c.sT;
     float cs[V / 2], sn[V / 2], w[2][V];
     turns_of<V>(a.turns, max(pos, 0), d0, c.hs, cs, sn);
-    weights_of<T, V>((const T*)a.wq, d0, c.hs, w[0]);
-    weights_of<T, V>((const T*)a.wk, d0, c.hs, w[1]);
+    weights_of<T, V, VEC>((const T*)a.wq, d0, c.hs, w[0]);
+    weights_of<T, V, VEC>((const T*)a.wk, d0, c.hs, w[1]);
     // the walk is the wavefront's (its butterflies want all lanes); a lane group past the last head stores nothing
     for (int first = blockIdx.y * HPW; first < heads; first += AHEAD * stride) {
 #pragma unroll
@@ -339,12 +361,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a)
                     for (int e = 0; e < V; e++) v[e] = v[e] * r * (isq ? w[0][e] : w[1][e]);
                 turn<V>(v, cs, sn);
             }
-            if (isq) piece_store<T, V, VEC>((T*)a.q + ((size_t)token * c.H + h) * c.hs, d0, c.hs, v);
+            if (isq) piece_store<T, V, VEC, true>((T*)a.q + ((size_t)token * c.H + h) * c.hs, d0, c.hs, v);
             else if (h < heads && page >= 0)
-                piece_store<TC, V, VEC>((TC*)(isk ? c.k : c.v) + at + (h - c.H - (isk ? 0 : c.kvH)) * c.sH, d0, c.hs, v);
+                piece_store<TC, V, VEC, true>((TC*)(isk ? c.k : c.v) + at + (h - c.H - (isk ? 0 : c.kvH)) * c.sH, d0, c.hs, v);
         }
         h0 += AHEAD * stride;
-        request();
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) request(i, h0 + i * stride);
     }
 }
 
@@ -389,13 +412,13 @@ hipError_t k_qk_norm_rope(hipStream_t s, DType dt, int B, int T, int H, int kvH,
     auto go = [&](auto type) {
         typedef decltype(type) T_;
         constexpr int V = values_a_lane<T_>();
-        const bool vec = hs % V == 0 && at16(q) && at16(k) && at16(yq) && at16(yk);
+        const bool vec = hs % V == 0 && at16(q) && at16(k) && at16(yq) && at16(yk) && at16(wq) && at16(wk);
         return with_bool(vec, [&](auto vec_) {
             return with_lanes(hs, V, [&](auto lanes) {
                 constexpr int LPH = decltype(lanes)::value, GROUPS = 256 / LPH;
                 const long long blocks = ((long long)B * T + GROUPS - 1) / GROUPS;
                 // few positions: their heads are dealt to several workgroups
-                const int parts = (int)std::max<long long>(1, std::min<long long>(H + kvH, 1024 / blocks));
+                const int parts = (int)std::max<long long>(1, std::min<long long>(H + kvH, 2048 / blocks));
                 hipLaunchKernelGGL((qk_norm_rope_kernel<T_, V, decltype(vec_)::value, LPH>), dim3((unsigned)blocks, parts), 256, 0, s, a);
                 return hipGetLastError();
             });
@@ -417,7 +440,7 @@ hipError_t k_qk_norm_rope_bwd(hipStream_t s, DType dt, int B, int T, int H, int 
     auto go = [&](auto type) {
         typedef decltype(type) T_;
         constexpr int V = values_a_lane<T_>();
-        const bool vec = hs % V == 0 && at16(q) && at16(k) && at16(dyq) && at16(dyk) && at16(dxq) && at16(dxk);
+        const bool vec = hs % V == 0 && at16(q) && at16(k) && at16(dyq) && at16(dyk) && at16(dxq) && at16(dxk) && at16(wq) && at16(wk);
         dim3 grid;
         hipError_t e = with_bool(vec, [&](auto vec_) {
             return with_lanes(hs, V, [&](auto lanes) {
@@ -428,7 +451,7 @@ hipError_t k_qk_norm_rope_bwd(hipStream_t s, DType dt, int B, int T, int H, int 
             });
         });
         if (e != hipSuccess || !a.part) return e;
-        hipLaunchKernelGGL((head_norm_dw_kernel<T_>), (2 * hs + 15) / 16, 256, 0, s, a.part, (int)(grid.x * grid.y), hs, (T_*)dwq, (T_*)dwk, accum ? 1 : 0);
+        hipLaunchKernelGGL((head_norm_dw_kernel<T_>), (2 * hs + 15) / 16, 1024, 0, s, a.part, (int)(grid.x * grid.y), hs, (T_*)dwq, (T_*)dwk, accum ? 1 : 0);
         return hipGetLastError();
     };
     return dt == F32 ? go(float()) : go(bf16_t());
@@ -443,7 +466,7 @@ hipError_t k_paged_append(hipStream_t s, DType dt, const PagedCache& c, const vo
         typedef decltype(type) T_;
         typedef decltype(ctype) TC_;
         constexpr int V = values_a_lane<T_>();
-        const bool vec = c.hs % V == 0 && c.sP % V == 0 && c.sH % V == 0 && c.sT % V == 0 && at16(qkv) && at16(q) && at16(c.k) && at16(c.v);
+        const bool vec = c.hs % V == 0 && c.sP % V == 0 && c.sH % V == 0 && c.sT % V == 0 && at16(qkv) && at16(q) && at16(c.k) && at16(c.v) && at16(wq) && at16(wk);
         return with_bool(vec, [&](auto vec_) {
             return with_lanes(c.hs, V, [&](auto lanes) {
                 constexpr int LPH = decltype(lanes)::value, HPW = 64 / LPH;
