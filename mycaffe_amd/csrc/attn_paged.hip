@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
     constexpr int KG = sizeof(TC) == 4 ? 1 : 2, KT = 16 * KG, UNIT = 4 * KT;   // groups of 16 keys a tile
     constexpr int VE = sizeof(TC) == 4 ? 4 : HSP / 16 < 8 ? HSP / 16 : 8, NH = HSP / (16 * VE), NO = HSP / 16;
     constexpr int ROWB = HSP * 2, STAGE = B16 ? KT * ROWB : 0;
-    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2);
+    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2), DEEP = 16;              // partial results in flight where an item is put together
     constexpr int SHARED = 4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4;
     static_assert(HSP == 64 || HSP == 128, "tile");
     __shared__ __attribute__((aligned(16))) unsigned char smem[SHARED];
@@ -537,21 +537,21 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                     const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
                     if (hd >= nh) continue;
                     float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-                    for (int i = wf; i <= we; i += 8) {
-                        float2 ml[8], v[8];
+                    for (int i = wf; i <= we; i += DEEP) {
+                        float2 ml[DEEP], v[DEEP];
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
+                        for (int j = 0; j < DEEP; j++) {
                             const float* from = w.part + ((size_t)min(i + j, we) * 2 + (i + j == wf ? 1 : 0)) * PART;
                             ml[j] = get2(from + 2 * r);
                             v[j] = get2(from + 32 + r * HSP + d);
                         }
                         float Mn = M;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) Mn = i + j <= we ? fmaxf(Mn, ml[j].x) : Mn;
+                        for (int j = 0; j < DEEP; j++) Mn = i + j <= we ? fmaxf(Mn, ml[j].x) : Mn;
                         const float f0 = weight_of(M, Mn);
                         L *= f0; x *= f0; y *= f0;
 #pragma unroll
-                        for (int j = 0; j < 8; j++) {
+                        for (int j = 0; j < DEEP; j++) {
                             const float f = weight_of(ml[j].x, Mn);
                             L += i + j <= we ? ml[j].y * f : 0.f;
                             x += i + j <= we ? v[j].x * f : 0.f;
@@ -584,10 +584,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
 // A workgroup has 128 rows of one key head (tokens times the heads that share it), 32 a wavefront, and stages blocks of KB keys and values in LDS for
 // all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
 // follow each other by key head), whose L2 then holds that head's keys and values.  Where tiles are few their blocks are split among
-// workgroups, and the last one puts a tile together.
+// workgroups and put together by a launch behind this one.
 struct ChunkArgs {
     float* part;      // [split][tile][key head x head tile][128 {maximum, sum} | 128 rows of HSP]
-    int* tickets;     // [tile][key head x head tile]; zero between launches
     int few;          // sequences of at most this many rows a key head are another kernel's
     int shift, perTile, tileHeads, headTiles, splits;
 };
@@ -615,6 +614,27 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
     return before + x - v;
 }
 
+// What workgroup `block` of a launch works on; b < 0: nothing
+struct ChunkTile { int b, tile, kh, ht; };
+__device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const ChunkArgs& w, unsigned block)
+{
+    __shared__ int sums[4], seq, tile;
+    const int groups = c.kvH * w.headTiles, want = block / groups, group = block - want * groups, tid = threadIdx.x;
+    if (tid == 0) { seq = -1; tile = 0; }
+    for (int b0 = 0, base = 0; b0 < c.batch && base <= want; b0 += 256) {
+        int tiles = 0, all;
+        if (b0 + tid < c.batch) {
+            const PagedSpan s = paged_span(c.starts[b0 + tid], c.starts[b0 + tid + 1], c.lens[b0 + tid], c.tokens, c.maxPages * c.pageSize);
+            if ((long long)s.count * (c.H / c.kvH) > w.few) tiles = (s.count + w.perTile - 1) / w.perTile;
+        }
+        const int at = base + block_scan(tiles, sums, &all);
+        if (at <= want && want < at + tiles) { seq = b0 + tid; tile = tiles - 1 - (want - at); }   // those that see most come first
+        base += all;
+    }
+    __syncthreads();
+    return ChunkTile{seq, tile, group / w.headTiles, group % w.headTiles};
+}
+
 template <typename TQ, typename TC, int HSP>
 __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs a, ChunkArgs w)
 {
@@ -628,31 +648,17 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     __shared__ __attribute__((aligned(16))) TQ sV[KB * LDV];
     __shared__ long long sPlace[2][KB];
     __shared__ uint64_t sGiven[2];
-    __shared__ int sSum[4], sSeq, sTile, sBad, sTicket, sFront;
+    __shared__ int sBad, sFront;
 
     const PagedCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
     const int G = c.H / c.kvH, positions = c.maxPages * c.pageSize;
-    const int groups = c.kvH * w.headTiles, want = blockIdx.x / groups, group = blockIdx.x - want * groups, kh = group / w.headTiles, ht = group - kh * w.headTiles;
-
-    // ---- the sequence and its tile ----
-    auto span_of = [&](int b) { return paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions); };
-    if (tid == 0) { sSeq = -1; sBad = 0; }
-    for (int b0 = 0, base = 0; b0 < c.batch && base <= want; b0 += 256) {
-        int tiles = 0, all;
-        if (b0 + tid < c.batch) {
-            const PagedSpan s = span_of(b0 + tid);
-            if ((long long)s.count * G > w.few) tiles = (s.count + w.perTile - 1) / w.perTile;
-        }
-        const int at = base + block_scan(tiles, sSum, &all);
-        if (at <= want && want < at + tiles) { sSeq = b0 + tid; sTile = tiles - 1 - (want - at); }   // those that see most come first
-        base += all;
-    }
-    __syncthreads();
-    const int b = sSeq;
-    if (b < 0) return;
-    const PagedSpan sp = span_of(b);
-    const int j0 = sTile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
+    if (tid == 0) sBad = 0;
+    const ChunkTile at = chunk_tile(c, w, blockIdx.x);
+    if (at.b < 0) return;
+    const int b = at.b, kh = at.kh, ht = at.ht;
+    const PagedSpan sp = paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions);
+    const int j0 = at.tile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
     const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads);
     const int end = min(sp.len, base + nt);                                                       // positions that some row sees
     const float* table = c.table + (size_t)b * c.maxPages;
@@ -680,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     const int row = 32 * wave + l32, token = row / w.tileHeads, head = row - token * w.tileHeads;
     const bool live = token < nt && head < nh;
     const int last = live ? base + token : -1;
-    const int waveEnd = min(end, base + min((32 * wave + 31) / w.tileHeads, nt - 1) + 1), waveOpen = base + 32 * wave / w.tileHeads + 1;   // past what any, and what every row sees
+    const int waveEnd = 32 * wave / w.tileHeads < nt ? min(end, base + min((32 * wave + 31) / w.tileHeads, nt - 1) + 1) : 0, waveOpen = base + 32 * wave / w.tileHeads + 1;   // past what any, and what every row sees
     auto row_at = [&](int t, int h) { return ((size_t)(sp.first + j0 + t) * c.H + h0 + h) * c.hs; };
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
     u32x4 qf[KF];
@@ -829,7 +835,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
         if (live) {
             TQ* y = (TQ*)a.y + row_at(token, head);
             const float inv = 1.f / l;
-            if (w.splits > 1 && half == 0) put2(part + 2 * row, m, l);
+            if (w.splits > 1 && half == 0) *(float2*)(part + 2 * row) = make_float2(m, l);
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -837,10 +843,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                     const int d = 32 * i + 8 * v + 4 * half;
                     if (d >= c.hs) continue;
                     float x[4] = {o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]};
-                    if (w.splits > 1) {
-                        put2(part + 256 + row * HSP + d, x[0], x[1]);
-                        put2(part + 256 + row * HSP + d + 2, x[2], x[3]);
-                    } else {
+                    if (w.splits > 1) *(float4*)(part + 256 + row * HSP + d) = make_float4(x[0], x[1], x[2], x[3]);
+                    else {
 #pragma unroll
                         for (int e = 0; e < 4; e++) x[e] = m > -INFINITY ? x[e] * inv : 0.f;
                         TR::store4(y + d, x[0], x[1], x[2], x[3]);
@@ -874,41 +878,59 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                 for (int i = 0; i < 2; i++) acc[i] = acc[i] * f + wt * val[i];
             }
             if (2 * lane < c.hs) {
-                if (w.splits > 1) put2(part + 256 + r * HSP + 2 * lane, acc[0], acc[1]);
+                if (w.splits > 1) *(float2*)(part + 256 + r * HSP + 2 * lane) = make_float2(acc[0], acc[1]);
                 else {
                     TQ* y = (TQ*)a.y + row_at(tk, hd) + 2 * lane;
                     y[0] = stored<TQ>(mr > -INFINITY ? acc[0] / lr : 0.f);
                     y[1] = stored<TQ>(mr > -INFINITY ? acc[1] / lr : 0.f);
                 }
             }
-            if (w.splits > 1 && lane == 0) put2(part + 2 * r, mr, lr);
+            if (w.splits > 1 && lane == 0) *(float2*)(part + 2 * r) = make_float2(mr, lr);
         }
     }
-    if (w.splits == 1) return;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0) sTicket = __hip_atomic_fetch_add(w.tickets + place, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (sTicket != w.splits - 1) return;
-    const int pairs = c.hs >> 1, rows = nt * w.tileHeads;
-    for (int e = tid; e < rows * pairs; e += 256) {
-        const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
-        if (hd >= nh) continue;
-        float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-        for (int z = 0; z < w.splits; z++) {
-            const float* from = w.part + (z * part0 + place) * PART;
-            const float2 ml = get2(from + 2 * r), v = get2(from + 256 + r * HSP + d);
-            const float Mn = fmaxf(M, ml.x), f0 = weight_of(M, Mn), f1 = weight_of(ml.x, Mn);
-            L = L * f0 + ml.y * f1;
-            x = x * f0 + v.x * f1;
-            y = y * f0 + v.y * f1;
-            M = Mn;
+}
+
+// The splits of a tile put together, 32 rows a workgroup, eight lanes a row.  A launch of its own: a tile has up to 64 KB a split, which one workgroup
+// takes longer to collect (its last one, 7 splits of 128 rows of 128: 100 us) than all of them to start anew.
+template <typename TQ, int HSP>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttnArgs a, ChunkArgs w)
+{
+    constexpr int PART = 128 * (HSP + 2), N = HSP / 32;
+    const PagedCache& c = a.c;
+    const ChunkTile at = chunk_tile(c, w, blockIdx.x);
+    if (at.b < 0) return;
+    const PagedSpan sp = paged_span(c.starts[at.b], c.starts[at.b + 1], c.lens[at.b], c.tokens, c.maxPages * c.pageSize);
+    const int G = c.H / c.kvH, j0 = at.tile * w.perTile, nt = min(w.perTile, sp.count - j0), nh = min(w.tileHeads, G - at.ht * w.tileHeads);
+    const int row = blockIdx.y * 32 + (threadIdx.x >> 3), token = row / w.tileHeads, head = row - token * w.tileHeads;
+    if (token >= nt || head >= nh) return;
+    const float* part = w.part + (size_t)blockIdx.x * PART;
+    const size_t split = (size_t)gridDim.x * PART;
+    float M = -INFINITY, L = 0.f;
+    for (int z = 0; z < w.splits; z++) M = fmaxf(M, part[z * split + 2 * row]);
+    float4 x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < w.splits; z++) {
+        const float* from = part + z * split;
+        const float f = weight_of(from[2 * row], M);
+        L += from[2 * row + 1] * f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float4 v = *(const float4*)(from + 256 + row * HSP + 32 * i + 4 * (threadIdx.x & 7));
+            x[i].x += v.x * f; x[i].y += v.y * f; x[i].z += v.z * f; x[i].w += v.w * f;
         }
-        TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
-        out[0] = stored<TQ>(M > -INFINITY ? x / L : 0.f);
-        out[1] = stored<TQ>(M > -INFINITY ? y / L : 0.f);
     }
-    if (tid == 0) __hip_atomic_store(w.tickets + place, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
+    TQ* y = (TQ*)a.y + ((size_t)(sp.first + j0 + token) * c.H + at.kh * G + at.ht * w.tileHeads + head) * c.hs;
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int d = 32 * i + 4 * (threadIdx.x & 7);
+        if (d >= c.hs) continue;
+        if (M == -INFINITY) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        else { x[i].x *= inv; x[i].y *= inv; x[i].z *= inv; x[i].w *= inv; }
+        FlashTraits<TQ>::store4(y + d, x[i].x, x[i].y, x[i].z, x[i].w);
+    }
 }
 
 constexpr int SPLIT_GRID = 512;   // two workgroups a CU
@@ -923,13 +945,17 @@ inline bool in_pieces(const PagedCache& c, DType dt, const void* q, const void* 
 
 }  // namespace
 
-// Rows of a key head up to which a sequence's positions are what is split (16-row tiles read the cache once each), beyond which its rows are
-constexpr int FEW_ROWS = 64;
-constexpr int CHUNK_ROWS = 128, CHUNK_GRID = 512;
+// Rows of a key head up to which a sequence's positions are what is split, beyond which its rows are: one 16-row tile.  Two of them read the cache
+// twice (us, two kernels, 32 heads on 8 key heads of 128, 4096 positions, 16-bit storage: 4 sequences of 8 new tokens, 32 rows, 41 | 36; 8 of 16, 64 rows, 84 | 61).
+constexpr int FEW_ROWS = 16;
+// Workgroups a launch of the chunk kernel aims at.  Splitting tiles costs what their partial results take to write and read, which products in
+// fp32 are longer than by more (us, 512 | 1024: one chunk of 256 tokens over 8192, 16-bit, 79 | 93; 8 chunks of up to 1024, 12 heads of 64, 16-bit 43 | 48;
+// 2 prompts of 1024, 12 heads of 64, fp32 77 | 66; 12 chunks and single tokens of up to 1500 positions, fp32, 145 | 115).
+constexpr int CHUNK_ROWS = 128, CHUNK_GRID_16 = 512, CHUNK_GRID_32 = 1024;
 
 // how a launch of the chunk kernel looks: what it takes from the host are the numbers of tokens and sequences alone
 struct ChunkPlan { int headTiles, tileHeads, perTile, tiles, splits; };
-static ChunkPlan chunk_plan(const PagedCache& c)
+static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
 {
     const int G = c.H / c.kvH;
     ChunkPlan p;
@@ -940,23 +966,19 @@ static ChunkPlan chunk_plan(const PagedCache& c)
     const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1));
     p.tiles = (int)(c.tokens / p.perTile + having);
     const long long groups = (long long)p.tiles * c.kvH * p.headTiles;
-    p.splits = (int)std::max<long long>(1, std::min<long long>(16, CHUNK_GRID / std::max<long long>(1, groups)));
+    p.splits = (int)std::max<long long>(1, std::min<long long>(16, (dt == F32 ? CHUNK_GRID_32 : CHUNK_GRID_16) / std::max<long long>(1, groups)));
     return p;
 }
 static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : 128; }
 
-size_t attn_paged_workspace_bytes(const PagedCache& c)
+size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
 {
-    const ChunkPlan p = chunk_plan(c);
+    const ChunkPlan p = chunk_plan(c, dt);
     const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
     const size_t chunk = p.splits > 1 ? (size_t)p.splits * p.tiles * c.kvH * p.headTiles * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) : 0;
     return std::max(split, chunk);
 }
-size_t attn_paged_tickets(const PagedCache& c)
-{
-    const ChunkPlan p = chunk_plan(c);
-    return std::max<size_t>(SPLIT_GRID, p.splits > 1 ? (size_t)p.tiles * c.kvH * p.headTiles : 0);
-}
+size_t attn_paged_tickets() { return SPLIT_GRID; }
 
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets)
 {
@@ -978,13 +1000,17 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
             const bool chunks = (long long)most * G > FEW_ROWS;
             w.few = chunks ? FEW_ROWS : 0;
             if (chunks) {
-                const ChunkPlan p = chunk_plan(c);
-                ChunkArgs g = {(float*)workspace, tickets, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits};
+                const ChunkPlan p = chunk_plan(c, dt);
+                ChunkArgs g = {(float*)workspace, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits};
                 const long long blocks = (long long)c.kvH * p.headTiles * p.tiles;
                 if (blocks > 0x7fffffff) return hipErrorInvalidValue;
                 const dim3 grid((unsigned)blocks, p.splits);
                 if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid, 256, 0, s, a, g);
                 else hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 128>), grid, 256, 0, s, a, g);
+                if (p.splits > 1) {
+                    if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_join_kernel<T_, 64>), dim3((unsigned)blocks, 4), 256, 0, s, a, g);
+                    else hipLaunchKernelGGL((attn_paged_join_kernel<T_, 128>), dim3((unsigned)blocks, 4), 256, 0, s, a, g);
+                }
                 const hipError_t e = hipGetLastError();
                 if (e != hipSuccess) return e;
             }

@@ -280,8 +280,8 @@ hipError_t k_paged_append(hipStream_t s, DType dt, const PagedCache& c, const vo
                           const float* turns);
 // y (tokens, H, hs) = attention of q (tokens, H, hs) over the pages, every token over the positions up to its own.  maxNew: at most this many new
 // tokens in a sequence, 0 if not known (any value is right).  workspace, tickets (zero between launches): as much as these say
-size_t attn_paged_workspace_bytes(const PagedCache& c);
-size_t attn_paged_tickets(const PagedCache& c);
+size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt);
+size_t attn_paged_tickets();
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets);
 
 }  // namespace mch
