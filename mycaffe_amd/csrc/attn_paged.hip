@@ -635,17 +635,34 @@ __device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const Chunk
     return ChunkTile{seq, tile, group / w.headTiles, group % w.headTiles};
 }
 
+// Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
+template <int PARTS> struct Parts { u32x4 p[PARTS]; };
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+__device__ __forceinline__ float upper_half(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+template <int PARTS> __device__ __forceinline__ void two_parts(float x, float y, uint32_t (&out)[PARTS])
+{
+#pragma unroll
+    for (int i = 0; i < PARTS; i++) {
+        out[i] = upper_halves(x, y);
+        if (i + 1 < PARTS) {
+            x -= upper_half(x);
+            y -= upper_half(y);
+        }
+    }
+}
+
+// Products in fp32 are sums of products of bf16 parts: of the nine of two values of three parts the six that reach fp32's last bits, exact each and
+// added in fp32; over a 16-bit cache the three that there are.  (32 x 32 x 16 of them take 32 cycles a part, in fp32 512: 2.7 and 5.3 times as long.)
 template <typename TQ, typename TC, int HSP>
 __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs a, ChunkArgs w)
 {
-    typedef FlashTraits<TQ> TR;
-    constexpr bool B16 = sizeof(TQ) == 2;
-    constexpr int KB = B16 ? 64 : 32, KF = HSP / TR::CPF, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    typedef FlashTraits<bf16_t> TR;
+    constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;                     // parts of a query and a weight, of a key and a value
+    constexpr int KB = NK == 1 ? 64 : 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
-    constexpr int LDK = B16 ? HSP + 8 : HSP + 4, LDV = B16 ? HSP + 8 : HSP;                       // values a row in LDS
+    constexpr int LD = HSP + 8;                                                                   // values a row in LDS
     constexpr int PART = 128 * (HSP + 2);
-    __shared__ __attribute__((aligned(16))) TQ sK[KB * LDK];
-    __shared__ __attribute__((aligned(16))) TQ sV[KB * LDV];
+    __shared__ __attribute__((aligned(16))) bf16_t sK[NK][KB * LD], sV[NK][KB * LD];
     __shared__ long long sPlace[2][KB];
     __shared__ uint64_t sGiven[2];
     __shared__ int sBad, sFront;
@@ -689,13 +706,32 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     const int waveEnd = 32 * wave / w.tileHeads < nt ? min(end, base + min((32 * wave + 31) / w.tileHeads, nt - 1) + 1) : 0, waveOpen = base + 32 * wave / w.tileHeads + 1;   // past what any, and what every row sees
     auto row_at = [&](int t, int h) { return ((size_t)(sp.first + j0 + t) * c.H + h0 + h) * c.hs; };
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
-    u32x4 qf[KF];
+    bool bad = false;
+    Parts<NQ> qf[KF];
     {
         const TQ* q = (const TQ*)a.q + (live ? row_at(token, head) : 0);
 #pragma unroll
         for (int f = 0; f < KF; f++) {
-            const int d = f * TR::CPF + half * TR::EPC;
-            qf[f] = live && d < c.hs ? *(const u32x4*)(q + d) : zero4;
+            const int d = 16 * f + 8 * half;
+            if constexpr (NQ == 1) qf[f].p[0] = live && d < c.hs ? *(const u32x4*)(q + d) : zero4;
+            else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 y = live && d + e < c.hs ? *(const float4*)(q + d + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t out[NQ];
+                    two_parts<NQ>(x[2 * e], x[2 * e + 1], out);
+#pragma unroll
+                    for (int i = 0; i < NQ; i++) qf[f].p[i][e] = out[i];
+                }
+                // parts of a value that is not finite do not add up to it
+#pragma unroll
+                for (int e = 0; e < 8; e++) bad = bad || (__float_as_uint(x[e]) & 0x7f800000u) == 0x7f800000u;
+            }
         }
     }
     floatx16 o[DT];
@@ -704,7 +740,6 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 #pragma unroll
         for (int v = 0; v < 16; v++) o[i][v] = 0.f;
     float m = -INFINITY, l = 0.f;
-    bool bad = false;
 
     // ---- staging: places two blocks ahead, values one ----
     u32x4 rk[NP], rv[NP];
@@ -740,19 +775,25 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int r = tid / CPR + RPP * i, d = (tid % CPR) * EPL;
-            if constexpr (sizeof(TQ) == sizeof(TC)) {
-                *(u32x4*)(sK + r * LDK + d) = rk[i];
-                *(u32x4*)(sV + r * LDV + d) = rv[i];
+            if constexpr (NK == 1) {
+                *(u32x4*)(sK[0] + r * LD + d) = rk[i];
+                *(u32x4*)(sV[0] + r * LD + d) = rv[i];
             } else {
+                uint32_t k[2][NK], v[2][NK];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const u32x4 x = {rk[i][2 * e] << 16, rk[i][2 * e] & 0xffff0000u, rk[i][2 * e + 1] << 16, rk[i][2 * e + 1] & 0xffff0000u};
-                    const u32x4 y = {rv[i][2 * e] << 16, rv[i][2 * e] & 0xffff0000u, rv[i][2 * e + 1] << 16, rv[i][2 * e + 1] & 0xffff0000u};
-                    *(u32x4*)(sK + r * LDK + d + 4 * e) = x;
-                    *(u32x4*)(sV + r * LDV + d + 4 * e) = y;
+                    two_parts<NK>(__uint_as_float(rk[i][2 * e]), __uint_as_float(rk[i][2 * e + 1]), k[e]);
+                    two_parts<NK>(__uint_as_float(rv[i][2 * e]), __uint_as_float(rv[i][2 * e + 1]), v[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < NK; e++) {
+                    *(uint2*)(sK[e] + r * LD + d) = make_uint2(k[0][e], k[1][e]);
+                    *(uint2*)(sV[e] + r * LD + d) = make_uint2(v[0][e], v[1][e]);
                 }
             }
-            if (kb * KB + KB > base + 1) bad = bad || not_finite<TC>(rv[i]);
+            // what only some rows see, and where parts are multiplied anything, has to be finite
+            if (NK > 1 || NQ > 1 || kb * KB + KB > base + 1) bad = bad || not_finite<TC>(rv[i]);
+            if (NK > 1 || NQ > 1) bad = bad || not_finite<TC>(rk[i]);
         }
         if (wave == 0 && kb + 2 < stop) publish(kb + 2, ahead);
         __syncthreads();
@@ -766,9 +807,16 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
             floatx16 s;
 #pragma unroll
             for (int v = 0; v < 16; v++) s[v] = 0.f;
-            const TQ* k = sK + (32 * j + l32) * LDK + half * TR::EPC;
+            const int krow = (32 * j + l32) * LD + 8 * half;
 #pragma unroll
-            for (int f = 0; f < KF; f++) s = TR::mma(*(const u32x4*)(k + f * TR::CPF), qf[f], s);
+            for (int f = 0; f < KF; f++)
+#pragma unroll
+                for (int x = NK - 1; x >= 0; x--) {
+                    const u32x4 k = *(const u32x4*)(sK[x] + krow + 16 * f);
+#pragma unroll
+                    for (int y = NQ - 1; y >= 0; y--)
+                        if (x + y < 3) s = TR::mma(k, qf[f].p[y], s);
+                }
             float mx = -INFINITY;
             if (t + 32 <= waveOpen && there == 0xffffffffu) {
 #pragma unroll
@@ -803,26 +851,31 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                 for (int i = 0; i < DT; i++)
 #pragma unroll
                     for (int v = 0; v < 16; v++) o[i][v] *= alpha;
-            if constexpr (B16) {
-                const u32x4 w0 = TR::pack_p(s, 0), w1 = TR::pack_p(s, 1);
+            // weights in the operand layout: rounded to 16 bits (their sum is not: the roundings of many even out), or in three parts
+            Parts<NQ> p[2];
 #pragma unroll
-                for (int i = 0; i < DT; i++) {
-                    const TQ* tile = sV + 32 * j * LDV + 32 * i;
-                    o[i] = TR::mma(TR::load_vt_rowmajor(tile, LDV, 0, lane), w0, o[i]);
-                    o[i] = TR::mma(TR::load_vt_rowmajor(tile, LDV, 1, lane), w1, o[i]);
-                }
-            } else {
+            for (int x = 0; x < 2; x++) {
+                if constexpr (NQ == 1) p[x].p[0] = TR::pack_p(s, x);
+                else
 #pragma unroll
-                for (int f = 0; f < 4; f++) {
-                    const u32x4 wt = TR::pack_p(s, f);
+                    for (int e = 0; e < 4; e++) {
+                        uint32_t out[NQ];
+                        two_parts<NQ>(s[8 * x + 2 * e], s[8 * x + 2 * e + 1], out);
 #pragma unroll
-                    for (int i = 0; i < DT; i++) {
-                        const TQ* v = sV + (32 * j + 8 * f + 4 * half) * LDV + 32 * i + l32;
-                        const u32x4 x = {__float_as_uint((float)v[0]), __float_as_uint((float)v[LDV]), __float_as_uint((float)v[2 * LDV]), __float_as_uint((float)v[3 * LDV])};
-                        o[i] = TR::mma(x, wt, o[i]);
+                        for (int i = 0; i < NQ; i++) p[x].p[i][e] = out[i];
                     }
-                }
             }
+#pragma unroll
+            for (int i = 0; i < DT; i++)
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int z = NK - 1; z >= 0; z--) {
+                        const u32x4 v = TR::load_vt_rowmajor(sV[z] + 32 * j * LD + 32 * i, LD, x, lane);
+#pragma unroll
+                        for (int y = NQ - 1; y >= 0; y--)
+                            if (z + y < 3) o[i] = TR::mma(v, p[x].p[y], o[i]);
+                    }
         }
     }
     l = add_lane_xor<32>(l);
@@ -847,12 +900,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                     else {
 #pragma unroll
                         for (int e = 0; e < 4; e++) x[e] = m > -INFINITY ? x[e] * inv : 0.f;
-                        TR::store4(y + d, x[0], x[1], x[2], x[3]);
+                        FlashTraits<TQ>::store4(y + d, x[0], x[1], x[2], x[3]);
                     }
                 }
         }
     } else {
-        // A value that is not finite lies where only some of the rows look: weights of zero would not keep it from the others.  Row by row, then.
+        // A value that is not finite lies where only some of the rows look, and weights of zero would not keep it from the others, or it has been cut in
+        // parts.  Row by row, then.
         for (int r = wave; r < nt * w.tileHeads; r += 4) {
             const int tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
             if (hd >= nh) continue;

@@ -209,6 +209,68 @@ def test_scores_that_are_all_minus_infinity(dev, act16, cache16):
 
 
 @pytest.mark.parametrize("act16,cache16", TYPES)
+@pytest.mark.parametrize("n", [1, 60])
+def test_keys_of_infinity(dev, act16, cache16, n):
+    """Scores of -inf are weights of zero and nothing else; a query that is no number spoils its own row alone."""
+    rng = np.random.default_rng(15)
+    H, kvH, hs, m = 2, 1, 64, 100
+    q = rounded(abs(rng.standard_normal((n, H, hs))) + 0.1, act16)
+    c = Cache(dev, rng, [(n, m, 0)], kvH, hs, 16, "head", cache16)
+    k, v = c.dense[0]
+    for at in (3, 35, 36):
+        k[at] = -np.inf
+        c.k[int(c.table[0, at // 16]), :, at % 16] = -np.inf
+    c.h["k"] = dev.put(c.laid(c.k), cache16)
+    q[n - 1, 1, 7] = np.nan
+    hq, hy = dev.put(q, act16), dev.zeros(q.size, act16)
+    c.attend(hq, hy, H)
+    got = dev.get(hy, q.shape)
+    assert np.isnan(got[n - 1, 1]).all()
+    keep = [t for t in range(m) if t not in (3, 35, 36)]
+    for j in range(n):
+        for h in range(H - (j == n - 1)):
+            seen = [t for t in keep if t <= m - n + j]
+            s = k[seen, 0].astype(np.float64) @ q[j, h] / 8
+            e = np.exp(s - s.max())
+            w = e / e.sum()
+            vv = v[seen, 0].astype(np.float64)
+            # as attention() counts it
+            off = 2 * ((hs + 8) * U32 * (abs(k[seen, 0].astype(np.float64)) @ abs(q[j, h])).max() / 8 + 4 * U32 * abs(s - s.max()).max() + 4 * U32) + (
+                2 * U16 if act16 else 0) + (len(w) + 8) * U32
+            assert (abs(got[j, h] - w @ vv) <= off * (w @ abs(vv)) + (U16 if act16 else U32) * abs(w @ vv)).all()
+
+
+@pytest.mark.parametrize("act16,cache16", TYPES)
+@pytest.mark.parametrize("size", [1e-30, 1e30, 3e38])
+def test_values_far_from_one(dev, act16, cache16, size):
+    """Values at the ends of the range come out as large as they went in."""
+    rng = np.random.default_rng(16)
+    H, kvH, hs, n, m = 1, 1, 64, 40, 90
+    c = Cache(dev, rng, [(n, m, 0)], kvH, hs, 16, "head", cache16)
+    k, v = c.dense[0]
+    v[:] = rounded(size * np.sign(v) * (1 + 0.1 * rng.random(v.shape)), cache16)
+    for t in range(m):
+        c.v[int(c.table[0, t // 16]), :, t % 16] = v[t]
+    c.h["v"] = dev.put(c.laid(c.v), cache16)
+    q = np.float32(np.zeros((n, H, hs)))
+    if size > 1e38:
+        v_ = v.copy()       # a mean of numbers of one sign, so that no sum leaves the range before it is divided
+        k[:] = 0
+        for t in range(m):
+            c.k[int(c.table[0, t // 16]), :, t % 16] = 0
+            c.v[int(c.table[0, t // 16]), :, t % 16] = abs(v_[t]) / 512
+        c.h["k"], c.h["v"] = dev.put(c.laid(c.k), cache16), dev.put(c.laid(c.v), cache16)
+        v[:] = rounded(abs(v_) / 512, cache16)
+    hq, hy = dev.put(q, act16), dev.zeros(q.size, act16)
+    c.attend(hq, hy, H)
+    got = dev.get(hy, q.shape)
+    for j in range(n):
+        vv = v[:m - n + j + 1, 0].astype(np.float64)
+        tol = ((len(vv) + 12) * U32 + (2 * U16 if act16 else 0)) * abs(vv).mean(0) + (U16 if act16 else U32) * abs(vv.mean(0))
+        assert (abs(got[j, 0] - vv.mean(0)) <= tol).all()
+
+
+@pytest.mark.parametrize("act16,cache16", TYPES)
 @pytest.mark.parametrize("max_new", [1, 40, 500])
 def test_hint(dev, act16, cache16, max_new):
     """The bound on new tokens changes nothing but kernels, even where it does not hold."""
