@@ -658,7 +658,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 {
     typedef FlashTraits<bf16_t> TR;
     constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;                     // parts of a query and a weight, of a key and a value
-    constexpr int KB = NK == 1 ? 64 : 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
     constexpr int LD = HSP + 8;                                                                   // values a row in LDS
     constexpr int PART = 128 * (HSP + 2);
@@ -799,14 +799,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
         __syncthreads();
         if (kb + 1 < stop) load((kb + 1) & 1);
         if (wave == 0) ahead = entry(kb + 3);
-#pragma unroll 1
-        for (int j = 0; j < KB / 32; j++) {
-            const int t = kb * KB + 32 * j;
-            const uint32_t there = (uint32_t)(given >> (32 * j));
-            if (t >= waveEnd || !there) continue;
-            floatx16 s;
+        const int t = kb * KB;
+        if (t >= waveEnd || !given) continue;
+        floatx16 s[KJ];
 #pragma unroll
-            for (int v = 0; v < 16; v++) s[v] = 0.f;
+        for (int j = 0; j < KJ; j++) {
+#pragma unroll
+            for (int v = 0; v < 16; v++) s[j][v] = 0.f;
             const int krow = (32 * j + l32) * LD + 8 * half;
 #pragma unroll
             for (int f = 0; f < KF; f++)
@@ -815,68 +814,80 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                     const u32x4 k = *(const u32x4*)(sK[x] + krow + 16 * f);
 #pragma unroll
                     for (int y = NQ - 1; y >= 0; y--)
-                        if (x + y < 3) s = TR::mma(k, qf[f].p[y], s);
+                        if (x + y < 3) s[j] = TR::mma(k, qf[f].p[y], s[j]);
                 }
-            float mx = -INFINITY;
-            if (t + 32 <= waveOpen && there == 0xffffffffu) {
+        }
+        float mx = -INFINITY;
+        if (t + KB <= waveOpen && given == (KB == 64 ? ~0ull : 0xffffffffull)) {
+#pragma unroll
+            for (int j = 0; j < KJ; j++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
-                    s[v] *= a.c2;
-                    mx = fmaxf(mx, s[v]);
+                    s[j][v] *= a.c2;
+                    mx = fmaxf(mx, s[j][v]);
                 }
-                mx = fmaxf(mx, SCORE_FLOOR);
-            } else {
+            mx = fmaxf(mx, SCORE_FLOOR);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KJ; j++) {
+                const uint32_t there = (uint32_t)(given >> (32 * j));
 #pragma unroll
                 for (int v = 0; v < 16; v++) {
                     const int key = 8 * (v >> 2) + 4 * half + (v & 3);
-                    const bool sees = (there >> key & 1) && t + key <= last;
-                    const float x = s[v] * a.c2;
+                    const bool sees = (there >> key & 1) && t + 32 * j + key <= last;
+                    const float x = s[j][v] * a.c2;
                     mx = fmaxf(mx, sees ? fmaxf(x, SCORE_FLOOR) : -INFINITY);
-                    s[v] = sees ? x : -INFINITY;
+                    s[j][v] = sees ? x : -INFINITY;
                 }
             }
-            mx = fmaxf(max_lane_xor<32>(mx), m);
-            const float ref = mx > -INFINITY ? mx : 0.f, alpha = __builtin_amdgcn_exp2f(m - ref);
-            const bool moved = __any(mx != m);
-            m = mx;
-            float sum = 0.f;
+        }
+        mx = fmaxf(max_lane_xor<32>(mx), m);
+        const float ref = mx > -INFINITY ? mx : 0.f, alpha = __builtin_amdgcn_exp2f(m - ref);
+        const bool moved = __any(mx != m);
+        m = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < KJ; j++)
 #pragma unroll
             for (int v = 0; v < 16; v++) {
-                s[v] = __builtin_amdgcn_exp2f(s[v] - ref);
-                sum += s[v];
+                s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ref);
+                sum += s[j][v];
             }
-            l = l * alpha + sum;
-            if (moved)
+        l = l * alpha + sum;
+        if (moved)
 #pragma unroll
-                for (int i = 0; i < DT; i++)
+            for (int i = 0; i < DT; i++)
 #pragma unroll
-                    for (int v = 0; v < 16; v++) o[i][v] *= alpha;
-            // weights in the operand layout: rounded to 16 bits (their sum is not: the roundings of many even out), or in three parts
-            Parts<NQ> p[2];
+                for (int v = 0; v < 16; v++) o[i][v] *= alpha;
+        // weights in the operand layout: rounded to 16 bits (their sum is not: the roundings of many even out), or in three parts
+        Parts<NQ> p[KJ][2];
+#pragma unroll
+        for (int j = 0; j < KJ; j++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                if constexpr (NQ == 1) p[x].p[0] = TR::pack_p(s, x);
+                if constexpr (NQ == 1) p[j][x].p[0] = TR::pack_p(s[j], x);
                 else
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         uint32_t out[NQ];
-                        two_parts<NQ>(s[8 * x + 2 * e], s[8 * x + 2 * e + 1], out);
+                        two_parts<NQ>(s[j][8 * x + 2 * e], s[j][8 * x + 2 * e + 1], out);
 #pragma unroll
-                        for (int i = 0; i < NQ; i++) p[x].p[i][e] = out[i];
+                        for (int i = 0; i < NQ; i++) p[j][x].p[i][e] = out[i];
                     }
             }
 #pragma unroll
-            for (int i = 0; i < DT; i++)
+        for (int j = 0; j < KJ; j++)
 #pragma unroll
-                for (int x = 0; x < 2; x++)
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < DT; i++)
 #pragma unroll
                     for (int z = NK - 1; z >= 0; z--) {
                         const u32x4 v = TR::load_vt_rowmajor(sV[z] + 32 * j * LD + 32 * i, LD, x, lane);
 #pragma unroll
                         for (int y = NQ - 1; y >= 0; y--)
-                            if (z + y < 3) o[i] = TR::mma(v, p[x].p[y], o[i]);
+                            if (z + y < 3) o[i] = TR::mma(v, p[j][x].p[y], o[i]);
                     }
-        }
     }
     l = add_lane_xor<32>(l);
     if (__any(bad) && lane == 0) sBad = 1;
