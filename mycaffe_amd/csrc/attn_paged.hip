@@ -651,6 +651,13 @@ template <int PARTS> __device__ __forceinline__ void two_parts(float x, float y,
     }
 }
 
+// l + both values of a pair of bf16
+__device__ __forceinline__ float pair_sum(uint32_t pair, float l)
+{
+    const bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+    return __builtin_amdgcn_fdot2_f32_bf16(*reinterpret_cast<bf16x2*>(&pair), ones, l, false);
+}
+
 // Products in fp32 are sums of products of bf16 parts: of the nine of two values of three parts the six that reach fp32's last bits, exact each and
 // added in fp32; over a 16-bit cache the three that there are.  (32 x 32 x 16 of them take 32 cycles a part, in fp32 512: 2.7 and 5.3 times as long.)
 template <typename TQ, typename TC, int HSP>
@@ -699,6 +706,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     const int kb0 = min(sFront, max(end, 0)) / KB, nkb = (max(end, 0) + KB - 1) / KB;
     const int first = kb0 + (int)((long long)(nkb - kb0) * blockIdx.y / w.splits), stop = kb0 + (int)((long long)(nkb - kb0) * (blockIdx.y + 1) / w.splits);
 
+    const float c2 = fabsf(a.c2);
+
     // ---- the lane's row ----
     const int row = 32 * wave + l32, token = row / w.tileHeads, head = row - token * w.tileHeads;
     const bool live = token < nt && head < nh;
@@ -713,14 +722,18 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 #pragma unroll
         for (int f = 0; f < KF; f++) {
             const int d = 16 * f + 8 * half;
-            if constexpr (NQ == 1) qf[f].p[0] = live && d < c.hs ? *(const u32x4*)(q + d) : zero4;
-            else {
+            if constexpr (NQ == 1) {
+                qf[f].p[0] = live && d < c.hs ? *(const u32x4*)(q + d) : zero4;
+                if (a.c2 < 0.f) qf[f].p[0] ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+            } else {
                 float x[8];
 #pragma unroll
                 for (int e = 0; e < 8; e += 4) {
                     const float4 y = live && d + e < c.hs ? *(const float4*)(q + d + e) : make_float4(0.f, 0.f, 0.f, 0.f);
                     x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
                 }
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = a.c2 < 0.f ? -x[e] : x[e];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     uint32_t out[NQ];
@@ -817,17 +830,17 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                         if (x + y < 3) s[j] = TR::mma(k, qf[f].p[y], s[j]);
                 }
         }
+        // Maxima are taken of the products themselves (the queries carry the scale's sign), and the running one moves only when a row's grows by 2^8:
+        // weights stay below that, and the sums are seldom scaled again.
         float mx = -INFINITY;
+        bool any = true;
         if (t + KB <= waveOpen && given == (KB == 64 ? ~0ull : 0xffffffffull)) {
 #pragma unroll
             for (int j = 0; j < KJ; j++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) {
-                    s[j][v] *= a.c2;
-                    mx = fmaxf(mx, s[j][v]);
-                }
-            mx = fmaxf(mx, SCORE_FLOOR);
+                for (int v = 0; v < 16; v++) mx = fmaxf(mx, s[j][v]);
         } else {
+            any = false;
 #pragma unroll
             for (int j = 0; j < KJ; j++) {
                 const uint32_t there = (uint32_t)(given >> (32 * j));
@@ -835,38 +848,43 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                 for (int v = 0; v < 16; v++) {
                     const int key = 8 * (v >> 2) + 4 * half + (v & 3);
                     const bool sees = (there >> key & 1) && t + 32 * j + key <= last;
-                    const float x = s[j][v] * a.c2;
-                    mx = fmaxf(mx, sees ? fmaxf(x, SCORE_FLOOR) : -INFINITY);
-                    s[j][v] = sees ? x : -INFINITY;
+                    any = any || sees;
+                    s[j][v] = sees ? s[j][v] : -INFINITY;
+                    mx = fmaxf(mx, s[j][v]);
                 }
             }
         }
-        mx = fmaxf(max_lane_xor<32>(mx), m);
-        const float ref = mx > -INFINITY ? mx : 0.f, alpha = __builtin_amdgcn_exp2f(m - ref);
-        const bool moved = __any(mx != m);
-        m = mx;
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < KJ; j++)
-#pragma unroll
-            for (int v = 0; v < 16; v++) {
-                s[j][v] = __builtin_amdgcn_exp2f(s[j][v] - ref);
-                sum += s[j][v];
-            }
-        l = l * alpha + sum;
-        if (moved)
+        mx = any ? fmaxf(mx * c2, SCORE_FLOOR) : -INFINITY;
+        mx = max_lane_xor<32>(mx);
+        if (__any(mx > m + 8.f)) {
+            mx = fmaxf(mx, m);
+            const float alpha = __builtin_amdgcn_exp2f(m - (mx > -INFINITY ? mx : 0.f));
+            m = mx;
+            l *= alpha;
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) o[i][v] *= alpha;
-        // weights in the operand layout: rounded to 16 bits (their sum is not: the roundings of many even out), or in three parts
+        }
+        const float ref = m > -INFINITY ? -m : 0.f;
+#pragma unroll
+        for (int j = 0; j < KJ; j++)
+#pragma unroll
+            for (int v = 0; v < 16; v++) {
+                s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], c2, ref));
+                if (NQ > 1) l += s[j][v];
+            }
+        // weights in the operand layout: rounded to 16 bits, and added up as rounded, or in three parts
         Parts<NQ> p[KJ][2];
 #pragma unroll
         for (int j = 0; j < KJ; j++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                if constexpr (NQ == 1) p[j][x].p[0] = TR::pack_p(s[j], x);
-                else
+                if constexpr (NQ == 1) {
+                    p[j][x].p[0] = TR::pack_p(s[j], x);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) l = pair_sum(p[j][x].p[0][e], l);
+                } else
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         uint32_t out[NQ];
