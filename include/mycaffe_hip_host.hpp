@@ -401,6 +401,33 @@ public:
     {
         m_cuda.AttnDecodeNoAlloc(m_hKernel, {fScale}, {nBatch, nHeads, nKvHeads, nSize, nLen, hQ, hKCache, hVCache, hY, nStrideBatch, nStrideHead, nStridePos});
     }
+    // norms of the heads of queries and keys with their rotation, forward and backward (hdWq, hdWk overwritten, or added to)
+    void QkNormRopeForward(int nBatch, int nT, int nHeads, int nKvHeads, int nSize, long hQ, long hK, long hWq, long hWk, long hYq, long hYk, long hRope = 0,
+                           float fEps = 1e-5f)
+    {
+        ex2(MCH_FN_QK_NORM_ROPE_FWD, {fEps}, {nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hRope, hYq, hYk});
+    }
+    void QkNormRopeBackward(int nBatch, int nT, int nHeads, int nKvHeads, int nSize, long hQ, long hK, long hWq, long hWk, long hdYq, long hdYk, long hdQ, long hdK,
+                            long hdWq, long hdWk, long hRope = 0, float fEps = 1e-5f, bool bAccumulate = false)
+    {
+        ex2(MCH_FN_QK_NORM_ROPE_BWD, {fEps}, {nBatch, nT, nHeads, nKvHeads, nSize, hQ, hK, hWq, hWk, hRope, hdYq, hdYk, hdQ, hdK, hdWq, hdWk, bAccumulate ? 1 : 0});
+    }
+    // a paged cache: its sizes, pages and sequences, as PAGED_APPEND and ATTN_PAGED_FWD take them
+    struct PagedCache {
+        int nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages;
+        long hKPages, hVPages, hTable, hStarts, hLens;
+        long long nStridePage, nStrideHead, nStridePos;
+    };
+    void PagedAppend(const PagedCache& c, long hQKV, long hQ, long hRope = 0, bool bNorm = false, long hWq = 0, long hWk = 0, float fEps = 1e-5f)
+    {
+        ex2(MCH_FN_PAGED_APPEND, {fEps}, {c.nBatch, c.nTokens, c.nHeads, c.nKvHeads, c.nSize, c.nPages, c.nPageSize, c.nMaxPages, hQKV, c.hKPages, c.hVPages, c.hTable,
+                                          c.hStarts, c.hLens, hQ, c.nStridePage, c.nStrideHead, c.nStridePos, hRope, bNorm ? 1 : 0, hWq, hWk});
+    }
+    void AttnPagedForward(const PagedCache& c, long hQ, long hY, float fScale = 0.f, int nMaxNew = 0)
+    {
+        ex2(MCH_FN_ATTN_PAGED_FWD, {fScale}, {c.nBatch, c.nTokens, c.nHeads, c.nKvHeads, c.nSize, c.nPages, c.nPageSize, c.nMaxPages, hQ, c.hKPages, c.hVPages, c.hTable,
+                                              c.hStarts, c.hLens, hY, c.nStridePage, c.nStrideHead, c.nStridePos, nMaxNew});
+    }
     // fused QKV projection: q, k, v = X W^T + bias written as (B,H,T,hs), q and k rotated when hRope is given (no
     // counterpart in the reference)
     void QkvProjHeads(int nBatch, int nT, int nHeads, int nSize, long hX, long hWeight, long hBias, long hQ, long hK, long hV,

@@ -2743,10 +2743,9 @@ long Kernel::qk_norm_rope(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool ba
 // hTable,hStarts,hLens,hOut,stridePage,strideHead,stridePos}, rows of rowHeads heads, output of `heads`
 long Kernel::paged_operands(const MCH_LONGLONG* pl, long long rowHeads, PagedCache* c, MemItem** rows, MemItem** out)
 {
-    const long long B = pl[0], N = pl[1], H = pl[2], KVH = pl[3], hs = pl[4], pages = pl[5], ps = pl[6], width = pl[7];
-    if (B < 1 || N < 1 || H < 1 || KVH < 1 || pages < 1 || ps < 1 || width < 1 || hs < 2 || (hs & 1) || hs > 256 || H > 65535 || KVH > H || H % KVH || B > PAGED_EXACT ||
-        N > PAGED_EXACT || pages > PAGED_EXACT || ps > PAGED_EXACT || width > PAGED_EXACT || ps * width > PAGED_EXACT)
-        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const long long* l = (const long long*)pl;
+    const long long B = l[0], N = l[1], H = l[2], KVH = l[3], hs = l[4], pages = l[5], ps = l[6], width = l[7];
+    if (!paged_sizes_ok(l)) return MCH_ERROR_PARAM_OUT_OF_RANGE;
     MemItem *K, *V, *table, *starts, *lens;
     ERRCHK(mem((long)pl[8], rows));
     ERRCHK(mem((long)pl[9], &K));
@@ -2765,23 +2764,18 @@ long Kernel::paged_operands(const MCH_LONGLONG* pl, long long rowHeads, PagedCac
     RANGE(table, 0, B * width);
     RANGE(starts, 0, B + 1);
     RANGE(lens, 0, B);
-    const long long sP = pl[15], sH = pl[16], sT = pl[17];
-    const long long most = (long long)std::min(K->count, V->count);
-    if (sP < 0 || sH < 0 || sT < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
-    if ((pages > 1 && sP > most) || (KVH > 1 && sH > most) || (ps > 1 && sT > most)) {
+    const long long need = paged_reach(l, (long long)std::min(K->count, V->count));
+    if (need < 0) {
         last_detail = "range exceeds the allocation behind the memory handle";
         return MCH_ERROR_MEMORY_RANGE_EXCEEDED;
     }
-    const long long need = (pages > 1 ? (pages - 1) * sP : 0) + (KVH > 1 ? (KVH - 1) * sH : 0) + (ps > 1 ? (ps - 1) * sT : 0) + hs;
-    RANGE(K, 0, need);
-    RANGE(V, 0, need);
     if (overlap(*out, N * H * hs, *rows, N * rowHeads * hs) || overlap(*out, N * H * hs, K, need) || overlap(*out, N * H * hs, V, need) || overlap(*out, N * H * hs, table, B * width) ||
         overlap(*out, N * H * hs, starts, B + 1) || overlap(*out, N * H * hs, lens, B)) {
         last_detail = "an output shares memory with another operand";
         return MCH_ERROR_PARAM_OUT_OF_RANGE;
     }
     *c = PagedCache{K->ptr, V->ptr, K->dt(), (const float*)table->ptr, (const float*)starts->ptr, (const float*)lens->ptr, (int)B, (int)N, (int)H, (int)KVH, (int)hs,
-                    (int)pages, (int)ps, (int)width, sP, sH, sT};
+                    (int)pages, (int)ps, (int)width, l[15], l[16], l[17]};
     return 0;
 }
 
@@ -2792,24 +2786,14 @@ long Kernel::paged_append(float* pf, long lf, MCH_LONGLONG* pl, long ll)
     NEED_L(22, 22);
     PagedCache c;
     MemItem *X, *Q, *K, *V, *W[2] = {}, *meta;
-    if (!(pf[0] >= 0.f) || pl[2] > 65535 || pl[3] > 65535) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    if (!(pf[0] >= 0.f) || !paged_sizes_ok((const long long*)pl)) return MCH_ERROR_PARAM_OUT_OF_RANGE;
     ERRCHK(paged_operands(pl, pl[2] + 2 * pl[3], &c, &X, &Q));
     ERRCHK(mem((long)pl[9], &K));
     ERRCHK(mem((long)pl[10], &V));
-    // every place of its own: each stride reaches past what the smaller ones span, the distance between keys and values in one piece of memory
-    // (rows k | v, say) among them
-    const long long apart = std::llabs((const char*)V->ptr - (const char*)K->ptr) / (long long)K->esize();
-    const long long reach = (c.pages - 1) * (c.pages > 1 ? c.sP : 0) + (c.kvH - 1) * (c.kvH > 1 ? c.sH : 0) + (c.pageSize - 1) * (c.pageSize > 1 ? c.sT : 0) + c.hs;
-    std::pair<long long, int> dims[4] = {{c.sP, c.pages}, {c.sH, c.kvH}, {c.sT, c.pageSize}, {apart, apart < reach ? 2 : 1}};
-    std::sort(dims, dims + 4);
-    long long span = c.hs;
-    for (const auto& d : dims) {
-        if (d.second == 1) continue;
-        if (d.first < span) {
-            last_detail = "the strides of the pages let positions overlap";
-            return MCH_ERROR_PARAM_OUT_OF_RANGE;
-        }
-        span += (d.second - 1) * d.first;
+    const long long reach = paged_reach((const long long*)pl, (long long)std::min(K->count, V->count));
+    if (!paged_apart((const long long*)pl, std::llabs((const char*)V->ptr - (const char*)K->ptr) / (long long)K->esize(), reach)) {
+        last_detail = "the strides of the pages let positions overlap";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
     }
     const long long rows = (long long)c.tokens * (c.H + 2 * c.kvH) * c.hs;
     bool clash = false;

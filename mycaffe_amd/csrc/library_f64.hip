@@ -11,15 +11,18 @@
 // in the message.  ALLOCMEM_HALF allocates doubles (no 16-bit storage under this base type).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <string>
 #include <vector>
 
 #include "gemm_f64.h"
+#include "paged.h"
 #include "runtime.h"
 
 namespace mch {
@@ -632,6 +635,170 @@ static hipError_t d_qkv_split(hipStream_t s, long long M, int T, int H, int hs, 
     return hipGetLastError();
 }
 
+// ---- norms of heads with their rotation, paged caches (ids 2013 - 2016): a wavefront a head, lane l of it the pairs l and l + 64 ----
+__device__ inline double d_wave_sum(double v)
+{
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// the pair (a, b) of a head turned to position t (theta 0: not), or back
+__device__ inline void d_turn(double& a, double& b, int t, int pair, int half, double theta, bool back)
+{
+    if (theta == 0.0) return;
+    double s, c;
+    sincos(t * pow(theta, -(double)pair / half), &s, &c);
+    if (back) s = -s;
+    const double x = a * c - b * s;
+    b = a * s + b * c;
+    a = x;
+}
+// y = R(t) (w x / rms(x)), or with norm false R(t) x
+__device__ inline void d_head(const double* x, const double* w, double* y, bool norm, double eps, int t, int hs, double theta)
+{
+    const int half = hs / 2, lane = threadIdx.x & 63;
+    double a[2], b[2], ss = 0.0;
+    for (int i = 0; i < 2; i++) {
+        const int p = lane + 64 * i;
+        a[i] = p < half ? x[2 * p] : 0.0;
+        b[i] = p < half ? x[2 * p + 1] : 0.0;
+        ss += a[i] * a[i] + b[i] * b[i];
+    }
+    const double r = norm ? 1.0 / sqrt(d_wave_sum(ss) / hs + eps) : 1.0;
+    for (int i = 0; i < 2; i++) {
+        const int p = lane + 64 * i;
+        if (p >= half) continue;
+        a[i] *= norm && w ? w[2 * p] * r : r;
+        b[i] *= norm && w ? w[2 * p + 1] * r : r;
+        d_turn(a[i], b[i], t, p, half, theta, false);
+        y[2 * p] = a[i];
+        y[2 * p + 1] = b[i];
+    }
+}
+__global__ __launch_bounds__(256) void d_head_norm_kernel(size_t rows, int T, int hs, const double* x, const double* w, double* y, double eps, double theta)
+{
+    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row < rows) d_head(x + row * hs, w, y + row * hs, true, eps, (int)(row % T), hs, theta);
+}
+// g = R(-t) dy, dx = r (g w - x r mean(g w x r)); gx: what the weights' gradient adds up, g x r
+__global__ __launch_bounds__(256) void d_head_norm_bwd_kernel(size_t rows, int T, int hs, const double* x, const double* w, const double* dy, double* dx, double* gx,
+                                                              double eps, double theta)
+{
+    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int half = hs / 2, lane = threadIdx.x & 63, t = (int)(row % T);
+    double a[2], b[2], ga[2], gb[2], ss = 0.0, dot = 0.0;
+    for (int i = 0; i < 2; i++) {
+        const int p = lane + 64 * i;
+        a[i] = b[i] = ga[i] = gb[i] = 0.0;
+        if (p >= half) continue;
+        a[i] = x[row * hs + 2 * p];
+        b[i] = x[row * hs + 2 * p + 1];
+        ga[i] = dy[row * hs + 2 * p];
+        gb[i] = dy[row * hs + 2 * p + 1];
+        d_turn(ga[i], gb[i], t, p, half, theta, true);
+        ss += a[i] * a[i] + b[i] * b[i];
+    }
+    const double r = 1.0 / sqrt(d_wave_sum(ss) / hs + eps);
+    for (int i = 0; i < 2; i++) {
+        const int p = lane + 64 * i;
+        if (p >= half) continue;
+        a[i] *= r;
+        b[i] *= r;
+        if (gx) {
+            gx[row * hs + 2 * p] = ga[i] * a[i];
+            gx[row * hs + 2 * p + 1] = gb[i] * b[i];
+        }
+        if (w) { ga[i] *= w[2 * p]; gb[i] *= w[2 * p + 1]; }
+        dot += ga[i] * a[i] + gb[i] * b[i];
+    }
+    const double mean = d_wave_sum(dot) / hs;
+    for (int i = 0; i < 2; i++) {
+        const int p = lane + 64 * i;
+        if (p >= half) continue;
+        dx[row * hs + 2 * p] = r * (ga[i] - a[i] * mean);
+        dx[row * hs + 2 * p + 1] = r * (gb[i] - b[i] * mean);
+    }
+}
+__global__ __launch_bounds__(1024) void d_head_norm_dw_kernel(size_t rows, int hs, const double* gx, double* dw, int accum)
+{
+    __shared__ double red[64][17];
+    const int r = threadIdx.x >> 4, j = blockIdx.x * 16 + (threadIdx.x & 15);
+    double acc = 0.0;
+    if (j < hs)
+        for (size_t i = r; i < rows; i += 64) acc += gx[i * hs + j];
+    acc = d_lane_sums(acc, red);
+    if (r == 0 && j < hs) dw[j] = accum ? dw[j] + acc : acc;
+}
+struct PagedD {
+    double *k, *v;
+    const double *table, *starts, *lens;
+    int batch, tokens, H, kvH, hs, pages, pageSize, maxPages;
+    long long sP, sH, sT;
+};
+// the sequence of a token and its span; false: none
+__device__ inline bool d_sequence(const PagedD& c, int token, int* b, PagedSpan* sp)
+{
+    for (*b = c.batch - 1; *b >= 0; --*b)
+        if (paged_int(c.starts[*b], 0, c.tokens) <= token) {
+            *sp = paged_span(c.starts[*b], c.starts[*b + 1], c.lens[*b], c.tokens, c.maxPages * c.pageSize);
+            return token < sp->first + sp->count;
+        }
+    return false;
+}
+// where position t >= 0 of sequence b lies, or -1
+__device__ inline long long d_place(const PagedD& c, int b, int t)
+{
+    const int e = t / c.pageSize, page = paged_page(c.table[(size_t)b * c.maxPages + e], c.pages);
+    return page >= 0 ? page * c.sP + (t - e * c.pageSize) * c.sT : -1;
+}
+__global__ __launch_bounds__(256) void d_paged_append_kernel(PagedD c, const double* qkv, double* q, const double* wq, const double* wk, int norm, double eps, double theta)
+{
+    const int token = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), heads = c.H + 2 * c.kvH;
+    int b;
+    PagedSpan sp;
+    if (h >= heads || !d_sequence(c, token, &b, &sp)) return;
+    const int pos = sp.len - sp.count + (token - sp.first), t = pos > 0 ? pos : 0;
+    const double* x = qkv + ((size_t)token * heads + h) * c.hs;
+    if (h < c.H) {
+        d_head(x, wq, q + ((size_t)token * c.H + h) * c.hs, norm != 0, eps, t, c.hs, theta);
+        return;
+    }
+    const long long at = pos >= 0 ? d_place(c, b, pos) : -1;
+    if (at < 0) return;
+    const bool key = h < c.H + c.kvH;
+    double* y = (key ? c.k : c.v) + at + (h - c.H - (key ? 0 : c.kvH)) * c.sH;
+    d_head(x, wk, y, key && norm, eps, t, c.hs, key ? theta : 0.0);
+}
+__global__ __launch_bounds__(256) void d_paged_attn_kernel(PagedD c, const double* q, double* y, double scale)
+{
+    const int token = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int b;
+    PagedSpan sp;
+    if (h >= c.H || !d_sequence(c, token, &b, &sp)) return;
+    const int last = sp.len - sp.count + (token - sp.first);
+    const size_t row = ((size_t)token * c.H + h) * c.hs;
+    double qv[4], acc[4] = {0.0, 0.0, 0.0, 0.0}, m = -INFINITY, l = 0.0;
+    bool seen = false;
+    for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < c.hs ? q[row + lane + 64 * i] : 0.0;
+    for (int t = 0; t <= last; t++) {
+        const long long at = d_place(c, b, t);
+        if (at < 0) continue;
+        seen = true;
+        const double *k = c.k + at + h / (c.H / c.kvH) * c.sH, *v = c.v + at + h / (c.H / c.kvH) * c.sH;
+        double s = 0.0;
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < c.hs) s += qv[i] * k[lane + 64 * i];
+        s = d_wave_sum(s) * scale;
+        const double mn = fmax(m, s), ref = mn > -INFINITY ? mn : 0.0, f = exp(m - ref), w = exp(s - ref);
+        m = mn;
+        l = l * f + w;
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < c.hs) acc[i] = acc[i] * f + w * v[lane + 64 * i];
+    }
+    for (int i = 0; i < 4; i++)
+        if (lane + 64 * i < c.hs) y[row + lane + 64 * i] = seen ? acc[i] / l : 0.0;
+}
+
 // ---- the kernel object --------------------------------------------------------------------------------------------
 struct MemD {
     double* ptr = nullptr; size_t count = 0; bool used = false; long base = 0;   // base != 0: a view into that handle's allocation
@@ -642,7 +809,7 @@ struct AttnD { bool set = false; int batch = 0, block = 0, heads = 0, hs = 0; do
                int lastTq = 0, lastTk = 0; long long lastBatchMask = 0; long lastMask = 0; };   // of the last forward call
 struct LayerNormD { bool set = false; int count = 0, outer = 0, channels = 0, inner = 0, backwards = 0; double eps = 1e-10; double* stdev = nullptr;
                     ~LayerNormD() { if (stdev) (void)hipFree(stdev); } };
-struct RopeD { bool set = false; int seq = 0, heads = 0, hs = 0; double* dcos = nullptr; double* dsin = nullptr;
+struct RopeD { bool set = false; int seq = 0, heads = 0, hs = 0; double theta = 10000.0; double* dcos = nullptr; double* dsin = nullptr;
                ~RopeD() { if (dcos) (void)hipFree(dcos); if (dsin) (void)hipFree(dsin); } };
 
 class KernelD {
@@ -769,6 +936,8 @@ private:
         *p = m_ws;
         return 0;
     }
+    long head_norm(const double* pf, const MCH_LONGLONG* pl, long ll, bool backward);
+    long paged(const double* pf, const MCH_LONGLONG* pl, bool append);
     // P (B, H, T, Tk) = softmax(mask(scale Q K^T))
     long attn_probs(const double* Q, const double* K, double* P, const AttnD* st, int T, int Tk, const MemD* M, int kind)
     {
@@ -811,6 +980,124 @@ static inline long set_out_d(double v, double** ppOut, MCH_LONG* plOut)
 #define RANGE(item, off, n) do { if ((long long)(off) < 0 || (long long)(n) < 0 || (size_t)(off) + (size_t)(n) > (item)->count) { \
         last_detail = "range exceeds the allocation behind the memory handle"; return MCH_ERROR_MEMORY_RANGE_EXCEEDED; } } while (0)
 #define LAUNCHED() HIPCHK(hipGetLastError())
+
+// whether n values of x and m of y share memory
+static bool d_overlap(const MemD* x, long long n, const MemD* y, long long m) { return x->ptr < y->ptr + m && y->ptr < x->ptr + n; }
+
+// QK_NORM_ROPE_FWD: f{eps}, l{batch,T,heads,kvHeads,hs,hQ,hK,hWq,hWk,hRope,hYq,hYk}
+// QK_NORM_ROPE_BWD: f{eps}, l{batch,T,heads,kvHeads,hs,hQ,hK,hWq,hWk,hRope,hdYq,hdYk,hdQ,hdK,hdWq,hdWk[,accumW]}
+long KernelD::head_norm(const double* pf, const MCH_LONGLONG* pl, long ll, bool backward)
+{
+    const long long B = pl[0], T = pl[1], H = pl[2], KVH = pl[3], hs = pl[4];
+    if (B < 1 || T < 1 || H < 1 || KVH < 1 || H > 65535 || KVH > 65535 || hs < 2 || hs > 256 || (hs & 1) || B > INT_MAX || T > INT_MAX || B * T > INT_MAX || !(pf[0] >= 0.0))
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const long long rows[2] = {B * H * T, B * KVH * T}, n[2] = {rows[0] * hs, rows[1] * hs};
+    if ((rows[0] + 3) / 4 > INT_MAX || (rows[1] + 3) / 4 > INT_MAX) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemD *X[2], *W[2] = {}, *dY[2] = {}, *Y[2], *dW[2] = {};
+    for (int i = 0; i < 2; i++) {
+        ERRCHK(mem((long)pl[5 + i], &X[i]));
+        if (pl[7 + i]) ERRCHK(mem((long)pl[7 + i], &W[i]));
+        if (backward) ERRCHK(mem((long)pl[10 + i], &dY[i]));
+        ERRCHK(mem((long)pl[(backward ? 12 : 10) + i], &Y[i]));
+        if (backward && pl[14 + i]) ERRCHK(mem((long)pl[14 + i], &dW[i]));
+        RANGE(X[i], 0, n[i]);
+        RANGE(Y[i], 0, n[i]);
+        if (W[i]) RANGE(W[i], 0, hs);
+        if (backward) RANGE(dY[i], 0, n[i]);
+        if (dW[i]) RANGE(dW[i], 0, hs);
+    }
+    bool clash = d_overlap(Y[0], n[0], Y[1], n[1]) || (dW[0] && dW[1] && d_overlap(dW[0], hs, dW[1], hs));
+    for (int i = 0; i < 2; i++)
+        for (int j = 0; j < 2; j++) {
+            clash = clash || (d_overlap(Y[i], n[i], X[j], n[j]) && !(i == j && Y[i]->ptr == X[j]->ptr));
+            if (backward) clash = clash || (d_overlap(Y[i], n[i], dY[j], n[j]) && !(i == j && Y[i]->ptr == dY[j]->ptr));
+            if (W[j]) clash = clash || d_overlap(Y[i], n[i], W[j], hs);
+            if (dW[j]) clash = clash || d_overlap(Y[i], n[i], dW[j], hs) || d_overlap(dW[j], hs, X[i], n[i]) || d_overlap(dW[j], hs, dY[i], n[i]) || (W[i] && d_overlap(dW[j], hs, W[i], hs));
+        }
+    if (clash) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    double theta = 0.0;
+    if (pl[9]) {
+        RopeD* r = m_rope.get((long)pl[9]);
+        if (!r || !r->set) return MCH_ERROR_ROPE_NOT_INITIALIZED;
+        if (r->hs != hs || r->seq < T) {
+            last_detail = "the rope handle was created for another head size or for fewer positions";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+        theta = r->theta;
+    }
+    double* gx = nullptr;
+    if (dW[0] || dW[1]) ERRCHK(workspace((size_t)std::max(n[0], n[1]), &gx));
+    for (int i = 0; i < 2; i++) {
+        const int grid = (int)((rows[i] + 3) / 4);
+        const double* w = W[i] ? W[i]->ptr : nullptr;
+        if (!backward) hipLaunchKernelGGL(d_head_norm_kernel, grid, 256, 0, m_stream, (size_t)rows[i], (int)T, (int)hs, (const double*)X[i]->ptr, w, Y[i]->ptr, pf[0], theta);
+        else {
+            hipLaunchKernelGGL(d_head_norm_bwd_kernel, grid, 256, 0, m_stream, (size_t)rows[i], (int)T, (int)hs, (const double*)X[i]->ptr, w, (const double*)dY[i]->ptr, Y[i]->ptr,
+                               dW[i] ? gx : nullptr, pf[0], theta);
+            if (dW[i]) hipLaunchKernelGGL(d_head_norm_dw_kernel, (int)((hs + 15) / 16), 1024, 0, m_stream, (size_t)rows[i], (int)hs, (const double*)gx, dW[i]->ptr, ll > 16 && pl[16] != 0 ? 1 : 0);
+        }
+        LAUNCHED();
+    }
+    return 0;
+}
+
+// PAGED_APPEND and ATTN_PAGED_FWD, arguments as in the float table
+long KernelD::paged(const double* pf, const MCH_LONGLONG* pl, bool append)
+{
+    const long long* l = (const long long*)pl;
+    if (!paged_sizes_ok(l) || (append && !(pf[0] >= 0.0))) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const long long B = l[0], N = l[1], H = l[2], KVH = l[3], hs = l[4], positions = l[6] * l[7], rowHeads = append ? H + 2 * KVH : H;
+    MemD* m[7];
+    for (int i = 0; i < 7; i++) ERRCHK(mem((long)pl[8 + i], &m[i]));
+    MemD *X = m[0], *K = m[1], *V = m[2], *out = m[6], *W[2] = {};
+    const long long count[7] = {N * rowHeads * hs, 0, 0, B * l[7], B + 1, B, N * H * hs};
+    for (int i = 0; i < 7; i++)
+        if (count[i]) RANGE(m[i], 0, count[i]);
+    const long long reach = paged_reach(l, (long long)std::min(K->count, V->count));
+    if (reach < 0) {
+        last_detail = "range exceeds the allocation behind the memory handle";
+        return MCH_ERROR_MEMORY_RANGE_EXCEEDED;
+    }
+    bool clash = d_overlap(out, count[6], K, reach) || d_overlap(out, count[6], V, reach);
+    for (int i = 0; i < 6; i++)
+        if (count[i]) clash = clash || d_overlap(out, count[6], m[i], count[i]) || (append && (d_overlap(K, reach, m[i], count[i]) || d_overlap(V, reach, m[i], count[i])));
+    double theta = 0.0;
+    if (append) {
+        if (!paged_apart(l, std::llabs(V->ptr - K->ptr), reach)) {
+            last_detail = "the strides of the pages let positions overlap";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+        for (int i = 0; i < 2; i++) {
+            if (!pl[20 + i]) continue;
+            ERRCHK(mem((long)pl[20 + i], &W[i]));
+            RANGE(W[i], 0, hs);
+            clash = clash || d_overlap(out, count[6], W[i], hs) || d_overlap(K, reach, W[i], hs) || d_overlap(V, reach, W[i], hs);
+        }
+        if (pl[18]) {
+            RopeD* r = m_rope.get((long)pl[18]);
+            if (!r || !r->set) return MCH_ERROR_ROPE_NOT_INITIALIZED;
+            if (r->hs != hs || r->seq < positions) {
+                last_detail = "the rope handle was created for another head size or for fewer positions";
+                return MCH_ERROR_PARAM_OUT_OF_RANGE;
+            }
+            theta = r->theta;
+        }
+    }
+    if (clash) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    const PagedD c = {K->ptr, V->ptr, m[3]->ptr, m[4]->ptr, m[5]->ptr, (int)B, (int)N, (int)H, (int)KVH, (int)hs, (int)l[5], (int)l[6], (int)l[7], l[15], l[16], l[17]};
+    const dim3 grid((unsigned)N, (unsigned)((rowHeads + 3) / 4));
+    if (append) hipLaunchKernelGGL(d_paged_append_kernel, grid, 256, 0, m_stream, c, (const double*)X->ptr, out->ptr, W[0] ? (const double*)W[0]->ptr : nullptr,
+                                   W[1] ? (const double*)W[1]->ptr : nullptr, (int)(pl[19] != 0), pf[0], theta);
+    else hipLaunchKernelGGL(d_paged_attn_kernel, grid, 256, 0, m_stream, c, (const double*)X->ptr, out->ptr, pf[0] != 0.0 ? pf[0] : 1.0 / sqrt((double)hs));
+    LAUNCHED();
+    return 0;
+}
 
 long KernelD::run(long fn, const double* pf, long lf, const MCH_LONGLONG* pl, long ll, double** ppOut, MCH_LONG* plOut)
 {
@@ -1948,7 +2235,7 @@ long KernelD::run(long fn, const double* pf, long lf, const MCH_LONGLONG* pl, lo
         long h;
         ERRCHK(m_rope.create(&h));
         RopeD* r = m_rope.get(h);
-        r->seq = (int)seq; r->heads = (int)heads; r->hs = (int)hs;
+        r->seq = (int)seq; r->heads = (int)heads; r->hs = (int)hs; r->theta = pf[0];
         const int half = (int)hs / 2;
         // the reference's host tables for T = double (rope.cu:535-553): the power and the cosines are single-precision
         // library calls on values held in double
@@ -2154,6 +2441,23 @@ long KernelD::run(long fn, const double* pf, long lf, const MCH_LONGLONG* pl, lo
                            r ? (const double*)r->dsin : nullptr, r ? r->seq : 1, true));
         return 0;
     }
+    case MCH_FN_QK_NORM_ROPE_FWD:
+        NEED_F(1, 1);
+        NEED_L(12, 12);
+        return head_norm(pf, pl, ll, false);
+    case MCH_FN_QK_NORM_ROPE_BWD:
+        NEED_F(1, 1);
+        NEED_L(16, 17);
+        return head_norm(pf, pl, ll, true);
+    case MCH_FN_PAGED_APPEND:
+        NEED_F(1, 1);
+        NEED_L(22, 22);
+        return paged(pf, pl, true);
+    case MCH_FN_ATTN_PAGED_FWD:
+        NEED_F(1, 1);
+        NEED_L(18, 19);
+        if (ll > 18 && pl[18] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        return paged(pf, pl, false);
     case MCH_FN_ATTN_DECODE_FWD: {
         // f{scale (0 = 1/sqrt(hs))}, l{batch, heads, kvHeads, hs, len, hQ, hKcache, hVcache, hY, strideKvBatch, strideKvHead,
         //   strideKvPos [, hRope, hKnew, hVnew]}

@@ -1,11 +1,14 @@
 // Sequences in a paged cache: which rows of a launch are whose, and where a position's keys and values lie.
 //
-// All of it comes in fp32 tensors, as every index of this ABI does (embedding ids, transposition counts): whole numbers, exact up
-// to 2^24, which the entry points hold every count to.  What the device reads is never trusted: every number is brought into
+// All of it comes in tensors of the base type, fp32 or double, as every index of this ABI does (embedding ids, transposition counts): whole numbers,
+// exact in fp32 up to 2^24, which the entry points hold every count to.  What the device reads is never trusted: every number is brought into
 // its range here before anything is addressed with it, and a number that is not a number counts as the lowest of its range or as
 // no page.  Host and device compile the same lines (the host's test feeds them everything that can go wrong).
 #pragma once
 #include <stdint.h>
+
+#include <algorithm>
+#include <utility>
 
 namespace mch {
 
@@ -18,19 +21,53 @@ namespace mch {
 constexpr int PAGED_EXACT = 1 << 24;   // whole numbers up to here are exact in fp32
 
 // v as a whole number in lo .. hi
-PAGED_FN int paged_int(float v, int lo, int hi) { return v >= (float)hi ? hi : v > (float)lo ? (int)v : lo; }
+template <typename T> PAGED_FN int paged_int(T v, int lo, int hi) { return v >= (T)hi ? hi : v > (T)lo ? (int)v : lo; }
 // an entry of a block table: a page, or -1
-PAGED_FN int paged_page(float v, int pages) { return v >= 0.f && v < (float)pages ? (int)v : -1; }
+template <typename T> PAGED_FN int paged_page(T v, int pages) { return v >= (T)0 && v < (T)pages ? (int)v : -1; }
 
 // New tokens of a sequence: rows first .. first + count - 1 of the launch, cached positions 0 .. len - 1 with the new ones last
 struct PagedSpan { int first, count, len; };
-PAGED_FN PagedSpan paged_span(float start, float next, float len, int tokens, int positions)
+template <typename T> PAGED_FN PagedSpan paged_span(T start, T next, T len, int tokens, int positions)
 {
     PagedSpan s;
     s.first = paged_int(start, 0, tokens);
     s.count = paged_int(next, s.first, tokens) - s.first;
     s.len = paged_int(len, 0, positions);
     return s;
+}
+
+// ---- what the entry points check, l as in the calls: {batch, tokens, heads, kvHeads, hs, pages, pageSize, maxPages, 7 handles, stridePage, strideHead, stridePos}
+inline bool paged_sizes_ok(const long long* l)
+{
+    for (int i = 0; i < 8; i++)
+        if (l[i] < 1 || l[i] > PAGED_EXACT) return false;
+    return l[2] <= 65535 && l[2] % l[3] == 0 && l[4] <= 256 && l[4] % 2 == 0 && l[6] * l[7] <= PAGED_EXACT && l[15] >= 0 && l[16] >= 0 && l[17] >= 0;
+}
+// values from the first of a cache to behind its last; -1: more than `most`
+inline long long paged_reach(const long long* l, long long most)
+{
+    const long long n[3] = {l[5], l[3], l[6]};
+    long long reach = l[4];
+    for (int i = 0; i < 3; i++) {
+        if (n[i] == 1) continue;
+        if (l[15 + i] > most) return -1;
+        reach += (n[i] - 1) * l[15 + i];
+    }
+    return reach <= most ? reach : -1;
+}
+// Whether every value of two caches, `apart` values from each other, has a place of its own: each stride reaches past what the smaller ones span, and so
+// does the distance where the two interleave (rows k | v, say)
+inline bool paged_apart(const long long* l, long long apart, long long reach)
+{
+    std::pair<long long, long long> dims[4] = {{l[15], l[5]}, {l[16], l[3]}, {l[17], l[6]}, {apart, apart < reach ? 2 : 1}};
+    std::sort(dims, dims + 4);
+    long long span = l[4];
+    for (const auto& d : dims) {
+        if (d.second == 1) continue;
+        if (d.first < span) return false;
+        span += (d.second - 1) * d.first;
+    }
+    return true;
 }
 
 }  // namespace mch

@@ -332,6 +332,56 @@ class SoftmaxLayer:
                                   top.gpu_diff, 0.0, self.hBottomDesc, bottom.gpu_diff)
 
 
+class PagedSequences:
+    """Which sequences are being served and which pages of a cache hold them (no counterpart in the reference, whose layer keeps one sequence of one
+    length).  One object serves all layers of a model: they keep pages of the same numbers.
+
+    ``Step({name: new tokens})`` before a model's pass: every named sequence grows by its tokens, in the order given, which is the order of the rows of
+    the pass; new names begin new sequences.  ``Drop(name, positions)`` gives up a sequence's oldest pages, ``End(name)`` all of them.
+    """
+
+    def __init__(self, cuda, pages, page_size, max_pages):
+        self.cuda, self.pages, self.page_size, self.max_pages = cuda, pages, page_size, max_pages
+        self._free = list(range(pages - 1, -1, -1))
+        self._table, self._len = {}, {}
+        self.table, self.starts, self.lens = (Blob(cuda) for _ in range(3))
+        self.batch = self.tokens = self.max_new = 0
+
+    def length(self, name):
+        return self._len.get(name, 0)
+
+    def Step(self, new):
+        need = {n: -(-(self.length(n) + k) // self.page_size) for n, k in new.items()}
+        if any(k < 1 for k in new.values()) or not new:
+            raise ValueError("a step has at least one token of every sequence it names")
+        if any(v > self.max_pages for v in need.values()):
+            raise ValueError("sequence longer than max_pages pages")
+        if sum(v - len(self._table.get(n, ())) for n, v in need.items()) > len(self._free):
+            raise MemoryError("no pages left: end or drop sequences first")
+        table = np.full((len(new), self.max_pages), -1, np.float32)
+        for i, (n, k) in enumerate(new.items()):
+            held = self._table.setdefault(n, [])
+            held += [self._free.pop() for _ in range(need[n] - len(held))]
+            self._len[n] = self.length(n) + k
+            table[i, :len(held)] = held
+        self.batch, self.tokens, self.max_new = len(new), sum(new.values()), max(new.values())
+        for blob, values in ((self.table, table), (self.starts, np.concatenate([[0], np.cumsum(list(new.values()))])), (self.lens, [self._len[n] for n in new])):
+            values = np.asarray(values, self.cuda.DTYPE)
+            blob.Reshape(*values.shape)
+            blob.mutable_cpu_data = values
+
+    def Drop(self, name, positions):
+        held = self._table[name]
+        for i in range(min(positions, self._len[name]) // self.page_size):
+            if held[i] >= 0:
+                self._free.append(held[i])
+                held[i] = -1
+
+    def End(self, name):
+        self._free += [p for p in self._table.pop(name) if p >= 0]
+        del self._len[name]
+
+
 class CausalSelfAttentionLayer:
     """MyCaffe.layers.gpt/layers.gpt/CausalSelfAttentionLayer.cs (setup :96-250, forward :526-628).
 
@@ -342,8 +392,11 @@ class CausalSelfAttentionLayer:
 
     def __init__(self, cuda, heads, embed, block_size, bias_term=True, enable_cuda_scaled_dot_product_attention=True,
                  enable_rotary_positional_embedding=False, rope_theta=10000.0, half=False, training=False,
-                 fused_qkv_heads=False):
+                 fused_qkv_heads=False, qk_norm=False):
         self.training = training
+        # RMS norms of the queries and keys of every head, in front of the rotation and in one pass with it
+        self.qk_norm, self.norm_eps = qk_norm, 1e-5
+        self.norms = []
         # inference with the fused attention handle as three calls: the handle writes its output head-merged
         self.fused_qkv_heads = fused_qkv_heads
         self.cuda, self.nHeads, self.nEmbed, self.nBlockSize = cuda, heads, embed, block_size
@@ -357,7 +410,7 @@ class CausalSelfAttentionLayer:
         self.transpose = TransposeLayer(cuda, (0, 2, 1, 3))
         self.transposeQ = TransposeLayer(cuda, (0, 1, 3, 2))
         self.softmax = SoftmaxLayer(cuda, -1)
-        names = "IpAttn Qt Kt Vt Kt1 AttA AttB Work Y".split()
+        names = "IpAttn Qt Kt Vt Kt1 AttA AttB Work Y".split() + (["Qraw", "Kraw"] if qk_norm else [])
         self.b = {n: Blob(cuda, half=half) for n in names}
         self.blobMask = Blob(cuda, (1, 1, block_size, block_size))
         mask = np.tril(np.ones((block_size, block_size), np.float32))  # fillMask :276-291
@@ -365,9 +418,14 @@ class CausalSelfAttentionLayer:
         self._masks, self._ropes = _Kept(Blob.Dispose), _Kept(cuda.FreeRope)
         self.hCudnn = self.hAttn = self.hRope = 0
         self._set_for = None
+        self._paged, self._page_rope = {}, None
 
-    def Setup(self, bottom, w_attn, b_attn, w_proj, b_proj):
+    def Setup(self, bottom, w_attn, b_attn, w_proj, b_proj, w_qnorm=None, w_knorm=None):
         self.c_attn.Setup(bottom, w_attn, b_attn)
+        if self.qk_norm:
+            self.norms = [Blob(self.cuda, (self.nSize,), self.half) for _ in range(2)]
+            for blob, w in zip(self.norms, (w_qnorm, w_knorm)):
+                blob.mutable_cpu_data = np.ones(self.nSize) if w is None else w
         y = Blob(self.cuda, bottom.shape_, self.half)
         self.c_proj.Setup(y, w_proj, b_proj)
         y.Dispose()
@@ -408,8 +466,15 @@ class CausalSelfAttentionLayer:
         for name in ("Qt", "Kt", "Vt"):
             b[name].Reshape(B, H, T, hs)
         w = self.c_attn.blobs
-        cuda.QkvProjHeads(B, T, H, hs, blobX.gpu_data, w[0].gpu_data, w[1].gpu_data if self.bias_term else 0, b["Qt"].gpu_data, b["Kt"].gpu_data,
-                          b["Vt"].gpu_data, self.hRope, self.c_attn.fp32_sums)
+        # with norms the rotation waits for them; a layer that trains keeps what they read
+        q, k = (b[n] for n in (("Qraw", "Kraw") if self.qk_norm and self.training else ("Qt", "Kt")))
+        q.Reshape(B, H, T, hs)
+        k.Reshape(B, H, T, hs)
+        cuda.QkvProjHeads(B, T, H, hs, blobX.gpu_data, w[0].gpu_data, w[1].gpu_data if self.bias_term else 0, q.gpu_data, k.gpu_data,
+                          b["Vt"].gpu_data, 0 if self.qk_norm else self.hRope, self.c_attn.fp32_sums)
+        if self.qk_norm:
+            cuda.QkNormRopeForward(B, T, H, H, hs, q.gpu_data, k.gpu_data, self.norms[0].gpu_data, self.norms[1].gpu_data, b["Qt"].gpu_data,
+                                   b["Kt"].gpu_data, self.hRope, self.norm_eps)
         if self.enable_sdpa:
             out = b["Work"]
             if self.fused_qkv_heads:
@@ -462,8 +527,39 @@ class CausalSelfAttentionLayer:
         # three transposes, two rotations and three channel copies (:700-740)
         ip = b["IpAttn"]
         ip.Reshape(B, T, 3 * C)
-        cuda.QkvHeadsGrad(B, T, H, hs, b["Qt"].gpu_diff, b["Kt"].gpu_diff, b["Vt"].gpu_diff, ip.gpu_diff, self.hRope)
+        if self.qk_norm:
+            cuda.QkNormRopeBackward(B, T, H, H, hs, b["Qraw"].gpu_data, b["Kraw"].gpu_data, self.norms[0].gpu_data, self.norms[1].gpu_data,
+                                    b["Qt"].gpu_diff, b["Kt"].gpu_diff, b["Qt"].gpu_diff, b["Kt"].gpu_diff, self.norms[0].gpu_diff,
+                                    self.norms[1].gpu_diff, self.hRope, self.norm_eps, True)
+        cuda.QkvHeadsGrad(B, T, H, hs, b["Qt"].gpu_diff, b["Kt"].gpu_diff, b["Vt"].gpu_diff, ip.gpu_diff, 0 if self.qk_norm else self.hRope)
         self.c_attn.Backward(ip, blobX)
+
+    def ForwardPaged(self, blobX, sequences, top):
+        """Inference of the new tokens of many sequences, (1, tokens, C) in the order of ``sequences.Step``, over their pages: projection, one call that
+        normalises, rotates and stores, attention, output projection."""
+        cuda, b, H, hs, seqs = self.cuda, self.b, self.nHeads, self.nSize, sequences
+        N, C = blobX.count(0, 2), self.nEmbed
+        if N != seqs.tokens:
+            raise ValueError("the pass has %d tokens, the step %d" % (N, seqs.tokens))
+        if id(seqs) not in self._paged:
+            # what a step does not write is never read; the sequences stay alive with their pages
+            self._paged[id(seqs)] = (seqs, Blob(cuda, (seqs.pages, H, seqs.page_size, hs), self.half), Blob(cuda, (seqs.pages, H, seqs.page_size, hs), self.half))
+        _, k, v = self._paged[id(seqs)]
+        positions = seqs.max_pages * seqs.page_size
+        if self.enable_rope and (self._page_rope is None or self._page_rope[0] < positions):
+            if self._page_rope is not None:
+                cuda.FreeRope(self._page_rope[1])
+            self._page_rope = (positions, cuda.CreateRope(0, 0, positions * C, 1, positions, H, hs, self.rope_theta))
+        self.c_attn.Forward(blobX, b["IpAttn"])
+        b["Qt"].Reshape(1, N, H, hs)
+        b["Y"].Reshape(1, N, C)
+        sizes = (seqs.batch, N, H, H, hs, seqs.pages, seqs.page_size, seqs.max_pages)
+        where = (k.gpu_data, v.gpu_data, seqs.table.gpu_data, seqs.starts.gpu_data, seqs.lens.gpu_data)
+        strides = (H * seqs.page_size * hs, seqs.page_size * hs, hs)
+        cuda.PagedAppend(*sizes, b["IpAttn"].gpu_data, b["Qt"].gpu_data, *where, *strides, self._page_rope[1] if self.enable_rope else 0, self.qk_norm,
+                         *([n.gpu_data for n in self.norms] or (0, 0)), self.norm_eps)
+        cuda.AttnPagedForward(*sizes, b["Qt"].gpu_data, *where, b["Y"].gpu_data, *strides, nMaxNew=seqs.max_new)
+        self.c_proj.Forward(b["Y"], top)
 
 
 class MultiheadAttentionLayer:
@@ -840,7 +936,7 @@ class TransformerBlockLayer:
     def __init__(self, cuda, heads, embed, block_size, activation="relu", bias_term=True, epsilon=1e-10,
                  enable_cuda_scaled_dot_product_attention=True, training=False, enable_llama_style_head=False, hidden_dim=0,
                  multiple_of=64, enable_layernorm_cuda_impl=True, fused_rmsnorm=None, block_type="causal_self_attention",
-                 enable_key_value_cache=False):
+                 enable_key_value_cache=False, qk_norm=False):
         if block_type not in ("causal_self_attention", "encoder"):
             raise ValueError(block_type)
         self.cuda = cuda
@@ -864,7 +960,7 @@ class TransformerBlockLayer:
                                                  enable_key_value_cache=enable_key_value_cache)
         else:
             self.attn1 = CausalSelfAttentionLayer(cuda, heads, embed, block_size, bias_term, enable_cuda_scaled_dot_product_attention,
-                                                  enable_rotary_positional_embedding=self.llama, training=training)
+                                                  enable_rotary_positional_embedding=self.llama, training=training, qk_norm=qk_norm)
         self.fc1 = InnerProductLayer(cuda, hidden_dim, bias_term, 2)
         self.fc2 = InnerProductLayer(cuda, hidden_dim, bias_term, 2) if self.llama else None
         self.proj = InnerProductLayer(cuda, embed, bias_term, 2)
@@ -881,11 +977,13 @@ class TransformerBlockLayer:
 
     def Setup(self, bottom, p):
         """``p``: attn_weight, attn_bias, attn_proj_weight, attn_proj_bias (ENCODER type: wq, bq, wk, bk, wv, bv, wo, bo),
-        fc_weight, fc_bias, proj_weight, proj_bias; Llama style also fc2_weight, rms1_weight, rms2_weight."""
+        fc_weight, fc_bias, proj_weight, proj_bias; Llama style also fc2_weight, rms1_weight, rms2_weight; with qk_norm attn_qnorm_weight,
+        attn_knorm_weight."""
         if self.block_type == "encoder":
             self.attn1.Setup(bottom, bottom, bottom, p)
         else:
-            self.attn1.Setup(bottom, p["attn_weight"], p.get("attn_bias"), p["attn_proj_weight"], p.get("attn_proj_bias"))
+            self.attn1.Setup(bottom, p["attn_weight"], p.get("attn_bias"), p["attn_proj_weight"], p.get("attn_proj_bias"), p.get("attn_qnorm_weight"),
+                             p.get("attn_knorm_weight"))
         self.fc1.Setup(bottom, p["fc_weight"], p.get("fc_bias"))
         if self.llama:
             self.fc2.Setup(bottom, p["fc2_weight"], p.get("fc2_bias"))

@@ -89,3 +89,31 @@ def test_a_single_fp32_row_goes_through_gemv_whatever_its_layout():
             cuda.calls.clear()
             forward()
             assert cuda.calls == want, (half, M, cuda.calls)
+
+
+def test_pages_are_handed_out_and_given_back():
+    from mycaffe_amd.layers import PagedSequences
+    import pytest
+    seqs = PagedSequences(Context(), 6, 4, 4)
+    seqs.Step({"a": 5, "b": 4})
+    assert (seqs.batch, seqs.tokens, seqs.max_new) == (2, 9, 5) and seqs.length("a") == 5
+    pages = {p for n in "ab" for p in seqs._table[n]}
+    assert len(pages) == 3 and len(seqs._free) == 3
+    seqs.Step({"b": 1})
+    seqs.Step({"a": 3})                       # fills its second page
+    assert len(seqs._free) == 2
+    with pytest.raises(ValueError):
+        seqs.Step({"a": 9})                   # five pages
+    with pytest.raises(ValueError):
+        seqs.Step({"a": 0})
+    with pytest.raises(MemoryError):
+        seqs.Step({"c": 12})
+    assert seqs.length("a") == 8 and seqs.length("c") == 0 and len(seqs._free) == 2     # a refused step changes nothing
+    seqs.Drop("a", 7)                         # one whole page
+    assert seqs._table["a"][0] == -1 and len(seqs._free) == 3
+    seqs.Drop("a", 7)
+    assert len(seqs._free) == 3
+    seqs.Step({"c": 12})
+    seqs.End("a")
+    seqs.End("b")
+    assert len(seqs._free) == 3 and seqs.length("a") == 0
