@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "attn_paged.h"
 #include "flash_traits.h"
 #include "kernels.h"
 #include "lane_ops.h"
@@ -16,13 +17,6 @@
 namespace mch {
 
 namespace {
-
-struct PagedAttnArgs {
-    PagedCache c;
-    const void* q;
-    void* y;
-    float c2;   // scale * log2(e)
-};
 
 template <typename T> __device__ __forceinline__ float value_of(T v);
 template <> __device__ __forceinline__ float value_of<float>(float v) { return v; }
@@ -155,29 +149,6 @@ template <typename T> __device__ __forceinline__ bool not_finite(u32x4 x)
         else r = r || (x[i] & 0x7f80u) == 0x7f80u || (x[i] & 0x7f800000u) == 0x7f800000u;
     }
     return r;
-}
-
-// over 256 threads: the sum of the numbers before the thread's own, and all of them
-__device__ __forceinline__ int block_scan(int v, int* sums, int* all)
-{
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = x;
-    __syncthreads();
-    int before = 0, sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        before += i < wave ? sums[i] : 0;
-        sum += sums[i];
-    }
-    *all = sum;
-    return before + x - v;
 }
 
 template <typename TQ, typename TC, int HSP>
@@ -589,33 +560,6 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
 // all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
 // follow each other by key head), whose L2 then holds that head's keys and values.  Where tiles are few their blocks are split among
 // workgroups and put together by a launch behind this one.
-struct ChunkArgs {
-    float* part;      // [split][tile][key head x head tile][128 {maximum, sum} | 128 rows of HSP]
-    int few;          // sequences of at most this many rows a key head are another kernel's
-    int shift, perTile, tileHeads, headTiles, splits;
-};
-
-// What workgroup `block` of a launch works on; b < 0: nothing
-struct ChunkTile { int b, tile, kh, ht; };
-__device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const ChunkArgs& w, unsigned block)
-{
-    __shared__ int sums[4], seq, tile;
-    const int groups = c.kvH * w.headTiles, want = block / groups, group = block - want * groups, tid = threadIdx.x;
-    if (tid == 0) { seq = -1; tile = 0; }
-    for (int b0 = 0, base = 0; b0 < c.batch && base <= want; b0 += 256) {
-        int tiles = 0, all;
-        if (b0 + tid < c.batch) {
-            const PagedSpan s = paged_span(c.starts[b0 + tid], c.starts[b0 + tid + 1], c.lens[b0 + tid], c.tokens, c.maxPages * c.pageSize);
-            if ((long long)s.count * (c.H / c.kvH) > w.few) tiles = (s.count + w.perTile - 1) / w.perTile;
-        }
-        const int at = base + block_scan(tiles, sums, &all);
-        if (at <= want && want < at + tiles) { seq = b0 + tid; tile = tiles - 1 - (want - at); }   // those that see most come first
-        base += all;
-    }
-    __syncthreads();
-    return ChunkTile{seq, tile, group / w.headTiles, group % w.headTiles};
-}
-
 // Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
 template <int PARTS> struct Parts { u32x4 p[PARTS]; };
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
@@ -659,11 +603,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
     const int G = c.H / c.kvH, positions = c.maxPages * c.pageSize;
     if (tid == 0) sBad = 0;
-    const ChunkTile at = chunk_tile(c, w, blockIdx.x);
+    if (w.redo && !w.redo[blockIdx.x / w.pair]) return;
+    const ChunkTile at = chunk_tile(c, w, blockIdx.x / w.pair);
     if (at.b < 0) return;
     const int b = at.b, kh = at.kh, ht = at.ht;
     const PagedSpan sp = paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions);
-    const int j0 = at.tile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
+    const int j0 = (at.tile * w.pair + (int)(blockIdx.x % w.pair)) * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
+    if (nt <= 0) return;
     const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads);
     const int end = min(sp.len, base + nt);                                                       // positions that some row sees
     const float* table = c.table + (size_t)b * c.maxPages;
@@ -1015,10 +961,14 @@ constexpr int FEW_ROWS = 16;
 // Workgroups a launch of the chunk kernel aims at.  Splitting tiles costs what their partial results take to write and read, which products in
 // fp32 are longer than by more (us, 512 | 1024: one chunk of 256 tokens over 8192, 16-bit, 79 | 93; 8 chunks of up to 1024, 12 heads of 64, 16-bit 43 | 48;
 // 2 prompts of 1024, 12 heads of 64, fp32 77 | 66; 12 chunks and single tokens of up to 1500 positions, fp32, 145 | 115).
+#ifndef V_PIPE
+#define V_PIPE 256
+#endif
+constexpr int PIPE_MIN = V_PIPE;
 constexpr int CHUNK_ROWS = 128, CHUNK_GRID_16 = 512, CHUNK_GRID_32 = 1024;
 
 // how a launch of the chunk kernel looks: what it takes from the host are the numbers of tokens and sequences alone
-struct ChunkPlan { int headTiles, tileHeads, perTile, tiles, splits; };
+struct ChunkPlan { int headTiles, tileHeads, perTile, tiles, splits, pipe; };   // pipe: workgroups of the pipe kernel, 0 without it
 static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
 {
     const int G = c.H / c.kvH;
@@ -1030,6 +980,14 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1));
     p.tiles = (int)(c.tokens / p.perTile + having);
     const long long groups = (long long)p.tiles * c.kvH * p.headTiles;
+    p.pipe = 0;
+    const long long pipe = (c.tokens / (2 * p.perTile) + having) * c.kvH * p.headTiles;
+    if (dt == BF16 && (c.hs == 64 || c.hs == 128) && (long long)c.tokens * G >= 256ll * c.batch && pipe >= PIPE_MIN && pipe < 0x3fffffff &&
+        ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll) {
+        p.pipe = (int)pipe;
+        p.splits = 1;
+        return p;
+    }
     p.splits = (int)std::max<long long>(1, std::min<long long>(16, (dt == F32 ? CHUNK_GRID_32 : CHUNK_GRID_16) / std::max<long long>(1, groups)));
     return p;
 }
@@ -1040,7 +998,7 @@ size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
     const ChunkPlan p = chunk_plan(c, dt);
     const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
     const size_t chunk = p.splits > 1 ? (size_t)p.splits * p.tiles * c.kvH * p.headTiles * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) : 0;
-    return std::max(split, chunk);
+    return std::max(split, std::max(chunk, (size_t)p.pipe * sizeof(int)));
 }
 size_t attn_paged_tickets() { return SPLIT_GRID; }
 
@@ -1067,8 +1025,12 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         if (in_pieces(c, dt, q, y) && units < 2e9) {
             if (chunks) {
                 const ChunkPlan p = chunk_plan(c, dt);
-                ChunkArgs g = {(float*)workspace, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits};
-                const long long blocks = (long long)c.kvH * p.headTiles * p.tiles;
+                ChunkArgs g = {(float*)workspace, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits, p.pipe ? 2 : 1, p.pipe ? (const int*)workspace : nullptr};
+                if (p.pipe) {
+                    const hipError_t e = attn_paged_pipe_launch(s, a, g, p.pipe, (int*)workspace);
+                    if (e != hipSuccess) return e;
+                }
+                const long long blocks = p.pipe ? 2ll * p.pipe : (long long)c.kvH * p.headTiles * p.tiles;
                 if (blocks > 0x7fffffff) return hipErrorInvalidValue;
                 const dim3 grid((unsigned)blocks, p.splits);
                 if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid, 256, 0, s, a, g);

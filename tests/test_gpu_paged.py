@@ -74,24 +74,28 @@ def attention(c, q, H, weights16, scale=None, out16=False):
     scale = hs ** -0.5 if scale is None else scale
     y, tol = np.full((c.tokens, H, hs), np.nan), np.full((c.tokens, H, hs), np.nan)
     at = 0
-    for (n, m, gone), (k, v) in zip(c.seqs, c.dense):
-        for j in range(n):
-            p = m - n + j
-            for h in range(H):
-                kk, vv = (x[gone:p + 1, h // G].astype(np.float64) for x in (k, v))
-                if p + 1 <= gone:
-                    y[at + j, h], tol[at + j, h] = 0, 0
-                    continue
-                qq = q[at + j, h].astype(np.float64)
-                s = scale * (kk @ qq)
-                e = np.exp(s - s.max())
-                w = e / e.sum()
-                y[at + j, h] = w @ vv
-                # scores: a dot product of hs terms, its scaling, the exponential's argument and the exponential
-                ds = (hs + 8) * U32 * (abs(scale) * (abs(kk) @ abs(qq))).max() + 4 * U32 * abs(s - s.max()).max() + 4 * U32
-                # weights each off by 2 ds (theirs and their sum's), rounded to 16 bits where the products are; sums of all of them
-                off = 2 * ds + (2 * U16 if weights16 else 0) + (len(w) + 8) * U32
-                tol[at + j, h] = off * (w @ abs(vv)) + (U16 if out16 else U32) * abs(y[at + j, h]) + 1e-30
+    for i, ((n, m, gone), (k, v)) in enumerate(zip(c.seqs, c.dense)):
+        there = np.arange(m) >= gone
+        for a, b in getattr(c, "holes", {}).get(i, ()):
+            there[a:b] = False
+        sees = there[None, :] & (np.arange(m)[None, :] <= np.arange(m - n, m)[:, None])
+        some = sees.any(1)
+        for h in range(H):
+            # what nobody sees may be anything
+            kk, vv = (np.where(there[:, None], x[:, h // G].astype(np.float64), 0) for x in (k, v))
+            qq = q[at:at + n, h].astype(np.float64)
+            s = np.where(sees, scale * (qq @ kk.T), -np.inf)
+            s = s - np.where(some, s.max(1, initial=-np.inf), 0)[:, None]
+            e = np.exp(s)
+            w = e / np.where(some, e.sum(1), 1)[:, None]
+            # scores: a dot product of hs terms, its scaling, the exponential's argument and the exponential
+            size = abs(scale) * (abs(qq) @ abs(kk).T)
+            ds = (hs + 8) * U32 * np.where(sees, size, 0).max(1, initial=0) + 4 * U32 * np.where(sees, abs(s), 0).max(1, initial=0) + 4 * U32
+            # weights each off by 2 ds (theirs and their sum's), rounded to 16 bits where the products are; sums of all of them
+            off = 2 * ds + (2 * U16 if weights16 else 0) + (sees.sum(1) + 8) * U32
+            y[at:at + n, h] = w @ vv
+            tol[at:at + n, h] = off[:, None] * (w @ abs(vv)) + (U16 if out16 else U32) * abs(y[at:at + n, h]) + 1e-30
+            tol[at:at + n, h][~some] = 0
         at += n
     return y, tol
 
@@ -268,6 +272,67 @@ def test_values_far_from_one(dev, act16, cache16, size):
         vv = v[:m - n + j + 1, 0].astype(np.float64)
         tol = ((len(vv) + 12) * U32 + (2 * U16 if act16 else 0)) * abs(vv).mean(0) + (U16 if act16 else U32) * abs(vv.mean(0))
         assert (abs(got[j, 0] - vv.mean(0)) <= tol).all()
+
+
+# Long chunks in 16-bit storage, enough tiles of 256 rows for the chip: heads and new tokens by the hundred
+LONG = [
+    # name, H, kvH, hs, page, order, [(new, positions, dropped)], padding rows
+    ("prompt", 128, 128, 64, 16, "head", [(300, 300, 0)], 3),
+    ("chunk_of_four_heads", 512, 128, 64, 32, "pos", [(70, 401, 0)], 0),
+    ("wide_two_sequences", 128, 64, 128, 16, "head", [(260, 517, 0), (140, 140, 0)], 0),
+    ("groups_of_seven", 448, 64, 128, 8, "pos", [(80, 300, 0), (37, 40, 0)], 1),
+    ("dropped", 128, 128, 64, 24, "head", [(270, 700, 168)], 0),
+    ("dropped_into_the_chunk", 128, 128, 64, 16, "head", [(300, 400, 160)], 0),
+    ("single_tokens_beside", 256, 64, 128, 16, "head", [(200, 500, 0), (1, 900, 0), (3, 70, 0), (0, 5, 0), (150, 160, 0)], 2),
+    ("more_new_than_positions", 128, 128, 64, 16, "head", [(300, 270, 0)], 0),
+    ("a_page_to_a_tile", 128, 64, 128, 128, "pos", [(320, 1000, 0)], 0),
+]
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 6.0])
+@pytest.mark.parametrize("name,H,kvH,hs,page,order,seqs,pad", LONG, ids=[s[0] for s in LONG])
+def test_long_chunks(dev, name, H, kvH, hs, page, order, seqs, pad, scale):
+    rng = np.random.default_rng(hs + len(name))
+    check_attention(dev, rng, Cache(dev, rng, seqs, kvH, hs, page, order, True, pad=pad), H, True, scale=scale)
+
+
+@pytest.mark.parametrize("act16,cache16", TYPES)
+def test_holes(dev, act16, cache16):
+    """Pages given up in the middle of sequences: the first page and a window kept, say."""
+    for H, kvH, hs, seqs in ((128, 128, 64, [(300, 700, 0)]), (4, 2, 64, [(40, 200, 0), (1, 300, 0), (2, 130, 0)])):
+        rng = np.random.default_rng(17)
+        c = Cache(dev, rng, seqs, kvH, hs, 16, "head", cache16)
+        c.holes = {}
+        for b, (n, m, _) in enumerate(seqs):
+            c.holes[b] = [(16, 16 * ((m - n) // 32))]
+            c.table[b, 1:(m - n) // 32] = -1
+        c.h["table"] = dev.put(c.table)
+        check_attention(dev, rng, c, H, act16)
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("where", ["k", "v", "q"])
+def test_long_chunks_with_values_that_are_not_finite(dev, where, bad):
+    rng = np.random.default_rng(18)
+    H, kvH, hs, n, m, at = 128, 128, 64, 280, 340, 250
+    c = Cache(dev, rng, [(n, m, 0)], kvH, hs, 16, "head", True)
+    q = rounded(rng.standard_normal((n, H, hs)), True)
+    want, tol = attention(c, q, H, True, None, True)
+    if where == "q":
+        q[at, :, 5] = bad
+        rows, touched = np.arange(n) != at, np.arange(n) == at
+    else:
+        a = c.k if where == "k" else c.v
+        a[int(c.table[0, (m - n + at) // 16]), :, (m - n + at) % 16, 5] = bad
+        c.h[where] = dev.put(c.laid(a), True)
+        rows = np.arange(n) < at
+        touched = ~rows
+    hq, hy = dev.put(q, True), dev.zeros(q.size, True)
+    c.attend(hq, hy, H)
+    got = dev.get(hy, q.shape)
+    assert (abs(got - want)[rows] <= tol[rows]).all()
+    if where != "k":      # (a key's infinity may be a weight of zero)
+        assert not np.isfinite(got[touched]).all(axis=2).any()
 
 
 @pytest.mark.parametrize("act16,cache16", TYPES)
