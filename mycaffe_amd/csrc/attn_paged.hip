@@ -590,7 +590,10 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 {
     typedef FlashTraits<bf16_t> TR;
     constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;                     // parts of a query and a weight, of a key and a value
-    constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    #ifndef V_KB
+#define V_KB (NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32)
+#endif
+    constexpr int KB = V_KB, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
     constexpr int LD = HSP + 8;                                                                   // values a row in LDS
     constexpr int PART = 128 * (HSP + 2);
@@ -961,10 +964,10 @@ constexpr int FEW_ROWS = 16;
 // Workgroups a launch of the chunk kernel aims at.  Splitting tiles costs what their partial results take to write and read, which products in
 // fp32 are longer than by more (us, 512 | 1024: one chunk of 256 tokens over 8192, 16-bit, 79 | 93; 8 chunks of up to 1024, 12 heads of 64, 16-bit 43 | 48;
 // 2 prompts of 1024, 12 heads of 64, fp32 77 | 66; 12 chunks and single tokens of up to 1500 positions, fp32, 145 | 115).
-#ifndef V_PIPE
-#define V_PIPE 256
-#endif
-constexpr int PIPE_MIN = V_PIPE;
+// Whole tiles of 256 rows from which on the pipe kernel takes a launch (it does not split them): half as many as CUs at head size 128, a workgroup
+// a CU, three quarters at 64, two a CU.  us, chunk kernel | pipe: heads of 128, 64 tiles 210 | 401, 128 225 | 217, 256 300 | 251; heads of 64, 128 160 | 163,
+// 168 39 | 45, 192 108 | 93 and 194 | 166, 384 54 | 47.
+constexpr int PIPE_TILES_128 = 128, PIPE_TILES_64 = 192;
 constexpr int CHUNK_ROWS = 128, CHUNK_GRID_16 = 512, CHUNK_GRID_32 = 1024;
 
 // how a launch of the chunk kernel looks: what it takes from the host are the numbers of tokens and sequences alone
@@ -981,8 +984,8 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     p.tiles = (int)(c.tokens / p.perTile + having);
     const long long groups = (long long)p.tiles * c.kvH * p.headTiles;
     p.pipe = 0;
-    const long long pipe = (c.tokens / (2 * p.perTile) + having) * c.kvH * p.headTiles;
-    if (dt == BF16 && (c.hs == 64 || c.hs == 128) && (long long)c.tokens * G >= 256ll * c.batch && pipe >= PIPE_MIN && pipe < 0x3fffffff &&
+    const long long whole = (long long)c.tokens / (2 * p.perTile) * c.kvH * p.headTiles, pipe = whole + having * c.kvH * p.headTiles;
+    if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 0x3fffffff &&
         ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll) {
         p.pipe = (int)pipe;
         p.splits = 1;
