@@ -12,13 +12,26 @@ struct PagedAttnArgs {
     float c2;   // scale * log2(e)
 };
 
+// place and last place of a tile's pieces (place -1: none), its first token and head, tokens, heads
+struct ChunkJoin { int place, to, token, head, tokens, heads, pad[2]; };
+
 struct ChunkArgs {
-    float* part;      // [split][tile][key head x head tile][128 {maximum, sum} | 128 rows of HSP]
+    float* part;      // partial results, [place in the list][2][128 {maximum, sum} | 128 rows of HSP]
+    ChunkJoin* join;   // of every workgroup: the tile that it began and left to the next ones
     int few;          // sequences of at most this many rows a key head are another kernel's
-    int shift, perTile, tileHeads, headTiles, splits;
+    int shift, perTile, tileHeads, headTiles;
+    int unit;         // shift of paged_units_before
     int pair;         // tiles of perTile tokens that a workgroup's tile stands for (the pipe kernel's are two of the chunk kernel's)
     const int* redo;  // chunk kernel: not null, workgroups 2 i and 2 i + 1 do what the pipe kernel's workgroup i left, if redo[i]
 };
+
+// what all lanes of a wavefront have alike, in scalar registers
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ PagedSpan uniform(const PagedSpan& s) { return PagedSpan{uniform(s.first), uniform(s.count), uniform(s.len)}; }
+__device__ __forceinline__ PagedSpan span_at(const PagedCache& c, int b)
+{
+    return uniform(paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize));
+}
 
 // over 256 threads: the sum of the numbers before the thread's own, and all of them
 __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
@@ -43,7 +56,58 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
     return before + x - v;
 }
 
-// What workgroup `block` of a launch works on; b < 0: nothing
+// The chunk kernel's list: sequences, their key heads and head tiles, their tiles, in units of about 32 positions of a tile.  All 256 threads.
+// Units a workgroup has at least: what a piece costs beside its blocks (its places, queries and partial results) is some of them.  us with 8 | 16 | 32: 2 prompts of 1024,
+// 12 heads of 64, fp32 50 | 63 | 99; 4 sequences of 8 new tokens over 4096, 32 heads of 128, 16-bit 37 | 38 | 50.
+constexpr int CHUNK_LEAST = 8;
+__device__ __forceinline__ int chunk_tiles(const PagedCache& c, const ChunkArgs& w, const PagedSpan& s)
+{
+    return (long long)s.count * (c.H / c.kvH) > w.few ? (s.count + w.perTile - 1) / w.perTile : 0;
+}
+__device__ __forceinline__ int chunk_work(const PagedCache& c, const ChunkArgs& w, const PagedSpan& s)   // of one key head and head tile
+{
+    return paged_units_before(max(s.len - s.count, 0), w.perTile, chunk_tiles(c, w, s), w.unit);
+}
+// the total, and where unit `begin(place)` of its runs is: sequence, its span, and the unit within it; place -1: nothing
+struct ChunkStart { int total, place, b, local; PagedSpan sp; };
+__device__ __forceinline__ ChunkStart chunk_start(const PagedCache& c, const ChunkArgs& w, int block, int most)
+{
+    __shared__ int sums[4], seq, first;
+    __shared__ PagedSpan span;
+    const int groups = c.kvH * w.headTiles, tid = threadIdx.x;
+    auto span_of = [&](int b) {
+        return b < c.batch ? paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize) : PagedSpan{0, 0, 0};
+    };
+    ChunkStart r = {};
+    PagedSpan mine = span_of(tid);
+    int work = chunk_work(c, w, mine) * groups, at = block_scan(work, sums, &r.total), all = r.total;
+    for (int b0 = 256; b0 < c.batch; b0 += 256) {
+        int more;
+        block_scan(chunk_work(c, w, span_of(b0 + tid)) * groups, sums, &more);
+        r.total += more;
+    }
+    r.total = uniform(r.total);
+    const PagedRuns runs(r.total, most, CHUNK_LEAST);
+    r.place = paged_place(block, runs.W);
+    if (r.place < 0) return r;
+    const int lo = runs.begin(r.place);
+    for (int b0 = 0, base = 0;;) {
+        if (at <= lo && lo < at + work) { seq = b0 + tid; first = at; span = mine; }
+        base += all;
+        if (lo < base) break;
+        if ((b0 += 256) >= c.batch) { r.place = -1; return r; }
+        mine = span_of(b0 + tid);
+        work = chunk_work(c, w, mine) * groups;
+        at = base + block_scan(work, sums, &all);
+    }
+    __syncthreads();
+    r.b = uniform(seq);
+    r.local = uniform(lo - first);
+    r.sp = uniform(span);
+    return r;
+}
+
+// What workgroup `block` of the pipe kernel works on; b < 0: nothing
 struct ChunkTile { int b, tile, kh, ht; };
 __device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const ChunkArgs& w, unsigned block)
 {
@@ -61,7 +125,7 @@ __device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const Chunk
         base += all;
     }
     __syncthreads();
-    return ChunkTile{seq, tile, group / w.headTiles, group % w.headTiles};
+    return ChunkTile{uniform(seq), uniform(tile), group / w.headTiles, group % w.headTiles};
 }
 
 // Chunks in 16-bit storage, head size 64 or 128, in tiles of 256 rows (w.pair 2); flags[i]: the tile of workgroup i is left to the chunk kernel

@@ -187,12 +187,10 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
         block_scan(b0 + tid < c.batch ? work_of(span_of(b0 + tid)) : 0, sScan, &all);
         total += all;
     }
-    // equal runs, the first `more` of them longer by one
-    const int W = min(total, (int)gridDim.x), run = total / max(W, 1), more = total - run * W;
-    if ((int)blockIdx.x >= W) return;
-    auto begin_of = [&](int i) { return run * i + min(i, more); };
-    auto run_of = [&](int u) { return u < (run + 1) * more ? u / (run + 1) : more + (u - (run + 1) * more) / run; };
-    const int lo = begin_of(blockIdx.x), hi = begin_of(blockIdx.x + 1);
+    total = uniform(total);
+    const PagedRuns runs(total, gridDim.x, 1);
+    if ((int)blockIdx.x >= runs.W) return;
+    const int lo = runs.begin(blockIdx.x), hi = runs.begin(blockIdx.x + 1);
     // the sequence that has unit `lo`
     for (int b0 = 0, base = 0, all = total256;;) {
         if (at <= lo && lo < at + work) { sSeq = b0 + tid; sAt = at; sSpan = mine; }
@@ -204,8 +202,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
         at = base + block_scan(work, sScan, &all);
     }
     __syncthreads();
-    int b = sSeq, local = lo - sAt;
-    PagedSpan sp = sSpan;
+    int b = uniform(sSeq), local = uniform(lo - sAt);
+    PagedSpan sp = uniform(sSpan);
 
     const TC *kp = (const TC*)c.k, *vp = (const TC*)c.v;
     for (int u = lo; u < hi;) {
@@ -499,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
         if (!whole) {
             // Who comes last puts the item together; its workgroups follow from the list alone.  Partial results go to the level that all XCDs
             // share, and are there before the ticket is taken.
-            const int wf = run_of(u - unit0), we = run_of(u - unit0 + units - 1);
+            const int wf = runs.of(u - unit0), we = runs.of(u - unit0 + units - 1);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (tid == 0) sTicket = __hip_atomic_fetch_add(w.tickets + wf, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -547,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                 local = 0;
                 do {
                     if (++b >= c.batch) return;
-                    sp = span_of(b);
+                    sp = span_at(c, b);
                 } while (tiles_of(sp) == 0);
             }
             __syncthreads();                                                     // LDS is read no more
@@ -558,8 +556,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
 // ---- chunks: rows by the hundred ----------------------------------------------------------------------------------------------------
 // A workgroup has 128 rows of one key head (tokens times the heads that share it), 32 a wavefront, and stages blocks of KB keys and values in LDS for
 // all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
-// follow each other by key head), whose L2 then holds that head's keys and values.  Where tiles are few their blocks are split among
-// workgroups and put together by a launch behind this one.
+// follow each other by key head), whose L2 then holds that head's keys and values.  The
+// blocks of all tiles are one list that is dealt to the workgroups in equal runs; tiles that a run ends in are put together by a launch behind this one.
 // Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
 template <int PARTS> struct Parts { u32x4 p[PARTS]; };
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
@@ -590,10 +588,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 {
     typedef FlashTraits<bf16_t> TR;
     constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;                     // parts of a query and a weight, of a key and a value
-    #ifndef V_KB
-#define V_KB (NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32)
-#endif
-    constexpr int KB = V_KB, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
     constexpr int LD = HSP + 8;                                                                   // values a row in LDS
     constexpr int PART = 128 * (HSP + 2);
@@ -604,15 +599,47 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
 
     const PagedCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
-    const int G = c.H / c.kvH, positions = c.maxPages * c.pageSize;
+    const int G = c.H / c.kvH;
+    const int groups = c.kvH * w.headTiles;
+    ChunkStart at = {};
+    ChunkTile left = {};
+    int u = 0, hi = 1;
+    if (w.redo) {
+        if (!w.redo[blockIdx.x / w.pair]) return;
+        left = chunk_tile(c, w, blockIdx.x / w.pair);
+        if (left.b < 0) return;
+        at.b = left.b;
+        at.sp = span_at(c, at.b);
+    } else {
+        at = chunk_start(c, w, blockIdx.x, gridDim.x);
+        if (tid == 0) w.join[blockIdx.x].place = -1;
+        if (at.place < 0) return;
+        const PagedRuns runs(at.total, gridDim.x, CHUNK_LEAST);
+        u = runs.begin(at.place);
+        hi = runs.begin(at.place + 1);
+    }
+    while (u < hi) {
+    // ---- the tile and the piece of it that is this workgroup's: units u0 .. u1 - 1 of `units` ----
+    const PagedSpan sp = at.sp;
+    const int b = at.b, before = max(sp.len - sp.count, 0);
+    int group, tile, u0 = 0, u1 = 1, units = 1;
+    if (w.redo) {
+        group = left.kh * w.headTiles + left.ht;
+        tile = left.tile * w.pair + (int)(blockIdx.x % w.pair);
+    } else {
+        const int tiles = chunk_tiles(c, w, sp), each = paged_units_before(before, w.perTile, tiles, w.unit), r = at.local - at.local / each * each;
+        group = at.local / each;
+        tile = paged_tile_of(before, w.perTile, tiles, w.unit, r);
+        const int start = paged_units_before(before, w.perTile, tile, w.unit);
+        units = paged_units_before(before, w.perTile, tile + 1, w.unit) - start;
+        u0 = r - start;
+        u1 = min(units, u0 + hi - u);
+    }
+    const bool whole = u0 == 0 && u1 == units;
+    const int kh = group / w.headTiles, ht = group - kh * w.headTiles;
+    const int j0 = tile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
+    if (nt <= 0) return;   // (redo: the second half of a tile that has none)
     if (tid == 0) sBad = 0;
-    if (w.redo && !w.redo[blockIdx.x / w.pair]) return;
-    const ChunkTile at = chunk_tile(c, w, blockIdx.x / w.pair);
-    if (at.b < 0) return;
-    const int b = at.b, kh = at.kh, ht = at.ht;
-    const PagedSpan sp = paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions);
-    const int j0 = (at.tile * w.pair + (int)(blockIdx.x % w.pair)) * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
-    if (nt <= 0) return;
     const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads);
     const int end = min(sp.len, base + nt);                                                       // positions that some row sees
     const float* table = c.table + (size_t)b * c.maxPages;
@@ -622,20 +649,6 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
         const int page = p < end ? paged_page(e, c.pages) : -1;
         return page >= 0 ? page * c.sP + (w.shift >= 0 ? p & (c.pageSize - 1) : p % c.pageSize) * c.sT : -1;
     };
-    // pages given up at the front are passed over
-    if (wave == 0) {
-        int front = 0;
-        const int entries = end > 0 ? (end - 1) / c.pageSize + 1 : 0;
-        for (; front < entries; front += 64) {
-            const uint64_t some = __ballot(front + lane < entries && paged_page(table[min(front + lane, entries - 1)], c.pages) >= 0);
-            if (some) { front += __ffsll((unsigned long long)some) - 1; break; }
-        }
-        if (lane == 0) sFront = min(front, entries) * c.pageSize;
-    }
-    __syncthreads();
-    const int kb0 = min(sFront, max(end, 0)) / KB, nkb = (max(end, 0) + KB - 1) / KB;
-    const int first = kb0 + (int)((long long)(nkb - kb0) * blockIdx.y / w.splits), stop = kb0 + (int)((long long)(nkb - kb0) * (blockIdx.y + 1) / w.splits);
-
     const float c2 = fabsf(a.c2);
 
     // ---- the lane's row ----
@@ -677,6 +690,20 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
             }
         }
     }
+    // pages given up at the front are passed over
+    if (wave == 0) {
+        int front = 0;
+        const int entries = end > 0 ? (end - 1) / c.pageSize + 1 : 0;
+        for (; front < entries; front += 64) {
+            const uint64_t some = __ballot(front + lane < entries && paged_page(table[min(front + lane, entries - 1)], c.pages) >= 0);
+            if (some) { front += __ffsll((unsigned long long)some) - 1; break; }
+        }
+        if (lane == 0) sFront = min(front, entries) * c.pageSize;
+    }
+    __syncthreads();
+    const int kb0 = min(uniform(sFront), max(end, 0)) / KB, nkb = (max(end, 0) + KB - 1) / KB;
+    const int first = kb0 + (int)((long long)(nkb - kb0) * u0 / units), stop = kb0 + (int)((long long)(nkb - kb0) * u1 / units);
+
     floatx16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; i++)
@@ -841,13 +868,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     if (__any(bad) && lane == 0) sBad = 1;
     __syncthreads();
 
-    const size_t place = blockIdx.x, part0 = gridDim.x;
-    float* part = w.part + (blockIdx.y * part0 + place) * PART;
+    float* part = w.part + ((size_t)at.place * 2 + (u0 == 0 ? 1 : 0)) * PART;
     if (!sBad) {
         if (live) {
             TQ* y = (TQ*)a.y + row_at(token, head);
             const float inv = 1.f / l;
-            if (w.splits > 1 && half == 0) *(float2*)(part + 2 * row) = make_float2(m, l);
+            if (!whole && half == 0) *(float2*)(part + 2 * row) = make_float2(m, l);
 #pragma unroll
             for (int i = 0; i < DT; i++)
 #pragma unroll
@@ -855,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                     const int d = 32 * i + 8 * v + 4 * half;
                     if (d >= c.hs) continue;
                     float x[4] = {o[i][4 * v], o[i][4 * v + 1], o[i][4 * v + 2], o[i][4 * v + 3]};
-                    if (w.splits > 1) *(float4*)(part + 256 + row * HSP + d) = make_float4(x[0], x[1], x[2], x[3]);
+                    if (!whole) *(float4*)(part + 256 + row * HSP + d) = make_float4(x[0], x[1], x[2], x[3]);
                     else {
 #pragma unroll
                         for (int e = 0; e < 4; e++) x[e] = m > -INFINITY ? x[e] * inv : 0.f;
@@ -891,54 +917,87 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                 for (int i = 0; i < 2; i++) acc[i] = acc[i] * f + wt * val[i];
             }
             if (2 * lane < c.hs) {
-                if (w.splits > 1) *(float2*)(part + 256 + r * HSP + 2 * lane) = make_float2(acc[0], acc[1]);
+                if (!whole) *(float2*)(part + 256 + r * HSP + 2 * lane) = make_float2(acc[0], acc[1]);
                 else {
                     TQ* y = (TQ*)a.y + row_at(tk, hd) + 2 * lane;
                     y[0] = stored<TQ>(mr > -INFINITY ? acc[0] / lr : 0.f);
                     y[1] = stored<TQ>(mr > -INFINITY ? acc[1] / lr : 0.f);
                 }
             }
-            if (w.splits > 1 && lane == 0) *(float2*)(part + 2 * r) = make_float2(mr, lr);
+            if (!whole && lane == 0) *(float2*)(part + 2 * r) = make_float2(mr, lr);
         }
+    }
+    if (u0 == 0 && !whole && tid == 0) {
+        const PagedRuns runs(at.total, gridDim.x, CHUNK_LEAST);
+        w.join[blockIdx.x] = ChunkJoin{at.place, runs.of(u + units - 1), sp.first + j0, h0, nt, nh, {0, 0}};
+    }
+    // ---- the next piece ----
+    const int done = u1 - u0;
+    u += done;
+    at.local += done;
+    if (u < hi) {
+        if (at.local == chunk_work(c, w, sp) * groups) {
+            at.local = 0;
+            do {
+                if (++at.b >= c.batch) return;
+                at.sp = span_at(c, at.b);
+            } while (chunk_tiles(c, w, at.sp) == 0);
+        }
+        __syncthreads();   // LDS is read no more
+    }
     }
 }
 
-// The splits of a tile put together, 32 rows a workgroup, eight lanes a row.  A launch of its own: a tile has up to 64 KB a split, which one workgroup
-// takes longer to collect (its last one, 7 splits of 128 rows of 128: 100 us) than all of them to start anew.
+// Tiles that a run ended in put together, 16 rows a workgroup, 16 lanes a row, from what the workgroup that began one has written down.
+// A launch of its own: a tile has up to 64 KB a piece, which one workgroup takes longer to collect (7 pieces of 128 rows of 128: 100 us) than
+// all of them to start anew.
 template <typename TQ, int HSP>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttnArgs a, ChunkArgs w)
 {
-    constexpr int PART = 128 * (HSP + 2), N = HSP / 32;
+    constexpr int PART = 128 * (HSP + 2), LANES = 16, N = HSP / (4 * LANES);
     const PagedCache& c = a.c;
-    const ChunkTile at = chunk_tile(c, w, blockIdx.x);
-    if (at.b < 0) return;
-    const PagedSpan sp = paged_span(c.starts[at.b], c.starts[at.b + 1], c.lens[at.b], c.tokens, c.maxPages * c.pageSize);
-    const int G = c.H / c.kvH, j0 = at.tile * w.perTile, nt = min(w.perTile, sp.count - j0), nh = min(w.tileHeads, G - at.ht * w.tileHeads);
-    const int row = blockIdx.y * 32 + (threadIdx.x >> 3), token = row / w.tileHeads, head = row - token * w.tileHeads;
-    if (token >= nt || head >= nh) return;
-    const float* part = w.part + (size_t)blockIdx.x * PART;
-    const size_t split = (size_t)gridDim.x * PART;
+    const ChunkJoin t = w.join[blockIdx.x];
+    const int row = blockIdx.y * 16 + threadIdx.x / LANES, token = row / w.tileHeads, head = row - token * w.tileHeads;
+    if (t.place < 0 || token >= t.tokens || head >= t.heads) return;
+    // piece z of the tile; eight of them in flight, past the last one that again with no weight
+    auto part_of = [&](int z) { return w.part + ((size_t)min(z, t.to) * 2 + (z == t.place ? 1 : 0)) * PART; };
     float M = -INFINITY, L = 0.f;
-    for (int z = 0; z < w.splits; z++) M = fmaxf(M, part[z * split + 2 * row]);
     float4 x[N];
 #pragma unroll
     for (int i = 0; i < N; i++) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int z = 0; z < w.splits; z++) {
-        const float* from = part + z * split;
-        const float f = weight_of(from[2 * row], M);
-        L += from[2 * row + 1] * f;
+    constexpr int DEEP = 8;
+    for (int z0 = t.place; z0 <= t.to; z0 += DEEP) {
+        float2 ml[DEEP];
+        float4 v[DEEP][N];
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const float4 v = *(const float4*)(from + 256 + row * HSP + 32 * i + 4 * (threadIdx.x & 7));
-            x[i].x += v.x * f; x[i].y += v.y * f; x[i].z += v.z * f; x[i].w += v.w * f;
+        for (int j = 0; j < DEEP; j++) {
+            const float* from = part_of(z0 + j);
+            ml[j] = *(const float2*)(from + 2 * row);
+#pragma unroll
+            for (int i = 0; i < N; i++) v[j][i] = *(const float4*)(from + 256 + row * HSP + 4 * LANES * i + 4 * (threadIdx.x % LANES));
         }
+        float Mn = M;
+#pragma unroll
+        for (int j = 0; j < DEEP; j++) Mn = z0 + j <= t.to ? fmaxf(Mn, ml[j].x) : Mn;
+        const float f0 = weight_of(M, Mn);
+        L *= f0;
+#pragma unroll
+        for (int i = 0; i < N; i++) { x[i].x *= f0; x[i].y *= f0; x[i].z *= f0; x[i].w *= f0; }
+#pragma unroll
+        for (int j = 0; j < DEEP; j++) {
+            if (z0 + j > t.to) break;
+            const float f = weight_of(ml[j].x, Mn);
+            L += ml[j].y * f;
+#pragma unroll
+            for (int i = 0; i < N; i++) { x[i].x += v[j][i].x * f; x[i].y += v[j][i].y * f; x[i].z += v[j][i].z * f; x[i].w += v[j][i].w * f; }
+        }
+        M = Mn;
     }
-    TQ* y = (TQ*)a.y + ((size_t)(sp.first + j0 + token) * c.H + at.kh * G + at.ht * w.tileHeads + head) * c.hs;
+    TQ* y = (TQ*)a.y + ((size_t)(t.token + token) * c.H + t.head + head) * c.hs;
     const float inv = 1.f / L;
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int d = 32 * i + 4 * (threadIdx.x & 7);
+        const int d = 4 * LANES * i + 4 * (threadIdx.x % LANES);
         if (d >= c.hs) continue;
         if (M == -INFINITY) x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         else { x[i].x *= inv; x[i].y *= inv; x[i].z *= inv; x[i].w *= inv; }
@@ -961,17 +1020,14 @@ inline bool in_pieces(const PagedCache& c, DType dt, const void* q, const void* 
 // Rows of a key head up to which a sequence's positions are what is split, beyond which its rows are: one 16-row tile.  Two of them read the cache
 // twice (us, two kernels, 32 heads on 8 key heads of 128, 4096 positions, 16-bit storage: 4 sequences of 8 new tokens, 32 rows, 41 | 36; 8 of 16, 64 rows, 84 | 61).
 constexpr int FEW_ROWS = 16;
-// Workgroups a launch of the chunk kernel aims at.  Splitting tiles costs what their partial results take to write and read, which products in
-// fp32 are longer than by more (us, 512 | 1024: one chunk of 256 tokens over 8192, 16-bit, 79 | 93; 8 chunks of up to 1024, 12 heads of 64, 16-bit 43 | 48;
-// 2 prompts of 1024, 12 heads of 64, fp32 77 | 66; 12 chunks and single tokens of up to 1500 positions, fp32, 145 | 115).
 // Whole tiles of 256 rows from which on the pipe kernel takes a launch (it does not split them): half as many as CUs at head size 128, a workgroup
 // a CU, three quarters at 64, two a CU.  us, chunk kernel | pipe: heads of 128, 64 tiles 210 | 401, 128 225 | 217, 256 300 | 251; heads of 64, 128 160 | 163,
 // 168 39 | 45, 192 108 | 93 and 194 | 166, 384 54 | 47.
 constexpr int PIPE_TILES_128 = 128, PIPE_TILES_64 = 192;
-constexpr int CHUNK_ROWS = 128, CHUNK_GRID_16 = 512, CHUNK_GRID_32 = 1024;
+constexpr int CHUNK_ROWS = 128, CHUNK_GRID = 512;   // two workgroups a CU
 
-// how a launch of the chunk kernel looks: what it takes from the host are the numbers of tokens and sequences alone
-struct ChunkPlan { int headTiles, tileHeads, perTile, tiles, splits, pipe; };   // pipe: workgroups of the pipe kernel, 0 without it
+// how a launch of the chunk kernels looks: what it takes from the host are the numbers of tokens and sequences alone
+struct ChunkPlan { int headTiles, tileHeads, perTile, grid, unit, pipe; };   // pipe: workgroups of the pipe kernel, 0 without it
 static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
 {
     const int G = c.H / c.kvH;
@@ -980,18 +1036,17 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     p.tileHeads = (G + p.headTiles - 1) / p.headTiles;
     p.perTile = CHUNK_ROWS / p.tileHeads;
     // every sequence may end inside a tile; those that have tiles have more than FEW_ROWS rows
-    const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1));
-    p.tiles = (int)(c.tokens / p.perTile + having);
-    const long long groups = (long long)p.tiles * c.kvH * p.headTiles;
+    const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1)), groups = (long long)c.kvH * p.headTiles;
+    const long long whole = (long long)c.tokens / (2 * p.perTile) * groups, pipe = whole + having * groups;
     p.pipe = 0;
-    const long long whole = (long long)c.tokens / (2 * p.perTile) * c.kvH * p.headTiles, pipe = whole + having * c.kvH * p.headTiles;
     if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 0x3fffffff &&
-        ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll) {
+        ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll)
         p.pipe = (int)pipe;
-        p.splits = 1;
-        return p;
-    }
-    p.splits = (int)std::max<long long>(1, std::min<long long>(16, (dt == F32 ? CHUNK_GRID_32 : CHUNK_GRID_16) / std::max<long long>(1, groups)));
+    // the list is counted in 32 bits
+    const double tiles = (double)(c.tokens / p.perTile + having) * groups, positions = std::max((double)c.tokens, c.maxPages * (double)c.pageSize) + CHUNK_ROWS;
+    p.unit = 0;
+    while (p.unit < 20 && tiles * (positions / (32 << p.unit) + 2) > 1e9) p.unit++;
+    p.grid = (int)std::min<double>(CHUNK_GRID, std::max(1.0, tiles * (positions / (32 << p.unit) + 2) / CHUNK_LEAST));
     return p;
 }
 static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : 128; }
@@ -1000,8 +1055,9 @@ size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
 {
     const ChunkPlan p = chunk_plan(c, dt);
     const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
-    const size_t chunk = p.splits > 1 ? (size_t)p.splits * p.tiles * c.kvH * p.headTiles * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) : 0;
-    return std::max(split, std::max(chunk, (size_t)p.pipe * sizeof(int)));
+    const bool chunks = (long long)c.tokens * (c.H / c.kvH) > FEW_ROWS;
+    const size_t chunk = !chunks ? 0 : p.pipe ? (size_t)p.pipe * sizeof(int) : (size_t)p.grid * (2 * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) + sizeof(ChunkJoin));
+    return std::max(split, chunk);
 }
 size_t attn_paged_tickets() { return SPLIT_GRID; }
 
@@ -1025,22 +1081,20 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         w.few = chunks ? FEW_ROWS : 0;
         // its list is counted in 32 bits
         const double units = (double)c.kvH * w.headTiles * (chunks ? c.batch : c.tokens / w.perTile + c.batch) * (c.maxPages * (double)c.pageSize / 64 + 1);
-        if (in_pieces(c, dt, q, y) && units < 2e9) {
+        if (workspace && in_pieces(c, dt, q, y) && units < 2e9) {
             if (chunks) {
                 const ChunkPlan p = chunk_plan(c, dt);
-                ChunkArgs g = {(float*)workspace, FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.splits, p.pipe ? 2 : 1, p.pipe ? (const int*)workspace : nullptr};
+                ChunkArgs g = {(float*)workspace, (ChunkJoin*)((float*)workspace + (size_t)p.grid * 2 * CHUNK_ROWS * (padded_size(c) + 2)), FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.unit, p.pipe ? 2 : 1, p.pipe ? (const int*)workspace : nullptr};
                 if (p.pipe) {
                     const hipError_t e = attn_paged_pipe_launch(s, a, g, p.pipe, (int*)workspace);
                     if (e != hipSuccess) return e;
                 }
-                const long long blocks = p.pipe ? 2ll * p.pipe : (long long)c.kvH * p.headTiles * p.tiles;
-                if (blocks > 0x7fffffff) return hipErrorInvalidValue;
-                const dim3 grid((unsigned)blocks, p.splits);
+                const int grid = p.pipe ? 2 * p.pipe : p.grid;
                 if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid, 256, 0, s, a, g);
                 else hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 128>), grid, 256, 0, s, a, g);
-                if (p.splits > 1) {
-                    if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_join_kernel<T_, 64>), dim3((unsigned)blocks, 4), 256, 0, s, a, g);
-                    else hipLaunchKernelGGL((attn_paged_join_kernel<T_, 128>), dim3((unsigned)blocks, 4), 256, 0, s, a, g);
+                if (!p.pipe && grid > 1) {
+                    if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_join_kernel<T_, 64>), dim3(grid, 8), 256, 0, s, a, g);
+                    else hipLaunchKernelGGL((attn_paged_join_kernel<T_, 128>), dim3(grid, 8), 256, 0, s, a, g);
                 }
                 const hipError_t e = hipGetLastError();
                 if (e != hipSuccess) return e;

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
     if (tid == 0) { sFirst = 0x7fffffff; sMissing = -1; sBad = 0; }
     const ChunkTile at = chunk_tile(c, w, blockIdx.x);
     if (at.b < 0) return;
-    const PagedSpan sp = paged_span(c.starts[at.b], c.starts[at.b + 1], c.lens[at.b], c.tokens, c.maxPages * c.pageSize);
+    const PagedSpan sp = span_at(c, at.b);
     const int G = c.H / c.kvH, perTile = w.perTile * w.pair, j0 = at.tile * perTile, nt = min(perTile, sp.count - j0), base = sp.len - sp.count + j0;
     const int h0 = at.kh * G + at.ht * w.tileHeads, nh = min(w.tileHeads, G - at.ht * w.tileHeads);
     const int end = min(sp.len, base + nt), entries = end > 0 ? (end - 1) / c.pageSize + 1 : 0;
@@ -64,8 +64,8 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
         if (missing >= 0) atomicMax(&sMissing, missing);
     }
     __syncthreads();
-    const int front = sFirst < entries ? sFirst * c.pageSize : 0;
-    if (sFirst >= entries || sMissing > sFirst || base < front) {
+    const int given = uniform(sFirst), front = given < entries ? given * c.pageSize : 0;
+    if (given >= entries || uniform(sMissing) > given || base < front) {
         if (tid == 0) flags[blockIdx.x] = 1;
         return;
     }

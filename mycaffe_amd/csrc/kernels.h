@@ -279,7 +279,7 @@ struct PagedCache {
 hipError_t k_paged_append(hipStream_t s, DType dt, const PagedCache& c, const void* qkv, void* q, const void* wq, const void* wk, bool norm, float eps,
                           const float* turns);
 // y (tokens, H, hs) = attention of q (tokens, H, hs) over the pages, every token over the positions up to its own.  maxNew: at most this many new
-// tokens in a sequence, 0 if not known (any value is right).  workspace, tickets (zero between launches): as much as these say
+// tokens in a sequence, 0 if not known (any value is right).  workspace (may be null: a plain kernel does all), tickets (zero between launches): as much as these say
 size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt);
 size_t attn_paged_tickets();
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets);

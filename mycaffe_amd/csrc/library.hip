@@ -2837,7 +2837,8 @@ long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll)
     const float scale = pf[0] != 0.f ? pf[0] : (float)(1.0 / sqrt((double)c.hs));
     void* ws;
     int* tk;
-    ERRCHK(workspace(attn_paged_workspace_bytes(c, Q->dt()), &ws));
+    size_t wsb = attn_paged_workspace_bytes(c, Q->dt());
+    workspace_or_none(&wsb, &ws);   // without scratch one wavefront a token and head does all of it
     ERRCHK(tickets(attn_paged_tickets(), &tk));
     HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)std::min<long long>(ll > 18 ? pl[18] : 0, c.tokens), ws, tk));
     m_mem.touch((long)pl[14]);

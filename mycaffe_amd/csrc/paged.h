@@ -36,6 +36,44 @@ template <typename T> PAGED_FN PagedSpan paged_span(T start, T next, T len, int 
     return s;
 }
 
+// A list of `total` units of work dealt to at most `most` workgroups, at least `least` units each: equal runs, the first ones longer by one
+struct PagedRuns {
+    int W, run, more;
+    PAGED_FN PagedRuns(int total, int most, int least)
+    {
+        const int want = total / least;
+        W = want < 1 ? (total > 0 ? 1 : 0) : want < most ? want : most;
+        run = W ? total / W : 0;
+        more = total - run * W;
+    }
+    PAGED_FN int begin(int i) const { return run * i + (i < more ? i : more); }
+    PAGED_FN int of(int u) const { return u < (run + 1) * more ? u / (run + 1) : more + (u - (run + 1) * more) / run; }   // whose unit u is
+};
+// Workgroup -> place in the list, so that an XCD (workgroup i is on XCD i % 8) has neighbouring runs; -1: none of W
+PAGED_FN int paged_place(int block, int W)
+{
+    const int x = block & 7, k = block >> 3, each = W >> 3, rest = W & 7;
+    return k < each + (x < rest ? 1 : 0) ? x * each + (x < rest ? x : rest) + k : -1;
+}
+// Units of the first t tiles of a chunk: tiles of perTile tokens, the first of them over `before` + perTile positions, every further one over perTile more;
+// about 32 << shift positions a unit, and one for the tile
+PAGED_FN int paged_units_before(int before, int perTile, int t, int shift)
+{
+    const unsigned long long n = t;
+    return (int)((n * (unsigned)before + (unsigned)perTile * (n * (n + 1) / 2)) >> (5 + shift)) + t;
+}
+// the tile that unit u is in, of those that begin before `tiles`
+PAGED_FN int paged_tile_of(int before, int perTile, int tiles, int shift, int u)
+{
+    int lo = 0, hi = tiles - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (paged_units_before(before, perTile, mid, shift) <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
 // ---- what the entry points check, l as in the calls: {batch, tokens, heads, kvHeads, hs, pages, pageSize, maxPages, 7 handles, stridePage, strideHead, stridePos}
 inline bool paged_sizes_ok(const long long* l)
 {
