@@ -120,6 +120,7 @@ struct SplitArgs {
     int perTile;      // tokens a row tile
     int tileHeads;    // heads a row tile, of G
     int headTiles;    // row tiles that the G heads of a key head take
+    int one;          // sequences of at most this many positions are one unit
 };
 
 // of a maximum over scores that a row sees: what tells "all of them -inf" from "none"
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
     constexpr int KG = sizeof(TC) == 4 ? 1 : 2, KT = 16 * KG, UNIT = 4 * KT;   // groups of 16 keys a tile
     constexpr int VE = sizeof(TC) == 4 ? 4 : HSP / 16 < 8 ? HSP / 16 : 8, NH = HSP / (16 * VE), NO = HSP / 16;
     constexpr int ROWB = HSP * 2, STAGE = B16 ? KT * ROWB : 0;
-    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2), DEEP = 16;              // partial results in flight where an item is put together
+    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2);
     constexpr int SHARED = 4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4;
     static_assert(HSP == 64 || HSP == 128, "tile");
     __shared__ __attribute__((aligned(16))) unsigned char smem[SHARED];
@@ -174,36 +175,46 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
 
     // units of a sequence; a row tile without positions is one all the same (its rows are zeros)
     auto span_of = [&](int b) { return paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions); };
-    // (two are one: going on for a tile takes less than putting two partial results together, us for 12 heads over 100 positions in fp32 9.6 | 8.6)
-    auto units_of = [&](const PagedSpan& s) { return s.len <= 2 * UNIT ? 1 : (s.len + UNIT - 1) / UNIT; };
+    auto units_of = [&](const PagedSpan& s) { return s.len <= max(w.one, UNIT) ? 1 : (s.len + UNIT - 1) / UNIT; };
     auto tiles_of = [&](const PagedSpan& s) -> int { return w.few && (long long)s.count * G > w.few ? 0 : (s.count + w.perTile - 1) / w.perTile * w.headTiles; };
     auto work_of = [&](const PagedSpan& s) -> int { return tiles_of(s) * c.kvH * units_of(s); };
-    const PagedSpan none = {0, 0, 0};
-    PagedSpan mine = tid < c.batch ? span_of(tid) : none;
-    int total, work = work_of(mine), at = block_scan(work, sScan, &total);
-    const int total256 = total;
-    for (int b0 = 256; b0 < c.batch; b0 += 256) {
-        int all;
-        block_scan(b0 + tid < c.batch ? work_of(span_of(b0 + tid)) : 0, sScan, &all);
-        total += all;
+    PagedRuns runs(0, 1, 1);
+    PagedSpan sp;
+    int b = 0, local, lo, hi;
+    if (c.batch == 1) {   // no sums, no sequence to be found
+        sp = span_at(c, 0);
+        runs = PagedRuns(work_of(sp), gridDim.x, 1);
+        if ((int)blockIdx.x >= runs.W) return;
+        local = lo = runs.begin(blockIdx.x);
+        hi = runs.begin(blockIdx.x + 1);
+    } else {
+        const PagedSpan none = {0, 0, 0};
+        PagedSpan mine = tid < c.batch ? span_of(tid) : none;
+        int total, work = work_of(mine), at = block_scan(work, sScan, &total), all = total;
+        for (int b0 = 256; b0 < c.batch; b0 += 256) {
+            int more;
+            block_scan(b0 + tid < c.batch ? work_of(span_of(b0 + tid)) : 0, sScan, &more);
+            total += more;
+        }
+        runs = PagedRuns(uniform(total), gridDim.x, 1);
+        if ((int)blockIdx.x >= runs.W) return;
+        lo = runs.begin(blockIdx.x);
+        hi = runs.begin(blockIdx.x + 1);
+        // the sequence that has unit `lo`
+        for (int b0 = 0, base = 0;;) {
+            if (at <= lo && lo < at + work) { sSeq = b0 + tid; sAt = at; sSpan = mine; }
+            base += all;
+            if (lo < base) break;
+            if ((b0 += 256) >= c.batch) return;
+            mine = b0 + tid < c.batch ? span_of(b0 + tid) : none;
+            work = work_of(mine);
+            at = base + block_scan(work, sScan, &all);
+        }
+        __syncthreads();
+        b = uniform(sSeq);
+        local = uniform(lo - sAt);
+        sp = uniform(sSpan);
     }
-    total = uniform(total);
-    const PagedRuns runs(total, gridDim.x, 1);
-    if ((int)blockIdx.x >= runs.W) return;
-    const int lo = runs.begin(blockIdx.x), hi = runs.begin(blockIdx.x + 1);
-    // the sequence that has unit `lo`
-    for (int b0 = 0, base = 0, all = total256;;) {
-        if (at <= lo && lo < at + work) { sSeq = b0 + tid; sAt = at; sSpan = mine; }
-        base += all;
-        if (lo < base) break;
-        if ((b0 += 256) >= c.batch) return;
-        mine = b0 + tid < c.batch ? span_of(b0 + tid) : none;
-        work = work_of(mine);
-        at = base + block_scan(work, sScan, &all);
-    }
-    __syncthreads();
-    int b = uniform(sSeq), local = uniform(lo - sAt);
-    PagedSpan sp = uniform(sSpan);
 
     const TC *kp = (const TC*)c.k, *vp = (const TC*)c.v;
     for (int u = lo; u < hi;) {
@@ -381,8 +392,14 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                     }
                 load_v(next);
                 wave_lds_fence();
-                // weights rounded to 16 bits, their sum not: the roundings of many weights even out
-                const u32x4 p = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]), pack_bf16x2(s[KG - 1][0], s[KG - 1][1]), pack_bf16x2(s[KG - 1][2], s[KG - 1][3])};
+                // weights as two bf16 numbers, sixteen bits of them: the second product is free beside the reading
+                u32x4 p, rest;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = s[e >> 1 ? KG - 1 : 0][2 * (e & 1)], y = s[e >> 1 ? KG - 1 : 0][2 * (e & 1) + 1];
+                    p[e] = pack_bf16x2(x, y);
+                    rest[e] = pack_bf16x2(x - __uint_as_float(p[e] << 16), y - __uint_as_float(p[e] & 0xffff0000u));
+                }
 #pragma unroll
                 for (int i = 0; i < NO; i++) {
                     uint2 half[2];
@@ -392,7 +409,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                         half[k] = lds_read_tr16((const bf16_t*)(stage + row * ROWB + ((piece ^ sw) << 4) + (r16 & 1) * 8));
                     }
                     u32x4 vt = {half[0].x, half[0].y, half[1].x, half[1].y};
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(bf16x8*)&vt, *(const bf16x8*)&p, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(bf16x8*)&vt, *(bf16x8*)&p, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(bf16x8*)&vt, *(bf16x8*)&rest, o[i], 0, 0, 0);
                 }
                 wave_lds_fence();
             } else {
@@ -503,37 +521,43 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
             if (tid == 0) sTicket = __hip_atomic_fetch_add(w.tickets + wf, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __syncthreads();
             if (sTicket == we - wf) {
-                for (int e = tid; e < rows * pairs; e += 256) {
-                    const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
-                    if (hd >= nh) continue;
-                    float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
-                    for (int i = wf; i <= we; i += DEEP) {
-                        float2 ml[DEEP], v[DEEP];
-#pragma unroll
-                        for (int j = 0; j < DEEP; j++) {
-                            const float* from = w.part + ((size_t)min(i + j, we) * 2 + (i + j == wf ? 1 : 0)) * PART;
-                            ml[j] = get2(from + 2 * r);
-                            v[j] = get2(from + 32 + r * HSP + d);
+                // DEEP partial results in flight (past the last one that again, with no weight)
+                auto join = [&](auto deep) __attribute__((always_inline)) {
+                    constexpr int DEEP = decltype(deep)::value;
+                    for (int e = tid; e < rows * pairs; e += 256) {
+                        const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
+                        if (hd >= nh) continue;
+                        float M = -INFINITY, L = 0.f, x = 0.f, y = 0.f;
+                        for (int i = wf; i <= we; i += DEEP) {
+                            float2 ml[DEEP], v[DEEP];
+    #pragma unroll
+                            for (int j = 0; j < DEEP; j++) {
+                                const float* from = w.part + ((size_t)min(i + j, we) * 2 + (i + j == wf ? 1 : 0)) * PART;
+                                ml[j] = get2(from + 2 * r);
+                                v[j] = get2(from + 32 + r * HSP + d);
+                            }
+                            float Mn = M;
+    #pragma unroll
+                            for (int j = 0; j < DEEP; j++) Mn = i + j <= we ? fmaxf(Mn, ml[j].x) : Mn;
+                            const float f0 = weight_of(M, Mn);
+                            L *= f0; x *= f0; y *= f0;
+    #pragma unroll
+                            for (int j = 0; j < DEEP; j++) {
+                                const float f = weight_of(ml[j].x, Mn);
+                                L += i + j <= we ? ml[j].y * f : 0.f;
+                                x += i + j <= we ? v[j].x * f : 0.f;
+                                y += i + j <= we ? v[j].y * f : 0.f;
+                            }
+                            M = Mn;
                         }
-                        float Mn = M;
-#pragma unroll
-                        for (int j = 0; j < DEEP; j++) Mn = i + j <= we ? fmaxf(Mn, ml[j].x) : Mn;
-                        const float f0 = weight_of(M, Mn);
-                        L *= f0; x *= f0; y *= f0;
-#pragma unroll
-                        for (int j = 0; j < DEEP; j++) {
-                            const float f = weight_of(ml[j].x, Mn);
-                            L += i + j <= we ? ml[j].y * f : 0.f;
-                            x += i + j <= we ? v[j].x * f : 0.f;
-                            y += i + j <= we ? v[j].y * f : 0.f;
-                        }
-                        M = Mn;
+                        TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
+                        const float xs = M > -INFINITY ? x / L : 0.f, ys = M > -INFINITY ? y / L : 0.f;
+                        if constexpr (B16) *(uint32_t*)out = pack_bf16x2(xs, ys);
+                        else *(float2*)out = make_float2(xs, ys);
                     }
-                    TQ* out = (TQ*)a.y + row_at(tk, hd) + d;
-                    const float xs = M > -INFINITY ? x / L : 0.f, ys = M > -INFINITY ? y / L : 0.f;
-                    if constexpr (B16) *(uint32_t*)out = pack_bf16x2(xs, ys);
-                    else *(float2*)out = make_float2(xs, ys);
-                }
+                };
+                if (we - wf < 4) join(std::integral_constant<int, 4>{});
+                else join(std::integral_constant<int, 16>{});
                 if (tid == 0) __hip_atomic_store(w.tickets + wf, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);   // for the next launch
             }
         }
@@ -1079,6 +1103,9 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         const int most = maxNew > 0 ? std::min(maxNew, c.tokens) : c.tokens;
         const bool chunks = (long long)most * G > FEW_ROWS && c.tokens > c.batch + c.batch / 4;
         w.few = chunks ? FEW_ROWS : 0;
+        // Up to two units in one where there are few sequences: going on for a tile takes less than putting two partial results together (us, 12 heads over 100
+        // positions, fp32, 9.6 | 8.2).  With many of them a unit has to stand for its length (64 sequences of up to 4096, 8 key heads, 120 | 124).
+        w.one = (long long)c.batch * c.kvH * w.headTiles < SPLIT_GRID / 2 ? 2 * 4 * 16 * (c.ct == F32 ? 1 : 2) : 0;
         // its list is counted in 32 bits
         const double units = (double)c.kvH * w.headTiles * (chunks ? c.batch : c.tokens / w.perTile + c.batch) * (c.maxPages * (double)c.pageSize / 64 + 1);
         if (workspace && in_pieces(c, dt, q, y) && units < 2e9) {
