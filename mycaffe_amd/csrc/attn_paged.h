@@ -33,7 +33,7 @@ __device__ __forceinline__ PagedSpan span_at(const PagedCache& c, int b)
     return uniform(paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize));
 }
 
-// over 256 threads: the sum of the numbers before the thread's own, and all of them
+// over 256 threads, numbers up to PAGED_MOST: the sum of those before the thread's own (PAGED_MOST: that or more), and of all of them
 __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -41,19 +41,20 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
+        if (lane >= o) x = paged_sum(x, y);
     }
+    const int mine = __shfl_up(x, 1);
     __syncthreads();
     if (lane == 63) sums[wave] = x;
     __syncthreads();
     int before = 0, sum = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        before += i < wave ? sums[i] : 0;
-        sum += sums[i];
+        before = i < wave ? paged_sum(before, sums[i]) : before;
+        sum = paged_sum(sum, sums[i]);
     }
     *all = sum;
-    return before + x - v;
+    return lane ? paged_sum(before, mine) : before;
 }
 
 // The chunk kernel's list: sequences, their key heads and head tiles, their tiles, in units of about 32 positions of a tile.  All 256 threads.
@@ -84,9 +85,10 @@ __device__ __forceinline__ ChunkStart chunk_start(const PagedCache& c, const Chu
     for (int b0 = 256; b0 < c.batch; b0 += 256) {
         int more;
         block_scan(chunk_work(c, w, span_of(b0 + tid)) * groups, sums, &more);
-        r.total += more;
+        r.total = paged_sum(r.total, more);
     }
     r.total = uniform(r.total);
+    if (r.total >= PAGED_MOST) { r.place = -1; return r; }
     const PagedRuns runs(r.total, most, CHUNK_LEAST);
     r.place = paged_place(block, runs.W);
     if (r.place < 0) return r;

@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a)
     constexpr int GROUPS = 64 / LPH;
     const PagedCache& c = a.c;
     const int lane = threadIdx.x & 63, d0 = (lane % LPH) * V;
-    const int token = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (h >= c.H) return;
+    const int token = blockIdx.z * gridDim.x + blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
+    if (h >= c.H || token >= c.tokens) return;
     const int b = sequence_of(c.starts, c.batch, c.tokens, token);
     if (b < 0) return;
     const PagedSpan sp = paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize);
@@ -194,8 +194,9 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
         for (int b0 = 256; b0 < c.batch; b0 += 256) {
             int more;
             block_scan(b0 + tid < c.batch ? work_of(span_of(b0 + tid)) : 0, sScan, &more);
-            total += more;
+            total = paged_sum(total, more);
         }
+        if (uniform(total) >= PAGED_MOST) return;
         runs = PagedRuns(uniform(total), gridDim.x, 1);
         if ((int)blockIdx.x >= runs.W) return;
         lo = runs.begin(blockIdx.x);
@@ -1051,7 +1052,7 @@ constexpr int PIPE_TILES_128 = 128, PIPE_TILES_64 = 192;
 constexpr int CHUNK_ROWS = 128, CHUNK_GRID = 512;   // two workgroups a CU
 
 // how a launch of the chunk kernels looks: what it takes from the host are the numbers of tokens and sequences alone
-struct ChunkPlan { int headTiles, tileHeads, perTile, grid, unit, pipe; };   // pipe: workgroups of the pipe kernel, 0 without it
+struct ChunkPlan { int headTiles, tileHeads, perTile, grid, unit, pipe; double units; };   // pipe: workgroups of the pipe kernel, 0 without it; units: no more than these
 static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
 {
     const int G = c.H / c.kvH;
@@ -1063,14 +1064,14 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1)), groups = (long long)c.kvH * p.headTiles;
     const long long whole = (long long)c.tokens / (2 * p.perTile) * groups, pipe = whole + having * groups;
     p.pipe = 0;
-    if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 0x3fffffff &&
+    if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 1 << 23 &&
         ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll)
         p.pipe = (int)pipe;
     // the list is counted in 32 bits
     const double tiles = (double)(c.tokens / p.perTile + having) * groups, positions = std::max((double)c.tokens, c.maxPages * (double)c.pageSize) + CHUNK_ROWS;
     p.unit = 0;
-    while (p.unit < 20 && tiles * (positions / (32 << p.unit) + 2) > 1e9) p.unit++;
-    p.grid = (int)std::min<double>(CHUNK_GRID, std::max(1.0, tiles * (positions / (32 << p.unit) + 2) / CHUNK_LEAST));
+    while (p.units = tiles * (positions / (32 << p.unit) + 2), p.unit < 20 && p.units > 1e9) p.unit++;
+    p.grid = (int)std::min<double>(CHUNK_GRID, std::max(1.0, p.units / CHUNK_LEAST));
     return p;
 }
 static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : 128; }
@@ -1108,7 +1109,8 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         w.one = (long long)c.batch * c.kvH * w.headTiles < SPLIT_GRID / 2 ? 2 * 4 * 16 * (c.ct == F32 ? 1 : 2) : 0;
         // its list is counted in 32 bits
         const double units = (double)c.kvH * w.headTiles * (chunks ? c.batch : c.tokens / w.perTile + c.batch) * (c.maxPages * (double)c.pageSize / 64 + 1);
-        if (workspace && in_pieces(c, dt, q, y) && units < 2e9) {
+        const bool fits = !chunks || chunk_plan(c, dt).units <= 1e9;
+        if (workspace && in_pieces(c, dt, q, y) && units < PAGED_MOST && fits) {
             if (chunks) {
                 const ChunkPlan p = chunk_plan(c, dt);
                 ChunkArgs g = {(float*)workspace, (ChunkJoin*)((float*)workspace + (size_t)p.grid * 2 * CHUNK_ROWS * (padded_size(c) + 2)), FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.unit, p.pipe ? 2 : 1, p.pipe ? (const int*)workspace : nullptr};
@@ -1130,7 +1132,8 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
             else hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
             return hipGetLastError();
         }
-        const dim3 grid(c.tokens, (c.H + 3) / 4);
+        const int x = std::min(c.tokens, 1 << 23);   // an axis of a launch has less than 2^32 threads
+        const dim3 grid(x, (c.H + 3) / 4, (c.tokens + x - 1) / x);
         if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 16>), grid, 256, 0, s, a);
         else if (c.hs <= 128) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 32>), grid, 256, 0, s, a);
         else hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 64>), grid, 256, 0, s, a);

@@ -143,13 +143,13 @@ struct HeadNormArgs {
 constexpr int AHEAD = 3, AHEAD_BWD = 2;      // heads a lane group has in flight
 
 // A lane group keeps one position and walks the heads of its part, so that cosines, sines and weights are read once for all of them.
-// grid: (groups of positions, parts of the heads)
+// grid: (groups of positions, parts of the heads, groups of positions beyond one axis)
 template <typename T, int V, bool VEC, int LPH>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(HeadNormArgs a)
 {
     constexpr int GROUPS = 256 / LPH;
     const int d0 = (threadIdx.x % LPH) * V;
-    const long long at = (long long)blockIdx.x * GROUPS + threadIdx.x / LPH;
+    const long long at = ((long long)blockIdx.z * gridDim.x + blockIdx.x) * GROUPS + threadIdx.x / LPH;
     const bool live = at < (long long)a.B * a.T;
     const int b = live ? (int)(at / a.T) : 0, t = live ? (int)(at - (long long)b * a.T) : 0;
     float c[V / 2], s[V / 2], w[2][V];
@@ -419,7 +419,8 @@ hipError_t k_qk_norm_rope(hipStream_t s, DType dt, int B, int T, int H, int kvH,
                 const long long blocks = ((long long)B * T + GROUPS - 1) / GROUPS;
                 // few positions: their heads are dealt to several workgroups
                 const int parts = (int)std::max<long long>(1, std::min<long long>(H + kvH, 2048 / blocks));
-                hipLaunchKernelGGL((qk_norm_rope_kernel<T_, V, decltype(vec_)::value, LPH>), dim3((unsigned)blocks, parts), 256, 0, s, a);
+                const unsigned x = (unsigned)std::min<long long>(blocks, 1 << 23);   // an axis of a launch has less than 2^32 threads
+                hipLaunchKernelGGL((qk_norm_rope_kernel<T_, V, decltype(vec_)::value, LPH>), dim3(x, parts, (unsigned)((blocks + x - 1) / x)), 256, 0, s, a);
                 return hipGetLastError();
             });
         });

@@ -676,14 +676,14 @@ __device__ inline void d_head(const double* x, const double* w, double* y, bool 
 }
 __global__ __launch_bounds__(256) void d_head_norm_kernel(size_t rows, int T, int hs, const double* x, const double* w, double* y, double eps, double theta)
 {
-    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t row = ((size_t)blockIdx.z * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row < rows) d_head(x + row * hs, w, y + row * hs, true, eps, (int)(row % T), hs, theta);
 }
 // g = R(-t) dy, dx = r (g w - x r mean(g w x r)); gx: what the weights' gradient adds up, g x r
 __global__ __launch_bounds__(256) void d_head_norm_bwd_kernel(size_t rows, int T, int hs, const double* x, const double* w, const double* dy, double* dx, double* gx,
                                                               double eps, double theta)
 {
-    const size_t row = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t row = ((size_t)blockIdx.z * gridDim.x + blockIdx.x) * 4 + (threadIdx.x >> 6);
     if (row >= rows) return;
     const int half = hs / 2, lane = threadIdx.x & 63, t = (int)(row % T);
     double a[2], b[2], ga[2], gb[2], ss = 0.0, dot = 0.0;
@@ -729,6 +729,12 @@ __global__ __launch_bounds__(1024) void d_head_norm_dw_kernel(size_t rows, int h
     acc = d_lane_sums(acc, red);
     if (r == 0 && j < hs) dw[j] = accum ? dw[j] + acc : acc;
 }
+// n workgroups of 256 threads by y: an axis of a launch has less than 2^32 threads
+inline dim3 d_axes(long long n, long long y)
+{
+    const long long x = std::min<long long>(n, 1 << 23);
+    return dim3((unsigned)x, (unsigned)y, (unsigned)((n + x - 1) / x));
+}
 struct PagedD {
     double *k, *v;
     const double *table, *starts, *lens;
@@ -753,10 +759,10 @@ __device__ inline long long d_place(const PagedD& c, int b, int t)
 }
 __global__ __launch_bounds__(256) void d_paged_append_kernel(PagedD c, const double* qkv, double* q, const double* wq, const double* wk, int norm, double eps, double theta)
 {
-    const int token = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), heads = c.H + 2 * c.kvH;
+    const int token = blockIdx.z * gridDim.x + blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), heads = c.H + 2 * c.kvH;
     int b;
     PagedSpan sp;
-    if (h >= heads || !d_sequence(c, token, &b, &sp)) return;
+    if (h >= heads || token >= c.tokens || !d_sequence(c, token, &b, &sp)) return;
     const int pos = sp.len - sp.count + (token - sp.first), t = pos > 0 ? pos : 0;
     const double* x = qkv + ((size_t)token * heads + h) * c.hs;
     if (h < c.H) {
@@ -771,10 +777,10 @@ __global__ __launch_bounds__(256) void d_paged_append_kernel(PagedD c, const dou
 }
 __global__ __launch_bounds__(256) void d_paged_attn_kernel(PagedD c, const double* q, double* y, double scale)
 {
-    const int token = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int token = blockIdx.z * gridDim.x + blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     int b;
     PagedSpan sp;
-    if (h >= c.H || !d_sequence(c, token, &b, &sp)) return;
+    if (h >= c.H || token >= c.tokens || !d_sequence(c, token, &b, &sp)) return;
     const int last = sp.len - sp.count + (token - sp.first);
     const size_t row = ((size_t)token * c.H + h) * c.hs;
     double qv[4], acc[4] = {0.0, 0.0, 0.0, 0.0}, m = -INFINITY, l = 0.0;
@@ -992,7 +998,6 @@ long KernelD::head_norm(const double* pf, const MCH_LONGLONG* pl, long ll, bool 
     if (B < 1 || T < 1 || H < 1 || KVH < 1 || H > 65535 || KVH > 65535 || hs < 2 || hs > 256 || (hs & 1) || B > INT_MAX || T > INT_MAX || B * T > INT_MAX || !(pf[0] >= 0.0))
         return MCH_ERROR_PARAM_OUT_OF_RANGE;
     const long long rows[2] = {B * H * T, B * KVH * T}, n[2] = {rows[0] * hs, rows[1] * hs};
-    if ((rows[0] + 3) / 4 > INT_MAX || (rows[1] + 3) / 4 > INT_MAX) return MCH_ERROR_PARAM_OUT_OF_RANGE;
     MemD *X[2], *W[2] = {}, *dY[2] = {}, *Y[2], *dW[2] = {};
     for (int i = 0; i < 2; i++) {
         ERRCHK(mem((long)pl[5 + i], &X[i]));
@@ -1031,7 +1036,7 @@ long KernelD::head_norm(const double* pf, const MCH_LONGLONG* pl, long ll, bool 
     double* gx = nullptr;
     if (dW[0] || dW[1]) ERRCHK(workspace((size_t)std::max(n[0], n[1]), &gx));
     for (int i = 0; i < 2; i++) {
-        const int grid = (int)((rows[i] + 3) / 4);
+        const dim3 grid = d_axes((rows[i] + 3) / 4, 1);
         const double* w = W[i] ? W[i]->ptr : nullptr;
         if (!backward) hipLaunchKernelGGL(d_head_norm_kernel, grid, 256, 0, m_stream, (size_t)rows[i], (int)T, (int)hs, (const double*)X[i]->ptr, w, Y[i]->ptr, pf[0], theta);
         else {
@@ -1091,7 +1096,7 @@ long KernelD::paged(const double* pf, const MCH_LONGLONG* pl, bool append)
         return MCH_ERROR_PARAM_OUT_OF_RANGE;
     }
     const PagedD c = {K->ptr, V->ptr, m[3]->ptr, m[4]->ptr, m[5]->ptr, (int)B, (int)N, (int)H, (int)KVH, (int)hs, (int)l[5], (int)l[6], (int)l[7], l[15], l[16], l[17]};
-    const dim3 grid((unsigned)N, (unsigned)((rowHeads + 3) / 4));
+    const dim3 grid = d_axes(N, (rowHeads + 3) / 4);
     if (append) hipLaunchKernelGGL(d_paged_append_kernel, grid, 256, 0, m_stream, c, (const double*)X->ptr, out->ptr, W[0] ? (const double*)W[0]->ptr : nullptr,
                                    W[1] ? (const double*)W[1]->ptr : nullptr, (int)(pl[19] != 0), pf[0], theta);
     else hipLaunchKernelGGL(d_paged_attn_kernel, grid, 256, 0, m_stream, c, (const double*)X->ptr, out->ptr, pf[0] != 0.0 ? pf[0] : 1.0 / sqrt((double)hs));

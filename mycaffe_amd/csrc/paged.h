@@ -19,6 +19,10 @@ namespace mch {
 #endif
 
 constexpr int PAGED_EXACT = 1 << 24;   // whole numbers up to here are exact in fp32
+// Lists of work are counted up to here and no further.  The host sees to it that sequences whose starts never decrease stay below; a list that does
+// reach it (starts that decrease give the same tokens to many sequences) is none.
+constexpr int PAGED_MOST = 0x3fffffff;
+PAGED_FN int paged_sum(int a, int b) { return a + b < PAGED_MOST ? a + b : PAGED_MOST; }   // of two up to PAGED_MOST
 
 // v as a whole number in lo .. hi
 template <typename T> PAGED_FN int paged_int(T v, int lo, int hi) { return v >= (T)hi ? hi : v > (T)lo ? (int)v : lo; }
