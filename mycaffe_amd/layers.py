@@ -337,13 +337,14 @@ class PagedSequences:
     length).  One object serves all layers of a model: they keep pages of the same numbers.
 
     ``Step({name: new tokens})`` before a model's pass: every named sequence grows by its tokens, in the order given, which is the order of the rows of
-    the pass; new names begin new sequences.  ``Drop(name, positions)`` gives up a sequence's oldest pages, ``End(name)`` all of them.
+    the pass; new names begin new sequences.  ``Drop(name, positions)`` gives up a sequence's oldest pages, ``End(name)`` all of them.  ``Dispose()``
+    frees the pages of all layers.
     """
 
     def __init__(self, cuda, pages, page_size, max_pages):
         self.cuda, self.pages, self.page_size, self.max_pages = cuda, pages, page_size, max_pages
         self._free = list(range(pages - 1, -1, -1))
-        self._table, self._len = {}, {}
+        self._table, self._len, self._caches = {}, {}, {}
         self.table, self.starts, self.lens = (Blob(cuda) for _ in range(3))
         self.batch = self.tokens = self.max_new = 0
 
@@ -380,6 +381,17 @@ class PagedSequences:
     def End(self, name):
         self._free += [p for p in self._table.pop(name) if p >= 0]
         del self._len[name]
+
+    def Cache(self, layer, heads, size, half):
+        """Keys and values of a layer, (pages, heads, page size, head size); what a step does not write is never read."""
+        if layer not in self._caches:
+            self._caches[layer] = tuple(Blob(self.cuda, (self.pages, heads, self.page_size, size), half) for _ in range(2))
+        return self._caches[layer]
+
+    def Dispose(self):
+        for blob in [self.table, self.starts, self.lens] + [b for kv in self._caches.values() for b in kv]:
+            blob.Dispose()
+        self._caches.clear()
 
 
 class CausalSelfAttentionLayer:
@@ -418,7 +430,7 @@ class CausalSelfAttentionLayer:
         self._masks, self._ropes = _Kept(Blob.Dispose), _Kept(cuda.FreeRope)
         self.hCudnn = self.hAttn = self.hRope = 0
         self._set_for = None
-        self._paged, self._page_rope = {}, None
+        self._page_rope = None
 
     def Setup(self, bottom, w_attn, b_attn, w_proj, b_proj, w_qnorm=None, w_knorm=None):
         self.c_attn.Setup(bottom, w_attn, b_attn)
@@ -541,10 +553,7 @@ class CausalSelfAttentionLayer:
         N, C = blobX.count(0, 2), self.nEmbed
         if N != seqs.tokens:
             raise ValueError("the pass has %d tokens, the step %d" % (N, seqs.tokens))
-        if id(seqs) not in self._paged:
-            # what a step does not write is never read; the sequences stay alive with their pages
-            self._paged[id(seqs)] = (seqs, Blob(cuda, (seqs.pages, H, seqs.page_size, hs), self.half), Blob(cuda, (seqs.pages, H, seqs.page_size, hs), self.half))
-        _, k, v = self._paged[id(seqs)]
+        k, v = seqs.Cache(self, H, hs, self.half)
         positions = seqs.max_pages * seqs.page_size
         if self.enable_rope and (self._page_rope is None or self._page_rope[0] < positions):
             if self._page_rope is not None:
