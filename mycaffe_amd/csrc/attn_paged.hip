@@ -616,6 +616,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
     constexpr int LD = HSP + 8;                                                                   // values a row in LDS
+    constexpr int AHEAD = 2;                                                                      // value fragments under way
     constexpr int PART = 128 * (HSP + 2);
     __shared__ __attribute__((aligned(16))) bf16_t sK[NK][KB * LD], sV[NK][KB * LD];
     __shared__ long long sPlace[2][KB];
@@ -812,6 +813,16 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                         if (x + y < 3) s[j] = TR::mma(k, qf[f].p[y], s[j]);
                 }
         }
+        // values travel while the weights are made, AHEAD fragments in front of the product that they are for (us with none | 1 | 2 | 4: a step of chunks and
+        // single tokens in fp32 73.9 | 73.2 | 72.0 | 73.3, 4 sequences of 8 new tokens over 4096 in 16 bits 37.3 | 37.2 | 36.7 | 38.8)
+        u32x4 vf[AHEAD][NK];
+        auto value = [&](int n) {
+            const int j = n / (2 * DT), x = n / DT % 2, i = n % DT;
+#pragma unroll
+            for (int z = 0; z < NK; z++) vf[n % AHEAD][z] = TR::load_vt_rowmajor(sV[z] + 32 * j * LD + 32 * i, LD, x, lane);
+        };
+#pragma unroll
+        for (int n = 0; n < AHEAD; n++) value(n);
         // Maxima are taken of the products themselves (the queries carry the scale's sign), and the running one moves only when a row's grows by 2^8:
         // weights stay below that, and the sums are seldom scaled again.
         float mx = -INFINITY;
@@ -876,18 +887,15 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
                     }
             }
 #pragma unroll
-        for (int j = 0; j < KJ; j++)
+        for (int n = 0; n < KJ * 2 * DT; n++) {
+            const int j = n / (2 * DT), x = n / DT % 2, i = n % DT;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int z = NK - 1; z >= 0; z--)
 #pragma unroll
-                for (int i = 0; i < DT; i++)
-#pragma unroll
-                    for (int z = NK - 1; z >= 0; z--) {
-                        const u32x4 v = TR::load_vt_rowmajor(sV[z] + 32 * j * LD + 32 * i, LD, x, lane);
-#pragma unroll
-                        for (int y = NQ - 1; y >= 0; y--)
-                            if (z + y < 3) o[i] = TR::mma(v, p[j][x].p[y], o[i]);
-                    }
+                for (int y = NQ - 1; y >= 0; y--)
+                    if (z + y < 3) o[i] = TR::mma(vf[n % AHEAD][z], p[j][x].p[y], o[i]);
+            if (n + AHEAD < KJ * 2 * DT) value(n + AHEAD);
+        }
     }
     l = add_lane_xor<32>(l);
     if (__any(bad) && lane == 0) sBad = 1;
