@@ -39,15 +39,21 @@ __device__ __forceinline__ int sequence_of(const float* starts, int batch, int t
     return n - 1;
 }
 
-// Any head size up to 256, any strides: a wavefront has one token's head, a group of LPH lanes every (64 / LPH)-th position, V values a lane.
-template <typename T, typename TC, int V, int LPH>
-__global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a)
+// Any head size up to 256, any strides and addresses, no workspace: a workgroup has one token's head, a group of LPH lanes of its WAVES wavefronts
+// every (64 WAVES / LPH)-th position, V values a lane, value by value in runs of LPH; ANY_DEEP positions' reads are under way together.  What
+// bounds it is waiting for them, and every head reads its keys for itself.  Sixteen wavefronts where there are few tokens' heads, four else (us: one token over
+// 1000 positions, 6 heads of 198, fp32 56 | 134, sixteen of them 69 | 191; 64 tokens over up to 60, 12 heads of 46, 16.1 | 7.1; 4 chunks of 300, 97 | 56).
+constexpr int ANY_DEEP = 4;
+template <typename T, typename TC, int V, int LPH, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void attn_paged_any_kernel(PagedAttnArgs a)
 {
-    constexpr int GROUPS = 64 / LPH;
+    constexpr int GROUPS = 64 / LPH, STEP = WAVES * GROUPS;
+    __shared__ float sM[WAVES], sL[WAVES], sAcc[WAVES][LPH * V];
+    __shared__ int sSeen[WAVES];
     const PagedCache& c = a.c;
-    const int lane = threadIdx.x & 63, d0 = (lane % LPH) * V;
-    const int token = blockIdx.z * gridDim.x + blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (h >= c.H || token >= c.tokens) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d0 = lane % LPH;
+    const int token = blockIdx.z * gridDim.x + blockIdx.x, h = blockIdx.y;
+    if (token >= c.tokens) return;
     const int b = sequence_of(c.starts, c.batch, c.tokens, token);
     if (b < 0) return;
     const PagedSpan sp = paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize);
@@ -55,31 +61,45 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a)
     const int last = sp.len - sp.count + (token - sp.first), kh = h / (c.H / c.kvH);
     const T* q = (const T*)a.q + ((size_t)token * c.H + h) * c.hs;
     float qv[V], acc[V], m = -INFINITY, l = 0.f;
+    int at_d[V];
     bool seen = false;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        qv[i] = d0 + i < c.hs ? value_of<T>(q[d0 + i]) : 0.f;
+        at_d[i] = min(d0 + LPH * i, c.hs - 1);
+        qv[i] = d0 + LPH * i < c.hs ? value_of<T>(q[d0 + LPH * i]) : 0.f;
         acc[i] = 0.f;
     }
-    for (int t = lane / LPH; t <= last; t += GROUPS) {
-        const int entry = t / c.pageSize, page = paged_page(c.table[(size_t)b * c.maxPages + entry], c.pages);
-        const bool given = page >= 0;
-        const long long at = given ? page * c.sP + kh * c.sH + (t - entry * c.pageSize) * c.sT : 0;
-        const TC *k = (const TC*)c.k + at, *v = (const TC*)c.v + at;
-        float dot = 0.f;
+    for (int t0 = wave * GROUPS + lane / LPH; t0 <= last; t0 += ANY_DEEP * STEP) {
+        TC k[ANY_DEEP][V], v[ANY_DEEP][V];
+        bool given[ANY_DEEP];
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (d0 + i < c.hs) dot += qv[i] * value_of<TC>(k[d0 + i]);
-        dot = group_sum<LPH>(dot) * a.c2;
-        if (!given) continue;
-        seen = true;
-        const float mn = fmaxf(m, dot), ref = mn > -INFINITY ? mn : 0.f, f = exp2f(m - ref), w = exp2f(dot - ref);
-        m = mn;
-        l = l * f + w;
+        for (int j = 0; j < ANY_DEEP; j++) {
+            const int t = t0 + j * STEP, entry = min(t, last) / c.pageSize, page = paged_page(c.table[(size_t)b * c.maxPages + entry], c.pages);
+            given[j] = page >= 0 && t <= last;
+            // what is not there: the cache's first values, left out below
+            const long long at = given[j] ? page * c.sP + kh * c.sH + (t - entry * c.pageSize) * c.sT : 0;
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] = acc[i] * f + (d0 + i < c.hs ? w * value_of<TC>(v[d0 + i]) : 0.f);
+            for (int i = 0; i < V; i++) {
+                k[j][i] = ((const TC*)c.k)[at + at_d[i]];
+                v[j][i] = ((const TC*)c.v)[at + at_d[i]];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < ANY_DEEP; j++) {
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; i++) dot += d0 + LPH * i < c.hs ? qv[i] * value_of<TC>(k[j][i]) : 0.f;
+            dot = group_sum<LPH>(dot) * a.c2;
+            if (!given[j]) continue;
+            seen = true;
+            const float mn = fmaxf(m, dot), ref = mn > -INFINITY ? mn : 0.f, f = exp2f(m - ref), w = exp2f(dot - ref);
+            m = mn;
+            l = l * f + w;
+#pragma unroll
+            for (int i = 0; i < V; i++) acc[i] = acc[i] * f + (d0 + LPH * i < c.hs ? w * value_of<TC>(v[j][i]) : 0.f);
+        }
     }
-    // the groups' sums meet; a group without positions has weight 0
+    // the groups' sums meet, then the wavefronts'; one without positions has weight 0
     float M = m;
 #pragma unroll
     for (int o = LPH; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -88,16 +108,32 @@ __global__ __launch_bounds__(256) void attn_paged_any_kernel(PagedAttnArgs a)
     l *= f;
 #pragma unroll
     for (int o = LPH; o < 64; o <<= 1) l += __shfl_xor(l, o);
-    T* y = (T*)a.y + ((size_t)token * c.H + h) * c.hs;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         float s = acc[i] * f;
 #pragma unroll
         for (int o = LPH; o < 64; o <<= 1) s += __shfl_xor(s, o);
-        if (lane < LPH && d0 + i < c.hs) y[d0 + i] = stored<T>(seen ? s / l : 0.f);
+        if (lane < LPH) sAcc[wave][d0 + LPH * i] = s;
+    }
+    if (lane == 0) { sM[wave] = M; sL[wave] = l; sSeen[wave] = seen; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        M = fmaxf(M, sM[i]);
+        seen = seen || sSeen[i];
+    }
+    T* y = (T*)a.y + ((size_t)token * c.H + h) * c.hs;
+    for (int d = threadIdx.x; d < c.hs; d += 64 * WAVES) {
+        float x = 0.f, n = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) {
+            const float g = exp2f(sM[i] - (M > -INFINITY ? M : 0.f));
+            x += sSeen[i] ? sAcc[i][d] * g : 0.f;
+            n += sSeen[i] ? sL[i] * g : 0.f;
+        }
+        y[d] = stored<T>(seen ? x / n : 0.f);
     }
 }
-
 
 // ---- few rows a sequence: the positions are what is split --------------------------------------------------------------------------
 // 16 rows - tokens times the heads that share a key head - make the columns of one 16 x 16 matrix product, so every key and value is read once
@@ -153,7 +189,7 @@ template <typename T> __device__ __forceinline__ bool not_finite(u32x4 x)
 }
 
 template <typename TQ, typename TC, int HSP>
-__global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs a, SplitArgs w)
+__global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kernel(PagedAttnArgs a, SplitArgs w)
 {
     constexpr bool B16 = sizeof(TQ) == 2;
     constexpr int EPL = 16 / (int)sizeof(TC), NF = HSP / (4 * EPL);            // values a piece, pieces a lane and key
@@ -162,7 +198,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
     constexpr int ROWB = HSP * 2, STAGE = B16 ? KT * ROWB : 0;
     constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2);
     constexpr int SHARED = 4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4;
-    static_assert(HSP == 64 || HSP == 128, "tile");
+    static_assert(HSP == 64 || HSP == 128 || HSP == 256, "tile");
     __shared__ __attribute__((aligned(16))) unsigned char smem[SHARED];
     __shared__ float sM[4][16], sL[4][16];
     __shared__ PagedSpan sSpan;
@@ -455,16 +491,19 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                 const int tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
                 if (hd >= nh) continue;
                 const TQ* q = (const TQ*)a.q + row_at(tk, hd);
-                float qv[2], acc[2] = {0.f, 0.f}, mr = -INFINITY, lr = 0.f;
+                constexpr int VPL = HSP <= 128 ? 2 : HSP / 64;
+                float qv[VPL], acc[VPL], mr = -INFINITY, lr = 0.f;
 #pragma unroll
-                for (int i = 0; i < 2; i++) qv[i] = lane + 64 * i < c.hs ? value_of<TQ>(q[lane + 64 * i]) : 0.f;
+                for (int i = 0; i < VPL; i++) acc[i] = 0.f;
+#pragma unroll
+                for (int i = 0; i < VPL; i++) qv[i] = lane + 64 * i < c.hs ? value_of<TQ>(q[lane + 64 * i]) : 0.f;
                 for (int p = p0; p < p1 && p <= base + tk; p++) {
                     const int e = p / c.pageSize, page = paged_page(table[e], c.pages);
                     if (page < 0) continue;
                     const long long at = page * c.sP + (p - e * c.pageSize) * c.sT + kh * c.sH;
-                    float x = 0.f, val[2];
+                    float x = 0.f, val[VPL];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
+                    for (int i = 0; i < VPL; i++) {
                         const int d = lane + 64 * i;
                         x += d < c.hs ? qv[i] * value_of<TC>(kp[at + d]) : 0.f;
                         val[i] = d < c.hs ? value_of<TC>(vp[at + d]) : 0.f;
@@ -474,13 +513,13 @@ __global__ __launch_bounds__(256, 2) void attn_paged_split_kernel(PagedAttnArgs 
                     mr = mn;
                     lr = lr * f + wt;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) acc[i] = acc[i] * f + wt * val[i];
+                    for (int i = 0; i < VPL; i++) acc[i] = acc[i] * f + wt * val[i];
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if (lane == 0) { sM[i][r] = i ? -INFINITY : mr; sL[i][r] = i ? 0.f : lr; }
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int j = 0; j < VPL; j++)
                         if (lane + 64 * j < HSP) sO[(i * 16 + r) * LDO + lane + 64 * j] = i ? 0.f : acc[j];
                 }
             }
@@ -1038,14 +1077,15 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttnArgs a, C
     }
 }
 
-constexpr int SPLIT_GRID = 512;   // two workgroups a CU
+constexpr int SPLIT_GRID = 512;   // two workgroups a CU; of heads of more than 128, one (64 tokens over 4096 positions, 2 key heads of 256, 16 bits: 103 us, with 512 112)
+constexpr int ANY_MANY = 512;     // tokens' heads from which on the plain kernel has four wavefronts for one
 
 inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // rows and cache in pieces of 16 bytes
 inline bool in_pieces(const PagedCache& c, DType dt, const void* q, const void* y)
 {
     const int e = dt == BF16 || c.ct == BF16 ? 8 : 4;
-    return c.hs <= 128 && c.hs % e == 0 && c.sP % e == 0 && c.sH % e == 0 && c.sT % e == 0 && at16(c.k) && at16(c.v) && at16(q) && at16(y);
+    return c.hs % e == 0 && c.sP % e == 0 && c.sH % e == 0 && c.sT % e == 0 && at16(c.k) && at16(c.v) && at16(q) && at16(y);
 }
 
 }  // namespace
@@ -1082,13 +1122,13 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     p.grid = (int)std::min<double>(CHUNK_GRID, std::max(1.0, p.units / CHUNK_LEAST));
     return p;
 }
-static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : 128; }
+static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : c.hs <= 128 ? 128 : 256; }
 
 size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
 {
     const ChunkPlan p = chunk_plan(c, dt);
     const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
-    const bool chunks = (long long)c.tokens * (c.H / c.kvH) > FEW_ROWS;
+    const bool chunks = c.hs <= 128 && (long long)c.tokens * (c.H / c.kvH) > FEW_ROWS;
     const size_t chunk = !chunks ? 0 : p.pipe ? (size_t)p.pipe * sizeof(int) : (size_t)p.grid * (2 * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) + sizeof(ChunkJoin));
     return std::max(split, chunk);
 }
@@ -1110,7 +1150,7 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         w.tileHeads = (G + w.headTiles - 1) / w.headTiles;
         w.perTile = 16 / w.tileHeads;
         const int most = maxNew > 0 ? std::min(maxNew, c.tokens) : c.tokens;
-        const bool chunks = (long long)most * G > FEW_ROWS && c.tokens > c.batch + c.batch / 4;
+        const bool chunks = c.hs <= 128 && (long long)most * G > FEW_ROWS && c.tokens > c.batch + c.batch / 4;
         w.few = chunks ? FEW_ROWS : 0;
         // Up to two units in one where there are few sequences: going on for a tile takes less than putting two partial results together (us, 12 heads over 100
         // positions, fp32, 9.6 | 8.2).  With many of them a unit has to stand for its length (64 sequences of up to 4096, 8 key heads, 120 | 124).
@@ -1137,14 +1177,20 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
                 if (e != hipSuccess) return e;
             }
             if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 64>), SPLIT_GRID, 256, 0, s, a, w);
-            else hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
+            else if (c.hs <= 128) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
+            else hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 256>), SPLIT_GRID / 2, 256, 0, s, a, w);
             return hipGetLastError();
         }
-        const int x = std::min(c.tokens, 1 << 23);   // an axis of a launch has less than 2^32 threads
-        const dim3 grid(x, (c.H + 3) / 4, (c.tokens + x - 1) / x);
-        if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 16>), grid, 256, 0, s, a);
-        else if (c.hs <= 128) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 32>), grid, 256, 0, s, a);
-        else hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, 64>), grid, 256, 0, s, a);
+        const int x = std::min(c.tokens, 1 << 21);   // an axis of a launch has less than 2^32 threads
+        const dim3 grid(x, c.H, (c.tokens + x - 1) / x);
+        auto any = [&](auto lanes) {
+            constexpr int LPH = decltype(lanes)::value;
+            if ((long long)c.tokens * c.H < ANY_MANY) hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, LPH, 16>), grid, 1024, 0, s, a);
+            else hipLaunchKernelGGL((attn_paged_any_kernel<T_, TC_, 4, LPH, 4>), grid, 256, 0, s, a);
+        };
+        if (c.hs <= 64) any(std::integral_constant<int, 16>{});
+        else if (c.hs <= 128) any(std::integral_constant<int, 32>{});
+        else any(std::integral_constant<int, 64>{});
         return hipGetLastError();
     };
     if (dt == F32) return c.ct == F32 ? go(float(), float()) : go(float(), bf16_t());
