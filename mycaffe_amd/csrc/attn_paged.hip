@@ -25,20 +25,6 @@ template <typename T> __device__ __forceinline__ T stored(float v);
 template <> __device__ __forceinline__ float stored<float>(float v) { return v; }
 template <> __device__ __forceinline__ bf16_t stored<bf16_t>(float v) { return f32_to_bf16(v); }
 
-// the sequence whose rows hold token `i`: the last one that starts at or before it.  All 64 lanes ask.
-__device__ __forceinline__ int sequence_of(const float* starts, int batch, int tokens, int i)
-{
-    int n = 0;
-    for (int b0 = 0; b0 < batch; b0 += 64) {
-        const int b = b0 + (threadIdx.x & 63);
-        const bool before = b < batch && paged_int(starts[b], 0, tokens) <= i;
-        const uint64_t m = __ballot(before);
-        if (!m) break;
-        n = b0 + 64 - __builtin_clzll(m);
-    }
-    return n - 1;
-}
-
 // Any head size up to 256, any strides and addresses, no workspace: a workgroup has one token's head, a group of LPH lanes of its WAVES wavefronts
 // every (64 WAVES / LPH)-th position, V values a lane, value by value in runs of LPH; ANY_DEEP positions' reads are under way together.  What
 // bounds it is waiting for them, and every head reads its keys for itself.  Sixteen wavefronts where there are few tokens' heads, four else (us: one token over
@@ -140,7 +126,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_any_kernel(PagedAttnArg
 // for all of them: what bounds this kernel is reading the cache.  All positions of all sequences, in units of four tiles of KT positions, are
 // one list that is dealt to the workgroups in equal runs, whatever the lengths: a run ends inside an item (a sequence's key head and row
 // tile), which the last workgroup to finish puts together.  A wavefront has every fourth tile, with statistics of its own; tiles of the wavefronts
-// meet in LDS at the end of an item.
+// meet in LDS at the end of an item.  Measured: 64 sequences of up to 4096 positions, 32 heads on 8 of 128, 16 bits, 559 MB 117 us (4.8 TB/s, what a large copy
+// reaches); one of 131000, 537 MB 120 us; one of 100, 12 heads of 64 in fp32, 7.2 us.
 //
 // Scores are S^T = K Q^T, so that a lane has one row: register v of a tile holds key 4 (lane / 16) + v of row lane % 16, which is the operand
 // layout that O^T = V^T P^T wants of P (which slot of the contraction is which key only has to agree between the two).  Keys go from memory to the
@@ -622,6 +609,8 @@ __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kern
 // all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
 // follow each other by key head), whose L2 then holds that head's keys and values.  The
 // blocks of all tiles are one list that is dealt to the workgroups in equal runs; tiles that a run ends in are put together by a launch behind this one.
+// Measured: 8 prompts of 2048, 12 heads of 64, fp32, 366 us (0.14 PFLOP/s of useful products, 0.9 of bf16 ones, which a large library product has 1.2 of);
+// a step of 12 chunks and single tokens, ragged, 60 us and 7 for the launch behind: half of it starts, ends and tiles that are not full.
 // Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
 template <int PARTS> struct Parts { u32x4 p[PARTS]; };
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }

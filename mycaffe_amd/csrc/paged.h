@@ -6,6 +6,9 @@
 // no page.  Host and device compile the same lines (the host's test feeds them everything that can go wrong).
 #pragma once
 #include <stdint.h>
+#ifdef __HIPCC__
+#include <hip/hip_runtime.h>
+#endif
 
 #include <algorithm>
 #include <utility>
@@ -59,6 +62,21 @@ PAGED_FN int paged_place(int block, int W)
     const int x = block & 7, k = block >> 3, each = W >> 3, rest = W & 7;
     return k < each + (x < rest ? 1 : 0) ? x * each + (x < rest ? x : rest) + k : -1;
 }
+#ifdef __HIPCC__
+// the sequence whose rows hold token `i`: the last one that starts at or before it.  All 64 lanes ask.
+__device__ __forceinline__ int sequence_of(const float* starts, int batch, int tokens, int i)
+{
+    int n = 0;
+    for (int b0 = 0; b0 < batch; b0 += 64) {
+        const int b = b0 + (threadIdx.x & 63);
+        const bool before = b < batch && paged_int(starts[b], 0, tokens) <= i;
+        const uint64_t m = __ballot(before);
+        if (!m) break;
+        n = b0 + 64 - __builtin_clzll(m);
+    }
+    return n - 1;
+}
+#endif
 // Units of the first t tiles of a chunk: tiles of perTile tokens, the first of them over `before` + perTile positions, every further one over perTile more;
 // about 32 << shift positions a unit, and one for the tile
 PAGED_FN int paged_units_before(int before, int perTile, int t, int shift)
