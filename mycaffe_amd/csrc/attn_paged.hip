@@ -175,21 +175,29 @@ template <typename T> __device__ __forceinline__ bool not_finite(u32x4 x)
     return r;
 }
 
+template <typename TQ, typename TC, int HSP> struct SplitShared {
+    static constexpr int KT = sizeof(TC) == 4 ? 16 : 32, STAGE = sizeof(TQ) == 2 ? KT * HSP * 2 : 0, LDO = HSP + 4;
+    __attribute__((aligned(16))) unsigned char mem[4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4];
+    float m[4][16], l[4][16];
+    PagedSpan span;
+    int scan[4], seq, at, bad, ticket;
+};
+// what workgroup `block` of `blocks` has of the list
 template <typename TQ, typename TC, int HSP>
-__global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kernel(PagedAttnArgs a, SplitArgs w)
+__device__ __forceinline__ void split_run(const PagedAttnArgs& a, const SplitArgs& w, int block, int blocks, SplitShared<TQ, TC, HSP>& shared)
 {
+    typedef SplitShared<TQ, TC, HSP> S;
     constexpr bool B16 = sizeof(TQ) == 2;
     constexpr int EPL = 16 / (int)sizeof(TC), NF = HSP / (4 * EPL);            // values a piece, pieces a lane and key
     constexpr int KG = sizeof(TC) == 4 ? 1 : 2, KT = 16 * KG, UNIT = 4 * KT;   // groups of 16 keys a tile
     constexpr int VE = sizeof(TC) == 4 ? 4 : HSP / 16 < 8 ? HSP / 16 : 8, NH = HSP / (16 * VE), NO = HSP / 16;
-    constexpr int ROWB = HSP * 2, STAGE = B16 ? KT * ROWB : 0;
-    constexpr int LDO = HSP + 4, PART = 16 * (HSP + 2);
-    constexpr int SHARED = 4 * STAGE > 4 * 16 * LDO * 4 ? 4 * STAGE : 4 * 16 * LDO * 4;
-    static_assert(HSP == 64 || HSP == 128 || HSP == 256, "tile");
-    __shared__ __attribute__((aligned(16))) unsigned char smem[SHARED];
-    __shared__ float sM[4][16], sL[4][16];
-    __shared__ PagedSpan sSpan;
-    __shared__ int sScan[4], sSeq, sAt, sBad, sTicket;
+    constexpr int ROWB = HSP * 2, STAGE = S::STAGE, LDO = S::LDO, PART = 16 * (HSP + 2);
+    static_assert(KT == S::KT && (HSP == 64 || HSP == 128 || HSP == 256), "tile");
+    unsigned char* smem = shared.mem;
+    auto &sM = shared.m, &sL = shared.l;
+    auto& sSpan = shared.span;
+    auto& sScan = shared.scan;
+    int &sSeq = shared.seq, &sAt = shared.at, &sBad = shared.bad, &sTicket = shared.ticket;
     float* sO = (float*)smem;                                                   // [wavefront][row][LDO], once the stages are done with
 
     const PagedCache& c = a.c;
@@ -206,10 +214,10 @@ __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kern
     int b = 0, local, lo, hi;
     if (c.batch == 1) {   // no sums, no sequence to be found
         sp = span_at(c, 0);
-        runs = PagedRuns(work_of(sp), gridDim.x, 1);
-        if ((int)blockIdx.x >= runs.W) return;
-        local = lo = runs.begin(blockIdx.x);
-        hi = runs.begin(blockIdx.x + 1);
+        runs = PagedRuns(work_of(sp), blocks, 1);
+        if (block >= runs.W) return;
+        local = lo = runs.begin(block);
+        hi = runs.begin(block + 1);
     } else {
         const PagedSpan none = {0, 0, 0};
         PagedSpan mine = tid < c.batch ? span_of(tid) : none;
@@ -220,10 +228,10 @@ __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kern
             total = paged_sum(total, more);
         }
         if (uniform(total) >= PAGED_MOST) return;
-        runs = PagedRuns(uniform(total), gridDim.x, 1);
-        if ((int)blockIdx.x >= runs.W) return;
-        lo = runs.begin(blockIdx.x);
-        hi = runs.begin(blockIdx.x + 1);
+        runs = PagedRuns(uniform(total), blocks, 1);
+        if (block >= runs.W) return;
+        lo = runs.begin(block);
+        hi = runs.begin(block + 1);
         // the sequence that has unit `lo`
         for (int b0 = 0, base = 0;;) {
             if (at <= lo && lo < at + work) { sSeq = b0 + tid; sAt = at; sSpan = mine; }
@@ -514,7 +522,7 @@ __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kern
         }
         const bool whole = count == units;
         const int rows = nt * w.tileHeads, pairs = c.hs >> 1;
-        float* part = w.part + ((size_t)blockIdx.x * 2 + (unit0 == 0 ? 1 : 0)) * PART;
+        float* part = w.part + ((size_t)block * 2 + (unit0 == 0 ? 1 : 0)) * PART;
         for (int e = tid; e < rows * pairs; e += 256) {
             const int r = e / pairs, d = 2 * (e - r * pairs), tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
             if (hd >= nh) continue;
@@ -610,7 +618,7 @@ __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kern
 // follow each other by key head), whose L2 then holds that head's keys and values.  The
 // blocks of all tiles are one list that is dealt to the workgroups in equal runs; tiles that a run ends in are put together by a launch behind this one.
 // Measured: 8 prompts of 2048, 12 heads of 64, fp32, 366 us (0.14 PFLOP/s of useful products, 0.9 of bf16 ones, which a large library product has 1.2 of);
-// a step of 12 chunks and single tokens, ragged, 60 us and 7 for the launch behind: half of it starts, ends and tiles that are not full.
+// a step of 12 chunks and single tokens, ragged, 64 us with the launch behind: half of it starts, ends and tiles that are not full.
 // Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
 template <int PARTS> struct Parts { u32x4 p[PARTS]; };
 __device__ __forceinline__ uint32_t upper_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
@@ -636,20 +644,28 @@ __device__ __forceinline__ float pair_sum(uint32_t pair, float l)
 
 // Products in fp32 are sums of products of bf16 parts: of the nine of two values of three parts the six that reach fp32's last bits, exact each and
 // added in fp32; over a 16-bit cache the three that there are.  (32 x 32 x 16 of them take 32 cycles a part, in fp32 512: 2.7 and 5.3 times as long.)
+template <typename TQ, typename TC, int HSP> struct ChunkShared {
+    static constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;              // parts of a query and a weight, of a key and a value
+    static constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, LD = HSP + 8;          // keys a block, values a row
+    __attribute__((aligned(16))) bf16_t k[NK][KB * LD], v[NK][KB * LD];
+    long long place[2][KB];
+    uint64_t given[2];
+    int bad, front;
+};
 template <typename TQ, typename TC, int HSP>
-__global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs a, ChunkArgs w)
+__device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArgs& w, int block, int blocks, ChunkShared<TQ, TC, HSP>& shared)
 {
     typedef FlashTraits<bf16_t> TR;
-    constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;                     // parts of a query and a weight, of a key and a value
-    constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
+    typedef ChunkShared<TQ, TC, HSP> S;
+    constexpr int NQ = S::NQ, NK = S::NK, KB = S::KB, LD = S::LD;
+    constexpr int KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
-    constexpr int LD = HSP + 8;                                                                   // values a row in LDS
     constexpr int AHEAD = 2;                                                                      // value fragments under way
     constexpr int PART = 128 * (HSP + 2);
-    __shared__ __attribute__((aligned(16))) bf16_t sK[NK][KB * LD], sV[NK][KB * LD];
-    __shared__ long long sPlace[2][KB];
-    __shared__ uint64_t sGiven[2];
-    __shared__ int sBad, sFront;
+    auto &sK = shared.k, &sV = shared.v;
+    auto& sPlace = shared.place;
+    auto& sGiven = shared.given;
+    int &sBad = shared.bad, &sFront = shared.front;
 
     const PagedCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
@@ -659,16 +675,16 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     ChunkTile left = {};
     int u = 0, hi = 1;
     if (w.redo) {
-        if (!w.redo[blockIdx.x / w.pair]) return;
-        left = chunk_tile(c, w, blockIdx.x / w.pair);
+        if (!w.redo[block / w.pair]) return;
+        left = chunk_tile(c, w, block / w.pair);
         if (left.b < 0) return;
         at.b = left.b;
         at.sp = span_at(c, at.b);
     } else {
-        at = chunk_start(c, w, blockIdx.x, gridDim.x);
-        if (tid == 0) w.join[blockIdx.x].place = -1;
+        at = chunk_start(c, w, block, blocks);
+        if (tid == 0) w.join[block].place = -1;
         if (at.place < 0) return;
-        const PagedRuns runs(at.total, gridDim.x, CHUNK_LEAST);
+        const PagedRuns runs(at.total, blocks, CHUNK_LEAST);
         u = runs.begin(at.place);
         hi = runs.begin(at.place + 1);
     }
@@ -679,7 +695,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
     int group, tile, u0 = 0, u1 = 1, units = 1;
     if (w.redo) {
         group = left.kh * w.headTiles + left.ht;
-        tile = left.tile * w.pair + (int)(blockIdx.x % w.pair);
+        tile = left.tile * w.pair + (block % w.pair);
     } else {
         const int tiles = chunk_tiles(c, w, sp), each = paged_units_before(before, w.perTile, tiles, w.unit), r = at.local - at.local / each * each;
         group = at.local / each;
@@ -989,8 +1005,8 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
         }
     }
     if (u0 == 0 && !whole && tid == 0) {
-        const PagedRuns runs(at.total, gridDim.x, CHUNK_LEAST);
-        w.join[blockIdx.x] = ChunkJoin{at.place, runs.of(u + units - 1), sp.first + j0, h0, nt, nh, {0, 0}};
+        const PagedRuns runs(at.total, blocks, CHUNK_LEAST);
+        w.join[block] = ChunkJoin{at.place, runs.of(u + units - 1), sp.first + j0, h0, nt, nh, {0, 0}};
     }
     // ---- the next piece ----
     const int done = u1 - u0;
@@ -1007,6 +1023,23 @@ __global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs 
         __syncthreads();   // LDS is read no more
     }
     }
+}
+
+// single tokens and other short ones: the split of positions by itself
+template <typename TQ, typename TC, int HSP>
+__global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_paged_split_kernel(PagedAttnArgs a, SplitArgs w)
+{
+    __shared__ SplitShared<TQ, TC, HSP> shared;
+    split_run<TQ, TC, HSP>(a, w, blockIdx.x, gridDim.x, shared);
+}
+// chunks, and the short ones among them: the first `chunks` workgroups have the chunks' list, the others the split's (us, two launches | one, the split behind | in front: a step
+// of chunks and single tokens in fp32 72.4 | 64.3 | 67.2, chunks alone 47.6 | 43.7 | 45.1)
+template <typename TQ, typename TC, int HSP>
+__global__ __launch_bounds__(256, 2) void attn_paged_chunk_kernel(PagedAttnArgs a, ChunkArgs w, SplitArgs few, int chunks)
+{
+    __shared__ union { SplitShared<TQ, TC, HSP> split; ChunkShared<TQ, TC, HSP> chunk; } shared;
+    if ((int)blockIdx.x < chunks) chunk_run<TQ, TC, HSP>(a, w, blockIdx.x, chunks, shared.chunk);
+    else split_run<TQ, TC, HSP>(a, few, blockIdx.x - chunks, gridDim.x - chunks, shared.split);
 }
 
 // Tiles that a run ended in put together, 16 rows a workgroup, 16 lanes a row, from what the workgroup that began one has written down.
@@ -1101,7 +1134,7 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
     const long long having = std::min<long long>(c.batch, (long long)c.tokens * G / (FEW_ROWS + 1)), groups = (long long)c.kvH * p.headTiles;
     const long long whole = (long long)c.tokens / (2 * p.perTile) * groups, pipe = whole + having * groups;
     p.pipe = 0;
-    if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 1 << 23 &&
+    if (dt == BF16 && ((c.hs == 128 && whole >= PIPE_TILES_128) || (c.hs == 64 && whole >= PIPE_TILES_64)) && (long long)c.tokens * G >= 256ll * c.batch && pipe < 1 << 22 &&
         ((c.pages - 1) * c.sP + (c.pageSize - 1) * c.sT) >> 3 < 0xffffffffll)
         p.pipe = (int)pipe;
     // the list is counted in 32 bits
@@ -1113,13 +1146,15 @@ static ChunkPlan chunk_plan(const PagedCache& c, DType dt)
 }
 static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : c.hs <= 128 ? 128 : 256; }
 
+// the split kernel's partial results, and behind them the chunk kernel's or the pipe kernel's flags
+static size_t split_bytes(const PagedCache& c) { return (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float); }
+
 size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
 {
     const ChunkPlan p = chunk_plan(c, dt);
-    const size_t split = (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float);
     const bool chunks = c.hs <= 128 && (long long)c.tokens * (c.H / c.kvH) > FEW_ROWS;
     const size_t chunk = !chunks ? 0 : p.pipe ? (size_t)p.pipe * sizeof(int) : (size_t)p.grid * (2 * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) + sizeof(ChunkJoin));
-    return std::max(split, chunk);
+    return split_bytes(c) + chunk;
 }
 size_t attn_paged_tickets() { return SPLIT_GRID; }
 
@@ -1150,20 +1185,20 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         if (workspace && in_pieces(c, dt, q, y) && units < PAGED_MOST && fits) {
             if (chunks) {
                 const ChunkPlan p = chunk_plan(c, dt);
-                ChunkArgs g = {(float*)workspace, (ChunkJoin*)((float*)workspace + (size_t)p.grid * 2 * CHUNK_ROWS * (padded_size(c) + 2)), FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.unit, p.pipe ? 2 : 1, p.pipe ? (const int*)workspace : nullptr};
+                float* own = (float*)((char*)workspace + split_bytes(c));
+                ChunkArgs g = {own, (ChunkJoin*)(own + (size_t)p.grid * 2 * CHUNK_ROWS * (padded_size(c) + 2)), FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.unit, p.pipe ? 2 : 1, p.pipe ? (const int*)own : nullptr};
                 if (p.pipe) {
-                    const hipError_t e = attn_paged_pipe_launch(s, a, g, p.pipe, (int*)workspace);
+                    const hipError_t e = attn_paged_pipe_launch(s, a, g, p.pipe, (int*)own);
                     if (e != hipSuccess) return e;
                 }
                 const int grid = p.pipe ? 2 * p.pipe : p.grid;
-                if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid, 256, 0, s, a, g);
-                else hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 128>), grid, 256, 0, s, a, g);
+                if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 64>), grid + SPLIT_GRID, 256, 0, s, a, g, w, grid);
+                else hipLaunchKernelGGL((attn_paged_chunk_kernel<T_, TC_, 128>), grid + SPLIT_GRID, 256, 0, s, a, g, w, grid);
                 if (!p.pipe && grid > 1) {
                     if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_join_kernel<T_, 64>), dim3(grid, 8), 256, 0, s, a, g);
                     else hipLaunchKernelGGL((attn_paged_join_kernel<T_, 128>), dim3(grid, 8), 256, 0, s, a, g);
                 }
-                const hipError_t e = hipGetLastError();
-                if (e != hipSuccess) return e;
+                return hipGetLastError();
             }
             if (c.hs <= 64) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 64>), SPLIT_GRID, 256, 0, s, a, w);
             else if (c.hs <= 128) hipLaunchKernelGGL((attn_paged_split_kernel<T_, TC_, 128>), SPLIT_GRID, 256, 0, s, a, w);
