@@ -660,7 +660,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     constexpr int NQ = S::NQ, NK = S::NK, KB = S::KB, LD = S::LD;
     constexpr int KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
-    constexpr int AHEAD = 2;                                                                      // value fragments under way
+    constexpr int AHEAD = NK == 3 && HSP == 128 ? 1 : 2;                                          // value fragments under way (1: registers are full)
     constexpr int PART = 128 * (HSP + 2);
     auto &sK = shared.k, &sV = shared.v;
     auto& sPlace = shared.place;
@@ -858,7 +858,8 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
                 }
         }
         // values travel while the weights are made, AHEAD fragments in front of the product that they are for (us with none | 1 | 2 | 4: a step of chunks and
-        // single tokens in fp32 73.9 | 73.2 | 72.0 | 73.3, 4 sequences of 8 new tokens over 4096 in 16 bits 37.3 | 37.2 | 36.7 | 38.8)
+        // single tokens in fp32 73.9 | 73.2 | 72.0 | 73.3, 4 sequences of 8 new tokens over 4096 in 16 bits 37.3 | 37.2 | 36.7 | 38.8; fp32 heads
+        // of 128, 8 chunks of 1500 over 3000, 826 with 1, 873 with 2)
         u32x4 vf[AHEAD][NK];
         auto value = [&](int n) {
             const int j = n / (2 * DT), x = n / DT % 2, i = n % DT;
