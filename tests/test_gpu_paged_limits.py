@@ -191,3 +191,18 @@ def test_wide_and_odd_heads_with_values_that_are_not_finite(dev, hs, act16, cach
     clean = [0, 1, 2, 3, 4, 5, 12]
     assert (abs(got[clean] - want[clean]) <= tol[clean]).all()
     assert np.isnan(got[6:12, :, 5]).all()
+
+
+MANY = [
+    # more sequences than one scan has threads, chunks and single tokens among each other
+    ("chunks", 4, 2, 64, 16, [(1 if b % 3 else 20 + b % 17, 40 + 13 * b % 90, 0) for b in range(600)], (True, False)),
+    ("long_chunks_64", 8, 1, 64, 16, [(1 if b % 29 == 0 else 40 + b % 5, 60 + b % 50, 16 * (b % 2)) for b in range(300)], (True,)),
+    ("long_chunks_128", 8, 1, 128, 32, [(1 if b % 29 == 0 else 40 + b % 5, 60 + b % 50, 0) for b in range(300)], (True,)),
+]
+
+
+@pytest.mark.parametrize("name,H,kvH,hs,page,seqs,types", MANY, ids=[m[0] for m in MANY])
+def test_more_chunks_than_a_scan(dev, name, H, kvH, hs, page, seqs, types):
+    for act16 in types:
+        rng = np.random.default_rng(38)
+        check_attention(dev, rng, Cache(dev, rng, seqs, kvH, hs, page, "head", act16, pad=3), H, act16)
