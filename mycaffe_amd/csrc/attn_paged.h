@@ -33,17 +33,21 @@ __device__ __forceinline__ PagedSpan span_at(const PagedCache& c, int b)
     return uniform(paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, c.maxPages * c.pageSize));
 }
 
+// over a wavefront, numbers up to PAGED_MOST: the sums up to and with the lane's own (a row of sixteen lanes, then the rows before it)
+__device__ __forceinline__ int wave_scan(int x)
+{
+    x = paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));   // row_shr 1, 2, 4, 8
+    x = paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));   // row_bcast 15 to rows 1 and 3
+    return paged_sum(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));   // row_bcast 31 to rows 2 and 3
+}
 // over 256 threads, numbers up to PAGED_MOST: the sum of those before the thread's own (PAGED_MOST: that or more), and of all of them
 __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x = paged_sum(x, y);
-    }
-    const int mine = __shfl_up(x, 1);
+    const int x = wave_scan(v), mine = __builtin_amdgcn_update_dpp(0, x, 0x138, 0xf, 0xf, false);   // wave_shr 1
     __syncthreads();
     if (lane == 63) sums[wave] = x;
     __syncthreads();
@@ -54,7 +58,7 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
         sum = paged_sum(sum, sums[i]);
     }
     *all = sum;
-    return lane ? paged_sum(before, mine) : before;
+    return paged_sum(before, mine);
 }
 
 // The chunk kernel's list: sequences, their key heads and head tiles, their tiles, in units of about 32 positions of a tile.  All 256 threads.

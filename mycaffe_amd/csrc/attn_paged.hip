@@ -218,6 +218,17 @@ __device__ __forceinline__ void split_run(const PagedAttnArgs& a, const SplitArg
         if (block >= runs.W) return;
         local = lo = runs.begin(block);
         hi = runs.begin(block + 1);
+    } else if (c.batch <= 64) {   // every wavefront for itself
+        const PagedSpan mine = lane < c.batch ? span_of(lane) : PagedSpan{0, 0, 0};
+        const int work = lane < c.batch ? work_of(mine) : 0, upTo = wave_scan(work), total = __builtin_amdgcn_readlane(upTo, 63);
+        if (total >= PAGED_MOST) return;
+        runs = PagedRuns(total, blocks, 1);
+        if (block >= runs.W) return;
+        lo = runs.begin(block);
+        hi = runs.begin(block + 1);
+        b = __builtin_ctzll(__ballot(lo < upTo));   // the sequence that has unit `lo`
+        local = lo - (__builtin_amdgcn_readlane(upTo, b) - __builtin_amdgcn_readlane(work, b));
+        sp = PagedSpan{__builtin_amdgcn_readlane(mine.first, b), __builtin_amdgcn_readlane(mine.count, b), __builtin_amdgcn_readlane(mine.len, b)};
     } else {
         const PagedSpan none = {0, 0, 0};
         PagedSpan mine = tid < c.batch ? span_of(tid) : none;
