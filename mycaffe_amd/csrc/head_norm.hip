@@ -227,7 +227,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(HeadNormArgs a)
                 piece_floats<T, V>(x[i], xv);
                 piece_floats<T, V>(g[i], gv);
                 turn<V>(gv, c, s);
-                const float r = head_rms<LPH, V>(xv, a.inv_hs, a.eps);
+                // a lane group without a position has no part in the sums, also where its zeros have no norm (eps 0)
+                const float rms = head_rms<LPH, V>(xv, a.inv_hs, a.eps), r = live ? rms : 0.f;
                 float dot = 0.f;
 #pragma unroll
                 for (int e = 0; e < V; e++) {
