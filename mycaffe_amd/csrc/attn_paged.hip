@@ -655,13 +655,25 @@ __device__ __forceinline__ float pair_sum(uint32_t pair, float l)
 
 // Products in fp32 are sums of products of bf16 parts: of the nine of two values of three parts the six that reach fp32's last bits, exact each and
 // added in fp32; over a 16-bit cache the three that there are.  (32 x 32 x 16 of them take 32 cycles a part, in fp32 512: 2.7 and 5.3 times as long.)
+// Three parts hold every bit from 2^-133 up, all 24 of values from 2^-110 up.  What is cut off of smaller queries and keys changes no score if the other factor is below
+// 2^65 (2^-133 2^65 2^8 a score, times a scale of up to SCALE: 2^-29), and of values no sum that is not small itself.  Rows where a factor is larger, or a sum of weights times
+// values is below SMALL of the sum of weights, are made one by one (below).  A weight below 2^-110 of its row's largest loses bits and is left as it is.
+// (us, 2 prompts of 1024, 12 heads of 64, as before 43; a column of values all zero, looked through for smaller ones, 59 for 47 in the same loop; rows one by one 4800.)
+constexpr float SCALE = 0x1p31f, SMALL = 0x1p-100f;
+// 2^65, from which on an exponent's two upper bits are set: of a piece, what has them so in `large_bits` (infinities and NaN among them)
+template <typename T> __device__ __forceinline__ void take_large(u32x4 x, uint32_t& bits)
+{
+#pragma unroll
+    for (int i = 0; i < 4; i++) bits |= x[i] & (x[i] << 1);
+}
+template <typename T> constexpr uint32_t large_bits() { return sizeof(T) == 4 ? 0x40000000u : 0x40004000u; }
 template <typename TQ, typename TC, int HSP> struct ChunkShared {
     static constexpr int NQ = sizeof(TQ) == 4 ? 3 : 1, NK = sizeof(TC) == 4 ? 3 : 1;              // parts of a query and a weight, of a key and a value
     static constexpr int KB = NK == 1 && (NQ == 1 || HSP == 64) ? 64 : 32, LD = HSP + 8;          // keys a block, values a row
     __attribute__((aligned(16))) bf16_t k[NK][KB * LD], v[NK][KB * LD];
     long long place[2][KB];
     uint64_t given[2];
-    int bad, front;
+    int bad, front, zero;
 };
 template <typename TQ, typename TC, int HSP>
 __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArgs& w, int block, int blocks, ChunkShared<TQ, TC, HSP>& shared)
@@ -676,7 +688,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     auto &sK = shared.k, &sV = shared.v;
     auto& sPlace = shared.place;
     auto& sGiven = shared.given;
-    int &sBad = shared.bad, &sFront = shared.front;
+    int &sBad = shared.bad, &sFront = shared.front, &sZero = shared.zero;
 
     const PagedCache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l32 = lane & 31, half = lane >> 5;
@@ -720,7 +732,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     const int kh = group / w.headTiles, ht = group - kh * w.headTiles;
     const int j0 = tile * w.perTile, nt = min(w.perTile, sp.count - j0), base = sp.len - sp.count + j0;
     if (nt <= 0) return;   // (redo: the second half of a tile that has none)
-    if (tid == 0) sBad = 0;
+    if (tid == 0) sBad = sZero = 0;
     const int h0 = kh * G + ht * w.tileHeads, nh = min(w.tileHeads, G - ht * w.tileHeads);
     const int end = min(sp.len, base + nt);                                                       // positions that some row sees
     const float* table = c.table + (size_t)b * c.maxPages;
@@ -739,7 +751,8 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     const int waveEnd = 32 * wave / w.tileHeads < nt ? min(end, base + min((32 * wave + 31) / w.tileHeads, nt - 1) + 1) : 0, waveOpen = base + 32 * wave / w.tileHeads + 1;   // past what any, and what every row sees
     auto row_at = [&](int t, int h) { return ((size_t)(sp.first + j0 + t) * c.H + h0 + h) * c.hs; };
     const u32x4 zero4 = {0u, 0u, 0u, 0u};
-    bool bad = false;
+    bool bad = NQ > 1 && !(c2 < SCALE);
+    uint32_t largeQ = 0;
     Parts<NQ> qf[KF];
     {
         const TQ* q = (const TQ*)a.q + (live ? row_at(token, head) : 0);
@@ -765,12 +778,12 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
 #pragma unroll
                     for (int i = 0; i < NQ; i++) qf[f].p[i][e] = out[i];
                 }
-                // parts of a value that is not finite do not add up to it
 #pragma unroll
-                for (int e = 0; e < 8; e++) bad = bad || (__float_as_uint(x[e]) & 0x7f800000u) == 0x7f800000u;
+                for (int e = 0; e < 8; e++) largeQ |= __float_as_uint(x[e]) & (__float_as_uint(x[e]) << 1);
             }
         }
     }
+    if (NQ > 1) bad = bad || (largeQ & large_bits<float>());
     // pages given up at the front are passed over
     if (wave == 0) {
         int front = 0;
@@ -823,6 +836,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     for (int kb = first; kb < stop; kb++) {
         const uint64_t given = sGiven[kb & 1];
         __syncthreads();                                                         // everybody has left the previous block
+        uint32_t large = 0;
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int r = tid / CPR + RPP * i, d = (tid % CPR) * EPL;
@@ -842,10 +856,14 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
                     *(uint2*)(sV[e] + r * LD + d) = make_uint2(v[0][e], v[1][e]);
                 }
             }
-            // what only some rows see, and where parts are multiplied anything, has to be finite
+            // what only some rows see, and where parts are multiplied anything, has to be finite (parts of a value that is not do not add up to it)
             if (NK > 1 || NQ > 1 || kb * KB + KB > base + 1) bad = bad || not_finite<TC>(rv[i]);
-            if (NK > 1 || NQ > 1) bad = bad || not_finite<TC>(rk[i]);
+            if (NK > 1 || NQ > 1) {
+                take_large<TC>(rk[i], large);
+                asm volatile("" : "+v"(large));   // here and now: else pieces are kept for it until the end, and registers spilt (8 chunks of 1500 over 3000, fp32, 940 us for 840)
+            }
         }
+        if (NK > 1 || NQ > 1) bad = bad || (large & large_bits<TC>());
         if (wave == 0 && kb + 2 < stop) publish(kb + 2, ahead);
         __syncthreads();
         if (kb + 1 < stop) load((kb + 1) & 1);
@@ -954,8 +972,54 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
         }
     }
     l = add_lane_xor<32>(l);
+    if constexpr (NQ > 1) {
+        // sums that are small or zero
+        float least = INFINITY;
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                const float x = fminf(fminf(fabsf(o[i][v]), fabsf(o[i][v + 1])), fminf(fabsf(o[i][v + 2]), fabsf(o[i][v + 3])));
+                least = fminf(least, 32 * i + 2 * v + 4 * half < c.hs ? x : INFINITY);
+            }
+        if (__any(live && least < l * SMALL)) {
+            bool zero = false;
+            if (live)
+#pragma unroll
+                for (int i = 0; i < DT; i++)
+#pragma unroll
+                    for (int v = 0; v < 16; v++)
+                        if (32 * i + 8 * (v >> 2) + 4 * half < c.hs) {
+                            zero = zero || o[i][v] == 0.f;
+                            bad = bad || (fabsf(o[i][v]) < l * SMALL && o[i][v] != 0.f);
+                        }
+            if (__any(zero) && lane == 0) sZero = 1;
+        }
+    }
     if (__any(bad) && lane == 0) sBad = 1;
     __syncthreads();
+    if (NK > 1 && sZero && !sBad) {
+        // of values that are zero, or of such as lie below the last part?  (Reads of DEEP positions under way.)
+        constexpr int DEEP = 4;
+        const int d = min((tid % CPR) * EPL, c.hs - EPL), until = min(stop * KB, end);
+        bool found = false;
+        for (int p0 = first * KB + tid / CPR; p0 < until; p0 += DEEP * RPP) {
+            float e[DEEP];
+            u32x4 x[DEEP];
+#pragma unroll
+            for (int i = 0; i < DEEP; i++) e[i] = page_at(min(p0 + i * RPP, until - 1));
+#pragma unroll
+            for (int i = 0; i < DEEP; i++) {
+                const long long at = place_of(min(p0 + i * RPP, until - 1), e[i]);
+                x[i] = at >= 0 ? *(const u32x4*)(vp + at + d) : zero4;
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * DEEP; i++) found = found || (x[i / 4][i % 4] & 0x7fffffffu) - 1 < __float_as_uint(0x1p-110f) - 1;
+        }
+        __syncthreads();
+        if (__any(found) && lane == 0) sBad = 1;
+        __syncthreads();
+    }
 
     float* part = w.part + ((size_t)at.place * 2 + (u0 == 0 ? 1 : 0)) * PART;
     if (!sBad) {
@@ -980,7 +1044,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
         }
     } else {
         // A value that is not finite lies where only some of the rows look, and weights of zero would not keep it from the others, or it has been cut in
-        // parts.  Row by row, then.
+        // parts, or parts do not hold what matters.  Row by row, then.
         for (int r = wave; r < nt * w.tileHeads; r += 4) {
             const int tk = r / w.tileHeads, hd = r - tk * w.tileHeads;
             if (hd >= nh) continue;
