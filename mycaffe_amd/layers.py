@@ -948,6 +948,8 @@ class TransformerBlockLayer:
                  enable_key_value_cache=False, qk_norm=False):
         if block_type not in ("causal_self_attention", "encoder"):
             raise ValueError(block_type)
+        if qk_norm and block_type != "causal_self_attention":
+            raise ValueError("norms of queries and keys are the causal self attention's (block type %s)" % block_type)
         self.cuda = cuda
         self.block_type = block_type
         self.llama = enable_llama_style_head
