@@ -334,17 +334,17 @@ class SoftmaxLayer:
 
 class PagedSequences:
     """Which sequences are being served and which pages of a cache hold them (no counterpart in the reference, whose layer keeps one sequence of one
-    length).  One object serves all layers of a model: they keep pages of the same numbers.
+    length).  One object serves all attention layers of a model: they keep pages of the same numbers.
 
     ``Step({name: new tokens})`` before a model's pass: every named sequence grows by its tokens, in the order given, which is the order of the rows of
     the pass; new names begin new sequences.  ``Drop(name, positions)`` gives up a sequence's oldest pages, ``End(name)`` all of them.  ``Dispose()``
-    frees the pages of all layers.
+    frees the pages of all layers and the angles that they share.
     """
 
     def __init__(self, cuda, pages, page_size, max_pages):
         self.cuda, self.pages, self.page_size, self.max_pages = cuda, pages, page_size, max_pages
         self._free = list(range(pages - 1, -1, -1))
-        self._table, self._len, self._caches = {}, {}, {}
+        self._table, self._len, self._caches, self._ropes = {}, {}, {}, {}
         self.table, self.starts, self.lens = (Blob(cuda) for _ in range(3))
         self.batch = self.tokens = self.max_new = 0
 
@@ -388,10 +388,20 @@ class PagedSequences:
             self._caches[layer] = tuple(Blob(self.cuda, (self.pages, heads, self.page_size, size), half) for _ in range(2))
         return self._caches[layer]
 
+    def Rope(self, heads, size, theta):
+        """The handle with the angles of every position that a sequence can have: one for all layers of this head size and base."""
+        if (size, theta) not in self._ropes:
+            positions = self.max_pages * self.page_size
+            self._ropes[size, theta] = self.cuda.CreateRope(0, 0, positions * heads * size, 1, positions, heads, size, theta)
+        return self._ropes[size, theta]
+
     def Dispose(self):
         for blob in [self.table, self.starts, self.lens] + [b for kv in self._caches.values() for b in kv]:
             blob.Dispose()
+        for rope in self._ropes.values():
+            self.cuda.FreeRope(rope)
         self._caches.clear()
+        self._ropes.clear()
 
 
 class CausalSelfAttentionLayer:
@@ -430,7 +440,6 @@ class CausalSelfAttentionLayer:
         self._masks, self._ropes = _Kept(Blob.Dispose), _Kept(cuda.FreeRope)
         self.hCudnn = self.hAttn = self.hRope = 0
         self._set_for = None
-        self._page_rope = None
 
     def Setup(self, bottom, w_attn, b_attn, w_proj, b_proj, w_qnorm=None, w_knorm=None):
         self.c_attn.Setup(bottom, w_attn, b_attn)
@@ -554,18 +563,14 @@ class CausalSelfAttentionLayer:
         if N != seqs.tokens:
             raise ValueError("the pass has %d tokens, the step %d" % (N, seqs.tokens))
         k, v = seqs.Cache(self, H, hs, self.half)
-        positions = seqs.max_pages * seqs.page_size
-        if self.enable_rope and (self._page_rope is None or self._page_rope[0] < positions):
-            if self._page_rope is not None:
-                cuda.FreeRope(self._page_rope[1])
-            self._page_rope = (positions, cuda.CreateRope(0, 0, positions * C, 1, positions, H, hs, self.rope_theta))
+        rope = seqs.Rope(H, hs, self.rope_theta) if self.enable_rope else 0
         self.c_attn.Forward(blobX, b["IpAttn"])
         b["Qt"].Reshape(1, N, H, hs)
         b["Y"].Reshape(1, N, C)
         sizes = (seqs.batch, N, H, H, hs, seqs.pages, seqs.page_size, seqs.max_pages)
         where = (k.gpu_data, v.gpu_data, seqs.table.gpu_data, seqs.starts.gpu_data, seqs.lens.gpu_data)
         strides = (H * seqs.page_size * hs, seqs.page_size * hs, hs)
-        cuda.PagedAppend(*sizes, b["IpAttn"].gpu_data, b["Qt"].gpu_data, *where, *strides, self._page_rope[1] if self.enable_rope else 0, self.qk_norm,
+        cuda.PagedAppend(*sizes, b["IpAttn"].gpu_data, b["Qt"].gpu_data, *where, *strides, rope, self.qk_norm,
                          *([n.gpu_data for n in self.norms] or (0, 0)), self.norm_eps)
         cuda.AttnPagedForward(*sizes, b["Qt"].gpu_data, *where, b["Y"].gpu_data, *strides, nMaxNew=seqs.max_new)
         self.c_proj.Forward(b["Y"], top)
