@@ -62,9 +62,9 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* all)
 }
 
 // The chunk kernel's list: sequences, their key heads and head tiles, their tiles, in units of about 32 positions of a tile.  All 256 threads.
-// Units a workgroup has at least: what a piece costs beside its blocks (its places, queries and partial results) is some of them.  us with 3 | 4 | 6 | 8: 16 new tokens
-// over 1811, 32 heads on 4 of 128, 16 bits 19.4 | 21.1 | 22.2 | 23.5; 2 sequences of 123 over 997, 28 heads on 4 of 96, fp32 over a 16-bit cache 41.6 | 37.8 | 40.7 | 42.6; 2 prompts
-// of 958, 10 heads of 128, fp32 78.8 | 78.1 | 79.2 | 83.7.  With 16 and 32: 2 prompts of 1024, 12 heads of 64, fp32 63 and 99 for 50.
+// Units a workgroup has at least: what a piece costs beside its blocks (its places, queries and partial results) is some of them.  us with 3 | 4 | 6 | 8: 8 new tokens
+// over 727 positions, 32 heads on 4 of 128, 16 bits 19.4 | 21.1 | 22.2 | 23.5; 68 over 400 and 121 over 985, 28 heads on 4 of 96, fp32 over a 16-bit cache 41.6 | 37.8 | 40.7 | 42.6; 2 prompts
+// of 958 over 978, 10 heads of 128, fp32 78.8 | 78.1 | 79.2 | 83.7.  With 16 and 32: 2 prompts of 1024, 12 heads of 64, fp32 63 and 99 for 50.
 constexpr int CHUNK_LEAST = 4;
 __device__ __forceinline__ int chunk_tiles(const PagedCache& c, const ChunkArgs& w, const PagedSpan& s)
 {

@@ -28,7 +28,7 @@ template <> __device__ __forceinline__ bf16_t stored<bf16_t>(float v) { return f
 // Any head size up to 256, any strides and addresses, no workspace: a workgroup has one token's head, a group of LPH lanes of its WAVES wavefronts
 // every (64 WAVES / LPH)-th position, V values a lane, value by value in runs of LPH; ANY_DEEP positions' reads are under way together.  What
 // bounds it is waiting for them, and every head reads its keys for itself.  Sixteen wavefronts where there are few tokens' heads, four else (us: one token over
-// 1000 positions, 6 heads of 198, fp32 56 | 134, sixteen of them 69 | 191; 64 tokens over up to 60, 12 heads of 46, 16.1 | 7.1; 4 chunks of 300, 97 | 56).
+// 1000 positions, 6 heads of 198, fp32 56 | 134, sixteen of them 69 | 191; 64 tokens over up to 60, 12 heads of 46, 16.1 | 7.1; chunks of 167 over 240, 297 over 593 and 137 over 157 and one token over 375, 6 heads of 46, 97 | 56).
 constexpr int ANY_DEEP = 4;
 template <typename T, typename TC, int V, int LPH, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void attn_paged_any_kernel(PagedAttnArgs a)
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(64 * WAVES) void attn_paged_any_kernel(PagedAttnArg
 // for all of them: what bounds this kernel is reading the cache.  All positions of all sequences, in units of four tiles of KT positions, are
 // one list that is dealt to the workgroups in equal runs, whatever the lengths: a run ends inside an item (a sequence's key head and row
 // tile), which the last workgroup to finish puts together.  A wavefront has every fourth tile, with statistics of its own; tiles of the wavefronts
-// meet in LDS at the end of an item.  Measured: 64 sequences of up to 4096 positions, 32 heads on 8 of 128, 16 bits, 559 MB 117 us (4.8 TB/s, what a large copy
-// reaches); one of 131000, 537 MB 120 us; one of 100, 12 heads of 64 in fp32, 7.2 us.
+// meet in LDS at the end of an item.  Measured: 64 sequences of up to 4096 positions, 32 heads on 8 of 128, 16 bits, 559 MB 117 us (4.8 TB/s; single tokens over a
+// contiguous cache of that size are read at 5.6); one of 131000, 537 MB 120 us; one of 100, 12 heads of 64 in fp32, 7.2 us.
 //
 // Scores are S^T = K Q^T, so that a lane has one row: register v of a tile holds key 4 (lane / 16) + v of row lane % 16, which is the operand
 // layout that O^T = V^T P^T wants of P (which slot of the contraction is which key only has to agree between the two).  Keys go from memory to the
@@ -628,7 +628,7 @@ __device__ __forceinline__ void split_run(const PagedAttnArgs& a, const SplitArg
 // all of them: every value read from the cache meets 128 rows, and the matrix cores bound it.  Tiles of one key head go to one XCD (workgroups
 // follow each other by key head), whose L2 then holds that head's keys and values.  The
 // blocks of all tiles are one list that is dealt to the workgroups in equal runs; tiles that a run ends in are put together by a launch behind this one.
-// Measured: 8 prompts of 2048, 12 heads of 64, fp32, 366 us (0.14 PFLOP/s of useful products, 0.9 of bf16 ones, which a large library product has 1.2 of);
+// Measured: 8 prompts of 2048, 12 heads of 64, fp32, 350 us (0.15 PFLOP/s of useful products, 0.9 of bf16 ones, which a large library product has 1.2 of);
 // a step of 12 chunks and single tokens, ragged, 64 us with the launch behind: half of it starts, ends and tiles that are not full.
 // Eight values as PARTS fragments of bf16: themselves, or of fp32 the three parts that hold its 24 bits, cut off (never rounded up to an infinity)
 template <int PARTS> struct Parts { u32x4 p[PARTS]; };
@@ -941,7 +941,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
                 s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], c2, ref));
                 if (NQ > 1) l += s[j][v];
             }
-        // weights in the operand layout: rounded to 16 bits, and added up as rounded, or in three parts
+        // weights in the operand layout: rounded to one bf16 number (eight bits, as the pipe kernel's) and added up as rounded, or in three parts
         Parts<NQ> p[KJ][2];
 #pragma unroll
         for (int j = 0; j < KJ; j++)
@@ -1250,6 +1250,11 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
         w.tileHeads = (G + w.headTiles - 1) / w.headTiles;
         w.perTile = 16 / w.tileHeads;
         const int most = maxNew > 0 ? std::min(maxNew, c.tokens) : c.tokens;
+        // Steps of single tokens with few others among them are the split's as a whole, up to a quarter more tokens than sequences: it reads the cache of a longer sequence once for
+        // 16 rows, and the chunk kernel's launch is longer by its registers, its list and the launch behind.  us, chunk kernel | split, one chunk of 1 + x times the sequences' number among
+        // single tokens, 32 heads on 8 of 128 in 16 bits: x 1/4 over 2000 positions, 16 sequences 38.7 | 32.4, 64 92 | 73, 256 126 | 107; over 8000, 64 312 | 256.  12 heads of 64 in fp32,
+        // 256 over 500 69 | 58.  From there on lengths decide, which are not known here: x 1/2, 32 heads on 4, 16 over 2000 37.5 | 23.7, 256 over 4000 123 | 139; x 2, 32 on 8, 64 over 2000
+        // 109 | 96, over 8000 306 | 344.
         const bool chunks = c.hs <= 128 && (long long)most * G > FEW_ROWS && c.tokens > c.batch + c.batch / 4;
         w.few = chunks ? FEW_ROWS : 0;
         // Up to two units in one where there are few sequences: going on for a tile takes less than putting two partial results together (us, 12 heads over 100

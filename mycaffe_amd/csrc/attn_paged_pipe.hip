@@ -9,7 +9,8 @@
 //    up and leaves their places in a ring of eight blocks in LDS (a place is 32 bits, in pieces of 16 bytes), from where the staging reads them.
 //  * Weights are exp2(scale log2(e) s - m) with a fixed m a row: the largest score of its first 32 keys.  The scale stays in fp32 (one fused
 //    multiply-add a score), and a row leaves the range only if a later score is higher by 44 than all of those.
-//  * Weights are cut off to 16 bits and added up as they are then, so that a row's weights still sum to one (y is off by 2e-3 of its norm, most of it its own rounding).
+//  * Weights are cut off to 16 bits and added up as they are then, so that a row's weights still sum to one: eight
+//    bits each, y is off by 2.4e-3 of its norm, where its own rounding is 1.7e-3.  (A second product of what is cut off is half as many matrix instructions again.)
 //  * What does not suit the pipeline is left to the chunk kernel, which runs behind this one for such tiles alone: tiles with a hole in their pages, rows
 //    before the first page given, row sums outside [2^-60, 2^64], values that are not finite where not all rows look.
 //

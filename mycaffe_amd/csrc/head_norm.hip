@@ -8,7 +8,7 @@
 // Everything is held in fp32 and rounded once, when it is stored.
 //
 // All three read and write every value once and compute a handful of operations on it, so memory bounds them (50 MB forward in 10.1 us, 252 MB backward in 53,
-// 201 MB appended in 46: 5.0, 4.7 and 4.3 TB/s, where a copy of 4 GiB has 4.8).  A head belongs to a group of
+// 201 MB appended in 46: 5.0, 4.7 and 4.3 TB/s, where a copy of 4 GiB has 4.5 - 4.8).  A head belongs to a group of
 // LPH adjacent lanes, V values a lane (16 bytes), so that the mean is LPH's butterfly and a pair never leaves its lane.
 #include <algorithm>
 #include <type_traits>

@@ -2838,7 +2838,7 @@ long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll)
     void* ws;
     int* tk;
     size_t wsb = attn_paged_workspace_bytes(c, Q->dt());
-    workspace_or_none(&wsb, &ws);   // without scratch one wavefront a token and head does all of it
+    workspace_or_none(&wsb, &ws);   // without scratch one workgroup a token and head does all of it
     ERRCHK(tickets(attn_paged_tickets(), &tk));
     HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)std::min<long long>(ll > 18 ? pl[18] : 0, c.tokens), ws, tk));
     m_mem.touch((long)pl[14]);
