@@ -245,6 +245,8 @@ enum {
      *   f{scale (0 = 1/sqrt(hs))}  l{batch, tokens, heads, kvHeads, hs, pages, pageSize, maxPages, hQ, hKpages, hVpages, hTable, hStarts,
      *             hLens, hY, stridePage, strideHead, stridePos [, maxNew]}
      * maxNew: no sequence has more new tokens than this (0: not known); only the choice of kernels follows from it.
+     * Weights of 16-bit rows have sixteen bits, in sequences of many rows eight (which these are depends on the whole call); all else is
+     * held in fp32.
      */
     MCH_FN_ATTN_DECODE_FWD = 2001,
     MCH_FN_RMSNORM_FWD = 2002,
