@@ -10,10 +10,10 @@ pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -149      # between the smallest numbers of fp32
 
 
-def definition(c, q, H):
+def definition(c, q, H, scale):
     """y and its tolerance: roundings as the other tests of this call count them, and half a step of the smallest numbers for every product and sum"""
     G, hs, y, tol, at = H // c.kvH, c.hs, [], [], 0
-    scale = hs ** -0.5
+    scale = scale or hs ** -0.5
     for (n, m, _), (k, v) in zip(c.seqs, c.dense):
         sees = np.arange(m)[None, :] <= np.arange(m - n, m)[:, None]
         ys, ts = np.zeros((n, H, hs)), np.zeros((n, H, hs))
@@ -23,7 +23,7 @@ def definition(c, q, H):
             s -= s.max(1, keepdims=True)
             w = np.exp(s)
             w /= w.sum(1, keepdims=True)
-            size = scale * (abs(qq) @ abs(kk).T)
+            size = abs(scale) * (abs(qq) @ abs(kk).T)      # a magnitude, whatever the sign of the scale
             ds = (hs + 8) * U32 * np.where(sees, size, 0).max(1) + 4 * U32 * np.where(sees, abs(s), 0).max(1) + 4 * U32
             off = 2 * ds + (sees.sum(1) + 8) * U32
             ys[:, h] = w @ vv
@@ -34,18 +34,18 @@ def definition(c, q, H):
     return np.concatenate(y), np.concatenate(tol)
 
 
-def check(dev, c, q, H):
+def check(dev, c, q, H, scale=0.0):
     for b, (k, v) in enumerate(c.dense):
         for t in range(len(k)):
             page, slot = int(c.table[b, t // c.page]), t % c.page
             c.k[page, :, slot], c.v[page, :, slot] = k[t], v[t]
     c.h["k"], c.h["v"] = dev.put(c.laid(c.k), c.half), dev.put(c.laid(c.v), c.half)
     hq, hy = dev.put(q), dev.zeros(q.size)
-    c.attend(hq, hy, H)
+    c.attend(hq, hy, H, fScale=scale)
     got = dev.get(hy, q.shape)
-    c.attend(hq, hy, H)
+    c.attend(hq, hy, H, fScale=scale)
     assert np.array_equal(got, dev.get(hy, q.shape))
-    want, tol = definition(c, q, H)
+    want, tol = definition(c, q, H, scale)
     over = abs(got - want) - tol
     at = np.unravel_index(over.argmax(), over.shape)
     assert over.max() <= 0, "%s: %g, not %g +- %g" % (at, got[at], want[at], tol[at])
@@ -102,3 +102,26 @@ def test_a_small_factor_beside_ordinary_ones(dev, cache16):
         c.dense[0][0][10, 0, 7] = 3.21e-37
         c.dense[1][0][0, 1] = 0
     check(dev, c, q, 4)
+
+
+@pytest.mark.parametrize("seqs", SEQS, ids=["chunk", "steps", "pieces", "mixed"])
+@pytest.mark.parametrize("hs", [48, 64, 128])
+def test_columns_of_zeros_and_of_the_smallest_numbers(dev, hs, seqs):
+    """A column of zeros comes out as zeros, also beside one of numbers that no 16-bit part holds, which come out as they are."""
+    for size in (0.0, 1e-41):
+        rng = np.random.default_rng(63)
+        c = Cache(dev, rng, seqs, 2, hs, 16, "head", False)
+        for _, v in c.dense:
+            v[:, :, 3] = 0
+            if size:
+                v[:, 1, hs - 1] = np.float32(size * (1 + abs(v[:, 1, hs - 1])))
+        check(dev, c, np.float32(rng.standard_normal((c.tokens, 4, hs))), 4)
+
+
+@pytest.mark.parametrize("cache16", [False, True])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_small_queries_at_a_large_scale(dev, sign, cache16):
+    for seqs in SEQS:
+        rng = np.random.default_rng(64)
+        c = Cache(dev, rng, seqs, 2, 64, 16, "head", cache16)
+        check(dev, c, np.float32(1e-36 * rng.standard_normal((c.tokens, 4, 64))), 4, sign * float(np.float32(1.25e35)))
