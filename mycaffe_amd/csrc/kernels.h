@@ -284,15 +284,4 @@ size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt);
 size_t attn_paged_tickets();
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets);
 
-// ---- a step of a server (paged_plan.hip, sample.hip): numbers fp32, or double (`wide`) -----------------------------------------
-// Room for the new tokens of a step.  In: wish (tokens that a sequence wants, below 0: it ends), lens, table (batch, maxPages), free (number of free pages, then
-// those), from and shared (may be null).  Out, each its input or memory of its own: lensOut, tableOut, freeOut, sharedOut (with shared); starts (batch + 1), last
-// (batch), positions and slots (tokens; may be null).
-struct PagedPlanArgs {
-    const void *wish, *lens, *table, *free, *from, *shared;
-    void *lensOut, *tableOut, *freeOut, *sharedOut, *starts, *last, *positions, *slots;
-    int batch, tokens, pages, pageSize, maxPages;
-};
-hipError_t k_paged_plan(hipStream_t s, bool wide, const PagedPlanArgs& a);
-
 }  // namespace mch
