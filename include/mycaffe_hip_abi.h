@@ -246,7 +246,34 @@ enum {
      *             hLens, hY, stridePage, strideHead, stridePos [, maxNew]}
      * maxNew: no sequence has more new tokens than this (0: not known); only the choice of kernels follows from it.
      * Weights of 16-bit rows have sixteen bits, in sequences of many rows eight (which these are depends on the whole call); all else is
+     * Weights of 16-bit rows have sixteen bits, in sequences of many rows eight (which these are depends on the whole call); all else is
      * held in fp32.
+     * ATTN_PAGED_PREFIX_FWD: the same result for sequences that share prefixes, which are read and multiplied once for all of a group's tokens:
+     *   f{scale}  l{...the 18 of ATTN_PAGED_FWD, groups, hGroups (groups + 1), hShared (groups) [, maxNew]}
+     * Group g are the sequences hGroups[g] .. hGroups[g + 1] - 1 (never decreasing; sequences in no group share nothing), which have their first hShared[g] positions
+     * in common: as far as these are whole pages, the rows of hTable name the same ones.  (What counts is what lies in front of every new token of the group.)
+     *
+     * PAGED_PLAN: room for the next tokens of `batch` sequences.  hNew[b] tokens are wanted behind hLens[b] positions; hNew[b] below 0 ends a sequence.
+     *   l{batch, tokens, pages, pageSize, maxPages, hNew, hLens, hTable, hFree, hLensOut, hTableOut, hFreeOut, hStarts, hPositions (0), hSlots (0), hLast
+     *     [, hFrom, hShared, hSharedOut]}
+     * hFree (pages + 1) is a stack: the number of free pages, then these.  First the pages of sequences that end go on it, in the order of the sequences (their row
+     * of the table becomes -1, their length 0); then each sequence in turn takes the pages that it needs off its top.  The first one for which the pages or the `tokens`
+     * rows of the call do not reach waits, unchanged, and so do all behind it; one that is longer than maxPages pages can hold is passed over.  hLensOut, hTableOut and
+     * hFreeOut (entries behind its number mean nothing) are the three inputs, or all memory of their own.  hStarts (batch + 1) as above; of every new row its position
+     * in its sequence and its slot, page * pageSize + place in the page (-1: no page; pages * pageSize is then at most 2^24); hLast (batch): a sequence's last row, or -1.
+     * hFrom, hShared, hSharedOut (batch; the last one the second or memory of its own, as the other three): a sequence without positions begins behind
+     * the first hShared[b] positions of sequence hFrom[b], as far as they are whole pages that it has; hSharedOut[b] says how many these are, and of a sequence that
+     * goes on what hShared[b] does: its first pages, up to there, are not its own, and not given back when it ends.
+     *
+     * SAMPLE_FWD: the next token of every row of logits (fp32 or 16 bits), drawn with the random number u = hRandom[row]:
+     *   l{rows, vocab, hLogits, hRandom, hIds, hTemperature, hTopK, hTopP, hMinP [, hLogProb, hRows, logitsRows, rowStride]}    (from hTemperature on each may be 0)
+     * Weights are exp((x - max x) / temperature); tokens count in falling order of x, equal ones by their index.  top-k (1 .. vocab - 1, else off) keeps the first k, top-p
+     * (below 1, else off) of these the fewest whose weights add up to at least p of theirs, one at least, min-p (above 0, else off) those whose weight is at least m times the
+     * largest; above 1: the first.  Drawn is the first token by index at which the sum of the weights left exceeds u times all of it (u below 0 or not a number: 0, from 1 on
+     * the last one).  A temperature that is not above 0: the likeliest token.  A logit that is not a number is -inf; of infinite ones each weighs 1.  hLogProb: the
+     * logarithm of the token's share of the weights left (0 without a draw).  hRows: which row, of logitsRows (0: rows) at rowStride (0: vocab) values each, a
+     * row's logits are; no such row, or one of -inf alone: id -1.  vocab up to 2^20.  Weights are exact to 2^-50 and sums exact, so the same numbers draw the same tokens
+     * in any batch.
      */
     MCH_FN_ATTN_DECODE_FWD = 2001,
     MCH_FN_RMSNORM_FWD = 2002,
@@ -263,7 +290,10 @@ enum {
     MCH_FN_QK_NORM_ROPE_FWD = 2013,
     MCH_FN_QK_NORM_ROPE_BWD = 2014,
     MCH_FN_PAGED_APPEND = 2015,
-    MCH_FN_ATTN_PAGED_FWD = 2016
+    MCH_FN_ATTN_PAGED_FWD = 2016,
+    MCH_FN_PAGED_PLAN = 2017,
+    MCH_FN_ATTN_PAGED_PREFIX_FWD = 2018,
+    MCH_FN_SAMPLE_FWD = 2019
 };
 
 /* DEVINIT flags (CudaDnnDLL/Cuda Files/device.h:18-22) */

@@ -284,4 +284,27 @@ size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt);
 size_t attn_paged_tickets();
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets);
 
+// ---- a step of a server (paged_plan.hip, sample.hip): numbers fp32, or double (`wide`) -----------------------------------------
+// Room for the new tokens of a step.  In: wish (tokens that a sequence wants, below 0: it ends), lens, table (batch, maxPages), free (number of free pages, then
+// those), from and shared (may be null).  Out, each its input or memory of its own: lensOut, tableOut, freeOut, sharedOut (with shared); starts (batch + 1), last
+// (batch), positions and slots (tokens; may be null).
+struct PagedPlanArgs {
+    const void *wish, *lens, *table, *free, *from, *shared;
+    void *lensOut, *tableOut, *freeOut, *sharedOut, *starts, *last, *positions, *slots;
+    int batch, tokens, pages, pageSize, maxPages;
+};
+hipError_t k_paged_plan(hipStream_t s, bool wide, const PagedPlanArgs& a);
+// The next token of `count` rows of logits (rows: which of the logitsRows rows each is; null: row i).  Numbers a row, each may be null: temperature (1), k (0: all), p (1:
+// all), m (0: all); u, the random number, may not.  Out: ids (-1 where there is no row, or nothing in it), logs (may be null).
+enum SampleType { SAMPLE_F32, SAMPLE_BF16, SAMPLE_F64 };   // of the logits; numbers are fp32 beside the first two, double beside the last
+constexpr int SAMPLE_VOCAB = 1 << 20;
+struct SampleArgs {
+    const void *x, *u, *temperature, *k, *p, *m, *rows;
+    void *ids, *logs;
+    long long stride;
+    int count, vocab, logitsRows;
+    int perWave, bits;   // the kernel's own
+};
+hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a);
+
 }  // namespace mch

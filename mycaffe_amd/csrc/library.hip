@@ -2340,7 +2340,10 @@ long Kernel::run(long fn, float* pf, long lf, MCH_LONGLONG* pl, long ll, float**
     case MCH_FN_QK_NORM_ROPE_FWD: return qk_norm_rope(pf, lf, pl, ll, false);
     case MCH_FN_QK_NORM_ROPE_BWD: return qk_norm_rope(pf, lf, pl, ll, true);
     case MCH_FN_PAGED_APPEND: return paged_append(pf, lf, pl, ll);
-    case MCH_FN_ATTN_PAGED_FWD: return attn_paged_fwd(pf, lf, pl, ll);
+    case MCH_FN_ATTN_PAGED_FWD: return attn_paged_fwd(pf, lf, pl, ll, false);
+    case MCH_FN_PAGED_PLAN: return paged_plan(pl, ll);
+    case MCH_FN_ATTN_PAGED_PREFIX_FWD: return attn_paged_fwd(pf, lf, pl, ll, true);
+    case MCH_FN_SAMPLE_FWD: return sample_fwd(pl, ll);
 
     // ---- RoPE ------------------------------------------------------------------
     case MCH_FN_CREATE_ROPE: {
@@ -2826,22 +2829,109 @@ long Kernel::paged_append(float* pf, long lf, MCH_LONGLONG* pl, long ll)
 }
 
 // ATTN_PAGED_FWD: f{scale}, l{...[, maxNew]} behind what paged_operands reads
-long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll)
+// ATTN_PAGED_PREFIX_FWD: f{scale}, l{..., groups, hGroups, hShared[, maxNew]}
+long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool prefix)
 {
     NEED_F(1, 1);
-    NEED_L(18, 19);
-    if (ll > 18 && pl[18] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const int hint = prefix ? 21 : 18;
+    NEED_L(hint, hint + 1);
+    if (ll > hint && pl[hint] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
     PagedCache c;
-    MemItem *Q, *Y;
+    MemItem *Q, *Y, *groups = nullptr, *shared = nullptr;
     ERRCHK(paged_operands(pl, pl[2], &c, &Q, &Y));
+    if (prefix) {
+        if (pl[18] < 1 || pl[18] > c.batch) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        ERRCHK(mem((long)pl[19], &groups));
+        ERRCHK(mem((long)pl[20], &shared));
+        if (groups->half || shared->half) {
+            last_detail = "groups and shared positions are fp32 tensors";
+            return MCH_ERROR_MEMORY_HALF_TYPE_NOT_SUPPORTED;
+        }
+        RANGE(groups, 0, pl[18] + 1);
+        RANGE(shared, 0, pl[18]);
+        const long long n = (long long)c.tokens * c.H * c.hs;
+        if (overlap(Y, n, groups, pl[18] + 1) || overlap(Y, n, shared, pl[18])) {
+            last_detail = "an output shares memory with another operand";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+    }
     const float scale = pf[0] != 0.f ? pf[0] : (float)(1.0 / sqrt((double)c.hs));
+    const int maxNew = (int)std::min<long long>(ll > hint ? pl[hint] : 0, c.tokens);
     void* ws;
     int* tk;
     size_t wsb = attn_paged_workspace_bytes(c, Q->dt());
     workspace_or_none(&wsb, &ws);   // without scratch one workgroup a token and head does all of it
     ERRCHK(tickets(attn_paged_tickets(), &tk));
-    HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)std::min<long long>(ll > 18 ? pl[18] : 0, c.tokens), ws, tk));
+    HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, maxNew, ws, tk));
     m_mem.touch((long)pl[14]);
+    return 0;
+}
+
+// PAGED_PLAN: l{batch,tokens,pages,pageSize,maxPages, hNew,hLens,hTable,hFree,hLensOut,hTableOut,hFreeOut,hStarts,hPositions,hSlots,hLast[,hFrom,hShared,hSharedOut]}
+long Kernel::paged_plan(MCH_LONGLONG* pl, long ll)
+{
+    NEED_L(16, 19);
+    if (ll != 16 && ll != 19) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const long long* l = (const long long*)pl;
+    const bool borrow = ll == 19 && (pl[16] || pl[17] || pl[18]);
+    if (!plan_sizes_ok(l, pl[14] != 0) || (borrow && !(pl[16] && pl[17] && pl[18]))) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemItem* m[PLAN_OPERANDS] = {};
+    for (int i = 0; i < PLAN_OPERANDS; i++) {
+        if (i >= 11 ? !borrow : (i == 8 || i == 9) && !pl[5 + i]) continue;
+        ERRCHK(mem((long)pl[5 + i], &m[i]));
+        if (m[i]->half) {
+            last_detail = "the numbers of a plan are fp32 tensors";
+            return MCH_ERROR_MEMORY_HALF_TYPE_NOT_SUPPORTED;
+        }
+        RANGE(m[i], 0, plan_values(l, i));
+    }
+    if (const char* why = plan_clash(l, [&](int i) -> const void* { return m[i] ? m[i]->ptr : nullptr; }, sizeof(float))) {
+        last_detail = why;
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
+    PagedPlanArgs a = {at(0), at(1), at(2), at(3), at(11), at(12), at(4), at(5), at(6), at(13), at(7), at(10), at(8), at(9), (int)l[0], (int)l[1], (int)l[2], (int)l[3], (int)l[4]};
+    HIPCHK(k_paged_plan(m_stream, false, a));
+    for (int i = 0; i < PLAN_OPERANDS; i++)
+        if (m[i] && plan_writes(i)) m_mem.touch((long)pl[5 + i]);
+    return 0;
+}
+
+// SAMPLE_FWD: l{rows,vocab,hLogits,hRandom,hIds,hTemperature,hTopK,hTopP,hMinP[,hLogProb,hRows,logitsRows,rowStride]}
+long Kernel::sample_fwd(MCH_LONGLONG* pl, long ll)
+{
+    NEED_L(9, 13);
+    const long long rows = pl[0], vocab = pl[1], of = ll > 11 && pl[11] ? pl[11] : rows, stride = ll > 12 && pl[12] ? pl[12] : vocab;
+    if (!sample_sizes_ok(rows, vocab, of, stride, SAMPLE_VOCAB)) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemItem* X;
+    MemItem* m[8] = {};   // random, ids, temperature, k, p, m, logs, rows
+    ERRCHK(mem((long)pl[2], &X));
+    for (int i = 0; i < 8; i++) {
+        const long h = 3 + i < ll ? (long)pl[3 + i] : 0;
+        if (i > 1 && !h) continue;
+        ERRCHK(mem(h, &m[i]));
+        if (m[i]->half) {
+            last_detail = "all numbers of a draw but the logits are fp32 tensors";
+            return MCH_ERROR_MEMORY_HALF_TYPE_NOT_SUPPORTED;
+        }
+        RANGE(m[i], 0, rows);
+    }
+    const long long reach = (of - 1) * stride + vocab;
+    RANGE(X, 0, reach);
+    for (int o : {1, 6}) {
+        if (!m[o]) continue;
+        bool clash = overlap(m[o], rows, X, reach);
+        for (int i = 0; i < 8; i++) clash = clash || (i != o && m[i] && overlap(m[o], rows, m[i], rows));
+        if (clash) {
+            last_detail = "an output shares memory with another operand";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+    }
+    auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
+    SampleArgs a = {X->ptr, at(0), at(2), at(3), at(4), at(5), at(7), at(1), at(6), stride, (int)rows, (int)vocab, (int)of, 0, 0};
+    HIPCHK(k_sample(m_stream, X->half ? SAMPLE_BF16 : SAMPLE_F32, a));
+    m_mem.touch((long)pl[4]);
+    if (m[6]) m_mem.touch((long)pl[9]);
     return 0;
 }
 
@@ -2954,7 +3044,7 @@ static const char* api_name(long fn)
 #define N(x) {MCH_FN_##x, "CUDA_FN_" #x}
     static const struct { long id; const char* name; } table[] = {
         {MCH_DLL_FREEMEM, "CUDA_DLL_FREEMEM"}, {MCH_DLL_INITIALIZE, "CUDA_DLL_INITIALIZE"}, {MCH_DLL_CLEANUP, "CUDA_DLL_CLEANUP"},
-        N(SETDEVICE), N(GETDEVICE), N(SYNCHRONIZEDEVICE), N(CREATE_MEMORYPOINTER), N(FREE_MEMORYPOINTER), N(ALLOCMEM_HALF), N(ALLOCMEM), N(FREEMEM), N(GETMEM), N(SETMEM), N(CREATE_CUDNN), N(FREE_CUDNN), N(CREATE_TENSORDESC), N(FREE_TENSORDESC), N(SET_TENSORDESC), N(CREATE_EXTENSION), N(FREE_EXTENSION), N(EXTENSION_RUN), N(SOFTMAX_FWD), N(SOFTMAX_BWD), N(ATTN_CREATE), N(ATTN_FREE), N(ATTN_SET), N(ATTN_FWD), N(ATTN_BWD), N(SET), N(COPY), N(GEMM2), N(GEMM), N(GEMV), N(AXPY), N(SCAL), N(SCALE), N(ADD_SCALAR), N(ADD), N(SUB), N(MUL), N(DIV), N(EXP), N(LOG), N(POWX), N(SQRT), N(TRANSPOSE), N(MASK), N(MASK_BATCH), N(TRANSPOSE_HW), N(INVERT), N(CHANNEL_MEAN), N(CHANNEL_MAX), N(CHANNEL_SUB), N(CHANNEL_SUM), N(CHANNEL_DIV), N(CHANNEL_DOT), N(CHANNEL_COPY), N(CHANNEL_FILLFROM), N(CHANNEL_COPYALL), N(CHANNEL_DUP), N(CHANNEL_SUM2), N(EMBED_FWD), N(RELU_FWD), N(RELU_BWD), N(GELU_FWD), N(GELU_BWD), N(SILU_FWD), N(SILU_BWD), N(CREATE_LAYERNORM), N(FREE_LAYERNORM), N(LAYERNORM_FWD), N(LAYERNORM_BWD), N(CREATE_ROPE), N(FREE_ROPE), N(ROPE_FWD), N(ROPE_BWD), N(CREATE_BLOBLOADER), N(FREE_BLOBLOADER), N(BLOBLOADER_LOAD), N(BLOBLOADER_RESETOFFSET), N(BLOBLOADER_ADDTOOFFSET), N(ATTN_DECODE_FWD), N(RMSNORM_FWD), N(SWIGLU_FWD), N(QKV_PROJ_HEADS), N(LINEAR_FWD), N(LINEAR_BWD), N(QKV_HEADS_GRAD), N(RMSNORM_BWD), N(SWIGLU_BWD), N(NORM_ADD_FWD), N(NORM_ADD_BWD), N(LINEAR_HEADS_GROUP), N(QK_NORM_ROPE_FWD), N(QK_NORM_ROPE_BWD), N(PAGED_APPEND), N(ATTN_PAGED_FWD)};
+        N(SETDEVICE), N(GETDEVICE), N(SYNCHRONIZEDEVICE), N(CREATE_MEMORYPOINTER), N(FREE_MEMORYPOINTER), N(ALLOCMEM_HALF), N(ALLOCMEM), N(FREEMEM), N(GETMEM), N(SETMEM), N(CREATE_CUDNN), N(FREE_CUDNN), N(CREATE_TENSORDESC), N(FREE_TENSORDESC), N(SET_TENSORDESC), N(CREATE_EXTENSION), N(FREE_EXTENSION), N(EXTENSION_RUN), N(SOFTMAX_FWD), N(SOFTMAX_BWD), N(ATTN_CREATE), N(ATTN_FREE), N(ATTN_SET), N(ATTN_FWD), N(ATTN_BWD), N(SET), N(COPY), N(GEMM2), N(GEMM), N(GEMV), N(AXPY), N(SCAL), N(SCALE), N(ADD_SCALAR), N(ADD), N(SUB), N(MUL), N(DIV), N(EXP), N(LOG), N(POWX), N(SQRT), N(TRANSPOSE), N(MASK), N(MASK_BATCH), N(TRANSPOSE_HW), N(INVERT), N(CHANNEL_MEAN), N(CHANNEL_MAX), N(CHANNEL_SUB), N(CHANNEL_SUM), N(CHANNEL_DIV), N(CHANNEL_DOT), N(CHANNEL_COPY), N(CHANNEL_FILLFROM), N(CHANNEL_COPYALL), N(CHANNEL_DUP), N(CHANNEL_SUM2), N(EMBED_FWD), N(RELU_FWD), N(RELU_BWD), N(GELU_FWD), N(GELU_BWD), N(SILU_FWD), N(SILU_BWD), N(CREATE_LAYERNORM), N(FREE_LAYERNORM), N(LAYERNORM_FWD), N(LAYERNORM_BWD), N(CREATE_ROPE), N(FREE_ROPE), N(ROPE_FWD), N(ROPE_BWD), N(CREATE_BLOBLOADER), N(FREE_BLOBLOADER), N(BLOBLOADER_LOAD), N(BLOBLOADER_RESETOFFSET), N(BLOBLOADER_ADDTOOFFSET), N(ATTN_DECODE_FWD), N(RMSNORM_FWD), N(SWIGLU_FWD), N(QKV_PROJ_HEADS), N(LINEAR_FWD), N(LINEAR_BWD), N(QKV_HEADS_GRAD), N(RMSNORM_BWD), N(SWIGLU_BWD), N(NORM_ADD_FWD), N(NORM_ADD_BWD), N(LINEAR_HEADS_GROUP), N(QK_NORM_ROPE_FWD), N(QK_NORM_ROPE_BWD), N(PAGED_APPEND), N(ATTN_PAGED_FWD), N(PAGED_PLAN), N(ATTN_PAGED_PREFIX_FWD), N(SAMPLE_FWD)};
 #undef N
     for (const auto& t : table)
         if (t.id == fn) return t.name;

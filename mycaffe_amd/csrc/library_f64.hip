@@ -944,6 +944,9 @@ private:
     }
     long head_norm(const double* pf, const MCH_LONGLONG* pl, long ll, bool backward);
     long paged(const double* pf, const MCH_LONGLONG* pl, bool append);
+    long paged_prefix(const double* pf, const MCH_LONGLONG* pl);
+    long paged_plan(const MCH_LONGLONG* pl, long ll);
+    long sample(const MCH_LONGLONG* pl, long ll);
     // P (B, H, T, Tk) = softmax(mask(scale Q K^T))
     long attn_probs(const double* Q, const double* K, double* P, const AttnD* st, int T, int Tk, const MemD* M, int kind)
     {
@@ -1101,6 +1104,77 @@ long KernelD::paged(const double* pf, const MCH_LONGLONG* pl, bool append)
                                    W[1] ? (const double*)W[1]->ptr : nullptr, (int)(pl[19] != 0), pf[0], theta);
     else hipLaunchKernelGGL(d_paged_attn_kernel, grid, 256, 0, m_stream, c, (const double*)X->ptr, out->ptr, pf[0] != 0.0 ? pf[0] : 1.0 / sqrt((double)hs));
     LAUNCHED();
+    return 0;
+}
+
+// ATTN_PAGED_PREFIX_FWD: every sequence over its own pages, which are the group's (what the float table saves by reading them once is not saved here)
+long KernelD::paged_prefix(const double* pf, const MCH_LONGLONG* pl)
+{
+    const long long* l = (const long long*)pl;
+    if (!paged_sizes_ok(l) || l[18] < 1 || l[18] > l[0]) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemD *Y, *groups, *shared;
+    ERRCHK(mem((long)pl[14], &Y));
+    ERRCHK(mem((long)pl[19], &groups));
+    ERRCHK(mem((long)pl[20], &shared));
+    RANGE(groups, 0, l[18] + 1);
+    RANGE(shared, 0, l[18]);
+    const long long n = l[1] * l[2] * l[4];
+    if (d_overlap(Y, n, groups, l[18] + 1) || d_overlap(Y, n, shared, l[18])) {
+        last_detail = "an output shares memory with another operand";
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    return paged(pf, pl, false);
+}
+
+// PAGED_PLAN and SAMPLE_FWD: the float table's kernels, arguments as there
+long KernelD::paged_plan(const MCH_LONGLONG* pl, long ll)
+{
+    const long long* l = (const long long*)pl;
+    if (ll != 16 && ll != 19) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    const bool borrow = ll == 19 && (pl[16] || pl[17] || pl[18]);
+    if (!plan_sizes_ok(l, pl[14] != 0) || (borrow && !(pl[16] && pl[17] && pl[18]))) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemD* m[PLAN_OPERANDS] = {};
+    for (int i = 0; i < PLAN_OPERANDS; i++) {
+        if (i >= 11 ? !borrow : (i == 8 || i == 9) && !pl[5 + i]) continue;
+        ERRCHK(mem((long)pl[5 + i], &m[i]));
+        RANGE(m[i], 0, plan_values(l, i));
+    }
+    auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
+    if (const char* why = plan_clash(l, at, sizeof(double))) {
+        last_detail = why;
+        return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    }
+    PagedPlanArgs a = {at(0), at(1), at(2), at(3), at(11), at(12), at(4), at(5), at(6), at(13), at(7), at(10), at(8), at(9), (int)l[0], (int)l[1], (int)l[2], (int)l[3], (int)l[4]};
+    HIPCHK(k_paged_plan(m_stream, true, a));
+    return 0;
+}
+long KernelD::sample(const MCH_LONGLONG* pl, long ll)
+{
+    const long long rows = pl[0], vocab = pl[1], of = ll > 11 && pl[11] ? pl[11] : rows, stride = ll > 12 && pl[12] ? pl[12] : vocab;
+    if (!sample_sizes_ok(rows, vocab, of, stride, SAMPLE_VOCAB)) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+    MemD* X;
+    MemD* m[8] = {};   // random, ids, temperature, k, p, m, logs, rows
+    ERRCHK(mem((long)pl[2], &X));
+    for (int i = 0; i < 8; i++) {
+        const long h = 3 + i < ll ? (long)pl[3 + i] : 0;
+        if (i > 1 && !h) continue;
+        ERRCHK(mem(h, &m[i]));
+        RANGE(m[i], 0, rows);
+    }
+    const long long reach = (of - 1) * stride + vocab;
+    RANGE(X, 0, reach);
+    for (int o : {1, 6}) {
+        if (!m[o]) continue;
+        bool clash = d_overlap(m[o], rows, X, reach);
+        for (int i = 0; i < 8; i++) clash = clash || (i != o && m[i] && d_overlap(m[o], rows, m[i], rows));
+        if (clash) {
+            last_detail = "an output shares memory with another operand";
+            return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        }
+    }
+    auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
+    SampleArgs a = {X->ptr, at(0), at(2), at(3), at(4), at(5), at(7), at(1), at(6), stride, (int)rows, (int)vocab, (int)of, 0, 0};
+    HIPCHK(k_sample(m_stream, SAMPLE_F64, a));
     return 0;
 }
 
@@ -2463,6 +2537,17 @@ long KernelD::run(long fn, const double* pf, long lf, const MCH_LONGLONG* pl, lo
         NEED_L(18, 19);
         if (ll > 18 && pl[18] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
         return paged(pf, pl, false);
+    case MCH_FN_PAGED_PLAN:
+        NEED_L(16, 19);
+        return paged_plan(pl, ll);
+    case MCH_FN_ATTN_PAGED_PREFIX_FWD:
+        NEED_F(1, 1);
+        NEED_L(21, 22);
+        if (ll > 21 && pl[21] < 0) return MCH_ERROR_PARAM_OUT_OF_RANGE;
+        return paged_prefix(pf, pl);
+    case MCH_FN_SAMPLE_FWD:
+        NEED_L(9, 13);
+        return sample(pl, ll);
     case MCH_FN_ATTN_DECODE_FWD: {
         // f{scale (0 = 1/sqrt(hs))}, l{batch, heads, kvHeads, hs, len, hQ, hKcache, hVcache, hY, strideKvBatch, strideKvHead,
         //   strideKvPos [, hRope, hKnew, hVnew]}

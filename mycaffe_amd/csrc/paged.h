@@ -130,4 +130,45 @@ inline bool paged_apart(const long long* l, long long apart, long long reach)
     return true;
 }
 
+// PAGED_PLAN, l{batch, tokens, pages, pageSize, maxPages, ...}; slots are page * pageSize + position in it
+inline bool plan_sizes_ok(const long long* l, bool slots)
+{
+    for (int i = 0; i < 5; i++)
+        if (l[i] < 1 || l[i] > PAGED_EXACT) return false;
+    return l[3] * l[4] <= PAGED_EXACT && (!slots || l[2] * l[3] <= PAGED_EXACT);
+}
+constexpr int PLAN_OPERANDS = 14;
+// Values of its handles: wish, lens, table, free, lensOut, tableOut, freeOut, starts, positions, slots, last, from, shared, sharedOut
+inline long long plan_values(const long long* l, int operand)
+{
+    const long long B = l[0], N = l[1], table = B * l[4], free = l[2] + 1;
+    const long long n[PLAN_OPERANDS] = {B, B, table, free, B, table, free, B + 1, N, N, B, B, B, B};
+    return n[operand];
+}
+inline bool plan_writes(int operand) { return (operand >= 4 && operand <= 10) || operand == 13; }
+// What is wrong with where its operands lie, null if nothing: lengths, table, free pages and shared positions are written all in place or all elsewhere, and no
+// output shares memory with anything else.  at(i): address of operand i, null if it is not given
+template <typename F> const char* plan_clash(const long long* l, F at, size_t size)
+{
+    static const int pairs[4][2] = {{1, 4}, {2, 5}, {3, 6}, {12, 13}};
+    int in = 0, apart = 0;
+    for (const auto& p : pairs)
+        if (at(p[0])) (at(p[0]) == at(p[1]) ? in : apart)++;
+    if (in && apart) return "lengths, table, free pages and shared positions are written all in place or all elsewhere";
+    for (int o = 0; o < PLAN_OPERANDS; o++)
+        for (int i = 0; i < PLAN_OPERANDS; i++) {
+            bool pair = i == o;
+            for (const auto& p : pairs) pair = pair || (in && i == p[0] && o == p[1]);
+            if (pair || !plan_writes(o) || !at(o) || !at(i)) continue;
+            const char *a = (const char*)at(o), *b = (const char*)at(i);
+            if (a < b + plan_values(l, i) * size && b < a + plan_values(l, o) * size) return "an output shares memory with another operand";
+        }
+    return nullptr;
+}
+// SAMPLE_FWD, l{rows, vocab, ..., logitsRows, stride}
+inline bool sample_sizes_ok(long long rows, long long vocab, long long logitsRows, long long stride, long long most)
+{
+    return rows >= 1 && rows <= PAGED_EXACT && vocab >= 1 && vocab <= most && logitsRows >= 1 && logitsRows <= PAGED_EXACT && stride >= vocab && stride <= (1ll << 38);
+}
+
 }  // namespace mch

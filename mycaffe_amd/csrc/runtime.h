@@ -182,7 +182,9 @@ private:
     long rope_turns(long hRope, long long hs, long long positions, const float** turns);
     long paged_operands(const MCH_LONGLONG* pl, long long rowHeads, PagedCache* c, MemItem** rows, MemItem** out);
     long paged_append(float* pf, long lf, MCH_LONGLONG* pl, long ll);
-    long attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll);
+    long attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool prefix);
+    long paged_plan(MCH_LONGLONG* pl, long ll);
+    long sample_fwd(MCH_LONGLONG* pl, long ll);
     long qk_norm_rope(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool backward);
     long attn_decode_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool staticScratch);
     long workspace(size_t bytes, void** p);

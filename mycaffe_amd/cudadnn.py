@@ -130,6 +130,9 @@ class CUDAFN:
     QK_NORM_ROPE_BWD = 2014
     PAGED_APPEND = 2015
     ATTN_PAGED_FWD = 2016
+    PAGED_PLAN = 2017
+    ATTN_PAGED_PREFIX_FWD = 2018
+    SAMPLE_FWD = 2019
 
 
 class CUDAQRY:
@@ -863,6 +866,38 @@ class CudaDnn:
         if nMaxNew:
             rgl.append(nMaxNew)
         self._ex2(CUDAFN.ATTN_PAGED_FWD, [fScale], rgl)
+
+    def AttnPagedPrefixForward(self, nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQ, hKPages, hVPages, hTable, hStarts, hLens, hY,
+                               nStridePage, nStrideHead, nStridePos, nGroups, hGroups, hShared, fScale=0.0, nMaxNew=0):
+        """AttnPagedForward for sequences that share prefixes, with the same result: group g, the sequences hGroups[g] .. hGroups[g + 1] - 1, has its first
+        hShared[g] positions in the same pages, which are read once for all of its tokens."""
+        rgl = [nBatch, nTokens, nHeads, nKvHeads, nSize, nPages, nPageSize, nMaxPages, hQ, hKPages, hVPages, hTable, hStarts, hLens, hY, nStridePage,
+               nStrideHead, nStridePos, nGroups, hGroups, hShared]
+        if nMaxNew:
+            rgl.append(nMaxNew)
+        self._ex2(CUDAFN.ATTN_PAGED_PREFIX_FWD, [fScale], rgl)
+
+    # ---- a server's step ------------------------------------------------------------------------
+    def PagedPlan(self, nBatch, nTokens, nPages, nPageSize, nMaxPages, hNew, hLens, hTable, hFree, hLensOut, hTableOut, hFreeOut, hStarts, hPositions, hSlots, hLast,
+                  hFrom=0, hShared=0, hSharedOut=0):
+        """Room in a paged cache for the next tokens of many sequences: hNew[b] of them behind hLens[b] positions (below 0: the sequence ends and gives its
+        pages back), pages off the stack hFree (their number, then the pages).  Sequences are served in their order; the first that pages or the nTokens rows do
+        not reach for waits, and all behind it.  Writes lengths, table and stack (each in place or elsewhere), hStarts as PagedAppend takes them, position and
+        slot (page * nPageSize + place in it) of every new row (0: not wanted) and the last row of every sequence (-1: none).  With hFrom, hShared
+        and hSharedOut a sequence without positions begins behind the first hShared[b] positions of sequence hFrom[b], whole pages of it."""
+        rgl = [nBatch, nTokens, nPages, nPageSize, nMaxPages, hNew, hLens, hTable, hFree, hLensOut, hTableOut, hFreeOut, hStarts, hPositions, hSlots, hLast]
+        if hFrom or hShared or hSharedOut:
+            rgl += [hFrom, hShared, hSharedOut]
+        self._ex2(CUDAFN.PAGED_PLAN, None, rgl)
+
+    def SampleForward(self, nRows, nVocab, hLogits, hRandom, hIds, hTemperature=0, hTopK=0, hTopP=0, hMinP=0, hLogProb=0, hRows=0, nLogitsRows=0, nRowStride=0):
+        """The next token of every row of logits, drawn with the row's random number (0 .. 1): weights exp((x - max x) / temperature) (0: the likeliest token), of them
+        the hTopK largest, of those the fewest that add up to hTopP of them, of those the ones of at least hMinP times the largest.  hLogProb: the logarithm of the
+        drawn token's share of what is left.  hRows: which row of the logits each is (not one of them: id -1).  Handles of 0: off."""
+        rgl = [nRows, nVocab, hLogits, hRandom, hIds, hTemperature, hTopK, hTopP, hMinP]
+        if hLogProb or hRows or nLogitsRows or nRowStride:
+            rgl += [hLogProb, hRows, nLogitsRows, nRowStride]
+        self._ex2(CUDAFN.SAMPLE_FWD, None, rgl)
 
     # ---- RoPE ---------------------------------------------------------------------------------
     def CreateRope(self, nSharedIndex, nGpuID, nCount, nBatch, nSeqLen, nHeads, nDim, fTheta=10000.0):
