@@ -246,7 +246,6 @@ enum {
      *             hLens, hY, stridePage, strideHead, stridePos [, maxNew]}
      * maxNew: no sequence has more new tokens than this (0: not known); only the choice of kernels follows from it.
      * Weights of 16-bit rows have sixteen bits, in sequences of many rows eight (which these are depends on the whole call); all else is
-     * Weights of 16-bit rows have sixteen bits, in sequences of many rows eight (which these are depends on the whole call); all else is
      * held in fp32.
      * ATTN_PAGED_PREFIX_FWD: the same result for sequences that share prefixes, which are read and multiplied once for all of a group's tokens:
      *   f{scale}  l{...the 18 of ATTN_PAGED_FWD, groups, hGroups (groups + 1), hShared (groups) [, maxNew]}
