@@ -2857,8 +2857,17 @@ long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool 
     }
     const float scale = pf[0] != 0.f ? pf[0] : (float)(1.0 / sqrt((double)c.hs));
     const int maxNew = (int)std::min<long long>(ll > hint ? pl[hint] : 0, c.tokens);
-    void* ws;
+    void* ws = nullptr;
     int* tk;
+    if (prefix) {
+        size_t wsb = attn_prefix_workspace_bytes(c, Q->dt(), Q->ptr, Y->ptr, (int)pl[18]);
+        workspace_or_none(&wsb, &ws);
+        if (ws) {
+            HIPCHK(k_attn_prefix(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)pl[18], (const float*)groups->ptr, (const float*)shared->ptr, ws));
+            m_mem.touch((long)pl[14]);
+            return 0;
+        }
+    }
     size_t wsb = attn_paged_workspace_bytes(c, Q->dt());
     workspace_or_none(&wsb, &ws);   // without scratch one workgroup a token and head does all of it
     ERRCHK(tickets(attn_paged_tickets(), &tk));

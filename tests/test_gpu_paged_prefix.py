@@ -12,8 +12,11 @@ class Shared(Cache):
     """Sequences of which groups [(first, end, shared positions)] have their first positions in common: whole pages of them are the first sequence's, the rest of the
     positions has the same keys and values."""
 
-    def __init__(self, dev, rng, seqs, groups, *args, **more):
-        super().__init__(dev, rng, seqs, *args, **more)
+    def __init__(self, dev, rng, seqs, groups, kvH, hs, page, order, half, wide=True, **more):
+        # sequences that cannot hold this many bytes are not worth sharing for, and go to attention over pages: room for more than they have
+        if wide:
+            more["width"] = max(max(-(-m // page) for _, m, _ in seqs) + 1, int(66e6 / (len(seqs) * page * kvH * hs * (4 if half else 8))) + 1)
+        super().__init__(dev, rng, seqs, kvH, hs, page, order, half, **more)
         self.groups = groups
         for first, end, shared in groups:
             for b in range(first + 1, end):
@@ -91,11 +94,12 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("wide", [True, False])
 @pytest.mark.parametrize("act16,cache16", TYPES)
 @pytest.mark.parametrize("name,H,kvH,hs,page,order,seqs,groups,pad", CASES, ids=[s[0] for s in CASES])
-def test_against_the_definition(dev, name, H, kvH, hs, page, order, seqs, groups, pad, act16, cache16):
+def test_against_the_definition(dev, name, H, kvH, hs, page, order, seqs, groups, pad, act16, cache16, wide):
     rng = np.random.default_rng(len(name) + hs)
-    check(dev, rng, Shared(dev, rng, seqs, groups, kvH, hs, page, order, cache16, pad=pad), H, act16)
+    check(dev, rng, Shared(dev, rng, seqs, groups, kvH, hs, page, order, cache16, wide, pad=pad), H, act16)
 
 
 @pytest.mark.parametrize("act16,cache16", TYPES)
@@ -112,7 +116,7 @@ def test_holes_and_entries_that_are_no_page(dev, act16, cache16):
     for missing in (-1.0, np.nan, np.inf, 1e9):
         rng = np.random.default_rng(17)
         seqs = [(2, 200, 0), (40, 300, 0), (1, 130, 0)]
-        c = Shared(dev, rng, seqs, [(0, 3, 96)], 2, 64, 16, "head", cache16, width=19, missing=missing)
+        c = Shared(dev, rng, seqs, [(0, 3, 96)], 2, 64, 16, "head", cache16, missing=missing)
         c.holes = {b: [(16, 64)] for b in range(3)}
         c.table[:, 1:4] = missing
         c.upload()
