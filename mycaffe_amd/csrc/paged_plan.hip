@@ -8,6 +8,7 @@
 // Numbers are whole ones in the base type; what is read is brought into its range here, as everywhere in a paged cache.
 #include <algorithm>
 
+#include "attn_paged.h"
 #include "kernels.h"
 #include "paged.h"
 
@@ -15,30 +16,18 @@ namespace mch {
 
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
-
-// sums over the workgroup of numbers up to PAGED_MOST: of those before the thread's own, and of all (sums: WAVES numbers a call, read until the next barrier)
-__device__ __forceinline__ int scan(int v, int* sums, int* all)
+// sums over the workgroup of numbers up to PAGED_MOST: of those before the thread's own, and of all (sums: as many numbers as wavefronts, read until the next call)
+template <int THREADS> __device__ __forceinline__ int scan(int v, int* sums, int* all)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        x = lane >= o ? paged_sum(x, y) : x;
-    }
-    const int mine = __shfl_up(x, 1);
+    constexpr int WAVES = THREADS / 64;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), x = wave_scan(v);
     __syncthreads();
     if (lane == 63) sums[wave] = x;
     __syncthreads();
-    int before = 0, sum = 0;
-#pragma unroll
-    for (int i = 0; i < WAVES; i++) {
-        before = i < wave ? paged_sum(before, sums[i]) : before;
-        sum = paged_sum(sum, sums[i]);
-    }
-    *all = sum;
-    return lane ? paged_sum(before, mine) : before;
+    const int upTo = wave_scan(lane < WAVES ? sums[lane] : 0);
+    *all = __builtin_amdgcn_readlane(upTo, WAVES - 1);
+    const int before = wave ? __builtin_amdgcn_readlane(upTo, wave ? wave - 1 : 0) : 0, mine = __builtin_amdgcn_update_dpp(0, x, 0x138, 0xf, 0xf, false);   // wave_shr 1
+    return paged_sum(before, mine);
 }
 
 template <typename T> struct Plan {
@@ -68,27 +57,35 @@ template <typename T> struct Plan {
 
 // What one sequence asks for: positions it has to begin with, entries first .. first + need - 1 that it needs, rows (0: it cannot grow)
 struct Ask { int begin, first, need, rows, take, lender; };
-template <typename T> __device__ Ask ask_of(const Plan<T>& p, int b)
+template <typename T> __device__ __forceinline__ Ask ask_of(const Plan<T>& p, int b, int wish, int len, int take, int lender)
 {
-    Ask k = {0, 0, 0, 0, 0, -1};
-    const int n = p.wish(b);
-    k.begin = p.len(b);
-    if (n <= 0) return k;
-    if (k.begin == 0) {
-        k.take = p.take(b, &k.lender);
-        k.begin = k.take * p.a.pageSize;
+    Ask k = {len, 0, 0, 0, 0, -1};
+    if (wish <= 0) return k;
+    if (len == 0) {
+        k.take = take;
+        k.lender = lender;
+        k.begin = take * p.a.pageSize;
     }
     k.first = p.pages_of(k.begin);
-    if (n > p.positions() - k.begin) return k;
-    k.rows = n;
-    k.need = p.pages_of(k.begin + n) - k.first;
+    if (wish > p.positions() - k.begin) return k;
+    k.rows = wish;
+    k.need = p.pages_of(k.begin + wish) - k.first;
     return k;
 }
-
-// Workgroup 0 decides and writes everything that its decisions change; the others copy what they do not, where the block table or the list of free pages
-// is not written in place (in place, they all are: a length that changes decides nothing then).
-template <typename T> __global__ __launch_bounds__(THREADS) void paged_plan_kernel(Plan<T> p, int writeTokens)
+template <typename T> __device__ __forceinline__ Ask ask_of(const Plan<T>& p, int b)
 {
+    int lender = -1;
+    const int wish = p.wish(b), len = p.len(b), take = wish > 0 && len == 0 ? p.take(b, &lender) : 0;
+    return ask_of(p, b, wish, len, take, lender);
+}
+
+// Workgroup 0 decides and writes everything that its decisions change; the others copy what they do not, where the block table and the list of free pages
+// are not written in place (in place, they all are: a length that changes decides nothing then).
+// What bounds it is one read behind the other in workgroup 0, so whatever it goes through - sequences, pages that come back, pages that are taken, entries that are copied -
+// is one list of items each, a thread an item, whose sequence it finds in the list's sums.
+template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void paged_plan_kernel(Plan<T> p, int writeTokens)
+{
+    constexpr int WAVES = THREADS / 64;
     const PagedPlanArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *table = (const T*)a.table, *free = (const T*)a.free;
@@ -111,119 +108,106 @@ template <typename T> __global__ __launch_bounds__(THREADS) void paged_plan_kern
             }
         return;
     }
-    __shared__ int sums[2][WAVES], sStart[THREADS + 1], sNeed[THREADS + 1], sFirst[THREADS], sBegin[THREADS];
-    // ---- the sequences that end: how many pages each gives back, then the pages themselves ----
+    __shared__ int sums[3][WAVES], sStart[THREADS + 1], sNeed[THREADS + 1], sCopy[THREADS + 1], sFirst[THREADS], sBegin[THREADS], sTake[THREADS], sRows, sPages;
+    // the sequence of item i of a list, by the sums in front of each
+    auto whose = [&](const int* starts, int i) __attribute__((always_inline)) -> int {
+        int lo = 0;
+#pragma unroll
+        for (int o = THREADS / 2; o > 0; o >>= 1) lo = starts[lo + o] <= i ? lo + o : lo;
+        return lo;
+    };
+    // ---- the pages of the sequences that end, in the order of the sequences ----
     int count = have;
     for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
         const int mine = b0 + tid;
         const bool ends = mine < a.batch && p.wish(mine) < 0;
         if (!__syncthreads_or(ends)) continue;
-        sNeed[tid] = 0;
-        const uint64_t some = __ballot(ends);
-        for (uint64_t m = some; m; m &= m - 1) {
-            const int at = 64 * wave + __builtin_ctzll(m), b = b0 + at, to = p.pages_of(p.len(b));
-            int n = 0;
-            for (int e0 = p.borrowed(b); e0 < to; e0 += 64)
-                n += __popcll(__ballot(e0 + lane < to && paged_page(table[(size_t)b * a.maxPages + e0 + lane], a.pages) >= 0));
-            if (lane == 0) sNeed[at] = n;
-        }
+        const int from = ends ? p.borrowed(mine) : 0;
+        int items;
+        sStart[tid] = scan<THREADS>(ends ? max(p.pages_of(p.len(mine)) - from, 0) : 0, sums[0], &items);
+        sFirst[tid] = from;
         __syncthreads();
-        int all;
-        const int before = scan(sNeed[tid], sums[0], &all);
-        sStart[tid] = before;
-        __syncthreads();
-        for (uint64_t m = some; m; m &= m - 1) {
-            const int at = 64 * wave + __builtin_ctzll(m), b = b0 + at, to = p.pages_of(p.len(b));
-            int n = paged_sum(count, sStart[at]);
-            for (int e0 = p.borrowed(b); e0 < to; e0 += 64) {
-                const int page = e0 + lane < to ? paged_page(table[(size_t)b * a.maxPages + e0 + lane], a.pages) : -1;
-                const uint64_t given = __ballot(page >= 0);
-                const int place = paged_sum(n, __popcll(given & ((1ull << lane) - 1)));
-                if (page >= 0 && place < a.pages) freeOut[1 + place] = (T)page;
-                n = paged_sum(n, __popcll(given));
+        constexpr int EACH = 4;   // entries of a thread, one behind the other
+        for (int i0 = 0; i0 < items; i0 += EACH * THREADS) {
+            int page[EACH], valid = 0;
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                const int i = i0 + EACH * tid + e, s = whose(sStart, i);
+                page[e] = i < items ? paged_page(table[(size_t)(b0 + s) * a.maxPages + sFirst[s] + i - sStart[s]], a.pages) : -1;
             }
+#pragma unroll
+            for (int e = 0; e < EACH; e++) valid += page[e] >= 0;
+            int all;
+            int place = paged_sum(count, scan<THREADS>(valid, sums[1], &all));
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+                if (page[e] >= 0 && place < a.pages) freeOut[1 + place++] = (T)page[e];
+            count = min(paged_sum(count, all), a.pages);
         }
-        count = min(paged_sum(count, all), a.pages);
+        __syncthreads();
     }
-    // what a lender has is what it had before the call: where lengths change in place, all of them are looked up before any is changed
-    if (a.from)
+    // What a lender has is what it had before the call: where lengths change in place and there are more sequences than threads, all of them are looked up before
+    // any is changed.
+    const bool ahead = a.from && a.batch > THREADS;
+    if (ahead)
         for (int b = tid; b < a.batch; b += THREADS) last[b] = (T)ask_of(p, b).take;
     __syncthreads();
-    // ---- sequence after sequence, 1024 of them at a time ----
+    // ---- sequence after sequence, as many at a time as there are threads ----
     int taken = 0, rows = 0, askedPages = 0, askedRows = 0;
     for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
-        const int b = b0 + tid, n = b < a.batch ? p.wish(b) : 0;
+        const int b = b0 + tid, n = b < a.batch ? p.wish(b) : 0, len = b < a.batch ? p.len(b) : 0;
         Ask k = {0, 0, 0, 0, 0, -1};
         T shared = (T)0;
         if (b < a.batch) {
-            // as ask_of, but for the lender's length
-            k.begin = p.len(b);
-            shared = a.shared ? (T)paged_int(((const T*)a.shared)[b], 0, p.positions()) : (T)0;
-            if (n > 0) {
-                if (k.begin == 0 && a.from) {
-                    k.take = (int)last[b];
-                    k.lender = k.take ? (int)((const T*)a.from)[b] : -1;
-                    k.begin = k.take * a.pageSize;
-                }
-                k.first = p.pages_of(k.begin);
-                if (n <= p.positions() - k.begin) {
-                    k.rows = n;
-                    k.need = p.pages_of(k.begin + n) - k.first;
-                }
+            int lender = -1, take = 0;
+            if (n > 0 && len == 0 && a.from) {
+                if (ahead) {
+                    take = (int)last[b];
+                    lender = take ? (int)((const T*)a.from)[b] : -1;
+                } else take = p.take(b, &lender);
             }
+            shared = a.shared ? (T)paged_int(((const T*)a.shared)[b], 0, p.positions()) : (T)0;
+            k = ask_of(p, b, n, len, take, lender);
         }
-        int allPages, allRows;
-        const int pagesBefore = paged_sum(askedPages, scan(k.need, sums[0], &allPages)), rowsBefore = paged_sum(askedRows, scan(k.rows, sums[1], &allRows));
+        if (tid == 0) { sRows = rows; sPages = taken; }
+        int allPages, allRows, copies;
+        const int pagesBefore = paged_sum(askedPages, scan<THREADS>(k.need, sums[0], &allPages)), rowsBefore = paged_sum(askedRows, scan<THREADS>(k.rows, sums[1], &allRows));
+        // Of those that are granted nobody waits in front: the sums of what is asked are what they get.
         const bool granted = k.rows && paged_sum(pagesBefore, k.need) <= count && paged_sum(rowsBefore, k.rows) <= a.tokens;
-        askedPages = paged_sum(askedPages, allPages);
-        askedRows = paged_sum(askedRows, allRows);
-        // those that wait are behind all that are granted: sums over the granted ones are these, up to the first that waits
-        const int grantedRows = granted ? k.rows : 0, grantedPages = granted ? k.need : 0;
-        int chunkRows, chunkPages;
-        const int rowAt = rows + scan(grantedRows, sums[0], &chunkRows), pageAt = taken + scan(grantedPages, sums[1], &chunkPages);
+        const uint64_t some = __ballot(granted);
+        if (granted && lane == 63 - __builtin_clzll(some)) {
+            atomicMax(&sRows, rowsBefore + k.rows);
+            atomicMax(&sPages, pagesBefore + k.need);
+        }
+        // borrowed entries, and of a row that is copied what the others have left for those that wait
+        const int copy = granted ? k.take : copyTable ? k.take + k.need : 0;
+        sCopy[tid] = scan<THREADS>(copy, sums[2], &copies);
+        const int rowsUpTo = sRows, pagesUpTo = sPages;   // (written before the scan's barriers)
+        const int rowAt = min(rowsBefore, rowsUpTo);   // a sequence that gets nothing stands where the next one that does begins
         sStart[tid] = rowAt;
-        sNeed[tid] = pageAt;
+        sNeed[tid] = min(pagesBefore, pagesUpTo);
         sFirst[tid] = k.first;
         sBegin[tid] = k.begin;
-        if (tid == 0) {
-            sStart[THREADS] = rows + chunkRows;
-            sNeed[THREADS] = taken + chunkPages;
-        }
-        const bool wasEmpty = b < a.batch && p.len(b) == 0;
-        __syncthreads();
+        sTake[tid] = granted ? k.lender : -1 - k.take;
+        askedPages = paged_sum(askedPages, allPages);
+        askedRows = paged_sum(askedRows, allRows);
         if (b < a.batch) {
-            ((T*)a.lensOut)[b] = n < 0 ? (T)0 : granted ? (T)(k.begin + k.rows) : (T)p.len(b);
+            ((T*)a.lensOut)[b] = n < 0 ? (T)0 : granted ? (T)(k.begin + k.rows) : (T)len;
             ((T*)a.starts)[b] = (T)rowAt;
             last[b] = granted ? (T)(rowAt + k.rows - 1) : (T)-1;
-            if (a.sharedOut) ((T*)a.sharedOut)[b] = n < 0 ? (T)0 : granted && wasEmpty ? (T)(k.take * a.pageSize) : shared;
+            if (a.sharedOut) ((T*)a.sharedOut)[b] = n < 0 ? (T)0 : granted && len == 0 ? (T)(k.take * a.pageSize) : shared;
         }
-        // pages: one thread each, that finds its sequence
-        auto whose = [&](const int* starts, int i) -> int {
-            int lo = 0, hi = THREADS;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (starts[mid] <= i) lo = mid;
-                else hi = mid;
-            }
-            return lo;
-        };
-        for (int i = taken + tid; i < taken + chunkPages; i += THREADS) {
-            const int s = whose(sNeed, i);
-            const int at = count - 1 - i;
+        __syncthreads();
+        for (int i = taken + tid; i < pagesUpTo; i += THREADS) {
+            const int s = whose(sNeed, i), at = count - 1 - i;
             const T page = at < have ? free[1 + at] : freeOut[1 + at];
             tableOut[(size_t)(b0 + s) * a.maxPages + sFirst[s] + i - sNeed[s]] = (T)paged_page(page, a.pages);
         }
-        // borrowed pages, and of a row that is copied what the others have left for those that wait
-        for (uint64_t m = __ballot(k.take > 0 || (copyTable && !granted && k.need > 0)); m; m &= m - 1) {
-            const int s = __builtin_ctzll(m), to = __shfl(k.take, s), lender = __shfl(k.lender, s), first = __shfl(k.first, s), need = __shfl(k.need, s);
-            const bool ok = __shfl((int)granted, s);
-            const size_t row = (size_t)(b0 + 64 * wave + s) * a.maxPages;
-            if (ok)
-                for (int e = lane; e < to; e += 64) tableOut[row + e] = table[(size_t)lender * a.maxPages + e];
-            else if (copyTable) {
-                for (int e = lane; e < to; e += 64) tableOut[row + e] = table[row + e];
-                for (int e = first + lane; e < first + need; e += 64) tableOut[row + e] = table[row + e];
-            }
+        for (int i = tid; i < copies; i += THREADS) {
+            const int s = whose(sCopy, i), j = i - sCopy[s], lender = sTake[s], row = b0 + s;
+            // of a row that waits: its first entries, as many as it would have borrowed, then those that it would have got
+            const int e = lender >= 0 || j < -1 - lender ? j : sFirst[s] + j - (-1 - lender);
+            tableOut[(size_t)row * a.maxPages + e] = table[(size_t)(lender >= 0 ? lender : row) * a.maxPages + e];
         }
         if (!copyTable)
             for (uint64_t m = __ballot(n < 0); m; m &= m - 1) {
@@ -232,7 +216,7 @@ template <typename T> __global__ __launch_bounds__(THREADS) void paged_plan_kern
             }
         __syncthreads();
         if (writeTokens)
-            for (int i = rows + tid; i < rows + chunkRows; i += THREADS) {
+            for (int i = rows + tid; i < rowsUpTo; i += THREADS) {
                 const int s = whose(sStart, i), pos = sBegin[s] + i - sStart[s], e = pos / a.pageSize;
                 // entries in front of the new ones are as they were
                 const T* from = e >= sFirst[s] ? (const T*)tableOut : table;
@@ -240,8 +224,8 @@ template <typename T> __global__ __launch_bounds__(THREADS) void paged_plan_kern
                 if (a.positions) ((T*)a.positions)[i] = (T)pos;
                 if (a.slots) ((T*)a.slots)[i] = page >= 0 ? (T)(page * a.pageSize + pos - e * a.pageSize) : (T)-1;
             }
-        rows += chunkRows;
-        taken += chunkPages;
+        rows = rowsUpTo;
+        taken = pagesUpTo;
         __syncthreads();
     }
     if (tid == 0) {
@@ -266,14 +250,16 @@ template <typename T> __global__ __launch_bounds__(256) void paged_plan_rows_ker
 }
 
 constexpr int ROWS_OF_ONE = 8192;   // rows up to which the first workgroup writes their places too
+constexpr int ROWS_OF_FEW = 1024;   // rows, and a quarter as many sequences, up to which four wavefronts do
 
 template <typename T> hipError_t launch(hipStream_t s, const PagedPlanArgs& a)
 {
     Plan<T> p = {a};
     const long long entries = (a.table != a.tableOut ? (long long)a.batch * a.maxPages : 0) + (a.free != a.freeOut ? a.pages : 0);
-    const int others = (int)std::min<long long>(256, (entries + 4 * THREADS - 1) / (4 * THREADS));
-    const bool rows = a.positions || a.slots, own = a.tokens <= ROWS_OF_ONE;
-    hipLaunchKernelGGL((paged_plan_kernel<T>), 1 + others, THREADS, 0, s, p, rows && own ? 1 : 0);
+    const bool rows = a.positions || a.slots, own = a.tokens <= ROWS_OF_ONE, few = a.tokens <= ROWS_OF_FEW && a.batch <= ROWS_OF_FEW / 4;
+    const int others = (int)std::min<long long>(few ? 1024 : 256, (entries + 4095) / 4096);
+    if (few) hipLaunchKernelGGL((paged_plan_kernel<T, 256>), 1 + others, 256, 0, s, p, rows ? 1 : 0);
+    else hipLaunchKernelGGL((paged_plan_kernel<T, 1024>), 1 + others, 1024, 0, s, p, rows && own ? 1 : 0);
     if (rows && !own) hipLaunchKernelGGL((paged_plan_rows_kernel<T>), std::min(a.batch, 65535), 256, 0, s, p);
     return hipGetLastError();
 }
