@@ -94,17 +94,36 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
     const int have = paged_int(free[0], 0, a.pages);
     if (blockIdx.x) {
         const int others = gridDim.x - 1, me = blockIdx.x - 1;
+        constexpr int EACH = 8;   // reads under way
         if (copyFree)
-            for (long long i = (long long)me * THREADS + tid; i < have; i += (long long)others * THREADS) freeOut[1 + i] = free[1 + i];
+            for (long long i0 = (long long)me * EACH * THREADS + tid; i0 < have; i0 += (long long)others * EACH * THREADS) {
+                T v[EACH];
+#pragma unroll
+                for (int j = 0; j < EACH; j++) v[j] = free[1 + min(i0 + j * THREADS, (long long)have - 1)];
+#pragma unroll
+                for (int j = 0; j < EACH; j++)
+                    if (i0 + j * THREADS < have) freeOut[1 + i0 + j * THREADS] = v[j];
+            }
         if (copyTable)
             for (int b = me * WAVES + wave; b < a.batch; b += others * WAVES) {
-                const Ask k = ask_of(p, b);
-                const bool ends = p.wish(b) < 0;
                 const T *from = table + (size_t)b * a.maxPages;
                 T* to = tableOut + (size_t)b * a.maxPages;
-                for (int e = lane; e < a.maxPages; e += 64)
-                    if (ends) to[e] = (T)-1;
-                    else if (e >= k.take && (e < k.first || e >= k.first + k.need)) to[e] = from[e];
+                T v[EACH];
+                auto read = [&](int e0) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int j = 0; j < EACH; j++) v[j] = from[min(e0 + 64 * j + lane, a.maxPages - 1)];
+                };
+                read(0);
+                const Ask k = ask_of(p, b);
+                const bool ends = p.wish(b) < 0;
+                for (int e0 = 0; e0 < a.maxPages; e0 += 64 * EACH) {
+#pragma unroll
+                    for (int j = 0; j < EACH; j++) {
+                        const int e = e0 + 64 * j + lane;
+                        if (e < a.maxPages && (ends || (e >= k.take && (e < k.first || e >= k.first + k.need)))) to[e] = ends ? (T)-1 : v[j];
+                    }
+                    if (e0 + 64 * EACH < a.maxPages) read(e0 + 64 * EACH);
+                }
             }
         return;
     }
@@ -116,15 +135,36 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         for (int o = THREADS / 2; o > 0; o >>= 1) lo = starts[lo + o] <= i ? lo + o : lo;
         return lo;
     };
+    // What a lender has is what it had before the call: where lengths change in place and there are more sequences than threads, all of them are looked up before
+    // any is changed.
+    const bool ahead = a.from && a.batch > THREADS;
+    struct Asks { int wish, len, shared; Ask k; };
+    auto asks_of = [&](int b, bool looked) __attribute__((always_inline)) -> Asks {
+        Asks q = {0, 0, 0, {0, 0, 0, 0, 0, -1}};
+        if (b >= a.batch) return q;
+        q.wish = p.wish(b);
+        q.len = p.len(b);
+        q.shared = a.shared ? paged_int(((const T*)a.shared)[b], 0, p.positions()) : 0;
+        int lender = -1, take = 0;
+        if (q.wish > 0 && q.len == 0 && a.from) {
+            if (looked) {
+                take = (int)last[b];
+                lender = take ? (int)((const T*)a.from)[b] : -1;
+            } else take = p.take(b, &lender);
+        }
+        q.k = ask_of(p, b, q.wish, q.len, take, lender);
+        return q;
+    };
+    const Asks first = asks_of(tid, false);   // read once, ahead of everything
     // ---- the pages of the sequences that end, in the order of the sequences ----
     int count = have;
     for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
-        const int mine = b0 + tid;
-        const bool ends = mine < a.batch && p.wish(mine) < 0;
+        const int mine = b0 + tid, wish = b0 ? mine < a.batch ? p.wish(mine) : 0 : first.wish;
+        const bool ends = wish < 0;
         if (!__syncthreads_or(ends)) continue;
-        const int from = ends ? p.borrowed(mine) : 0;
+        const int from = !ends ? 0 : b0 ? p.borrowed(mine) : first.shared / a.pageSize, to = !ends ? 0 : p.pages_of(b0 ? p.len(mine) : first.len);
         int items;
-        sStart[tid] = scan<THREADS>(ends ? max(p.pages_of(p.len(mine)) - from, 0) : 0, sums[0], &items);
+        sStart[tid] = scan<THREADS>(max(to - from, 0), sums[0], &items);
         sFirst[tid] = from;
         __syncthreads();
         constexpr int EACH = 4;   // entries of a thread, one behind the other
@@ -146,29 +186,16 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         }
         __syncthreads();
     }
-    // What a lender has is what it had before the call: where lengths change in place and there are more sequences than threads, all of them are looked up before
-    // any is changed.
-    const bool ahead = a.from && a.batch > THREADS;
     if (ahead)
         for (int b = tid; b < a.batch; b += THREADS) last[b] = (T)ask_of(p, b).take;
     __syncthreads();
     // ---- sequence after sequence, as many at a time as there are threads ----
     int taken = 0, rows = 0, askedPages = 0, askedRows = 0;
     for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
-        const int b = b0 + tid, n = b < a.batch ? p.wish(b) : 0, len = b < a.batch ? p.len(b) : 0;
-        Ask k = {0, 0, 0, 0, 0, -1};
-        T shared = (T)0;
-        if (b < a.batch) {
-            int lender = -1, take = 0;
-            if (n > 0 && len == 0 && a.from) {
-                if (ahead) {
-                    take = (int)last[b];
-                    lender = take ? (int)((const T*)a.from)[b] : -1;
-                } else take = p.take(b, &lender);
-            }
-            shared = a.shared ? (T)paged_int(((const T*)a.shared)[b], 0, p.positions()) : (T)0;
-            k = ask_of(p, b, n, len, take, lender);
-        }
+        const int b = b0 + tid;
+        const Asks asks = b0 ? asks_of(b, ahead) : first;
+        const int n = asks.wish, len = asks.len;
+        const Ask k = asks.k;
         if (tid == 0) { sRows = rows; sPages = taken; }
         int allPages, allRows, copies;
         const int pagesBefore = paged_sum(askedPages, scan<THREADS>(k.need, sums[0], &allPages)), rowsBefore = paged_sum(askedRows, scan<THREADS>(k.rows, sums[1], &allRows));
@@ -195,7 +222,7 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
             ((T*)a.lensOut)[b] = n < 0 ? (T)0 : granted ? (T)(k.begin + k.rows) : (T)len;
             ((T*)a.starts)[b] = (T)rowAt;
             last[b] = granted ? (T)(rowAt + k.rows - 1) : (T)-1;
-            if (a.sharedOut) ((T*)a.sharedOut)[b] = n < 0 ? (T)0 : granted && len == 0 ? (T)(k.take * a.pageSize) : shared;
+            if (a.sharedOut) ((T*)a.sharedOut)[b] = n < 0 ? (T)0 : granted && len == 0 ? (T)(k.take * a.pageSize) : (T)asks.shared;
         }
         __syncthreads();
         for (int i = taken + tid; i < pagesUpTo; i += THREADS) {
