@@ -309,6 +309,16 @@ struct SampleArgs {
     int count, vocab, logitsRows;
     int perWave, bits;   // the kernel's own
 };
-hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a);
+// scratch memory of the rows that many workgroups share, whole numbers of 64 bits first
+struct SampleCuts {
+    unsigned long long *sums, *list, *weights;
+    void* state;
+    unsigned* counts;
+    int* tickets;
+    float* tops;
+    int slices;
+};
+size_t sample_workspace_bytes(SampleType type, const SampleArgs& a);   // 0: none is needed; without it (null) a workgroup does a row
+hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspace);
 
 }  // namespace mch

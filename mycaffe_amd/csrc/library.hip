@@ -2938,7 +2938,11 @@ long Kernel::sample_fwd(MCH_LONGLONG* pl, long ll)
     }
     auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
     SampleArgs a = {X->ptr, at(0), at(2), at(3), at(4), at(5), at(7), at(1), at(6), stride, (int)rows, (int)vocab, (int)of, 0, 0};
-    HIPCHK(k_sample(m_stream, X->half ? SAMPLE_BF16 : SAMPLE_F32, a));
+    const SampleType type = X->half ? SAMPLE_BF16 : SAMPLE_F32;
+    void* ws;
+    size_t wsb = sample_workspace_bytes(type, a);
+    workspace_or_none(&wsb, &ws);
+    HIPCHK(k_sample(m_stream, type, a, ws));
     m_mem.touch((long)pl[4]);
     if (m[6]) m_mem.touch((long)pl[9]);
     return 0;

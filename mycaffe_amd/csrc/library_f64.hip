@@ -1174,7 +1174,7 @@ long KernelD::sample(const MCH_LONGLONG* pl, long ll)
     }
     auto at = [&](int i) -> void* { return m[i] ? m[i]->ptr : nullptr; };
     SampleArgs a = {X->ptr, at(0), at(2), at(3), at(4), at(5), at(7), at(1), at(6), stride, (int)rows, (int)vocab, (int)of, 0, 0};
-    HIPCHK(k_sample(m_stream, SAMPLE_F64, a));
+    HIPCHK(k_sample(m_stream, SAMPLE_F64, a, nullptr));
     return 0;
 }
 

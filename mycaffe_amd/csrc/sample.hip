@@ -7,8 +7,10 @@
 // A draw compares u with sums over the whole vocabulary: a sum that is off by e moves every border by e, so with 100000 tokens fp32 sums draw another token every
 // few hundred rows.  Weights are made in 64 bits and held as whole numbers of 2^-FB, which add up to the same in any order; their sums are exact.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
+#include "lane_ops.h"
 
 namespace mch {
 
@@ -80,7 +82,7 @@ __device__ __forceinline__ u64 shfl_xor64(u64 v, int o)
     return (u64)hi << 32 | lo;
 }
 // over the workgroup: the sum before the thread's own, and of all (sums: WAVES numbers, read until the next barrier)
-__device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64* all)
+template <int WAVES = THREADS / 64> __device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64* all)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const u64 x = wave_scan(v);
@@ -90,7 +92,7 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* sums, u64* all)
     u64 each = sums[lane & (WAVES - 1)];   // sums of the wavefronts up to the lane's
     each += dpp64<0x111, 0xf>(each);
     each += dpp64<0x112, 0xf>(each);
-    each += dpp64<0x114, 0xf>(each);
+    if (WAVES > 4) each += dpp64<0x114, 0xf>(each);
     if (WAVES > 8) each += dpp64<0x118, 0xf>(each);
     *all = lane_of(each, WAVES - 1);
     return (wave ? lane_of(each, wave ? wave - 1 : 0) : 0) + x - v;
@@ -275,6 +277,29 @@ template <typename R, typename B> __device__ __forceinline__ int locate_equal(co
         for (int e = 0; e < R::VEC; e++) n += v[e] == v0 && old.has(v[e], i0 + e);
         return n;
     }, [&](typename R::V v, int i) __attribute__((always_inline)) -> u64 { return v == v0 && old.has(v, i); }, [&](u64) { return count - 1; }, &total);
+}
+
+// what a row is drawn by
+struct Settings {
+    bool first, byK, byP;   // the largest logit alone; top-k, top-p
+    u64 k, run, share;      // top-k's number; top-p's part and the random number, of 2^64
+    double rate, least;     // Row's rate; min-p, 0: off
+    __device__ __forceinline__ u64 run_of(u64 all) const { return max(1ull, __umul64hi(all, run) + (all * run ? 1 : 0)); }
+};
+template <typename N> __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row)
+{
+    const N heat = a.temperature ? ((const N*)a.temperature)[row] : (N)1, k = a.k ? ((const N*)a.k)[row] : (N)0, p = a.p ? ((const N*)a.p)[row] : (N)1;
+    const N m = a.m ? ((const N*)a.m)[row] : (N)0, u = ((const N*)a.u)[row];
+    Settings t;
+    t.first = !(heat > (N)0) || m > (N)1;
+    t.byK = !t.first && k >= (N)1 && k < (N)a.vocab;
+    t.byP = !t.first && p < (N)1;
+    t.k = t.byK ? (u64)k : 0;
+    t.run = fraction((double)p);
+    t.share = t.first ? 0 : fraction((double)u);
+    t.rate = heat > (N)0 ? fmin(32 * 1.4426950408889634 / (double)heat, 1e300) : 0.0;
+    t.least = !t.first && m > (N)0 ? (double)m : 0.0;
+    return t;
 }
 
 // What is kept: logits above `at`, and equal ones up to index `last`
@@ -518,25 +543,80 @@ template <typename R, typename G> __device__ __forceinline__ int draw_of_few(con
     return s.found;
 }
 
-template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
+// where a row's logits are, and whether it has any
+template <typename L, typename N> __device__ __forceinline__ bool row_of(const SampleArgs& a, int row, Row<L>& r, const double* roots)
+{
+    const N which = a.rows ? ((const N*)a.rows)[row] : (N)row;
+    const bool there = which >= (N)0 && which < (N)a.logitsRows;
+    r.x = (const L*)a.x + (there ? (size_t)(int)which * a.stride : 0);
+    r.vocab = a.vocab;
+    r.perWave = a.perWave;
+    r.bits = a.bits;
+    r.least = -32.0 * (a.bits + 2);
+    r.infinite = false;
+    r.roots = roots;
+    return there;
+}
+template <typename L> __device__ __forceinline__ void top_is(Row<L>& r, typename Row<L>::V top)
+{
+    typedef typename Row<L>::V V;
+    r.infinite = top == (V)INFINITY;
+    r.top = r.infinite ? (V)0 : top;
+}
+template <typename L, typename N> __device__ __forceinline__ void write_draw(const SampleArgs& a, int row, const Row<L>& r, const Settings& t, int id, u64 total)
+{
+    typedef typename Row<L>::V V;
+    ((N*)a.ids)[row] = (N)id;
+    if (!a.logs) return;
+    const V v = r.infinite ? r.top : (V)read(r.x[id]);
+    ((N*)a.logs)[row] = t.first ? (N)0 : (N)(fmin(((double)v - (double)r.top) * t.rate, 0.0) * (0.69314718055994530942 / 32) - log(ldexp((double)total, -a.bits)));
+}
+template <typename N> __device__ __forceinline__ void write_none(const SampleArgs& a, int row)
+{
+    ((N*)a.ids)[row] = (N)-1;
+    if (a.logs) ((N*)a.logs)[row] = (N)0;
+}
+// sums of the weights that the border keeps, of a lane's piece
+template <typename R> __device__ __forceinline__ u64 kept_weights(const R& r, const typename R::V (&v)[R::VEC], int i0, const Border<typename R::V>& border)
+{
+    typedef typename R::V V;
+    u64 sum = 0;
+    if (!(border.at > -(V)INFINITY)) {
+#pragma unroll
+        for (int e0 = 0; e0 < R::VEC; e0 += R::SIDE) {
+#pragma unroll
+            for (int e = 0; e < R::SIDE; e++) sum += r.raw_weight(v[e0 + e]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return sum - R::VEC * RAW;
+    }
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < R::VEC; e++) any = any || v[e] >= border.at;
+    if (__any(any))
+#pragma unroll
+        for (int e0 = 0; e0 < R::VEC; e0 += R::SIDE) {
+#pragma unroll
+            for (int e = e0; e < e0 + R::SIDE; e++) {
+                const u64 w = r.weight(v[e]);
+                sum += border.has(v[e], i0 + e) ? w : 0;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    return sum;
+}
+
+// A row by one workgroup
+template <typename L, typename N> __device__ __forceinline__ void sample_row(const SampleArgs& a, int row, Shared& s, u64* parts)
 {
     typedef Row<L> R;
     typedef typename R::V V;
-    __shared__ Shared s;
     __shared__ V sTop[WAVES];
-    extern __shared__ u64 parts[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x;
-    N *ids = (N*)a.ids, *logs = (N*)a.logs;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid < 32) s.roots[tid] = ROOTS[tid];
-    const N which = a.rows ? ((const N*)a.rows)[row] : (N)row;
-    const bool none = !(which >= (N)0 && which < (N)a.logitsRows);
     R r;
-    r.x = (const L*)a.x + (none ? 0 : (size_t)(int)which * a.stride);
-    r.vocab = a.vocab;
-    r.perWave = a.perWave;
-    r.roots = s.roots;
+    const bool none = !row_of<L, N>(a, row, r, s.roots);
     // ---- the largest logit ----
-    r.infinite = false;
     V top = -(V)INFINITY;
     if (!none)
         r.each([&](int, int, const V (&v)[R::VEC]) __attribute__((always_inline)) {
@@ -551,79 +631,548 @@ template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sam
     __syncthreads();
     for (int i = 0; i < WAVES; i++) top = sTop[i] > top ? sTop[i] : top;
     if (!(top > -(V)INFINITY)) {   // no row, or nothing in it that could be drawn
-        if (tid == 0) {
-            ids[row] = (N)-1;
-            if (logs) logs[row] = (N)0;
-        }
+        if (tid == 0) write_none<N>(a, row);
         return;
     }
-    r.infinite = top == (V)INFINITY;
-    top = r.infinite ? (V)0 : top;
-    r.top = top;
-    r.bits = a.bits;
-    r.least = -32.0 * (a.bits + 2);
-    const N heat = a.temperature ? ((const N*)a.temperature)[row] : (N)1, k = a.k ? ((const N*)a.k)[row] : (N)0, p = a.p ? ((const N*)a.p)[row] : (N)1;
-    const N m = a.m ? ((const N*)a.m)[row] : (N)0;
-    r.rate = heat > (N)0 ? fmin(32 * 1.4426950408889634 / (double)heat, 1e300) : 0.0;
+    const Settings t = settings_of<N>(a, row);
+    top_is(r, top);
+    r.rate = t.rate;
     Border<V> border = {-(V)INFINITY, INT32_MAX};
-    const bool first = !(heat > (N)0) || m > (N)1;   // of the largest logits the first one, whatever else
-    const bool byK = !first && k >= (N)1 && k < (N)a.vocab, byP = !first && p < (N)1;
-    const u64 run = fraction((double)p), share = first ? 0 : fraction((double)((const N*)a.u)[row]);
-    const double least = !first && m > (N)0 ? (double)m : 0.0;
-    auto run_of = [&](u64 all) __attribute__((always_inline)) -> u64 { return max(1ull, __umul64hi(all, run) + (all * run ? 1 : 0)); };
     u64 total, target = 0;
     int id = -1, few;
 #pragma unroll 1
     for (int filter = 0; filter < 2; filter++) {
-        if (!(filter ? byP : byK)) continue;
-        border = select(r, s, parts, border, !filter || !byK, filter != 0, &target, &few, [&](u64 all) __attribute__((always_inline)) -> u64 { return filter ? run_of(all) : (u64)k; });
+        if (!(filter ? t.byP : t.byK)) continue;
+        border = select(r, s, parts, border, !filter || !t.byK, filter != 0, &target, &few, [&](u64 all) __attribute__((always_inline)) -> u64 { return filter ? t.run_of(all) : t.k; });
         if (few) {
-            id = draw_of_few(r, s, few, filter ? 0 : (u64)k, [&](u64 all) __attribute__((always_inline)) -> u64 { return filter ? target : byP ? run_of(all) : 0; }, least, share, &total);
+            id = draw_of_few(r, s, few, filter ? 0 : t.k, [&](u64 all) __attribute__((always_inline)) -> u64 { return filter ? target : t.byP ? t.run_of(all) : 0; }, t.least, t.share, &total);
             break;
         }
     }
-    if (id < 0 && least > 0.0) {   // weights from here on are logits from here on
-        const V at = r.smallest([&](V v) __attribute__((always_inline)) { return r.two_to(r.power(v), 0) >= least; });
+    if (id < 0 && t.least > 0.0) {   // weights from here on are logits from here on
+        const V at = r.smallest([&](V v) __attribute__((always_inline)) { return r.two_to(r.power(v), 0) >= t.least; });
         if (at > border.at) border = Border<V>{at, INT32_MAX};
     }
-    auto target_of = [&](u64 all) __attribute__((always_inline)) -> u64 { return __umul64hi(all, share); };
-    if (first) id = locate_equal(r, s, parts, top, border, 1);
-    else if (id < 0) {
-        const bool some = border.at > -(V)INFINITY;
-        id = locate(r, s, parts, [&](const V (&v)[R::VEC], int i0) __attribute__((always_inline)) -> u64 {
-            u64 sum = 0;
-            if (!some) {
+    if (t.first) id = locate_equal(r, s, parts, r.top, border, 1);
+    else if (id < 0)
+        id = locate(r, s, parts, [&](const V (&v)[R::VEC], int i0) __attribute__((always_inline)) -> u64 { return kept_weights(r, v, i0, border); },
+                    [&](V v, int i) __attribute__((always_inline)) -> u64 { return border.has(v, i) ? r.weight(v) : 0; },
+                    [&](u64 all) __attribute__((always_inline)) -> u64 { return __umul64hi(all, t.share); }, &total);
+    if (tid == 0) write_draw<L, N>(a, row, r, t, id, total);
+}
+template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a)
+{
+    __shared__ Shared s;
+    extern __shared__ u64 parts[];
+    sample_row<L, N>(a, blockIdx.x, s, parts);
+}
+
+// ---- a row by many workgroups ---------------------------------------------------------------------------------------------------------
+// Logits of 16 and 32 bits: slices of a row, one a workgroup, in launches that read them one after the other:
+//   top     the largest logit of every slice;
+//   weigh   the weights: added up, or counted and added up in bins;
+//   border  a workgroup a row: the draw, where neither top-k nor top-p is asked for, else the bin that has the border;
+//   list    what lies above the border's bin and in it, if LISTED tokens at most, else what lies in the bin;
+//   finish  a workgroup a row: with what is listed alone, to the draw, or to the border; rows of which too much would be listed as above, from their beginning;
+//   draw    rows with a border: all weights behind it are added up, and the last workgroup draws.
+// (The last launch alone, of few rows, has the last workgroup of a row, by a ticket, read what the others have written past the caches, at the level that all XCDs share: a
+// wait for that at the end of every slice costs more than a launch.  256 rows of 131072, weigh with it 48 us.)  Sums are whole numbers: any order gives the same.
+constexpr int CUT = 256, CUT_BINS = CUT, LISTED = 4096;
+enum RowMode { ROW_DONE, ROW_LIST_ALL, ROW_LIST_BIN, ROW_DRAW, ROW_WHOLE };
+struct RowState {
+    int mode, last;       // border: logits above `at`, equal ones up to index `last`
+    float top, lo, hi, at;
+    u64 above, target;    // of the border's bin: what is above it, and where the border is
+};
+
+__device__ __forceinline__ void put(u64* p, u64 v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put(uint32_t* p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T> __device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// whether this is the last of n workgroups to come here; what it wrote before is there then
+__device__ __forceinline__ bool last_of(int* ticket, int n, int* shared)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return *shared == n - 1;
+}
+
+// a slice: EACH logits a thread of T, in pieces, in the order of the vocabulary from piece to piece and within one from thread to thread
+template <typename L, int EACH, int T> struct Slice {
+    typedef Row<L> R;
+    static constexpr int VEC = R::VEC, PIECES = EACH / VEC, LOGITS = EACH * T;
+    __device__ static int index(int slice, int piece) { return slice * LOGITS + piece * T * VEC + (int)threadIdx.x * VEC; }
+    L raw[PIECES][VEC];
+    __device__ __forceinline__ void load(const R& r, int slice)   // all of it under way at once
+    {
 #pragma unroll
-                for (int e0 = 0; e0 < R::VEC; e0 += R::SIDE) {
-#pragma unroll
-                    for (int e = 0; e < R::SIDE; e++) sum += r.raw_weight(v[e0 + e]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                return sum - R::VEC * RAW;
-            }
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < R::VEC; e++) any = any || v[e] >= border.at;
-            if (__any(any))
-#pragma unroll
-                for (int e0 = 0; e0 < R::VEC; e0 += R::SIDE) {
-#pragma unroll
-                    for (int e = e0; e < e0 + R::SIDE; e++) {
-                        const u64 w = r.weight(v[e]);
-                        sum += border.has(v[e], i0 + e) ? w : 0;
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            return sum;
-        }, [&](V v, int i) __attribute__((always_inline)) -> u64 { return border.has(v, i) ? r.weight(v) : 0; }, target_of, &total);
+        for (int q = 0; q < PIECES; q++) r.fetch(index(slice, q), raw[q]);
     }
-    if (tid == 0) {
-        ids[row] = (N)id;
-        if (logs) {
-            const V v = r.infinite ? top : (V)read(r.x[id]);
-            logs[row] = first ? (N)0 : (N)(fmin(((double)v - (double)top) * r.rate, 0.0) * (0.69314718055994530942 / 32) - log(ldexp((double)total, -a.bits)));
+    template <typename F> __device__ __forceinline__ void each(const R& r, int slice, F f) const   // f(piece, first index, logits)
+    {
+#pragma unroll
+        for (int q = 0; q < PIECES; q++) {
+            float v[VEC];
+            r.logits(raw[q], v);
+            f(q, index(slice, q), v);
         }
     }
+};
+
+template <int T> struct DrawShared { u64 sums[T / 64], tot[16 * T / 64]; u64 before; int slice, ticket; };
+// The last workgroup of a row: from the sums of n slices, which it is that the draw falls into, and where in it
+template <typename L, typename N, int EACH, int T>
+__device__ __forceinline__ void draw_from(const SampleArgs& a, int row, const Row<L>& r, const Settings& t, const Border<float>& border, const u64* slices, int n, DrawShared<T>& s)
+{
+    typedef Slice<L, EACH, T> C;
+    constexpr int W = T / 64;
+    const int tid = threadIdx.x, wave = tid >> 6, per = (n + T - 1) / T;
+    u64 mine = 0, total;
+    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) mine += get(slices + i);
+    u64 before = block_scan<W>(mine, s.sums, &total);
+    const u64 want = __umul64hi(total, t.share);
+    if (before <= want && want < before + mine)
+        for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
+            const u64 x = get(slices + i);
+            if (want < before + x) { s.slice = i; s.before = before; break; }
+            before += x;
+        }
+    __syncthreads();
+    const int slice = s.slice;
+    u64 w[C::PIECES];
+    C c;
+    c.load(r, slice);
+    c.each(r, slice, [&](int q, int i0, const float (&v)[C::VEC]) __attribute__((always_inline)) {
+        w[q] = kept_weights(r, v, i0, border);
+        const u64 sum = wave_sum(w[q]);
+        if ((tid & 63) == 0) s.tot[q * W + wave] = sum;
+    });
+    __syncthreads();
+    u64 at = s.before;
+    int k = 0;
+#pragma unroll
+    for (int q = 0; q < C::PIECES; q++) {
+        for (; k < q * W + wave; k++) at += s.tot[k];
+        const u64 from = at + wave_scan(w[q]) - w[q];
+        if (from <= want && want < from + w[q]) {
+            float v[C::VEC];
+            const int i0 = C::index(slice, q);
+            r.logits(c.raw[q], v);
+            u64 x = from;
+            int id = -1;
+#pragma unroll
+            for (int e = 0; e < C::VEC; e++) {
+                const u64 one = border.has(v[e], i0 + e) ? r.weight(v[e]) : 0;
+                if (x <= want && want < x + one) id = i0 + e;
+                x += one;
+            }
+            write_draw<L, N>(a, row, r, t, id, total);
+        }
+    }
+}
+
+template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_top_kernel(SampleArgs a, SampleCuts w)
+{
+    __shared__ float sTop[CUT / 64];
+    const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+    Row<L> r;
+    float top = -INFINITY;
+    Slice<L, EACH, CUT> c;
+    if (row_of<L, float>(a, row, r, nullptr)) {
+        c.load(r, slice);
+        c.each(r, slice, [&](int, int, const float (&v)[Row<L>::VEC]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < Row<L>::VEC; e++) top = v[e] > top ? v[e] : top;
+        });
+    }
+    top = group_max<64>(top);
+    if ((tid & 63) == 0) sTop[tid >> 6] = top;
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < CUT / 64; i++) top = fmaxf(top, sTop[i]);
+        w.tops[row * w.slices + slice] = top;
+    }
+    if (slice == 0 && tid < 4) w.tickets[4 * row + tid] = 0;
+}
+
+// smallest logit that the weights' share `least` keeps
+template <typename R> __device__ __forceinline__ Border<float> border_of_least(const R& r, double least)
+{
+    Border<float> b = {-INFINITY, INT32_MAX};
+    if (least > 0.0) b.at = r.smallest([&](float v) __attribute__((always_inline)) { return r.two_to(r.power(v), 0) >= least; });
+    return b;
+}
+
+// the row's largest logit, and the first slice that has it
+__device__ __forceinline__ float top_of_row(const SampleCuts& w, int row, int* first)
+{
+    __shared__ float sTop[CUT / 64];
+    __shared__ int sAt[CUT / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float top = -INFINITY;
+    int at = INT32_MAX;
+    for (int i = tid; i < w.slices; i += CUT) {
+        const float x = w.tops[row * w.slices + i];
+        if (x > top) { top = x; at = i; }
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        const float x = __shfl_xor(top, o);
+        const int i = __shfl_xor(at, o);
+        if (x > top || (x == top && i < at)) { top = x; at = i; }
+    }
+    if (lane == 0) { sTop[wave] = top; sAt[wave] = at; }
+    __syncthreads();
+    for (int i = 0; i < CUT / 64; i++)
+        if (sTop[i] > top || (sTop[i] == top && sAt[i] < at)) { top = sTop[i]; at = sAt[i]; }
+    *first = at;
+    return top;
+}
+// bins a unit of the logits, twice: top-k's over all octaves of weights, top-p's over 24 (what lies below weighs too little to be reached, but for flat rows)
+template <typename R> __device__ __forceinline__ float bins_of(const R& r, const Settings& t)
+{
+    return (float)fmin(2.0 * r.rate * CUT_BINS / (t.byK ? -r.least : 32.0 * 24), 1e37);
+}
+
+template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_weigh_kernel(SampleArgs a, SampleCuts w)
+{
+    typedef Row<L> R;
+    typedef Slice<L, EACH, CUT> C;
+    __shared__ uint32_t sCount[CUT_BINS];
+    __shared__ u64 sWeight[CUT_BINS], sSums[CUT / 64];
+    __shared__ double sRoots[32];
+    const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+    R r;
+    if (!row_of<L, float>(a, row, r, sRoots)) return;
+    C c;
+    c.load(r, slice);
+    const Settings t = settings_of<float>(a, row);
+    if (t.first) return;
+    if (tid < 32) sRoots[tid] = ROOTS[tid];
+    sCount[tid] = 0;
+    sWeight[tid] = 0;
+    int first;
+    const float top = top_of_row(w, row, &first);   // (with the barrier that the lines above need)
+    if (!(top > -INFINITY)) return;
+    top_is(r, top);
+    r.rate = t.rate;
+    u64 sum = 0, all;
+    if (!t.byK && !t.byP) {
+        const Border<float> border = border_of_least(r, t.least);
+        c.each(r, slice, [&](int, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) { sum += kept_weights(r, v, i0, border); });
+        block_scan<CUT / 64>(sum, sSums, &all);
+        if (tid == 0) w.sums[row * w.slices + slice] = all;
+        return;
+    }
+    const bool byWeight = !t.byK;
+    const float half = r.top * 0.5f, scale = bins_of(r, t);
+    c.each(r, slice, [&](int, int, const float (&v)[R::VEC]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e0 = 0; e0 < R::VEC; e0 += R::SIDE) {
+            u64 x[R::SIDE];
+            if (byWeight) {
+#pragma unroll
+                for (int e = 0; e < R::SIDE; e++) sum += x[e] = r.raw_weight(v[e0 + e]);
+                sum -= R::SIDE * RAW;
+            }
+#pragma unroll
+            for (int e = 0; e < R::SIDE; e++) {
+                const float z = r.bins(v[e0 + e], half, scale);
+                if (!(z < (float)CUT_BINS)) continue;
+                atomicAdd(&sCount[(int)z], 1u);
+                if (byWeight) atomicAdd(&sWeight[(int)z], x[e] - RAW);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    });
+    block_scan<CUT / 64>(sum, sSums, &all);
+    const size_t bins = ((size_t)row * w.slices + slice) * CUT_BINS + tid;
+    w.counts[bins] = sCount[tid];
+    if (byWeight) {
+        w.weights[bins] = sWeight[tid];
+        if (tid == 0) w.sums[row * w.slices + slice] = all;
+    }
+}
+
+template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_border_kernel(SampleArgs a, SampleCuts w)
+{
+    typedef Row<L> R;
+    typedef Slice<L, EACH, CUT> C;
+    __shared__ DrawShared<CUT> s;
+    __shared__ int sFirst, sBin, sReached, sIn;
+    __shared__ double sRoots[32];
+    const int tid = threadIdx.x, row = blockIdx.x;
+    R r;
+    row_of<L, float>(a, row, r, sRoots);
+    const Settings t = settings_of<float>(a, row);
+    const bool byWeight = !t.byK, bins = t.byK || t.byP;
+    // this thread's bin of the row
+    uint32_t n = 0;
+    u64 x = 0, sum = 0, all = 0;
+    if (bins) {
+#pragma unroll 8
+        for (int i = 0; i < w.slices; i++) n += w.counts[((size_t)row * w.slices + i) * CUT_BINS + tid];
+        if (byWeight) {
+#pragma unroll 8
+            for (int i = 0; i < w.slices; i++) x += w.weights[((size_t)row * w.slices + i) * CUT_BINS + tid];
+            for (int i = tid; i < w.slices; i += CUT) sum += w.sums[row * w.slices + i];
+        }
+    }
+    if (tid < 32) sRoots[tid] = ROOTS[tid];
+    if (tid == 0) { sFirst = INT32_MAX; sBin = -1; }
+    int first;
+    const float top = top_of_row(w, row, &first);
+    RowState st = {};
+    st.mode = ROW_DONE;
+    st.top = top;
+    if (!(top > -INFINITY)) {   // no row, or nothing in it that could be drawn
+        if (tid == 0) {
+            write_none<float>(a, row);
+            ((RowState*)w.state)[row] = st;
+        }
+        return;
+    }
+    top_is(r, top);
+    r.rate = t.rate;
+    if (t.first) {
+        C c;
+        c.load(r, first);
+        c.each(r, first, [&](int, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = R::VEC - 1; e >= 0; e--)
+                if (v[e] == r.top) atomicMin(&sFirst, i0 + e);
+        });
+        __syncthreads();
+        if (tid == 0) write_draw<L, float>(a, row, r, t, sFirst, 0);
+    } else if (!bins) {
+        draw_from<L, float, EACH, CUT>(a, row, r, t, border_of_least(r, t.least), w.sums + row * w.slices, w.slices, s);
+    } else {
+        if (byWeight) block_scan<CUT / 64>(sum, s.sums, &all);
+        u64 any;
+        const u64 tokens = block_scan<CUT / 64>(n, s.sums, &any), before = byWeight ? block_scan<CUT / 64>(x, s.sums, &any) : tokens;
+        const u64 target = byWeight ? t.run_of(all) : t.k, amount = byWeight ? x : n;
+        if (before < target && target <= before + amount) { sBin = tid; s.before = before; sReached = (int)tokens + n; sIn = n; }
+        __syncthreads();
+        const int bin = sBin;
+        if (bin < 0) {
+            // top-k: as many as there are with weight; top-p: it goes further down than the bins
+            st.mode = t.byP ? ROW_WHOLE : ROW_DRAW;
+            const Border<float> border = border_of_least(r, t.least);
+            st.at = border.at;
+            st.last = border.last;
+        } else {
+            const float half = r.top * 0.5f, scale = bins_of(r, t);
+            st.lo = r.smallest([&](float v) __attribute__((always_inline)) { return r.bins(v, half, scale) < (float)(bin + 1); });
+            st.hi = bin ? of_key(key_of(r.smallest([&](float v) __attribute__((always_inline)) { return r.bins(v, half, scale) < (float)bin; })) - 1) : r.top;
+            st.above = s.before;
+            st.target = target;
+            st.mode = sReached <= LISTED ? ROW_LIST_ALL : sIn <= LISTED && !(t.byK && t.byP) ? ROW_LIST_BIN : ROW_WHOLE;
+        }
+    }
+    if (tid == 0) ((RowState*)w.state)[row] = st;
+}
+
+// Logit (-0 is 0) and index as one number: falling logits, and rising indexes of equal ones, fall.  Few bits, so that few rounds tell them apart: 16 of a 16-bit logit
+constexpr int INDEX_BITS = 20, LAST_INDEX = (1 << INDEX_BITS) - 1;
+static_assert(SAMPLE_VOCAB <= LAST_INDEX + 1, "index");
+template <typename L> __device__ __forceinline__ u64 place_of(float v, int i)
+{
+    const uint32_t k = key_of(v + 0.f);
+    return (u64)(sizeof(L) == 2 ? k >> 16 : k) << INDEX_BITS | (uint32_t)(LAST_INDEX - i);
+}
+// of a logit that need not be one of L: the least place of those that are not below it
+template <typename L> __device__ __forceinline__ u64 least_place(float v)
+{
+    const uint32_t k = key_of(v + 0.f);
+    // the lower half of a 16-bit logit's key is 0, of a negative one all bits
+    return sizeof(L) == 2 ? (u64)((k >> 16) + (k >> 31 && k & 0xffffu ? 1 : 0)) << INDEX_BITS : (u64)k << INDEX_BITS;
+}
+__device__ __forceinline__ int index_at(u64 place) { return LAST_INDEX - (int)(place & LAST_INDEX); }
+template <typename L> __device__ __forceinline__ float logit_at(u64 place)
+{
+    const uint32_t k = (uint32_t)(place >> INDEX_BITS);
+    return of_key(sizeof(L) == 2 ? k << 16 | (k & 0x8000u ? 0u : 0xffffu) : k);   // (of a negative one all bits are turned)
+}
+
+template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_list_kernel(SampleArgs a, SampleCuts w)
+{
+    typedef Row<L> R;
+    typedef Slice<L, EACH, CUT> C;
+    __shared__ u64 sSums[CUT / 64];
+    __shared__ int sBase;
+    const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
+    const RowState st = ((const RowState*)w.state)[row];
+    if (st.mode != ROW_LIST_ALL && st.mode != ROW_LIST_BIN) return;
+    R r;
+    row_of<L, float>(a, row, r, nullptr);
+    top_is(r, st.top);
+    const float lo = st.lo, hi = st.mode == ROW_LIST_ALL ? r.top : st.hi;
+    u64 hits = 0, all;
+    C c;
+    c.load(r, slice);
+    c.each(r, slice, [&](int q, int, const float (&v)[R::VEC]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < R::VEC; e++) hits |= (u64)(v[e] >= lo && v[e] <= hi) << (q * R::VEC + e);
+    });
+    int to = (int)block_scan<CUT / 64>(__popcll(hits), sSums, &all);
+    if (!all) return;
+    if (tid == 0) sBase = __hip_atomic_fetch_add(w.tickets + 4 * row + 3, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    to += sBase;
+    if (hits)
+        c.each(r, slice, [&](int q, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < R::VEC; e++)
+                if (hits >> (q * R::VEC + e) & 1) {
+                    if (to < LISTED) w.list[(size_t)row * LISTED + to] = place_of<L>(v[e], i0 + e);
+                    to++;
+                }
+        });
+}
+
+constexpr int OWN = LISTED / THREADS;
+struct ReachShared { uint32_t count[THREADS]; u64 amount[THREADS], sums[WAVES], above, key; int bin; };
+// Of numbers key[j], which are all different, with amounts: the one at which the sum of the amounts, from the largest number down, reaches the target; 0 if it does not.
+// In ever smaller ranges, a bin a thread.
+template <typename F> __device__ __forceinline__ u64 reach(ReachShared& s, const u64 (&key)[OWN], F amount, u64 lo, u64 hi, u64 target)
+{
+    const int tid = threadIdx.x;
+    u64 above = 0;
+#pragma unroll 1
+    for (;;) {
+        const int shift = max(0, 64 - 10 - __builtin_clzll((hi - lo) | 1));
+        __syncthreads();
+        s.count[tid] = 0;
+        s.amount[tid] = 0;
+        if (tid == 0) s.bin = -1;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < OWN; j++) {
+            const u64 w = amount(j);
+            if (!w || key[j] < lo || key[j] > hi) continue;
+            const int b = (int)((hi - key[j]) >> shift);
+            atomicAdd(&s.count[b], 1u);
+            atomicAdd(&s.amount[b], w);
+        }
+        __syncthreads();
+        u64 all;
+        const u64 mine = s.amount[tid], at = above + block_scan(mine, s.sums, &all);
+        if (at < target && target <= at + mine) { s.bin = tid; s.above = at; }
+        __syncthreads();
+        const int bin = s.bin;
+        if (bin < 0) return 0;
+        above = s.above;
+        hi -= (u64)bin << shift;
+        const u64 span = (1ull << shift) - 1;
+        lo = hi - lo > span ? hi - span : lo;
+        if (s.count[bin] == 1) break;
+    }
+#pragma unroll
+    for (int j = 0; j < OWN; j++)
+        if (key[j] >= lo && key[j] <= hi && amount(j)) s.key = key[j];
+    __syncthreads();
+    const u64 k = s.key;
+    __syncthreads();
+    return k;
+}
+
+template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleArgs a, SampleCuts w)
+{
+    static_assert(THREADS == 1024, "bins of reach()");
+    typedef Row<L> R;
+    __shared__ union { Shared row; ReachShared reach; } s;
+    __shared__ double sRoots[32];
+    extern __shared__ u64 parts[];
+    const int tid = threadIdx.x, row = blockIdx.x;
+    RowState st = ((const RowState*)w.state)[row];
+    if (st.mode == ROW_WHOLE) {
+        sample_row<L, float>(a, row, s.row, parts);
+        return;
+    }
+    if (st.mode != ROW_LIST_ALL && st.mode != ROW_LIST_BIN) return;
+    R r;
+    row_of<L, float>(a, row, r, sRoots);
+    top_is(r, st.top);
+    const Settings t = settings_of<float>(a, row);
+    r.rate = t.rate;
+    const int n = min(w.tickets[4 * row + 3], LISTED);
+    const u64* list = w.list + (size_t)row * LISTED;
+    if (tid < 32) sRoots[tid] = ROOTS[tid];
+    u64 key[OWN], weight[OWN], least = 0, all, total;
+#pragma unroll
+    for (int j = 0; j < OWN; j++) key[j] = tid + THREADS * j < n ? list[tid + THREADS * j] : 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < OWN; j++) weight[j] = key[j] ? r.weight(logit_at<L>(key[j])) : 0;
+    auto one = [&](int j) __attribute__((always_inline)) -> u64 { return key[j] != 0; };
+    auto kept = [&](int j) __attribute__((always_inline)) -> u64 { return key[j] >= least ? weight[j] : 0; };
+    if (n <= FEW) {
+        if (tid < n) {
+            s.row.values[tid] = logit_at<L>(key[0]);
+            s.row.weights[tid] = weight[0];
+            s.row.ids[tid] = index_at(key[0]);
+        }
+        __syncthreads();
+    }
+    if (st.mode == ROW_LIST_ALL && n <= FEW) {
+        const int id = draw_of_few(r, s.row, n, t.k, [&](u64 sum) __attribute__((always_inline)) -> u64 { return !t.byP ? 0 : t.byK ? t.run_of(sum) : st.target; }, t.least, t.share, &total);
+        if (tid == 0) write_draw<L, float>(a, row, r, t, id, total);
+        return;
+    }
+    const u64 from = place_of<L>(st.lo, LAST_INDEX), to = place_of<L>(st.mode == ROW_LIST_ALL ? r.top : st.hi, 0);
+    if (st.mode == ROW_LIST_BIN) {
+        const u64 target = st.target - st.above, border = t.byK ? reach(s.reach, key, one, from, to, target) : reach(s.reach, key, kept, from, to, target);
+        const Border<float> b = border_of_least(r, t.least);
+        st.at = logit_at<L>(border);
+        st.last = index_at(border);
+        if (b.at > st.at) { st.at = b.at; st.last = b.last; }
+        st.mode = ROW_DRAW;
+        if (tid == 0) ((RowState*)w.state)[row] = st;
+        return;
+    }
+    auto sum = [&]() __attribute__((always_inline)) -> u64 {
+        u64 x = 0;
+#pragma unroll
+        for (int j = 0; j < OWN; j++) x += kept(j);
+        block_scan(x, s.reach.sums, &all);
+        return all;
+    };
+    if (t.byK) least = max(least, reach(s.reach, key, one, from, to, t.k));
+    if (t.byP) least = max(least, reach(s.reach, key, kept, from, to, t.byK ? t.run_of(sum()) : st.target));
+    if (t.least > 0.0) least = max(least, least_place<L>(border_of_least(r, t.least).at));
+    total = sum();
+    // in the order of the vocabulary: the sum up to the token drawn exceeds u times all
+    u64 order[OWN];
+#pragma unroll
+    for (int j = 0; j < OWN; j++) order[j] = key[j] & LAST_INDEX;
+    const u64 drawn = reach(s.reach, order, kept, LAST_INDEX + 1 - a.vocab, LAST_INDEX, __umul64hi(total, t.share) + 1);
+    if (tid == 0) write_draw<L, float>(a, row, r, t, index_at(drawn), total);
+}
+
+template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_draw_kernel(SampleArgs a, SampleCuts w)
+{
+    typedef Slice<L, EACH, CUT> C;
+    typedef Row<L> R;
+    __shared__ DrawShared<CUT> s;
+    __shared__ double sRoots[32];
+    const int row = blockIdx.y, slice = blockIdx.x;
+    const RowState st = ((const RowState*)w.state)[row];
+    if (st.mode != ROW_DRAW) return;
+    R r;
+    row_of<L, float>(a, row, r, sRoots);
+    C c;
+    c.load(r, slice);
+    const Settings t = settings_of<float>(a, row);
+    top_is(r, st.top);
+    r.rate = t.rate;
+    if (threadIdx.x < 32) sRoots[threadIdx.x] = ROOTS[threadIdx.x];
+    __syncthreads();
+    const Border<float> border = {st.at, st.last};
+    u64 sum = 0, all;
+    c.each(r, slice, [&](int, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) { sum += kept_weights(r, v, i0, border); });
+    block_scan<CUT / 64>(sum, s.sums, &all);
+    if (threadIdx.x == 0) put(w.sums + row * w.slices + slice, all);
+    if (last_of(w.tickets + 4 * row + 2, w.slices, &s.ticket)) draw_from<L, float, EACH, CUT>(a, row, r, t, border, w.sums + row * w.slices, w.slices, s);
 }
 
 }  // namespace
@@ -636,12 +1185,66 @@ int sample_bits(int vocab)
     return std::min(50, 63 - log);
 }
 
-hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a)
+// Rows up to which slices of them are what workgroups have, logits of a row and of all from which on, and logits a thread of a slice: few where there are few slices
+constexpr int CUT_ROWS = 4096, CUT_VOCAB = 4096, CUT_LOGITS = 1 << 19;
+static int cut_each(const SampleArgs& a)
+{
+    const long long slices = (long long)a.count * ((a.vocab + 32 * CUT - 1) / (32 * CUT));
+    return slices < 256 && a.vocab <= 128 * 8 * CUT ? 8 : 32;
+}
+static bool cut_bins(const SampleArgs& a) { return a.k || a.p; }
+
+size_t sample_workspace_bytes(SampleType type, const SampleArgs& a)
+{
+    if (type == SAMPLE_F64 || a.count > CUT_ROWS || a.vocab <= CUT_VOCAB || (long long)a.count * a.vocab < CUT_LOGITS) return 0;
+    const int each = cut_each(a);
+    const size_t slices = (a.vocab + each * CUT - 1) / (each * CUT), rows = a.count;
+    return rows * (slices * (8 + 4) + sizeof(RowState) + 16 + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
+}
+
+hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspace)
 {
     const int chunk = 64 * 16 / (type == SAMPLE_BF16 ? 2 : type == SAMPLE_F32 ? 4 : 8);
     a.perWave = (a.vocab + chunk * WAVES - 1) / (chunk * WAVES);
     a.bits = sample_bits(a.vocab);
     const size_t parts = (size_t)a.perWave * WAVES * sizeof(u64);
+    if (workspace) {
+        const int each = cut_each(a);
+        const size_t rows = a.count;
+        SampleCuts w = {};
+        w.slices = (a.vocab + each * CUT - 1) / (each * CUT);
+        w.sums = (u64*)workspace;
+        w.state = w.sums + rows * w.slices;
+        char* at = (char*)w.state + rows * sizeof(RowState);
+        if (cut_bins(a)) {
+            w.list = (u64*)at;
+            w.weights = w.list + rows * LISTED;
+            w.counts = (uint32_t*)(w.weights + rows * w.slices * CUT_BINS);
+            at = (char*)(w.counts + rows * w.slices * CUT_BINS);
+        }
+        w.tickets = (int*)at;
+        w.tops = (float*)(w.tickets + 4 * rows);
+        const dim3 grid(w.slices, a.count);
+        auto go = [&](auto type, auto size) {
+            typedef decltype(type) L;
+            constexpr int EACH = decltype(size)::value;
+            hipLaunchKernelGGL((sample_top_kernel<L, EACH>), grid, CUT, 0, s, a, w);
+            hipLaunchKernelGGL((sample_weigh_kernel<L, EACH>), grid, CUT, 0, s, a, w);
+            hipLaunchKernelGGL((sample_border_kernel<L, EACH>), a.count, CUT, 0, s, a, w);
+            if (cut_bins(a)) {
+                hipLaunchKernelGGL((sample_list_kernel<L, EACH>), grid, CUT, 0, s, a, w);
+                hipLaunchKernelGGL((sample_finish_kernel<L>), a.count, THREADS, parts, s, a, w);
+                hipLaunchKernelGGL((sample_draw_kernel<L, EACH>), grid, CUT, 0, s, a, w);
+            }
+        };
+        auto sized = [&](auto type) {
+            if (each == 8) go(type, std::integral_constant<int, 8>{});
+            else go(type, std::integral_constant<int, 32>{});
+        };
+        if (type == SAMPLE_F32) sized(float());
+        else sized(bf16_t());
+        return hipGetLastError();
+    }
     if (type == SAMPLE_F32) hipLaunchKernelGGL((sample_kernel<float, float>), a.count, THREADS, parts, s, a);
     else if (type == SAMPLE_BF16) hipLaunchKernelGGL((sample_kernel<bf16_t, float>), a.count, THREADS, parts, s, a);
     else hipLaunchKernelGGL((sample_kernel<double, double>), a.count, THREADS, parts, s, a);
