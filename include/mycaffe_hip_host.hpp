@@ -428,6 +428,29 @@ public:
         ex2(MCH_FN_ATTN_PAGED_FWD, {fScale}, {c.nBatch, c.nTokens, c.nHeads, c.nKvHeads, c.nSize, c.nPages, c.nPageSize, c.nMaxPages, hQ, c.hKPages, c.hVPages, c.hTable,
                                               c.hStarts, c.hLens, hY, c.nStridePage, c.nStrideHead, c.nStridePos, nMaxNew});
     }
+    // the same for sequences that share prefixes: group g are the sequences hGroups[g] .. hGroups[g + 1] - 1, their first hShared[g] positions in the same pages
+    void AttnPagedPrefixForward(const PagedCache& c, long hQ, long hY, int nGroups, long hGroups, long hShared, float fScale = 0.f, int nMaxNew = 0)
+    {
+        ex2(MCH_FN_ATTN_PAGED_PREFIX_FWD, {fScale}, {c.nBatch, c.nTokens, c.nHeads, c.nKvHeads, c.nSize, c.nPages, c.nPageSize, c.nMaxPages, hQ, c.hKPages, c.hVPages,
+                                                     c.hTable, c.hStarts, c.hLens, hY, c.nStridePage, c.nStrideHead, c.nStridePos, nGroups, hGroups, hShared, nMaxNew});
+    }
+    // room for the next hNew tokens of a cache's sequences: lengths and table of the cache and the stack hFree in place; hPositions, hSlots may be 0, and
+    // hFrom with hShared (in place): sequences that begin behind another one's first positions
+    void PagedPlan(const PagedCache& c, long hNew, long hFree, long hLast, long hPositions = 0, long hSlots = 0, long hFrom = 0, long hShared = 0)
+    {
+        if (hFrom || hShared)
+            ex2(MCH_FN_PAGED_PLAN, {}, {c.nBatch, c.nTokens, c.nPages, c.nPageSize, c.nMaxPages, hNew, c.hLens, c.hTable, hFree, c.hLens, c.hTable, hFree, c.hStarts,
+                                        hPositions, hSlots, hLast, hFrom, hShared, hShared});
+        else
+            ex2(MCH_FN_PAGED_PLAN, {}, {c.nBatch, c.nTokens, c.nPages, c.nPageSize, c.nMaxPages, hNew, c.hLens, c.hTable, hFree, c.hLens, c.hTable, hFree, c.hStarts,
+                                        hPositions, hSlots, hLast});
+    }
+    // the next token of every row of logits; handles of 0 leave a setting out
+    void SampleForward(int nRows, int nVocab, long hLogits, long hRandom, long hIds, long hTemperature = 0, long hTopK = 0, long hTopP = 0, long hMinP = 0,
+                       long hLogProb = 0, long hRows = 0, int nLogitsRows = 0, long long nRowStride = 0)
+    {
+        ex2(MCH_FN_SAMPLE_FWD, {}, {nRows, nVocab, hLogits, hRandom, hIds, hTemperature, hTopK, hTopP, hMinP, hLogProb, hRows, nLogitsRows, nRowStride});
+    }
     // fused QKV projection: q, k, v = X W^T + bias written as (B,H,T,hs), q and k rotated when hRope is given (no
     // counterpart in the reference)
     void QkvProjHeads(int nBatch, int nT, int nHeads, int nSize, long hX, long hWeight, long hBias, long hQ, long hK, long hV,

@@ -332,7 +332,37 @@ class SoftmaxLayer:
                                   top.gpu_diff, 0.0, self.hBottomDesc, bottom.gpu_diff)
 
 
-class PagedSequences:
+class _Paged:
+    """What the layers of a model keep of the sequences that they serve: pages of the same numbers in every layer, angles that layers share."""
+
+    def __init__(self, cuda, pages, page_size, max_pages, *blobs):
+        self.cuda, self.pages, self.page_size, self.max_pages = cuda, pages, page_size, max_pages
+        self._caches, self._ropes, self._blobs = {}, {}, blobs
+        self.nGroups = self.max_new = 0
+
+    def Cache(self, layer, heads, size, half):
+        """Keys and values of a layer, (pages, heads, page size, head size); what a step does not write is never read."""
+        if layer not in self._caches:
+            self._caches[layer] = tuple(Blob(self.cuda, (self.pages, heads, self.page_size, size), half) for _ in range(2))
+        return self._caches[layer]
+
+    def Rope(self, heads, size, theta):
+        """The handle with the angles of every position that a sequence can have: one for all layers of this head size and base."""
+        if (size, theta) not in self._ropes:
+            positions = self.max_pages * self.page_size
+            self._ropes[size, theta] = self.cuda.CreateRope(0, 0, positions * heads * size, 1, positions, heads, size, theta)
+        return self._ropes[size, theta]
+
+    def Dispose(self):
+        for blob in list(self._blobs) + [b for kv in self._caches.values() for b in kv]:
+            blob.Dispose()
+        for rope in self._ropes.values():
+            self.cuda.FreeRope(rope)
+        self._caches.clear()
+        self._ropes.clear()
+
+
+class PagedSequences(_Paged):
     """Which sequences are being served and which pages of a cache hold them (no counterpart in the reference, whose layer keeps one sequence of one
     length).  One object serves all attention layers of a model: they keep pages of the same numbers.
 
@@ -342,11 +372,11 @@ class PagedSequences:
     """
 
     def __init__(self, cuda, pages, page_size, max_pages):
-        self.cuda, self.pages, self.page_size, self.max_pages = cuda, pages, page_size, max_pages
-        self._free = list(range(pages - 1, -1, -1))
-        self._table, self._len, self._caches, self._ropes = {}, {}, {}, {}
         self.table, self.starts, self.lens = (Blob(cuda) for _ in range(3))
-        self.batch = self.tokens = self.max_new = 0
+        super().__init__(cuda, pages, page_size, max_pages, self.table, self.starts, self.lens)
+        self._free = list(range(pages - 1, -1, -1))
+        self._table, self._len = {}, {}
+        self.batch = self.tokens = 0
 
     def length(self, name):
         return self._len.get(name, 0)
@@ -382,26 +412,73 @@ class PagedSequences:
         self._free += [p for p in self._table.pop(name) if p >= 0]
         del self._len[name]
 
-    def Cache(self, layer, heads, size, half):
-        """Keys and values of a layer, (pages, heads, page size, head size); what a step does not write is never read."""
-        if layer not in self._caches:
-            self._caches[layer] = tuple(Blob(self.cuda, (self.pages, heads, self.page_size, size), half) for _ in range(2))
-        return self._caches[layer]
 
-    def Rope(self, heads, size, theta):
-        """The handle with the angles of every position that a sequence can have: one for all layers of this head size and base."""
-        if (size, theta) not in self._ropes:
-            positions = self.max_pages * self.page_size
-            self._ropes[size, theta] = self.cuda.CreateRope(0, 0, positions * heads * size, 1, positions, heads, size, theta)
-        return self._ropes[size, theta]
+class PagedBatch(_Paged):
+    """A batch of sequences whose tables, lengths and free pages live on the device (no counterpart in the reference): ``batch`` places for sequences, each
+    with its own length, and passes of up to ``tokens`` rows.  Nothing of a step has to come from the host, so that a loop of steps can be captured.
 
-    def Dispose(self):
-        for blob in [self.table, self.starts, self.lens] + [b for kv in self._caches.values() for b in kv]:
-            blob.Dispose()
-        for rope in self._ropes.values():
-            self.cuda.FreeRope(rope)
-        self._caches.clear()
-        self._ropes.clear()
+    ``Step(new)`` before a model's pass: place b gets room for ``new[b]`` tokens (below 0: its sequence ends, its pages are free); without an argument what
+    the blob ``new`` holds.  Places for which pages or rows do not reach wait: ``lens`` does not grow, ``last`` is -1.  ``starts``, ``positions`` and ``last``
+    say which rows of the pass are whose; rows behind them are computed from and to whatever their memory holds.
+    ``Begin({place: (other, positions)})`` before a Step: an empty place begins behind the first positions of another one, in its pages (whole pages of it; they
+    are the other's, which has to end last).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
+    same pages; attention then reads these once for all of them.  ``Sample(...)`` draws a token for every place that got rows.
+    """
+
+    def __init__(self, cuda, batch, tokens, pages, page_size, max_pages):
+        shapes = dict(new=(batch,), lens=(batch,), table=(batch, max_pages), free=(pages + 1,), starts=(batch + 1,), positions=(tokens,), last=(batch,),
+                      origin=(batch,), shared=(batch,), ids=(batch,), logprobs=(batch,))
+        for name, shape in shapes.items():
+            setattr(self, name, Blob(cuda, shape))
+        self.bounds, self.common = Blob(cuda), Blob(cuda)
+        super().__init__(cuda, pages, page_size, max_pages, *(getattr(self, name) for name in shapes), self.bounds, self.common)
+        self.batch, self.tokens = batch, tokens
+        for blob in (self.new, self.lens, self.shared):
+            blob.mutable_cpu_data = np.zeros(batch, cuda.DTYPE)
+        self.table.mutable_cpu_data = np.full((batch, max_pages), -1, cuda.DTYPE)
+        self.origin.mutable_cpu_data = np.full(batch, -1, cuda.DTYPE)
+        self.free.mutable_cpu_data = np.concatenate([[pages], np.arange(pages - 1, -1, -1)]).astype(cuda.DTYPE)
+
+    def Step(self, new=None):
+        if new is not None:
+            new = np.asarray(new, self.cuda.DTYPE)
+            if new.shape != (self.batch,):
+                raise ValueError("a step has a number for each of its %d places" % self.batch)
+            self.new.mutable_cpu_data = new
+        at = lambda *blobs: [b.gpu_data for b in blobs]  # noqa: E731
+        state = at(self.lens, self.table, self.free)
+        self.cuda.PagedPlan(self.batch, self.tokens, self.pages, self.page_size, self.max_pages, self.new.gpu_data, *state, *state,
+                            *at(self.starts, self.positions), 0, *at(self.last, self.origin, self.shared, self.shared))
+
+    def Begin(self, places):
+        """What ``shared`` says of places that hold a sequence stays: the pages that are not theirs."""
+        if any(not 0 <= b < self.batch or not 0 <= other < self.batch or b == other for b, (other, _) in places.items()):
+            raise ValueError("a place begins behind another one of the %d" % self.batch)
+        origin, shared, lens = (blob.mutable_cpu_data for blob in (self.origin, self.shared, self.lens))
+        if any(lens[b] for b in places):
+            raise ValueError("only an empty place begins")
+        for b, (other, positions) in places.items():
+            origin[b], shared[b] = other, positions
+        self.origin.mutable_cpu_data, self.shared.mutable_cpu_data = origin, shared
+
+    def Share(self, bounds=(), positions=()):
+        bounds, positions = (np.asarray(v, self.cuda.DTYPE) for v in (bounds, positions))
+        if len(positions) and (len(bounds) != len(positions) + 1 or (np.diff(bounds) < 0).any() or bounds[0] < 0 or bounds[-1] > self.batch):
+            raise ValueError("groups are runs of the %d places, one bound more than groups" % self.batch)
+        self.nGroups = len(positions)
+        if self.nGroups:
+            for blob, values in ((self.bounds, bounds), (self.common, positions)):
+                blob.Reshape(*values.shape)
+                blob.mutable_cpu_data = values
+
+    def Sample(self, logits, random, temperature=None, top_k=None, top_p=None, min_p=None):
+        """The next token of every place from logits (1, tokens, vocab) into ``ids`` (-1: a place without rows) with a random number, 0 .. 1, for each place; the
+        settings are blobs with a number for each place too.  ``logprobs``: logarithm of the share that the token had."""
+        if logits.count(0, 2) != self.tokens or random.count() != self.batch or any(b is not None and b.count() != self.batch for b in (temperature, top_k, top_p, min_p)):
+            raise ValueError("logits of %d rows, numbers for %d places" % (self.tokens, self.batch))
+        vocab = logits.count(2)
+        self.cuda.SampleForward(self.batch, vocab, logits.gpu_data, random.gpu_data, self.ids.gpu_data, *(b.gpu_data if b is not None else 0 for b in (temperature, top_k, top_p, min_p)),
+                                hLogProb=self.logprobs.gpu_data, hRows=self.last.gpu_data, nLogitsRows=self.tokens)
 
 
 class CausalSelfAttentionLayer:
@@ -556,7 +633,8 @@ class CausalSelfAttentionLayer:
         self.c_attn.Backward(ip, blobX)
 
     def ForwardPaged(self, blobX, sequences, top):
-        """Inference of the new tokens of many sequences, (1, tokens, C) in the order of ``sequences.Step``, over their pages: projection, one call that
+        """Inference of the new tokens of many sequences, (1, tokens, C) in the order of ``sequences.Step`` (PagedSequences or
+        PagedBatch), over their pages: projection, one call that
         normalises, rotates and stores, attention, output projection."""
         cuda, b, H, hs, seqs = self.cuda, self.b, self.nHeads, self.nSize, sequences
         N, C = blobX.count(0, 2), self.nEmbed
@@ -572,7 +650,11 @@ class CausalSelfAttentionLayer:
         strides = (H * seqs.page_size * hs, seqs.page_size * hs, hs)
         cuda.PagedAppend(*sizes, b["IpAttn"].gpu_data, b["Qt"].gpu_data, *where, *strides, rope, self.qk_norm,
                          *([n.gpu_data for n in self.norms] or (0, 0)), self.norm_eps)
-        cuda.AttnPagedForward(*sizes, b["Qt"].gpu_data, *where, b["Y"].gpu_data, *strides, nMaxNew=seqs.max_new)
+        if seqs.nGroups:
+            cuda.AttnPagedPrefixForward(*sizes, b["Qt"].gpu_data, *where, b["Y"].gpu_data, *strides, seqs.nGroups, seqs.bounds.gpu_data, seqs.common.gpu_data,
+                                        nMaxNew=seqs.max_new)
+        else:
+            cuda.AttnPagedForward(*sizes, b["Qt"].gpu_data, *where, b["Y"].gpu_data, *strides, nMaxNew=seqs.max_new)
         self.c_proj.Forward(b["Y"], top)
 
 
