@@ -314,7 +314,7 @@ struct SampleCuts {
     unsigned long long *sums, *list, *weights;
     void* state;
     unsigned* counts;
-    int* tickets;
+    int* listed;
     float* tops;
     int slices;
 };

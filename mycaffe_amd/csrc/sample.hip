@@ -17,6 +17,7 @@ namespace mch {
 namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64, BINS = 2048, FEW = 256;
+static_assert(FEW <= THREADS / 4 && 2 * FEW <= BINS, "Rank, draw_of_few()");
 typedef unsigned long long u64;
 constexpr u64 RAW = 0x4330000000000000ull;   // the upper bits of a whole number in a double
 
@@ -318,7 +319,7 @@ struct Rank {
     int id;
     __device__ __forceinline__ Rank(const Shared& s, int n)
     {
-        shift = n <= THREADS / 16 ? 4 : n <= THREADS / 4 ? 2 : 1;
+        shift = n <= THREADS / 16 ? 4 : n <= THREADS / 8 ? 3 : 2;
         i = (int)threadIdx.x >> shift;
         part = (int)threadIdx.x & ((1 << shift) - 1);
         mine = i < n;
@@ -515,30 +516,35 @@ __device__ __forceinline__ Border<typename R::V> select(const R& r, Shared& s, u
     return Border<V>{(V)s.value, s.index};
 }
 
-// The draw from the listed tokens alone.  k: of them the first (0: all), targetOf(sum): the sum of weights at which top-p's run ends (0: all), least: weights from here on
+// The draw from the listed tokens alone.  k: of them the first (0: all), targetOf(sum): the sum of weights at which top-p's run ends (0: all), least: weights from here on.
+// Each is compared with each once, which says its place in both orders, by logit and by index; the rest are sums along these.
 template <typename R, typename G> __device__ __forceinline__ int draw_of_few(const R& r, Shared& s, int n, u64 k, G targetOf, double least, u64 share, u64* total)
 {
-    const int lane = threadIdx.x & 63;
+    const int tid = threadIdx.x;
     const Rank me(s, n);
-    const u64 rank = me.sum(n, [&](int j) __attribute__((always_inline)) -> u64 { return me.before(s, j); });
-    const u64 better = me.sum(n, [&](int j) __attribute__((always_inline)) -> u64 { return me.before(s, j) ? s.weights[j] : 0; });
-    auto all = [&]() __attribute__((always_inline)) -> u64 {   // every wavefront for itself
-        u64 x = 0;
-        for (int j = lane; j < n; j += 64) x += s.kept[j];
-        return wave_sum(x);
-    };
-    bool keep = me.mine && (k == 0 || rank < k);
-    if (me.lead) s.kept[me.i] = keep ? me.w : 0;
-    if (threadIdx.x == 0) s.found = -1;
+    uint32_t at = 0;   // tokens before it, and 2^16 those of smaller indexes
+    if (me.mine) {
+#pragma unroll 4
+        for (int j = me.part; j < n; j += 1 << me.shift) at += (me.before(s, j) ? 1u : 0u) + (s.ids[j] < me.id ? 0x10000u : 0u);
+    }
+    for (int o = 1; o < 1 << me.shift; o <<= 1) at += __shfl_xor(at, o);
+    const int rank = at & 0xffff, place = at >> 16;
+    uint32_t *tag = s.count, *ids = s.count + FEW;   // by rank: place and min-p's word; by place: index
+    if (me.lead) {
+        s.kept[rank] = me.w;
+        tag[rank] = (uint32_t)place << 1 | (least == 0.0 || r.two_to(r.power((typename R::V)me.v), 0) >= least);
+        ids[place] = me.id;
+    }
     __syncthreads();
-    const u64 target = targetOf(all());
-    keep = keep && (rank == 0 || ((target == 0 || better < target) && (least == 0.0 || r.two_to(r.power((typename R::V)me.v), 0) >= least)));
+    const bool first = tid < n && (k == 0 || (u64)tid < k);
+    const u64 w = first ? s.kept[tid] : 0;
+    u64 all;
+    const u64 better = block_scan(w, s.sums, &all), target = targetOf(all);
+    if (tid < n) s.weight[tag[tid] >> 1] = first && (tid == 0 || ((target == 0 || better < target) && tag[tid] & 1)) ? w : 0;
+    if (tid == 0) s.found = -1;
     __syncthreads();
-    if (me.lead) s.kept[me.i] = keep ? me.w : 0;
-    __syncthreads();
-    *total = all();
-    const u64 want = __umul64hi(*total, share), before = me.sum(n, [&](int j) __attribute__((always_inline)) -> u64 { return s.ids[j] < me.id ? s.kept[j] : 0; });
-    if (me.lead && keep && before <= want && want < before + me.w) s.found = me.id;
+    const u64 mine = tid < n ? s.weight[tid] : 0, before = block_scan(mine, s.sums, total), want = __umul64hi(*total, share);
+    if (before <= want && want < before + mine) s.found = ids[tid];
     __syncthreads();
     return s.found;
 }
@@ -673,30 +679,18 @@ template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sam
 //   weigh   the weights: added up, or counted and added up in bins;
 //   border  a workgroup a row: the draw, where neither top-k nor top-p is asked for, else the bin that has the border;
 //   list    what lies above the border's bin and in it, if LISTED tokens at most, else what lies in the bin;
-//   finish  a workgroup a row: with what is listed alone, to the draw, or to the border; rows of which too much would be listed as above, from their beginning;
-//   draw    rows with a border: all weights behind it are added up, and the last workgroup draws.
-// (The last launch alone, of few rows, has the last workgroup of a row, by a ticket, read what the others have written past the caches, at the level that all XCDs share: a
-// wait for that at the end of every slice costs more than a launch.  256 rows of 131072, weigh with it 48 us.)  Sums are whole numbers: any order gives the same.
+//   finish  a workgroup a row: the draw, with what is listed alone, or with that and the bins above it, slice by slice, and the logits of one slice; rows of which
+//           too much would be listed as above, from their beginning.
+// (No launch waits for its last workgroup: reading what the others have written past the caches, at the level that all XCDs share, at the end of every slice costs
+// more than a launch.  256 rows of 131072, weigh with it 48 us.)  Sums are whole numbers: any order gives the same.
 constexpr int CUT = 256, CUT_BINS = CUT, LISTED = 4096;
-enum RowMode { ROW_DONE, ROW_LIST_ALL, ROW_LIST_BIN, ROW_DRAW, ROW_WHOLE };
+enum RowMode { ROW_DONE, ROW_LIST_ALL, ROW_LIST_BIN, ROW_WHOLE };
 struct RowState {
-    int mode, last;       // border: logits above `at`, equal ones up to index `last`
+    int mode, last;       // min-p's border: logits above `at`, equal ones up to index `last`
     float top, lo, hi, at;
-    u64 above, target;    // of the border's bin: what is above it, and where the border is
+    u64 above, target;    // of what is listed of a bin: what is above it, and where top-k's or top-p's border is (0: not in it)
+    int bins, none;       // whole bins that are kept
 };
-
-__device__ __forceinline__ void put(u64* p, u64 v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void put(uint32_t* p, uint32_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <typename T> __device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-// whether this is the last of n workgroups to come here; what it wrote before is there then
-__device__ __forceinline__ bool last_of(int* ticket, int n, int* shared)
-{
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0) *shared = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    return *shared == n - 1;
-}
 
 // a slice: EACH logits a thread of T, in pieces, in the order of the vocabulary from piece to piece and within one from thread to thread
 template <typename L, int EACH, int T> struct Slice {
@@ -720,8 +714,8 @@ template <typename L, int EACH, int T> struct Slice {
     }
 };
 
-template <int T> struct DrawShared { u64 sums[T / 64], tot[16 * T / 64]; u64 before; int slice, ticket; };
-// The last workgroup of a row: from the sums of n slices, which it is that the draw falls into, and where in it
+template <int T> struct DrawShared { u64 sums[T / 64], tot[16 * T / 64]; u64 before; int slice; };
+// Of a row, from the sums of n slices, which it is that the draw falls into, and where in it
 template <typename L, typename N, int EACH, int T>
 __device__ __forceinline__ void draw_from(const SampleArgs& a, int row, const Row<L>& r, const Settings& t, const Border<float>& border, const u64* slices, int n, DrawShared<T>& s)
 {
@@ -729,12 +723,12 @@ __device__ __forceinline__ void draw_from(const SampleArgs& a, int row, const Ro
     constexpr int W = T / 64;
     const int tid = threadIdx.x, wave = tid >> 6, per = (n + T - 1) / T;
     u64 mine = 0, total;
-    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) mine += get(slices + i);
+    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) mine += slices[i];
     u64 before = block_scan<W>(mine, s.sums, &total);
     const u64 want = __umul64hi(total, t.share);
     if (before <= want && want < before + mine)
         for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
-            const u64 x = get(slices + i);
+            const u64 x = slices[i];
             if (want < before + x) { s.slice = i; s.before = before; break; }
             before += x;
         }
@@ -793,7 +787,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_to
         for (int i = 1; i < CUT / 64; i++) top = fmaxf(top, sTop[i]);
         w.tops[row * w.slices + slice] = top;
     }
-    if (slice == 0 && tid < 4) w.tickets[4 * row + tid] = 0;
+    if (slice == 0 && tid == 0) w.listed[row] = 0;
 }
 
 // smallest logit that the weights' share `least` keeps
@@ -828,11 +822,15 @@ __device__ __forceinline__ float top_of_row(const SampleCuts& w, int row, int* f
     *first = at;
     return top;
 }
-// bins a unit of the logits, twice: top-k's over all octaves of weights, top-p's over 24 (what lies below weighs too little to be reached, but for flat rows)
+// bins a unit of the logits, twice: top-k's over all octaves of weights, and a little more than these, so that no rounding leaves out a token with weight; top-p's over 24
+// (what lies below weighs too little to be reached, but for flat rows)
 template <typename R> __device__ __forceinline__ float bins_of(const R& r, const Settings& t)
 {
-    return (float)fmin(2.0 * r.rate * CUT_BINS / (t.byK ? -r.least : 32.0 * 24), 1e37);
+    return (float)fmin(2.0 * (1.0 - 0x1p-16) * r.rate * CUT_BINS / (t.byK ? -r.least : 32.0 * 24), 1e37);
 }
+
+// whether the bins' weights are added up: not where top-k leaves so few tokens that, with the others of the border's bin, they are all listed, but for flat rows
+__device__ __forceinline__ bool weighs(const Settings& t) { return !t.byK || t.k > LISTED / 4; }
 
 template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_weigh_kernel(SampleArgs a, SampleCuts w)
 {
@@ -864,7 +862,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_we
         if (tid == 0) w.sums[row * w.slices + slice] = all;
         return;
     }
-    const bool byWeight = !t.byK;
+    const bool byWeight = weighs(t);
     const float half = r.top * 0.5f, scale = bins_of(r, t);
     c.each(r, slice, [&](int, int, const float (&v)[R::VEC]) __attribute__((always_inline)) {
 #pragma unroll
@@ -899,26 +897,27 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_bo
     typedef Row<L> R;
     typedef Slice<L, EACH, CUT> C;
     __shared__ DrawShared<CUT> s;
-    __shared__ int sFirst, sBin, sReached, sIn;
+    __shared__ int sFirst, sBin, sReached, sIn[CUT_BINS];
     __shared__ double sRoots[32];
     const int tid = threadIdx.x, row = blockIdx.x;
     R r;
     row_of<L, float>(a, row, r, sRoots);
     const Settings t = settings_of<float>(a, row);
-    const bool byWeight = !t.byK, bins = t.byK || t.byP;
+    const bool bins = t.byK || t.byP;
     // this thread's bin of the row
     uint32_t n = 0;
     u64 x = 0, sum = 0, all = 0;
     if (bins) {
 #pragma unroll 8
         for (int i = 0; i < w.slices; i++) n += w.counts[((size_t)row * w.slices + i) * CUT_BINS + tid];
-        if (byWeight) {
+        if (!t.byK) {
 #pragma unroll 8
             for (int i = 0; i < w.slices; i++) x += w.weights[((size_t)row * w.slices + i) * CUT_BINS + tid];
             for (int i = tid; i < w.slices; i += CUT) sum += w.sums[row * w.slices + i];
         }
     }
     if (tid < 32) sRoots[tid] = ROOTS[tid];
+    sIn[tid] = n;
     if (tid == 0) { sFirst = INT32_MAX; sBin = -1; }
     int first;
     const float top = top_of_row(w, row, &first);
@@ -947,26 +946,40 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_bo
     } else if (!bins) {
         draw_from<L, float, EACH, CUT>(a, row, r, t, border_of_least(r, t.least), w.sums + row * w.slices, w.slices, s);
     } else {
-        if (byWeight) block_scan<CUT / 64>(sum, s.sums, &all);
-        u64 any;
-        const u64 tokens = block_scan<CUT / 64>(n, s.sums, &any), before = byWeight ? block_scan<CUT / 64>(x, s.sums, &any) : tokens;
-        const u64 target = byWeight ? t.run_of(all) : t.k, amount = byWeight ? x : n;
-        if (before < target && target <= before + amount) { sBin = tid; s.before = before; sReached = (int)tokens + n; sIn = n; }
+        u64 any, weight;
+        if (!t.byK) block_scan<CUT / 64>(sum, s.sums, &all);
+        const u64 tokens = block_scan<CUT / 64>(n, s.sums, &any), before = t.byK ? tokens : block_scan<CUT / 64>(x, s.sums, &weight);
+        const u64 target = t.byK ? t.k : t.run_of(all), amount = t.byK ? n : x;
+        if (before < target && target <= before + amount) { sBin = tid; s.before = before; sReached = (int)tokens + n; }
         __syncthreads();
-        const int bin = sBin;
-        if (bin < 0) {
-            // top-k: as many as there are with weight; top-p: it goes further down than the bins
-            st.mode = t.byP ? ROW_WHOLE : ROW_DRAW;
-            const Border<float> border = border_of_least(r, t.least);
-            st.at = border.at;
-            st.last = border.last;
-        } else {
-            const float half = r.top * 0.5f, scale = bins_of(r, t);
-            st.lo = r.smallest([&](float v) __attribute__((always_inline)) { return r.bins(v, half, scale) < (float)(bin + 1); });
-            st.hi = bin ? of_key(key_of(r.smallest([&](float v) __attribute__((always_inline)) { return r.bins(v, half, scale) < (float)bin; })) - 1) : r.top;
-            st.above = s.before;
+        const float half = r.top * 0.5f, scale = bins_of(r, t);
+        const Border<float> least = border_of_least(r, t.least);
+        const float z = r.bins(least.at, half, scale);
+        const int leastBin = z < (float)CUT_BINS ? (int)z : CUT_BINS;
+        st.at = least.at;
+        st.last = least.last;
+        // (top-k: no bin where there are not as many with weight, all of which stay then; top-p: none where it goes further down than the bins, unless min-p does not)
+        int bin = sBin >= 0 ? sBin : t.byK ? CUT_BINS : leastBin < CUT_BINS ? leastBin : -1;
+        const u64 reached = sBin >= 0 ? sReached : any;
+        if (bin < 0) st.mode = ROW_WHOLE;
+        else if (reached <= LISTED) {
+            st.mode = ROW_LIST_ALL;
             st.target = target;
-            st.mode = sReached <= LISTED ? ROW_LIST_ALL : sIn <= LISTED && !(t.byK && t.byP) ? ROW_LIST_BIN : ROW_WHOLE;
+        } else if (t.byK && (t.byP || !weighs(t))) st.mode = ROW_WHOLE;
+        else {
+            st.above = s.before;
+            st.target = sBin >= 0 && bin <= leastBin ? target : 0;
+            bin = min(bin, leastBin);
+            st.mode = bin < CUT_BINS && sIn[bin] > LISTED ? ROW_WHOLE : ROW_LIST_BIN;
+        }
+        st.bins = bin;
+        auto from = [&](int b) __attribute__((always_inline)) { return r.smallest([&](float v) __attribute__((always_inline)) { return r.bins(v, half, scale) < (float)b; }); };
+        if (bin < CUT_BINS) {
+            st.lo = from(bin + 1);
+            st.hi = bin > 0 ? of_key(key_of(from(bin)) - 1) : r.top;
+        } else {   // no bin more
+            st.lo = st.mode == ROW_LIST_ALL ? from(CUT_BINS) : INFINITY;
+            st.hi = -INFINITY;
         }
     }
     if (tid == 0) ((RowState*)w.state)[row] = st;
@@ -1016,7 +1029,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_li
     });
     int to = (int)block_scan<CUT / 64>(__popcll(hits), sSums, &all);
     if (!all) return;
-    if (tid == 0) sBase = __hip_atomic_fetch_add(w.tickets + 4 * row + 3, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) sBase = __hip_atomic_fetch_add(w.listed + row, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     to += sBase;
     if (hits)
@@ -1031,9 +1044,9 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_li
 }
 
 constexpr int OWN = LISTED / THREADS;
-struct ReachShared { uint32_t count[THREADS]; u64 amount[THREADS], sums[WAVES], above, key; int bin; };
+struct ReachShared { uint32_t count[THREADS]; u64 amount[THREADS], sums[WAVES], above, key, keys[64], amounts[64]; int bin, few; };
 // Of numbers key[j], which are all different, with amounts: the one at which the sum of the amounts, from the largest number down, reaches the target; 0 if it does not.
-// In ever smaller ranges, a bin a thread.
+// In ever smaller ranges, a bin a thread, until those of one wavefront are left, who look at each other.
 template <typename F> __device__ __forceinline__ u64 reach(ReachShared& s, const u64 (&key)[OWN], F amount, u64 lo, u64 hi, u64 target)
 {
     const int tid = threadIdx.x;
@@ -1044,7 +1057,7 @@ template <typename F> __device__ __forceinline__ u64 reach(ReachShared& s, const
         __syncthreads();
         s.count[tid] = 0;
         s.amount[tid] = 0;
-        if (tid == 0) s.bin = -1;
+        if (tid == 0) { s.bin = -1; s.few = 0; }
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < OWN; j++) {
@@ -1065,18 +1078,31 @@ template <typename F> __device__ __forceinline__ u64 reach(ReachShared& s, const
         hi -= (u64)bin << shift;
         const u64 span = (1ull << shift) - 1;
         lo = hi - lo > span ? hi - span : lo;
-        if (s.count[bin] == 1) break;
+        if (s.count[bin] <= 64) break;
     }
 #pragma unroll
-    for (int j = 0; j < OWN; j++)
-        if (key[j] >= lo && key[j] <= hi && amount(j)) s.key = key[j];
+    for (int j = 0; j < OWN; j++) {
+        const u64 w = amount(j);
+        if (key[j] < lo || key[j] > hi || !w) continue;
+        const int i = atomicAdd(&s.few, 1);
+        s.keys[i] = key[j];
+        s.amounts[i] = w;
+    }
+    __syncthreads();
+    const int few = s.few;
+    if (tid < few) {   // (of the first wavefront)
+        const u64 mine = s.keys[tid];
+        u64 at = above;
+        for (int i = 0; i < few; i++) at += s.keys[i] > mine ? s.amounts[i] : 0;
+        if (at < target && target <= at + s.amounts[tid]) s.key = mine;
+    }
     __syncthreads();
     const u64 k = s.key;
     __syncthreads();
     return k;
 }
 
-template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleArgs a, SampleCuts w)
+template <typename L, int EACH> __global__ __launch_bounds__(THREADS) void sample_finish_kernel(SampleArgs a, SampleCuts w)
 {
     static_assert(THREADS == 1024, "bins of reach()");
     typedef Row<L> R;
@@ -1084,7 +1110,7 @@ template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_k
     __shared__ double sRoots[32];
     extern __shared__ u64 parts[];
     const int tid = threadIdx.x, row = blockIdx.x;
-    RowState st = ((const RowState*)w.state)[row];
+    const RowState st = ((const RowState*)w.state)[row];
     if (st.mode == ROW_WHOLE) {
         sample_row<L, float>(a, row, s.row, parts);
         return;
@@ -1095,7 +1121,7 @@ template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_k
     top_is(r, st.top);
     const Settings t = settings_of<float>(a, row);
     r.rate = t.rate;
-    const int n = min(w.tickets[4 * row + 3], LISTED);
+    const int n = min(w.listed[row], LISTED);
     const u64* list = w.list + (size_t)row * LISTED;
     if (tid < 32) sRoots[tid] = ROOTS[tid];
     u64 key[OWN], weight[OWN], least = 0, all, total;
@@ -1121,13 +1147,48 @@ template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_k
     }
     const u64 from = place_of<L>(st.lo, LAST_INDEX), to = place_of<L>(st.mode == ROW_LIST_ALL ? r.top : st.hi, 0);
     if (st.mode == ROW_LIST_BIN) {
-        const u64 target = st.target - st.above, border = t.byK ? reach(s.reach, key, one, from, to, target) : reach(s.reach, key, kept, from, to, target);
-        const Border<float> b = border_of_least(r, t.least);
-        st.at = logit_at<L>(border);
-        st.last = index_at(border);
-        if (b.at > st.at) { st.at = b.at; st.last = b.last; }
-        st.mode = ROW_DRAW;
-        if (tid == 0) ((RowState*)w.state)[row] = st;
+        Border<float> border = {st.at, st.last};
+        if (st.target) {
+            const u64 target = st.target - st.above, at = t.byK ? reach(s.reach, key, one, from, to, target) : reach(s.reach, key, kept, from, to, target);
+            const Border<float> b = {logit_at<L>(at), index_at(at)};
+            if (!(border.at > b.at)) border = b;
+        }
+        // what is left of every slice: whole bins, and of the bin that is listed what the border leaves
+        constexpr int LOGITS = EACH * CUT, PER = LOGITS / THREADS;
+        u64* slices = s.reach.amount;
+        for (int i = tid >> 6; i < w.slices; i += WAVES) {
+            const u64* bins = w.weights + ((size_t)row * w.slices + i) * CUT_BINS;
+            u64 x = 0;
+#pragma unroll
+            for (int b = tid & 63; b < CUT_BINS; b += 64) x += b < st.bins ? bins[b] : 0;
+            x = wave_sum(x);
+            if ((tid & 63) == 0) slices[i] = x;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < OWN; j++)
+            if (key[j] && border.has(logit_at<L>(key[j]), index_at(key[j]))) atomicAdd(slices + index_at(key[j]) / LOGITS, weight[j]);
+        __syncthreads();
+        u64 mine = tid < w.slices ? slices[tid] : 0, at = block_scan(mine, s.reach.sums, &total);
+        const u64 want = __umul64hi(total, t.share);
+        if (at <= want && want < at + mine) { s.reach.bin = tid; s.reach.above = at; }
+        __syncthreads();
+        const int i0 = s.reach.bin * LOGITS + tid * PER;
+        const u64 before = s.reach.above;
+        u64 x[PER];
+        mine = 0;
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            float v = i0 + e < a.vocab ? read(r.x[i0 + e]) : -INFINITY;
+            if (r.infinite) v = v == INFINITY ? 0.f : -INFINITY;
+            mine += x[e] = border.has(v, i0 + e) ? r.weight(v) : 0;
+        }
+        at = before + block_scan(mine, s.reach.sums, &all);
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            if (at <= want && want < at + x[e]) write_draw<L, float>(a, row, r, t, i0 + e, total);
+            at += x[e];
+        }
         return;
     }
     auto sum = [&]() __attribute__((always_inline)) -> u64 {
@@ -1139,7 +1200,7 @@ template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_k
     };
     if (t.byK) least = max(least, reach(s.reach, key, one, from, to, t.k));
     if (t.byP) least = max(least, reach(s.reach, key, kept, from, to, t.byK ? t.run_of(sum()) : st.target));
-    if (t.least > 0.0) least = max(least, least_place<L>(border_of_least(r, t.least).at));
+    if (t.least > 0.0) least = max(least, least_place<L>(st.at));
     total = sum();
     // in the order of the vocabulary: the sum up to the token drawn exceeds u times all
     u64 order[OWN];
@@ -1147,32 +1208,6 @@ template <typename L> __global__ __launch_bounds__(THREADS) void sample_finish_k
     for (int j = 0; j < OWN; j++) order[j] = key[j] & LAST_INDEX;
     const u64 drawn = reach(s.reach, order, kept, LAST_INDEX + 1 - a.vocab, LAST_INDEX, __umul64hi(total, t.share) + 1);
     if (tid == 0) write_draw<L, float>(a, row, r, t, index_at(drawn), total);
-}
-
-template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_draw_kernel(SampleArgs a, SampleCuts w)
-{
-    typedef Slice<L, EACH, CUT> C;
-    typedef Row<L> R;
-    __shared__ DrawShared<CUT> s;
-    __shared__ double sRoots[32];
-    const int row = blockIdx.y, slice = blockIdx.x;
-    const RowState st = ((const RowState*)w.state)[row];
-    if (st.mode != ROW_DRAW) return;
-    R r;
-    row_of<L, float>(a, row, r, sRoots);
-    C c;
-    c.load(r, slice);
-    const Settings t = settings_of<float>(a, row);
-    top_is(r, st.top);
-    r.rate = t.rate;
-    if (threadIdx.x < 32) sRoots[threadIdx.x] = ROOTS[threadIdx.x];
-    __syncthreads();
-    const Border<float> border = {st.at, st.last};
-    u64 sum = 0, all;
-    c.each(r, slice, [&](int, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) { sum += kept_weights(r, v, i0, border); });
-    block_scan<CUT / 64>(sum, s.sums, &all);
-    if (threadIdx.x == 0) put(w.sums + row * w.slices + slice, all);
-    if (last_of(w.tickets + 4 * row + 2, w.slices, &s.ticket)) draw_from<L, float, EACH, CUT>(a, row, r, t, border, w.sums + row * w.slices, w.slices, s);
 }
 
 }  // namespace
@@ -1199,7 +1234,7 @@ size_t sample_workspace_bytes(SampleType type, const SampleArgs& a)
     if (type == SAMPLE_F64 || a.count > CUT_ROWS || a.vocab <= CUT_VOCAB || (long long)a.count * a.vocab < CUT_LOGITS) return 0;
     const int each = cut_each(a);
     const size_t slices = (a.vocab + each * CUT - 1) / (each * CUT), rows = a.count;
-    return rows * (slices * (8 + 4) + sizeof(RowState) + 16 + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
+    return rows * (slices * (8 + 4) + sizeof(RowState) + 8 + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
 }
 
 hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspace)
@@ -1222,8 +1257,8 @@ hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspac
             w.counts = (uint32_t*)(w.weights + rows * w.slices * CUT_BINS);
             at = (char*)(w.counts + rows * w.slices * CUT_BINS);
         }
-        w.tickets = (int*)at;
-        w.tops = (float*)(w.tickets + 4 * rows);
+        w.listed = (int*)at;
+        w.tops = (float*)(w.listed + rows);
         const dim3 grid(w.slices, a.count);
         auto go = [&](auto type, auto size) {
             typedef decltype(type) L;
@@ -1233,8 +1268,7 @@ hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspac
             hipLaunchKernelGGL((sample_border_kernel<L, EACH>), a.count, CUT, 0, s, a, w);
             if (cut_bins(a)) {
                 hipLaunchKernelGGL((sample_list_kernel<L, EACH>), grid, CUT, 0, s, a, w);
-                hipLaunchKernelGGL((sample_finish_kernel<L>), a.count, THREADS, parts, s, a, w);
-                hipLaunchKernelGGL((sample_draw_kernel<L, EACH>), grid, CUT, 0, s, a, w);
+                hipLaunchKernelGGL((sample_finish_kernel<L, EACH>), a.count, THREADS, parts, s, a, w);
             }
         };
         auto sized = [&](auto type) {
