@@ -64,7 +64,9 @@ struct PrefixUnits {
     SplitArgs split;
     ChunkArgs chunk;
     int unit, kvH, G;
+    int splitGrid;                // workgroups of split_run in a launch of its own; 0: those that chunk_run leaves
     float splitCost, chunkCost;   // of a unit
+    __device__ int split_blocks(int chunks) const { return splitGrid ? splitGrid : PREFIX_GRID - chunks; }
     __device__ bool is_chunk(const PrefixSpan& s) const { return split.few && (long long)s.count * G > split.few; }
     __device__ int units(const PrefixSpan& s) const { const int n = s.len - s.from; return n <= max(split.one, unit) ? 1 : (n + unit - 1) / unit; }
     __device__ int split_work(const PrefixSpan& s) const { return is_chunk(s) ? 0 : (s.count + split.perTile - 1) / split.perTile * split.headTiles * kvH * units(s); }
@@ -174,7 +176,7 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
     const float cost[2] = {total[0] * u.splitCost, total[1] * u.chunkCost};
     // (more than half of them only for runs of 512 positions: every run leaves 128 rows of sums behind)
     const int most = max(PREFIX_GRID / 2, min(PREFIX_GRID - (total[0] ? 8 : 0), total[1] / 16));
-    const int chunks = total[1] ? max(8, min((int)(PREFIX_GRID * cost[1] / (cost[0] + cost[1])), most) & ~7) : 0;
+    const int chunks = !total[1] ? 0 : u.splitGrid ? PREFIX_GRID : max(8, min((int)(PREFIX_GRID * cost[1] / (cost[0] + cost[1])), most) & ~7);
     if (tid == 0) {
         w.totals[0] = countable ? total[0] : 0;
         w.totals[1] = countable ? total[1] : 0;
@@ -185,7 +187,7 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
     // ---- where every run begins ----
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const PagedRuns runs(total[i], i ? chunks : PREFIX_GRID - chunks, i ? CHUNK_LEAST : 1);
+        const PagedRuns runs(total[i], i ? chunks : u.split_blocks(chunks), i ? CHUNK_LEAST : 1);
         for (int k = tid; k < runs.W; k += THREADS) {
             const int unit = runs.begin(k);
             int lo = 0, hi = w.n;
@@ -207,10 +209,16 @@ template <typename TQ, typename TC, int HSP> __global__ __launch_bounds__(256, 2
     if (block < chunks) chunk_run<TQ, TC, HSP>(a, chunk, block, chunks, shared.chunk, list);
     else split_run<TQ, TC, HSP>(a, split, block - chunks, PREFIX_GRID - chunks, shared.split, list);
 }
-template <typename TQ, typename TC, int HSP> __global__ __launch_bounds__(256, HSP <= 128 ? 2 : 1) void attn_prefix_split_kernel(PagedAttnArgs a, SplitArgs split, OfPrefixes list)
+template <typename TQ, typename TC, int HSP> __global__ __launch_bounds__(256, HSP <= 64 ? 4 : HSP <= 128 ? 2 : 1) void attn_prefix_split_kernel(PagedAttnArgs a, SplitArgs split, OfPrefixes list)
 {
     __shared__ SplitShared<TQ, TC, HSP, OfPrefixes> shared;
-    split_run<TQ, TC, HSP>(a, split, blockIdx.x, PREFIX_GRID, shared, list);
+    split_run<TQ, TC, HSP>(a, split, blockIdx.x, gridDim.x, shared, list);
+}
+template <typename TQ, typename TC, int HSP> __global__ __launch_bounds__(256, 2) void attn_prefix_chunk_kernel(PagedAttnArgs a, ChunkArgs chunk, OfPrefixes list)
+{
+    __shared__ ChunkShared<TQ, TC, HSP> shared;
+    const int chunks = list.chunk_blocks(), block = blockIdx.x;
+    if (block < chunks) chunk_run<TQ, TC, HSP>(a, chunk, block, chunks, shared, list);
 }
 
 // The sums of both sides, and of the pieces of each, put together: a wavefront a head of a token, LANES lanes of it four values each, and as many pieces at a time as
@@ -248,7 +256,7 @@ template <typename TQ, int HSP> __global__ __launch_bounds__(256) void attn_pref
                 values[i] = 256 - 2 * row + row * HSP;
             } else {
                 const int ht = j / u.split.tileHeads, units = u.units(s), tile = t / u.split.perTile, first = at.x + ((tile * u.split.headTiles + ht) * u.kvH + kh) * units;
-                const PagedRuns runs(total0, PREFIX_GRID - chunks, 1);
+                const PagedRuns runs(total0, u.split_blocks(chunks), 1);
                 from = runs.of(first);
                 to = runs.of(first + units - 1);
                 row = (t - tile * u.split.perTile) * u.split.tileHeads + j - ht * u.split.tileHeads;
@@ -327,6 +335,10 @@ PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups)
 {
     PrefixPlan p = {};
     const int G = c.H / c.kvH, n = groups + c.batch;
+    // Single tokens of heads that share no key heads leave little for the matrix cores, and at head sizes up to 64 four workgroups of split_run fit a CU where two of both kinds
+    // do: a launch for each.  12 heads of 64, 16 bits, 192 tokens behind 2048 and up to 700 positions 90 us for 97, up to 2000 169 for 209, 96 behind 512 and 700 60 for 82 (the
+    // other way 44 for 40 with nothing behind the prefix); 24 heads on 3 the other way, 42 for 34, 12 heads and 8 tokens each 57 for 51.
+    if (padded(c) == 64 && (long long)c.tokens * G <= (long long)c.batch * 5 / 4) p.u.splitGrid = 2 * PREFIX_GRID;
     p.chunks = c.hs <= 128;
     p.u.kvH = c.kvH;
     p.u.G = G;
@@ -355,11 +367,12 @@ PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups)
     auto take = [&](size_t n) { const size_t at = bytes; bytes += (n + 255) & ~(size_t)255; return at; };
     p.spans = take(n * sizeof(PrefixSpan));
     p.at = take(n * sizeof(int2));
-    p.splitBegin = take(PREFIX_GRID * sizeof(int2));
+    const int splits = std::max(PREFIX_GRID, p.u.splitGrid);
+    p.splitBegin = take(splits * sizeof(int2));
     p.chunkBegin = take(PREFIX_GRID * sizeof(int2));
     p.groupOf = take(c.batch * sizeof(int));
     p.totals = take(4 * sizeof(int));
-    p.splitPart = take((size_t)PREFIX_GRID * 2 * 16 * (padded(c) + 2) * sizeof(float));
+    p.splitPart = take((size_t)splits * 2 * 16 * (padded(c) + 2) * sizeof(float));
     p.chunkPart = take(p.chunks ? (size_t)PREFIX_GRID * 2 * 128 * (padded(c) + 2) * sizeof(float) : 0);
     p.sums = take((size_t)2 * c.tokens * c.H * (padded(c) + 4) * sizeof(float));
     p.bytes = bytes;
@@ -402,7 +415,12 @@ hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const voi
         typedef decltype(ctype) TC_;
         auto sized = [&](auto size) {
             constexpr int HSP = decltype(size)::value;
-            if constexpr (HSP <= 128) hipLaunchKernelGGL((attn_prefix_kernel<T_, TC_, HSP>), PREFIX_GRID, 256, 0, s, a, p.u.chunk, p.u.split, OfPrefixes{w});
+            if (HSP == 64 && p.u.splitGrid) {
+                if constexpr (HSP == 64) {
+                    hipLaunchKernelGGL((attn_prefix_split_kernel<T_, TC_, HSP>), p.u.splitGrid, 256, 0, s, a, p.u.split, OfPrefixes{w});
+                    hipLaunchKernelGGL((attn_prefix_chunk_kernel<T_, TC_, HSP>), PREFIX_GRID, 256, 0, s, a, p.u.chunk, OfPrefixes{w});
+                }
+            } else if constexpr (HSP <= 128) hipLaunchKernelGGL((attn_prefix_kernel<T_, TC_, HSP>), PREFIX_GRID, 256, 0, s, a, p.u.chunk, p.u.split, OfPrefixes{w});
             else hipLaunchKernelGGL((attn_prefix_split_kernel<T_, TC_, HSP>), PREFIX_GRID, 256, 0, s, a, p.u.split, OfPrefixes{w});
             hipLaunchKernelGGL((attn_prefix_join_kernel<T_, HSP>), join, 256, 0, s, a, w, p.u);
         };

@@ -90,6 +90,10 @@ CASES = [
     ("many", 2, 1, 32, 8, "head", [(1 + b % 3, 53 + 7 * b % 61, 0) for b in range(200)], [(0, 90, 48), (90, 91, 48), (91, 200, 40)], 0),
     ("more_than_a_scan", 1, 1, 32, 16, "pos", [(b % 3, 40 + 11 * b % 40, 0) for b in range(600)], [(5, 400, 32), (400, 590, 16)], 1),
     ("as_many_groups_as_sequences", 2, 1, 64, 16, "head", [(1 + b % 2, 40 + b, 0) for b in range(300)], [(b, b + 1, 32) for b in range(300)], 0),
+    ("single_tokens_of_unshared_heads", 4, 4, 64, 16, "head", [(1, 3000 + 17 * b, 0) for b in range(24)], [(0, 20, 2990), (20, 24, 100)], 0),
+    ("unshared_heads_and_one_chunk", 3, 3, 48, 8, "pos", [(20, 900, 0)] + [(b % 2, 300 + b, 0) for b in range(40)], [(0, 30, 288), (30, 41, 64)], 2),
+    ("more_groups_than_the_list_has", 1, 1, 32, 16, "head", [(1, 20 + b % 50, 0) for b in range(1100)], [(b, b + 1, 16) for b in range(1100)], 0),
+    ("more_entries_than_the_list_has", 1, 1, 32, 16, "pos", [(1, 20 + b % 30, 0) for b in range(4090)], [(b * 409, b * 409 + 409, 16) for b in range(10)], 0),
     ("three_groups_of_chunks", 8, 8, 64, 16, "head", [(65 + b % 3, 165 + b % 3 + 5 * b % 30, 0) for b in range(30)], [(0, 10, 96), (10, 11, 64), (11, 30, 80)], 4),
 ]
 
