@@ -382,17 +382,25 @@ inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// Rows of a sequence from which on its tokens fill tiles by themselves, and nothing is saved by sharing; bytes of keys and values that the sequences can hold up to which
-// reading them all takes less than two launches more.
-constexpr int PREFIX_ROWS = 128;
-constexpr double PREFIX_BYTES = 64e6;
+// What is shared is worth it if the sequences can be long or hold many bytes of keys and values, and have few rows (tokens times the heads that share a key head) each: with many, the
+// kernels of attention over pages have whole tiles of one sequence.  us, over pages | shared, 16 bits, heads of 128, single tokens with up to 64 - 300 positions of their own:
+//   32 heads on 8, 16 sequences behind 1024 (71 MB) 20.2 | 25.4, 64 (285 MB) 39.8 | 35.7, 64 behind 256 (84 MB) 17.4 | 29.0; behind 4096, 8 (136 MB) 29.3 | 28.6, 64 125 | 41;
+//   16 on one, 16 behind 1024 (11 MB) 19.1 | 26.6, behind 4096 (36 MB) 41.3 | 29.9; 64 on one, 64 behind 1024 (43 MB) 41.0 | 38.0, behind 4096 80 | 60, behind 12000 189 | 91;
+// in fp32 over 16 bits, 12 heads on 4 of 64, behind 1024, 24 (27 MB) 21.6 | 26.1, 96 (107 MB) 38.9 | 29.4, behind 4096 8 (34 MB) 26.1 | 23.7.
+// By rows a sequence, 16 sequences, 16 bits: 32 heads on 8 behind 2048 and behind 16384, 21 53 | 41, 42 45 | 59 and 178 | 132, 84 53 | 92 and 199 | 248, 167 71 | 125 and 323 | 450; 8 on 8 behind
+// 4096, 42 63 | 58, 83 73 | 92; fp32 behind 2048, 31 43 | 36, 62 38 | 56.
+constexpr int PREFIX_LONG = 3000;   // positions that the sequences can have
+constexpr int PREFIX_ROWS = 32, PREFIX_LONG_ROWS = 64;
+constexpr double PREFIX_BYTES = 120e6, PREFIX_BYTES_F32 = 60e6, PREFIX_LONG_BYTES = 32e6;
 
 size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups)
 {
     const int e = dt == BF16 || c.ct == BF16 ? 8 : 4;
     const bool pieces = c.hs % e == 0 && c.sP % e == 0 && c.sH % e == 0 && c.sT % e == 0 && at16(c.k) && at16(c.v) && at16(q) && at16(y);
-    if (!pieces || c.batch < 2 || groups > PREFIX_GROUPS || groups + c.batch > PREFIX_ENTRIES || (long long)c.tokens * (c.H / c.kvH) >= (long long)PREFIX_ROWS * c.batch ||
-        (double)c.batch * c.maxPages * c.pageSize * c.kvH * c.hs * 2 * (c.ct == F32 ? 4 : 2) < PREFIX_BYTES) return 0;
+    const bool far = c.maxPages * c.pageSize >= PREFIX_LONG;
+    const double bytes = (double)c.batch * c.maxPages * c.pageSize * c.kvH * c.hs * 2 * (c.ct == F32 ? 4 : 2);
+    if (!pieces || c.batch < 2 || groups > PREFIX_GROUPS || groups + c.batch > PREFIX_ENTRIES || (long long)c.tokens * (c.H / c.kvH) > (far ? PREFIX_LONG_ROWS : PREFIX_ROWS) * (long long)c.batch ||
+        bytes < (far ? PREFIX_LONG_BYTES : dt == F32 ? PREFIX_BYTES_F32 : PREFIX_BYTES)) return 0;
     const PrefixPlan p = prefix_plan(c, dt, groups);
     return p.splitUnits < 1e9 && p.chunkUnits <= 1e9 ? p.bytes : 0;
 }

@@ -683,7 +683,7 @@ template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sam
 //           too much would be listed as above, from their beginning.
 // (No launch waits for its last workgroup: reading what the others have written past the caches, at the level that all XCDs share, at the end of every slice costs
 // more than a launch.  256 rows of 131072, weigh with it 48 us.)  Sums are whole numbers: any order gives the same.
-constexpr int CUT = 256, CUT_BINS = CUT, LISTED = 4096;
+constexpr int CUT = 256, CUT_BINS = CUT, LISTED = 4096, COUNTERS = 32;   // (a row's counter has 128 bytes of its own)
 enum RowMode { ROW_DONE, ROW_LIST_ALL, ROW_LIST_BIN, ROW_WHOLE };
 struct RowState {
     int mode, last;       // min-p's border: logits above `at`, equal ones up to index `last`
@@ -787,7 +787,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_to
         for (int i = 1; i < CUT / 64; i++) top = fmaxf(top, sTop[i]);
         w.tops[row * w.slices + slice] = top;
     }
-    if (slice == 0 && tid == 0) w.listed[row] = 0;
+    if (slice == 0 && tid == 0) w.listed[row * COUNTERS] = 0;
 }
 
 // smallest logit that the weights' share `least` keeps
@@ -1029,7 +1029,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_li
     });
     int to = (int)block_scan<CUT / 64>(__popcll(hits), sSums, &all);
     if (!all) return;
-    if (tid == 0) sBase = __hip_atomic_fetch_add(w.listed + row, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) sBase = __hip_atomic_fetch_add(w.listed + row * COUNTERS, (int)all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     to += sBase;
     if (hits)
@@ -1121,7 +1121,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(THREADS) void sampl
     top_is(r, st.top);
     const Settings t = settings_of<float>(a, row);
     r.rate = t.rate;
-    const int n = min(w.listed[row], LISTED);
+    const int n = min(w.listed[row * COUNTERS], LISTED);
     const u64* list = w.list + (size_t)row * LISTED;
     if (tid < 32) sRoots[tid] = ROOTS[tid];
     u64 key[OWN], weight[OWN], least = 0, all, total;
@@ -1220,21 +1220,27 @@ int sample_bits(int vocab)
     return std::min(50, 63 - log);
 }
 
-// Rows up to which slices of them are what workgroups have, logits of a row and of all from which on, and logits a thread of a slice: few where there are few slices
-constexpr int CUT_ROWS = 4096, CUT_VOCAB = 4096, CUT_LOGITS = 1 << 19;
+// When slices of rows are what workgroups have.  Where every CU has a row or two at most, a row alone takes as long as it is, and five launches some 25 us; more rows than that
+// take turns.  us, a workgroup a row | slices: top-50 in fp32, 1 row of 32000 21.4 | 22.4, of 131072 41.3 | 24.2, 16 of 8000 17.8 | 24.0, 256 of 8000 19.1 | 27.4, of 32000
+// 30.4 | 39.2, 1024 of 4000 63.1 | 49.0; temperature, top-k, top-p and min-p in 16 bits, 1 row of 32000 25.7 | 25.5, 16 47.4 | 36.4, 256 55.5 | 54.7, 4 of 131072 67.0 | 35.3, 16 of 8000
+// 29.1 | 32.5, 1024 of 4000 91.5 | 65.2; top-p in fp32, 1 row of 32000 27.0 | 24.9, 64 38.0 | 39.3, 256 43.6 | 56.1.  (Above CUT_ROWS it is the scratch memory that costs.)
+constexpr int CUT_ROWS = 4096, CUT_FEW = 128, CUT_TURNS = 512;
+static bool cut(const SampleArgs& a) { return a.count <= CUT_ROWS && a.vocab >= (a.count <= CUT_FEW ? 24576 : a.count <= CUT_TURNS ? 49152 : 2048); }
+// Logits a thread of a slice: few where there are few slices.  us, 8 | 32: 64 rows of 32000, the four settings 41.2 | 43.8, temperature alone 15.7 | 18.6, 1024 of 4000 65.2 | 72.0; top-50
+// 256 rows of 32000 47.0 | 39.2, 1024 of 8000 60.2 | 56.6
 static int cut_each(const SampleArgs& a)
 {
-    const long long slices = (long long)a.count * ((a.vocab + 32 * CUT - 1) / (32 * CUT));
-    return slices < 256 && a.vocab <= 128 * 8 * CUT ? 8 : 32;
+    const long long slices = (long long)a.count * ((a.vocab + 8 * CUT - 1) / (8 * CUT));
+    return slices < 4096 && a.vocab <= 128 * 8 * CUT ? 8 : 32;
 }
 static bool cut_bins(const SampleArgs& a) { return a.k || a.p; }
 
 size_t sample_workspace_bytes(SampleType type, const SampleArgs& a)
 {
-    if (type == SAMPLE_F64 || a.count > CUT_ROWS || a.vocab <= CUT_VOCAB || (long long)a.count * a.vocab < CUT_LOGITS) return 0;
+    if (type == SAMPLE_F64 || !cut(a)) return 0;
     const int each = cut_each(a);
     const size_t slices = (a.vocab + each * CUT - 1) / (each * CUT), rows = a.count;
-    return rows * (slices * (8 + 4) + sizeof(RowState) + 8 + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
+    return rows * (slices * (8 + 4) + sizeof(RowState) + 4 * COUNTERS + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
 }
 
 hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspace)
@@ -1258,7 +1264,7 @@ hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspac
             at = (char*)(w.counts + rows * w.slices * CUT_BINS);
         }
         w.listed = (int*)at;
-        w.tops = (float*)(w.listed + rows);
+        w.tops = (float*)(w.listed + rows * COUNTERS);
         const dim3 grid(w.slices, a.count);
         auto go = [&](auto type, auto size) {
             typedef decltype(type) L;

@@ -15,7 +15,7 @@ class Shared(Cache):
     def __init__(self, dev, rng, seqs, groups, kvH, hs, page, order, half, wide=True, **more):
         # sequences that cannot hold this many bytes are not worth sharing for, and go to attention over pages: room for more than they have
         if wide:
-            more["width"] = max(max(-(-m // page) for _, m, _ in seqs) + 1, int(66e6 / (len(seqs) * page * kvH * hs * (4 if half else 8))) + 1)
+            more["width"] = max(max(-(-m // page) for _, m, _ in seqs) + 1, int(125e6 / (len(seqs) * page * kvH * hs * (4 if half else 8))) + 1)
         super().__init__(dev, rng, seqs, kvH, hs, page, order, half, **more)
         self.groups = groups
         for first, end, shared in groups:
@@ -94,6 +94,9 @@ CASES = [
     ("unshared_heads_and_one_chunk", 3, 3, 48, 8, "pos", [(20, 900, 0)] + [(b % 2, 300 + b, 0) for b in range(40)], [(0, 30, 288), (30, 41, 64)], 2),
     ("more_groups_than_the_list_has", 1, 1, 32, 16, "head", [(1, 20 + b % 50, 0) for b in range(1100)], [(b, b + 1, 16) for b in range(1100)], 0),
     ("more_entries_than_the_list_has", 1, 1, 32, 16, "pos", [(1, 20 + b % 30, 0) for b in range(4090)], [(b * 409, b * 409 + 409, 16) for b in range(10)], 0),
+    ("a_chunk_among_single_tokens", 4, 2, 64, 16, "head", [(150, 400, 0)] + [(1 + b % 3, 230 + 9 * b, 0) for b in range(24)], [(0, 25, 224)], 3),
+    ("chunks_among_single_tokens", 8, 2, 128, 32, "pos", [(1, 400 + 5 * b, 0) if b % 6 else (60 + b, 500 + b, 0) for b in range(26)], [(0, 13, 384), (13, 26, 320)], 0),
+    ("long_chunks_of_two_groups", 4, 4, 64, 16, "head", [(1, 1500 + 3 * b, 0) if b % 20 else (300 + b, 2000, 0) for b in range(60)], [(0, 30, 1400), (30, 60, 1024)], 1),
     ("three_groups_of_chunks", 8, 8, 64, 16, "head", [(65 + b % 3, 165 + b % 3 + 5 * b % 30, 0) for b in range(30)], [(0, 10, 96), (10, 11, 64), (11, 30, 80)], 4),
 ]
 
