@@ -325,8 +325,8 @@ MCH_LONG DLL_InvokeFloatEx(MCH_LONG lKernelIdx, MCH_LONG lFunctionIdx, float* pI
  * FREE_LAYERNORM and LAYERNORM_FWD / BWD, CREATE / FREE_CUDNN, CREATE / FREE / SET_TENSORDESC, SOFTMAX_FWD / BWD,
  * ATTN_CREATE / FREE / SET / FWD / BWD (no dropout; the tenth and eleventh values of ATTN_FWD as on the float side, the twelfth ignored),
  * CREATE_ROPE / FREE_ROPE / ROPE_FWD / BWD, and the fused ids ATTN_DECODE_FWD, QKV_PROJ_HEADS, QKV_HEADS_GRAD,
- * LINEAR_FWD / BWD, RMSNORM_BWD, SWIGLU_BWD and NORM_ADD_FWD / BWD - same packing as the float ids above: what the attention, multi-head attention and transformer block layers
- * call, forward and backward.  Products run on the double matrix cores, the rest in one-element-per-thread kernels.  Any other id (blob loaders, extensions), and DLL_InvokeDoubleEx (extensions and blob loaders are float objects),
+ * LINEAR_FWD / BWD, RMSNORM_BWD, SWIGLU_BWD, NORM_ADD_FWD / BWD, QK_NORM_ROPE_FWD / BWD, PAGED_APPEND, ATTN_PAGED_FWD, ATTN_PAGED_PREFIX_FWD, PAGED_PLAN and
+ * SAMPLE_FWD - same packing as the float ids above: what the attention, multi-head attention and transformer block layers call, forward and backward, and serving.  Products run on the double matrix cores, the rest in one-element-per-thread kernels.  Any other id (blob loaders, extensions), and DLL_InvokeDoubleEx (extensions and blob loaders are float objects),
  * returns MCH_ERROR_NOT_IMPLEMENTED with the id in the message. */
 MCH_LONG DLL_InvokeDouble(MCH_LONG lKernelIdx, MCH_LONG lFunctionIdx, double* pInput, MCH_LONG lInput,
                           double** ppOutput, MCH_LONG* plOutput, MCH_TCHAR* szErr, MCH_LONG lszErrMax);

@@ -82,7 +82,8 @@ template <typename T> __device__ __forceinline__ Ask ask_of(const Plan<T>& p, in
 // Workgroup 0 decides and writes everything that its decisions change; the others copy what they do not, where the block table and the list of free pages
 // are not written in place (in place, they all are: a length that changes decides nothing then).
 // What bounds it is one read behind the other in workgroup 0, so whatever it goes through - sequences, pages that come back, pages that are taken, entries that are copied -
-// is one list of items each, a thread an item, whose sequence it finds in the list's sums.
+// is one list of items each, a thread an item, whose sequence it finds in the list's sums.  Measured, all memory of its own: 4 sequences of one token 4.5 us (an empty call takes 3.3 - 3.8), 512
+// with tables of 512 entries, a tenth of which end or begin, 17 - 20 us (13.3 and 5.2 for the rows), 256 prompts 16.6; with loops over the sequences in place of the lists 8.4, 30 and 33.
 template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void paged_plan_kernel(Plan<T> p, int writeTokens)
 {
     constexpr int WAVES = THREADS / 64;
@@ -276,14 +277,17 @@ template <typename T> __global__ __launch_bounds__(256) void paged_plan_rows_ker
     }
 }
 
-constexpr int ROWS_OF_ONE = 8192;   // rows up to which the first workgroup writes their places too
-constexpr int ROWS_OF_FEW = 1024;   // rows, and a quarter as many sequences, up to which four wavefronts do
+// Rows up to which the first workgroup writes their places too.  us, it | a launch more: 32 prompts, 4096 rows 7.6 | 9.5, 16384 8.8 | 10.4, 256 prompts, 32768 rows 15.3 | 12.0, 65536
+// 57 | 15
+constexpr int ROWS_OF_ONE = 16384;
+// Sequences and rows up to which four wavefronts do.  us, four | sixteen: 4 sequences of one token 4.8 | 5.3, 8 prompts, 1024 rows 5.6 | 6.5, 32 sequences of one token 7.0 | 5.5
+constexpr int BATCH_OF_FEW = 16, ROWS_OF_FEW = 1024;
 
 template <typename T> hipError_t launch(hipStream_t s, const PagedPlanArgs& a)
 {
     Plan<T> p = {a};
     const long long entries = (a.table != a.tableOut ? (long long)a.batch * a.maxPages : 0) + (a.free != a.freeOut ? a.pages : 0);
-    const bool rows = a.positions || a.slots, own = a.tokens <= ROWS_OF_ONE, few = a.tokens <= ROWS_OF_FEW && a.batch <= ROWS_OF_FEW / 4;
+    const bool rows = a.positions || a.slots, own = a.tokens <= ROWS_OF_ONE, few = a.tokens <= ROWS_OF_FEW && a.batch <= BATCH_OF_FEW;
     const int others = (int)std::min<long long>(few ? 1024 : 256, (entries + 4095) / 4096);
     if (few) hipLaunchKernelGGL((paged_plan_kernel<T, 256>), 1 + others, 256, 0, s, p, rows ? 1 : 0);
     else hipLaunchKernelGGL((paged_plan_kernel<T, 1024>), 1 + others, 1024, 0, s, p, rows && own ? 1 : 0);
