@@ -6,6 +6,11 @@
 //
 // A draw compares u with sums over the whole vocabulary: a sum that is off by e moves every border by e, so with 100000 tokens fp32 sums draw another token every
 // few hundred rows.  Weights are made in 64 bits and held as whole numbers of 2^-FB, which add up to the same in any order; their sums are exact.
+//
+// A logit takes some 20 instructions of 64 bits where its weight counts, and none where only its place does (top-k): long rows are bound by these, and by their bins, short ones by one
+// pass and one barrier behind the other.  A row is one workgroup's, its logits read two or three times (they stay in the caches); or slices of it are (below).  Measured: top-p
+// of a row of 32000 in fp32 27 us by one workgroup, 24 in slices; 64 rows of 50261 in fp32, top-50, 28 us; 256 rows of 131072 in 16 bits with settings of their own 95 us
+// (67 MB; largest logits 13, weights 38, borders 11, candidates 17, the rest 17); 48 rows of 200003 in 16 bits by temperature alone 27 us.
 #include <algorithm>
 #include <type_traits>
 
