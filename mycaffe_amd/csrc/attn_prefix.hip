@@ -86,7 +86,7 @@ struct PrefixUnits {
 template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THREADS) void attn_prefix_plan_kernel(PagedCache c, PrefixWork w, PrefixUnits u)
 {
     constexpr int WAVES = THREADS / 64;
-    __shared__ int sBound[GROUPS + 1], sPrefix[GROUPS], sFirst[ENTRIES + 1], sSums[2][WAVES], sAt[2][ENTRIES];
+    __shared__ int sBound[GROUPS + 1], sPrefix[GROUPS], sRow[GROUPS], sFirst[ENTRIES + 1], sSums[2][WAVES], sAt[2][ENTRIES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, positions = c.maxPages * c.pageSize;
     const int said = tid < w.nGroups ? paged_int(w.shared[tid], 0, positions) : 0;
     // bounds of the groups, never decreasing: the largest so far
@@ -107,6 +107,7 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
     if (tid < w.nGroups) {
         sBound[tid] = bound;
         sPrefix[tid] = positions + 1;
+        sRow[tid] = c.batch;
     }
     if (tid == w.nGroups - 1) sSums[1][0] = bound;
     __syncthreads();
@@ -115,7 +116,7 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
         sFirst[c.batch] = rows;
     }
     __syncthreads();
-    // of sequence b its group, or -1; the least position of a group's new tokens
+    // of sequence b its group, or -1; the least position of a group's new tokens, and the first sequence with any, whose pages are read (others need not have any more)
     auto group_of = [&](int b) -> int {
         if (b < sBound[0] || b >= sBound[w.nGroups]) return -1;
         int lo = 0, hi = w.nGroups;
@@ -130,7 +131,10 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
         const PagedSpan s = b == tid ? span : paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions);
         sFirst[b] = s.first;
         const int g = group_of(b);
-        if (g >= 0 && s.count > 0) atomicMin(&sPrefix[g], max(s.len - s.count, 0));
+        if (g >= 0 && s.count > 0) {
+            atomicMin(&sPrefix[g], max(s.len - s.count, 0));
+            atomicMin(&sRow[g], b);
+        }
     }
     __syncthreads();
     if (tid < w.nGroups) sPrefix[tid] = sPrefix[tid] > positions ? 0 : min(sPrefix[tid], said) / c.pageSize * c.pageSize;
@@ -144,7 +148,7 @@ template <int THREADS, int ENTRIES, int GROUPS> __global__ __launch_bounds__(THR
             PrefixSpan s;
             if (v < w.nGroups) {
                 const int first = sBound[v], prefix = sPrefix[v];
-                s = PrefixSpan{sFirst[first], prefix > 0 ? max(sFirst[sBound[v + 1]] - sFirst[first], 0) : 0, prefix, 0, prefix, first, 1, 0};
+                s = PrefixSpan{sFirst[first], prefix > 0 ? max(sFirst[sBound[v + 1]] - sFirst[first], 0) : 0, prefix, 0, prefix, sRow[v], 1, 0};
             } else {
                 const int b = v - w.nGroups, g = group_of(b), from = g >= 0 ? sPrefix[g] : 0;
                 const PagedSpan x = v0 == 0 && w.nGroups <= THREADS && sequence >= 0 ? own : paged_span(c.starts[b], c.starts[b + 1], c.lens[b], c.tokens, positions);

@@ -131,6 +131,20 @@ def test_holes_and_entries_that_are_no_page(dev, act16, cache16):
 
 
 @pytest.mark.parametrize("act16,cache16", TYPES)
+@pytest.mark.parametrize("wide", [True, False])
+def test_first_sequences_of_groups_that_have_ended(dev, act16, cache16, wide):
+    """Their rows of the block table name no pages any more, and count for nothing."""
+    rng = np.random.default_rng(23)
+    c = Shared(dev, rng, [(0, 150, 0), (0, 120, 0), (1, 140, 0), (2, 130, 0), (0, 99, 0), (1, 90, 0), (1, 100, 0)], [(0, 4, 96), (4, 7, 64)], 2, 64, 16, "head", cache16, wide=wide)
+    for b in (0, 1, 4):
+        c.table[b] = -1
+        c.lens[b] = 0
+    c.upload()
+    c.h["lens"] = dev.put(c.lens)
+    check(dev, rng, c, 4, act16)
+
+
+@pytest.mark.parametrize("act16,cache16", TYPES)
 def test_groups_and_prefixes_that_are_none(dev, act16, cache16):
     """Numbers out of range count as its nearest end: the result is the definition's whatever they say, as long as what is said to be shared is."""
     rng = np.random.default_rng(18)
