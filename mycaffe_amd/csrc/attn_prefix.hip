@@ -400,6 +400,7 @@ inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // 4096, 42 63 | 58, 83 73 | 92; fp32 behind 2048, 31 43 | 36, 62 38 | 56.
 constexpr int PREFIX_LONG = 3000;   // positions that the sequences can have
 constexpr int PREFIX_ROWS = 32, PREFIX_LONG_ROWS = 64;
+constexpr size_t PREFIX_SCRATCH = 1ull << 30;   // sums of every row on both sides: 4096 tokens of 32 heads of 128 take 138 MB
 constexpr double PREFIX_BYTES = 120e6, PREFIX_BYTES_F32 = 60e6, PREFIX_LONG_BYTES = 32e6;
 
 size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups)
@@ -411,7 +412,7 @@ size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q,
     if (!pieces || c.batch < 2 || groups > PREFIX_GROUPS || groups + c.batch > PREFIX_ENTRIES || (long long)c.tokens * (c.H / c.kvH) > (far ? PREFIX_LONG_ROWS : PREFIX_ROWS) * (long long)c.batch ||
         bytes < (far ? PREFIX_LONG_BYTES : dt == F32 ? PREFIX_BYTES_F32 : PREFIX_BYTES)) return 0;
     const PrefixPlan p = prefix_plan(c, dt, groups);
-    return p.splitUnits < 1e9 && p.chunkUnits <= 1e9 ? p.bytes : 0;
+    return p.splitUnits < 1e9 && p.chunkUnits <= 1e9 && p.bytes <= PREFIX_SCRATCH ? p.bytes : 0;
 }
 
 hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int groups, const float* bounds, const float* shared, void* workspace)

@@ -675,7 +675,8 @@ template <typename L, typename N> __global__ __launch_bounds__(THREADS) void sam
 {
     __shared__ Shared s;
     extern __shared__ u64 parts[];
-    sample_row<L, N>(a, blockIdx.x, s, parts);
+    const long long row = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+    if (row < a.count) sample_row<L, N>(a, (int)row, s, parts);
 }
 
 // ---- a row by many workgroups ---------------------------------------------------------------------------------------------------------
@@ -1290,9 +1291,11 @@ hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspac
         else sized(bf16_t());
         return hipGetLastError();
     }
-    if (type == SAMPLE_F32) hipLaunchKernelGGL((sample_kernel<float, float>), a.count, THREADS, parts, s, a);
-    else if (type == SAMPLE_BF16) hipLaunchKernelGGL((sample_kernel<bf16_t, float>), a.count, THREADS, parts, s, a);
-    else hipLaunchKernelGGL((sample_kernel<double, double>), a.count, THREADS, parts, s, a);
+    const int x = std::min(a.count, 1 << 21);   // an axis of a launch has less than 2^32 threads
+    const dim3 grid(x, (a.count + x - 1) / x);
+    if (type == SAMPLE_F32) hipLaunchKernelGGL((sample_kernel<float, float>), grid, THREADS, parts, s, a);
+    else if (type == SAMPLE_BF16) hipLaunchKernelGGL((sample_kernel<bf16_t, float>), grid, THREADS, parts, s, a);
+    else hipLaunchKernelGGL((sample_kernel<double, double>), grid, THREADS, parts, s, a);
     return hipGetLastError();
 }
 

@@ -3,6 +3,7 @@ first ones.  Caches, the definition and its tolerances are those of attention ov
 import numpy as np
 import pytest
 
+from tests.conftest import Dev
 from tests.test_gpu_paged import TYPES, U16, U32, Cache, attention, refused, rounded
 
 pytestmark = pytest.mark.gpu
@@ -242,6 +243,32 @@ def test_the_same_as_attention_over_pages(dev, act16, cache16):
         c.attend(hq, hz, H)
         want, tol = attention(c, q, H, act16, None, act16)
         assert (abs(dev.get(hy, q.shape) - want) <= tol).all() and (abs(dev.get(hz, q.shape) - want) <= tol).all()
+
+
+def test_without_scratch_memory(dev, monkeypatch):
+    """Every sequence reads its pages for itself then, a workgroup a token and head."""
+    rng = np.random.default_rng(31)
+    monkeypatch.setenv("MYCAFFE_HIP_SCRATCH_LIMIT", "20000")
+    small = Dev()
+    c = Shared(small, rng, [(1, 90, 0), (3, 100, 0), (1, 70, 0), (2, 80, 0)], [(0, 3, 64)], 2, 64, 16, "head", False)
+    check(small, rng, c, 4, False)
+    small.close()
+
+
+def test_two_kernel_objects_in_turn(dev):
+    """Each has scratch memory of its own."""
+    rng = np.random.default_rng(32)
+    other = Dev()
+    cases = [Shared(d, rng, [(1, 500 + 9 * b, 0) for b in range(12)], [(0, 12, 400 + 16 * i)], 2, 128, 16, "pos", True) for i, d in enumerate((dev, other))]
+    q = [rounded(rng.standard_normal((12, 8, 128)), True) for _ in cases]
+    put = [(c.dev.put(v, True), c.dev.zeros(v.size, True)) for c, v in zip(cases, q)]
+    for _ in range(3):
+        for c, (hq, hy) in zip(cases, put):
+            c.attend_shared(hq, hy, 8)
+    for c, v, (_, hy) in zip(cases, q, put):
+        want, tol = attention(c, v, 8, True, None, True)
+        assert (abs(c.dev.get(hy, v.shape) - want) <= tol).all()
+    other.close()
 
 
 @pytest.mark.parametrize("act16,cache16", TYPES)

@@ -191,6 +191,21 @@ def test_draws_follow_the_weights(kind):
     assert np.array_equal(np.bincount(ids.astype(int), minlength=12), w * n)
 
 
+def test_more_rows_than_an_axis_of_a_launch_has():
+    """2^22 rows and some, of three logits each; the largest logit, and draws at the borders of equal ones."""
+    cuda = CudaDnn(0)
+    rng = np.random.default_rng(20)
+    n = (1 << 22) + 5
+    x = rng.integers(-2, 3, (n, 3)).astype(np.float32)
+    heat = np.where(np.arange(n) % 2, 0.0, 1.0)
+    u = rng.integers(0, 8, n) / 8 + 1 / 16
+    ids, _ = draw(cuda, "f32", x, u, heat, logs=False)
+    w = np.cumsum(np.exp(np.float64(x)), 1)
+    want = np.where(np.arange(n) % 2, x.argmax(1), (w <= u[:, None] * w[:, -1:]).sum(1))
+    assert np.array_equal(ids, want)
+    cuda.Dispose()
+
+
 def test_calls_in_turn_leave_nothing_behind(kind):
     cuda, t = kind
     rng = np.random.default_rng(6)
