@@ -701,7 +701,7 @@ struct RowState {
 // a slice: EACH logits a thread of T, in pieces, in the order of the vocabulary from piece to piece and within one from thread to thread
 template <typename L, int EACH, int T> struct Slice {
     typedef Row<L> R;
-    static constexpr int VEC = R::VEC, PIECES = EACH / VEC, LOGITS = EACH * T;
+    static constexpr int VEC = R::VEC, PIECES = EACH / VEC, LOGITS = EACH * T, CELLS = PIECES * T / 64;   // cells: a wavefront's part of a piece
     __device__ static int index(int slice, int piece) { return slice * LOGITS + piece * T * VEC + (int)threadIdx.x * VEC; }
     L raw[PIECES][VEC];
     __device__ __forceinline__ void load(const R& r, int slice)   // all of it under way at once
@@ -720,56 +720,48 @@ template <typename L, int EACH, int T> struct Slice {
     }
 };
 
-template <int T> struct DrawShared { u64 sums[T / 64], tot[16 * T / 64]; u64 before; int slice; };
-// Of a row, from the sums of n slices, which it is that the draw falls into, and where in it
-template <typename L, typename N, int EACH, int T>
-__device__ __forceinline__ void draw_from(const SampleArgs& a, int row, const Row<L>& r, const Settings& t, const Border<float>& border, const u64* slices, int n, DrawShared<T>& s)
+struct DrawShared { u64 sums[CUT / 64], before; int cell; };
+// The draw of a row from the sums of its n cells: which it falls into, and, for one wavefront, where in it
+template <typename L, int EACH>
+__device__ __forceinline__ void draw_from(const SampleArgs& a, int row, const Row<L>& r, const Settings& t, const Border<float>& border, const u64* cells, int n, DrawShared& s)
 {
-    typedef Slice<L, EACH, T> C;
-    constexpr int W = T / 64;
-    const int tid = threadIdx.x, wave = tid >> 6, per = (n + T - 1) / T;
+    typedef Slice<L, EACH, CUT> C;
+    constexpr int VEC = C::VEC;
+    const int tid = threadIdx.x, per = (n + CUT - 1) / CUT, from = tid * per, to = min(n, from + per);
     u64 mine = 0, total;
-    for (int i = tid * per; i < min(n, (tid + 1) * per); i++) mine += slices[i];
-    u64 before = block_scan<W>(mine, s.sums, &total);
+#pragma unroll 8
+    for (int i = from; i < to; i++) mine += cells[i];
+    u64 before = block_scan<CUT / 64>(mine, s.sums, &total);
     const u64 want = __umul64hi(total, t.share);
     if (before <= want && want < before + mine)
-        for (int i = tid * per; i < min(n, (tid + 1) * per); i++) {
-            const u64 x = slices[i];
-            if (want < before + x) { s.slice = i; s.before = before; break; }
+        for (int i = from; i < to; i++) {
+            const u64 x = cells[i];
+            if (want < before + x) { s.cell = i; s.before = before; break; }
             before += x;
         }
     __syncthreads();
-    const int slice = s.slice;
-    u64 w[C::PIECES];
-    C c;
-    c.load(r, slice);
-    c.each(r, slice, [&](int q, int i0, const float (&v)[C::VEC]) __attribute__((always_inline)) {
-        w[q] = kept_weights(r, v, i0, border);
-        const u64 sum = wave_sum(w[q]);
-        if ((tid & 63) == 0) s.tot[q * W + wave] = sum;
-    });
-    __syncthreads();
-    u64 at = s.before;
-    int k = 0;
+    if (tid >= 64) return;
+    const int i0 = s.cell * 64 * VEC + tid * VEC;   // (the order of the cells is that of the vocabulary)
+    L raw[VEC];
+    float v[VEC];
+    u64 w[VEC], sum = 0;
+    r.fetch(i0, raw);
+    r.logits(raw, v);
 #pragma unroll
-    for (int q = 0; q < C::PIECES; q++) {
-        for (; k < q * W + wave; k++) at += s.tot[k];
-        const u64 from = at + wave_scan(w[q]) - w[q];
-        if (from <= want && want < from + w[q]) {
-            float v[C::VEC];
-            const int i0 = C::index(slice, q);
-            r.logits(c.raw[q], v);
-            u64 x = from;
-            int id = -1;
+    for (int e = 0; e < VEC; e++) sum += w[e] = r.weight(v[e]);
+    if (border.at > -INFINITY) {
+        sum = 0;
 #pragma unroll
-            for (int e = 0; e < C::VEC; e++) {
-                const u64 one = border.has(v[e], i0 + e) ? r.weight(v[e]) : 0;
-                if (x <= want && want < x + one) id = i0 + e;
-                x += one;
-            }
-            write_draw<L, N>(a, row, r, t, id, total);
-        }
+        for (int e = 0; e < VEC; e++) sum += w[e] = border.has(v[e], i0 + e) ? w[e] : 0;
     }
+    u64 at = s.before + wave_scan(sum) - sum;
+    int id = -1;
+#pragma unroll
+    for (int e = 0; e < VEC; e++) {
+        if (at <= want && want < at + w[e]) id = i0 + e;
+        at += w[e];
+    }
+    if (id >= 0) write_draw<L, float>(a, row, r, t, id, total);
 }
 
 template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_top_kernel(SampleArgs a, SampleCuts w)
@@ -804,27 +796,25 @@ template <typename R> __device__ __forceinline__ Border<float> border_of_least(c
     return b;
 }
 
-// the row's largest logit, and the first slice that has it
-__device__ __forceinline__ float top_of_row(const SampleCuts& w, int row, int* first)
+// the row's largest logit, and the first slice that has it, from that of slice i in thread i
+constexpr int SLICES = 128;   // of a row, at most
+static_assert(SLICES <= CUT && SAMPLE_VOCAB <= SLICES * 32 * CUT, "a thread a slice");
+__device__ __forceinline__ float top_of_slice(const SampleCuts& w, int row) { return (int)threadIdx.x < w.slices ? w.tops[row * w.slices + threadIdx.x] : -INFINITY; }
+__device__ __forceinline__ float top_of_row(float mine, int* first)
 {
-    __shared__ float sTop[CUT / 64];
-    __shared__ int sAt[CUT / 64];
+    __shared__ float sTop[SLICES / 64];
+    __shared__ int sAt[SLICES / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    float top = -INFINITY;
-    int at = INT32_MAX;
-    for (int i = tid; i < w.slices; i += CUT) {
-        const float x = w.tops[row * w.slices + i];
-        if (x > top) { top = x; at = i; }
+    if (tid < SLICES) {
+        const float top = group_max<64>(mine);
+        const u64 there = __ballot(mine == top);
+        if (lane == 0) { sTop[wave] = top; sAt[wave] = tid + __builtin_ctzll(there | 1ull << 63); }
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const float x = __shfl_xor(top, o);
-        const int i = __shfl_xor(at, o);
-        if (x > top || (x == top && i < at)) { top = x; at = i; }
-    }
-    if (lane == 0) { sTop[wave] = top; sAt[wave] = at; }
     __syncthreads();
-    for (int i = 0; i < CUT / 64; i++)
-        if (sTop[i] > top || (sTop[i] == top && sAt[i] < at)) { top = sTop[i]; at = sAt[i]; }
+    float top = sTop[0];
+    int at = sAt[0];
+    for (int i = 1; i < SLICES / 64; i++)
+        if (sTop[i] > top) { top = sTop[i]; at = sAt[i]; }
     *first = at;
     return top;
 }
@@ -847,25 +837,28 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_we
     __shared__ double sRoots[32];
     const int tid = threadIdx.x, slice = blockIdx.x, row = blockIdx.y;
     R r;
+    const float mine = top_of_slice(w, row);
     if (!row_of<L, float>(a, row, r, sRoots)) return;
-    C c;
-    c.load(r, slice);
     const Settings t = settings_of<float>(a, row);
+    C c;
+    c.load(r, slice);   // (behind what is waited for first)
     if (t.first) return;
     if (tid < 32) sRoots[tid] = ROOTS[tid];
     sCount[tid] = 0;
     sWeight[tid] = 0;
     int first;
-    const float top = top_of_row(w, row, &first);   // (with the barrier that the lines above need)
+    const float top = top_of_row(mine, &first);   // (with the barrier that the lines above need)
     if (!(top > -INFINITY)) return;
     top_is(r, top);
     r.rate = t.rate;
     u64 sum = 0, all;
     if (!t.byK && !t.byP) {
         const Border<float> border = border_of_least(r, t.least);
-        c.each(r, slice, [&](int, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) { sum += kept_weights(r, v, i0, border); });
-        block_scan<CUT / 64>(sum, sSums, &all);
-        if (tid == 0) w.sums[row * w.slices + slice] = all;
+        u64* cells = w.sums + (size_t)(row * w.slices + slice) * C::CELLS + (tid >> 6);
+        c.each(r, slice, [&](int q, int i0, const float (&v)[R::VEC]) __attribute__((always_inline)) {
+            const u64 x = wave_sum(kept_weights(r, v, i0, border));
+            if ((tid & 63) == 0) cells[q * (CUT / 64)] = x;
+        });
         return;
     }
     const bool byWeight = weighs(t);
@@ -894,7 +887,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_we
     w.counts[bins] = sCount[tid];
     if (byWeight) {
         w.weights[bins] = sWeight[tid];
-        if (tid == 0) w.sums[row * w.slices + slice] = all;
+        if (tid == 0) w.sums[(size_t)(row * w.slices + slice) * C::CELLS] = all;
     }
 }
 
@@ -902,7 +895,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_bo
 {
     typedef Row<L> R;
     typedef Slice<L, EACH, CUT> C;
-    __shared__ DrawShared<CUT> s;
+    __shared__ DrawShared s;
     __shared__ int sFirst, sBin, sReached, sIn[CUT_BINS];
     __shared__ double sRoots[32];
     const int tid = threadIdx.x, row = blockIdx.x;
@@ -910,23 +903,35 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_bo
     row_of<L, float>(a, row, r, sRoots);
     const Settings t = settings_of<float>(a, row);
     const bool bins = t.byK || t.byP;
-    // this thread's bin of the row
+    const float mine = top_of_slice(w, row);
+    const u64* cells = w.sums + (size_t)row * w.slices * C::CELLS;
+    // this thread's bin of the row, and its slice
     uint32_t n = 0;
     u64 x = 0, sum = 0, all = 0;
     if (bins) {
-#pragma unroll 8
-        for (int i = 0; i < w.slices; i++) n += w.counts[((size_t)row * w.slices + i) * CUT_BINS + tid];
-        if (!t.byK) {
-#pragma unroll 8
-            for (int i = 0; i < w.slices; i++) x += w.weights[((size_t)row * w.slices + i) * CUT_BINS + tid];
-            for (int i = tid; i < w.slices; i += CUT) sum += w.sums[row * w.slices + i];
+        constexpr int AHEAD = 16;   // slices read at once
+        sum = !t.byK && tid < w.slices ? cells[tid * C::CELLS] : 0;
+        for (int i0 = 0; i0 < w.slices; i0 += AHEAD) {
+            uint32_t some[AHEAD];
+            u64 heavy[AHEAD];
+            const size_t at = (size_t)row * w.slices * CUT_BINS + tid;
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) some[j] = w.counts[at + min(i0 + j, w.slices - 1) * CUT_BINS];
+            if (!t.byK)
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++) heavy[j] = w.weights[at + min(i0 + j, w.slices - 1) * CUT_BINS];
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                n += i0 + j < w.slices ? some[j] : 0;
+                if (!t.byK) x += i0 + j < w.slices ? heavy[j] : 0;
+            }
         }
     }
     if (tid < 32) sRoots[tid] = ROOTS[tid];
     sIn[tid] = n;
     if (tid == 0) { sFirst = INT32_MAX; sBin = -1; }
     int first;
-    const float top = top_of_row(w, row, &first);
+    const float top = top_of_row(mine, &first);
     RowState st = {};
     st.mode = ROW_DONE;
     st.top = top;
@@ -950,7 +955,7 @@ template <typename L, int EACH> __global__ __launch_bounds__(CUT) void sample_bo
         __syncthreads();
         if (tid == 0) write_draw<L, float>(a, row, r, t, sFirst, 0);
     } else if (!bins) {
-        draw_from<L, float, EACH, CUT>(a, row, r, t, border_of_least(r, t.least), w.sums + row * w.slices, w.slices, s);
+        draw_from<L, EACH>(a, row, r, t, border_of_least(r, t.least), cells, w.slices * C::CELLS, s);
     } else {
         u64 any, weight;
         if (!t.byK) block_scan<CUT / 64>(sum, s.sums, &all);
@@ -1117,6 +1122,13 @@ template <typename L, int EACH> __global__ __launch_bounds__(THREADS) void sampl
     extern __shared__ u64 parts[];
     const int tid = threadIdx.x, row = blockIdx.x;
     const RowState st = ((const RowState*)w.state)[row];
+    // (read at once, whatever it is good for)
+    const int n = min(w.listed[row * COUNTERS], LISTED);
+    const u64* list = w.list + (size_t)row * LISTED;
+    const Settings t = settings_of<float>(a, row);
+    u64 key[OWN];
+#pragma unroll
+    for (int j = 0; j < OWN; j++) key[j] = list[tid + THREADS * j];
     if (st.mode == ROW_WHOLE) {
         sample_row<L, float>(a, row, s.row, parts);
         return;
@@ -1125,14 +1137,11 @@ template <typename L, int EACH> __global__ __launch_bounds__(THREADS) void sampl
     R r;
     row_of<L, float>(a, row, r, sRoots);
     top_is(r, st.top);
-    const Settings t = settings_of<float>(a, row);
     r.rate = t.rate;
-    const int n = min(w.listed[row * COUNTERS], LISTED);
-    const u64* list = w.list + (size_t)row * LISTED;
     if (tid < 32) sRoots[tid] = ROOTS[tid];
-    u64 key[OWN], weight[OWN], least = 0, all, total;
+    u64 weight[OWN], least = 0, all, total;
 #pragma unroll
-    for (int j = 0; j < OWN; j++) key[j] = tid + THREADS * j < n ? list[tid + THREADS * j] : 0;
+    for (int j = 0; j < OWN; j++) key[j] = tid + THREADS * j < n ? key[j] : 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < OWN; j++) weight[j] = key[j] ? r.weight(logit_at<L>(key[j])) : 0;
@@ -1241,12 +1250,14 @@ static int cut_each(const SampleArgs& a)
 }
 static bool cut_bins(const SampleArgs& a) { return a.k || a.p; }
 
+static size_t cells_of(SampleType type, int each) { return each / (type == SAMPLE_BF16 ? 8 : 4) * (CUT / 64); }
+
 size_t sample_workspace_bytes(SampleType type, const SampleArgs& a)
 {
     if (type == SAMPLE_F64 || !cut(a)) return 0;
     const int each = cut_each(a);
     const size_t slices = (a.vocab + each * CUT - 1) / (each * CUT), rows = a.count;
-    return rows * (slices * (8 + 4) + sizeof(RowState) + 4 * COUNTERS + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
+    return rows * (slices * (8 * cells_of(type, each) + 4) + sizeof(RowState) + 4 * COUNTERS + (cut_bins(a) ? LISTED * 8 + slices * CUT_BINS * 12 : 0));
 }
 
 hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspace)
@@ -1261,7 +1272,7 @@ hipError_t k_sample(hipStream_t s, SampleType type, SampleArgs a, void* workspac
         SampleCuts w = {};
         w.slices = (a.vocab + each * CUT - 1) / (each * CUT);
         w.sums = (u64*)workspace;
-        w.state = w.sums + rows * w.slices;
+        w.state = w.sums + rows * w.slices * cells_of(type, each);
         char* at = (char*)w.state + rows * sizeof(RowState);
         if (cut_bins(a)) {
             w.list = (u64*)at;
