@@ -135,7 +135,45 @@ __device__ __forceinline__ ChunkTile chunk_tile(const PagedCache& c, const Chunk
     return ChunkTile{uniform(seq), uniform(tile), group / w.headTiles, group % w.headTiles};
 }
 
-// Chunks in 16-bit storage, head size 64 or 128, in tiles of 256 rows (w.pair 2); flags[i]: the tile of workgroup i is left to the chunk kernel
-hipError_t attn_paged_pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* flags);
+// Tiles take turns, one a CU at head size 128 and two at 64, and the last turn is seldom full: where the positions of a tile are done in pieces, each by a workgroup, more and
+// shorter turns leave less of the chip idle, at the price of writing and reading a piece's sums (132 KB at 128).  Pieces: as many as make it shortest, counted in turns.  us, whole | in pieces, 32 heads on 8 of 128 behind 16384 positions: 144 tiles 408 | 333, 200
+// (one piece: what finding that out costs) 411 | 424, 304 847 | 664, 384 851 | 770; behind 8000, 304 438 | 379, behind 4000 244 | 239; 368 tiles of heads of 64 511 | 467.
+constexpr int PIECES = 4, PIECE_KEYS = 1024;   // at most, and keys from which on a piece of a tile is worth its sums
+__host__ __device__ constexpr int turn_of(int hs) { return hs == 64 ? 512 : 256; }   // tiles of a turn
+__host__ __device__ inline int pieces_of(int tiles, int hs)
+{
+    const int turn = turn_of(hs);
+    if (tiles > (hs == 64 ? turn : 2 * turn)) return 1;   // (two workgroups a CU: those of a turn that is half full are faster)
+    int best = 1;
+    float least = (float)((tiles + turn - 1) / turn);
+    for (int n = 2; n <= PIECES && tiles * n <= 4 * turn; n++) {
+        const float cost = (float)((tiles * n + turn - 1) / turn) / n + 0.03f * n * tiles / turn;
+        if (cost < least) { least = cost; best = n; }
+    }
+    return best;
+}
+// the tiles of a launch of the pipe kernel
+__device__ __forceinline__ int chunk_tile_count(const PagedCache& c, const ChunkArgs& w)
+{
+    __shared__ int sums[4];
+    const int tid = threadIdx.x;
+    int total = 0;
+    for (int b0 = 0; b0 < c.batch; b0 += 256) {
+        int tiles = 0, all;
+        if (b0 + tid < c.batch) {
+            const PagedSpan s = paged_span(c.starts[b0 + tid], c.starts[b0 + tid + 1], c.lens[b0 + tid], c.tokens, c.maxPages * c.pageSize);
+            if ((long long)s.count * (c.H / c.kvH) > w.few) tiles = (s.count + w.perTile * w.pair - 1) / (w.perTile * w.pair);
+        }
+        block_scan(tiles, sums, &all);
+        total = paged_sum(total, all);
+    }
+    return uniform(min(total, PAGED_MOST / (c.kvH * w.headTiles)) * c.kvH * w.headTiles);
+}
+
+// Chunks in 16-bit storage, head size 64 or 128, in tiles of 256 rows (w.pair 2); redo[i]: tile i is left to the chunk kernel
+hipError_t attn_paged_pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* redo);
+// The same with the positions of each tile in up to four pieces, where that fills the chip better; part: as many bytes as these say
+size_t attn_paged_pieces_bytes(const PagedCache& c, int blocks);
+hipError_t attn_paged_pieces_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* redo, void* part);
 
 }  // namespace mch

@@ -239,16 +239,27 @@ static int padded_size(const PagedCache& c) { return c.hs <= 64 ? 64 : c.hs <= 1
 // the split kernel's partial results, and behind them the chunk kernel's or the pipe kernel's flags
 static size_t split_bytes(const PagedCache& c) { return (size_t)SPLIT_GRID * 2 * 16 * (padded_size(c) + 2) * sizeof(float); }
 
-size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt)
+// Whether a launch of the pipe kernel may have its tiles in pieces: at about as many tiles as there are if the last one of every sequence is half full, and over long tables
+static bool in_turns(const PagedCache& c, DType dt)
+{
+    const ChunkPlan p = chunk_plan(c, dt);
+    const int about = (int)std::min<long long>(((long long)c.tokens / (2 * p.perTile) * c.kvH * p.headTiles + p.pipe) / 2, 1 << 16);
+    bool some = false;
+    for (int tiles = about - about / 10; tiles <= about + about / 10; tiles++) some = some || pieces_of(tiles, c.hs) > 1;
+    return p.pipe && some && c.maxPages * c.pageSize >= 6144;
+}
+
+size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt, bool pieces)
 {
     const ChunkPlan p = chunk_plan(c, dt);
     const bool chunks = c.hs <= 128 && (long long)c.tokens * (c.H / c.kvH) > FEW_ROWS;
-    const size_t chunk = !chunks ? 0 : p.pipe ? (size_t)p.pipe * sizeof(int) : (size_t)p.grid * (2 * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) + sizeof(ChunkJoin));
+    if (pieces && (!chunks || !in_turns(c, dt))) return 0;
+    const size_t chunk = !chunks ? 0 : p.pipe ? ((size_t)p.pipe * sizeof(int) + 255 & ~(size_t)255) + (pieces ? attn_paged_pieces_bytes(c, p.pipe) : 0) : (size_t)p.grid * (2 * CHUNK_ROWS * (padded_size(c) + 2) * sizeof(float) + sizeof(ChunkJoin));
     return split_bytes(c) + chunk;
 }
 size_t attn_paged_tickets() { return SPLIT_GRID; }
 
-hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets)
+hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets, bool pieces)
 {
     PagedAttnArgs a = {};
     a.c = c; a.q = q; a.y = y; a.c2 = scale * 1.44269504088896340736f;
@@ -283,7 +294,8 @@ hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void
                 float* own = (float*)((char*)workspace + split_bytes(c));
                 ChunkArgs g = {own, (ChunkJoin*)(own + (size_t)p.grid * 2 * CHUNK_ROWS * (padded_size(c) + 2)), FEW_ROWS, w.shift, p.perTile, p.tileHeads, p.headTiles, p.unit, p.pipe ? 2 : 1, p.pipe ? (const int*)own : nullptr};
                 if (p.pipe) {
-                    const hipError_t e = attn_paged_pipe_launch(s, a, g, p.pipe, (int*)own);
+                    const hipError_t e = pieces ? attn_paged_pieces_launch(s, a, g, p.pipe, (int*)own, (char*)own + ((size_t)p.pipe * sizeof(int) + 255 & ~(size_t)255))
+                                                : attn_paged_pipe_launch(s, a, g, p.pipe, (int*)own);
                     if (e != hipSuccess) return e;
                 }
                 const int grid = p.pipe ? 2 * p.pipe : p.grid;

@@ -14,6 +14,8 @@
 //  * What does not suit the pipeline is left to the chunk kernel, which runs behind this one for such tiles alone: tiles with a hole in their pages, rows
 //    before the first page given, row sums outside [2^-60, 2^64], values that are not finite where not all rows look.
 //
+//  * Behind a shared prefix (CUT) the positions of a tile may be in pieces, which leave their sums to a launch behind.
+//
 // Measured: 4 chunks of 1024 tokens over 8192 positions, 32 heads on 8 of 128, 515 GFLOP in 477 us (1080 TFLOP/s; a large library product has 1197).
 #include <algorithm>
 #include <type_traits>
@@ -29,8 +31,10 @@ namespace {
 constexpr float PIPE_HI = 1.8446744e19f, PIPE_LO = 8.6736174e-19f;   // 2^64, 2^-60
 constexpr int RING = 8;                                              // blocks whose places are kept
 
-template <int HS>
-__global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(PagedAttnArgs a, ChunkArgs w, int* flags)
+// (part: of a piece {m, sum of weights} of 256 rows, then the 256 rows; flags: 1 it is not to be trusted, -1 it has none)
+
+template <int HS, bool CUT = false>
+__global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(PagedAttnArgs a, ChunkArgs w, int* flags, float* part)
 {
     typedef FlashTraits<bf16_t> TR;
     constexpr int NST = 4;                        // LDS stages of 64 keys
@@ -51,7 +55,16 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
 
     // ---- the tile, and whether it is one for this kernel ----
     if (tid == 0) { sFirst = 0x7fffffff; sMissing = -1; sBad = 0; }
-    const ChunkTile at = chunk_tile(c, w, blockIdx.x);
+    int pieces = 1, piece = 0, index = blockIdx.x;
+    if constexpr (CUT) {
+        const int tiles = chunk_tile_count(c, w);
+        pieces = pieces_of(tiles, HS);
+        if (tiles == 0 || index >= tiles * pieces) return;
+        // (first pieces first: what runs side by side reads the same positions, and of as few key heads as whole tiles on an XCD)
+        piece = index / tiles;
+        index -= piece * tiles;
+    }
+    const ChunkTile at = chunk_tile(c, w, index);
     if (at.b < 0) return;
     const PagedSpan sp = span_at(c, at.b);
     const int G = c.H / c.kvH, perTile = w.perTile * w.pair, j0 = at.tile * perTile, nt = min(perTile, sp.count - j0), base = sp.len - sp.count + j0;
@@ -68,12 +81,31 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
         if (missing >= 0) atomicMax(&sMissing, missing);
     }
     __syncthreads();
-    const int given = uniform(sFirst), front = given < entries ? given * c.pageSize : 0;
+    const int given = uniform(sFirst);
+    int front = given < entries ? given * c.pageSize : 0;
     if (given >= entries || uniform(sMissing) > given || base < front) {
         if (tid == 0) flags[blockIdx.x] = 1;
         return;
     }
-    const int Tk = end - front, lim0 = base - front;   // keys, and the last one that the tile's first token sees
+    int Tk = end - front, lim0 = base - front, more = 1;   // keys, the last one that the tile's first token sees, and how many more each further token does
+    if (CUT && pieces > 1) {
+        // as many pieces as the keys that all rows see are enough for; every one but the last has whole blocks of these
+        const int mine = min(pieces, max((lim0 + 1) / PIECE_KEYS, 1)), each = (lim0 + 1) / mine & ~63;
+        if (piece >= mine) {
+            if (tid == 0) flags[blockIdx.x] = -1;
+            return;
+        }
+        if (piece < mine - 1) {
+            front += piece * each;
+            Tk = each;
+            lim0 = each - 1;
+            more = 0;
+        } else {
+            front += piece * each;
+            Tk -= piece * each;
+            lim0 -= piece * each;
+        }
+    }
     const unsigned char *kp = (const unsigned char*)((const bf16_t*)c.k + at.kh * c.sH), *vp = (const unsigned char*)((const bf16_t*)c.v + at.kh * c.sH);
     auto page_at = [&](int key) -> float { const int p = front + min(key, Tk - 1); return table[w.shift >= 0 ? p >> w.shift : p / c.pageSize]; };
     auto place_at = [&](int key, float entry) -> uint32_t {
@@ -87,9 +119,9 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const int r = row0 + 32 * x;
-        lim[x] = lim0 + min((r + l32) / w.tileHeads, nt - 1);
-        firstLim[x] = lim0 + min(r / w.tileHeads, nt - 1);
-        jobs[x] = ((lim0 + min((r + 31) / w.tileHeads, nt - 1)) >> 5) + 1;
+        lim[x] = lim0 + more * min((r + l32) / w.tileHeads, nt - 1);
+        firstLim[x] = lim0 + more * min(r / w.tileHeads, nt - 1);
+        jobs[x] = ((lim0 + more * min((r + 31) / w.tileHeads, nt - 1)) >> 5) + 1;
     }
     const int nplain = (firstLim[0] + 1) >> 5;         // steps that all rows see whole
     const int nkb = (Tk + 63) >> 6;
@@ -391,13 +423,39 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
         lsum[x] = f2_pair_sum(ls[x][0] + ls[x][1]);
         bad = bad || !(lsum[x] >= PIPE_LO && lsum[x] <= PIPE_HI);
     }
-    for (int e = tid; e < (nt - 1) * CPRW; e += 256) {
+    for (int e = tid; e < more * (nt - 1) * CPRW; e += 256) {
         const int key = lim0 + 1 + e / CPRW;
         const u32x4 v = *(const u32x4*)(vp + ((size_t)place_at(key, page_at(key)) << 4) + ((e % CPRW) << 4));
 #pragma unroll
         for (int i = 0; i < 4; i++) bad = bad || (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
     }
     __syncthreads();   // everybody is done with the stages
+    if (CUT && pieces > 1) {
+        // ---- the piece's sums, as they are ----
+        float* sums = part + (size_t)blockIdx.x * 256 * (HS + 2);
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int r = row0 + 32 * x + l32;
+            if (half == 0) *(float2*)(sums + 2 * r) = make_float2(-nref[x], lsum[x]);
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float4 v;
+                    float* f = &v.x;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        f[i] = o[x][dt][4 * g + i];
+                        bad = bad || (__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u;
+                    }
+                    *(float4*)(sums + 512 + r * HS + 32 * dt + 8 * g + 4 * half) = v;
+                }
+        }
+        if (__any(bad) && lane == 0) sBad = 1;
+        __syncthreads();
+        if (tid == 0) flags[blockIdx.x] = sBad;
+        return;
+    }
 
     // ---- y = O^T / l; register v of tile dt is value 32 dt + 8 (v / 4) + 4 half + v % 4.  A lane owns a row, so its values are scattered over it; they go
     // through the wavefront's own 64 rows of LDS and leave as whole rows, 16 bytes a lane.  The pieces of a row are permuted by its number so that
@@ -434,24 +492,85 @@ __global__ __launch_bounds__(256, HS == 64 ? 2 : 1) void attn_paged_pipe_kernel(
     if (tid == 0) flags[blockIdx.x] = sBad;
 }
 
-template <int HS> hipError_t pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* flags)
+// The pieces of a tile put together, 32 rows a workgroup, four values a lane; and whether the tile is left to the chunk kernel
+template <int HS> __global__ __launch_bounds__(256) void attn_paged_pieces_kernel(PagedAttnArgs a, ChunkArgs w, const int* flags, const float* part, int* redo)
+{
+    constexpr int LANES = HS / 4, ROWS = 256 / LANES;
+    const PagedCache& c = a.c;
+    const int tiles = chunk_tile_count(c, w), tile = blockIdx.x, tid = threadIdx.x;
+    if (tile >= tiles) return;
+    const int pieces = pieces_of(tiles, HS);
+    int flag[PIECES];
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) flag[p] = p < pieces ? uniform(flags[p * tiles + tile]) : -1;
+    bool bad = false;
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) bad = bad || flag[p] == 1;
+    if (blockIdx.y == 0 && tid == 0) redo[tile] = bad;
+    if (bad || pieces == 1) return;
+    const ChunkTile at = chunk_tile(c, w, tile);
+    if (at.b < 0) return;
+    const PagedSpan sp = span_at(c, at.b);
+    const int G = c.H / c.kvH, perTile = w.perTile * w.pair, j0 = at.tile * perTile, nt = min(perTile, sp.count - j0);
+    const int h0 = at.kh * G + at.ht * w.tileHeads, nh = min(w.tileHeads, G - at.ht * w.tileHeads);
+    for (int r = blockIdx.y * 32 + tid / LANES; r < (int)blockIdx.y * 32 + 32; r += ROWS) {
+        const int token = r / w.tileHeads, head = r - token * w.tileHeads;
+        if (token >= nt || head >= nh) continue;
+        float2 ml[PIECES];
+        float4 v[PIECES];
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            const float* sums = part + (size_t)((flag[p] < 0 ? 0 : p) * tiles + tile) * 256 * (HS + 2);   // (the first one always has some)
+            ml[p] = *(const float2*)(sums + 2 * r);
+            v[p] = *(const float4*)(sums + 512 + r * HS + 4 * (tid % LANES));
+        }
+        float M = -INFINITY, L = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) M = flag[p] < 0 ? M : fmaxf(M, ml[p].x);
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            const float f = flag[p] < 0 ? 0.f : __builtin_amdgcn_exp2f(ml[p].x - M);
+            L += f * ml[p].y;
+            y.x += f * v[p].x; y.y += f * v[p].y; y.z += f * v[p].z; y.w += f * v[p].w;
+        }
+        const float inv = 1.f / L;
+        *(uint2*)((bf16_t*)a.y + ((size_t)(sp.first + j0 + token) * c.H + h0 + head) * HS + 4 * (tid % LANES)) =
+            make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+    }
+}
+
+template <int HS> int pieces_grid(int blocks) { return std::max(blocks, 4 * turn_of(HS)); }
+template <int HS, bool CUT = false> hipError_t pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* flags, int* redo = nullptr, float* part = nullptr)
 {
     constexpr int LDSB = 2 * 4 * 64 * HS * 2 + RING * 64 * 4;   // four K and four V stages, the places
     static bool attr = false;
     if (!attr) {
-        const hipError_t e = hipFuncSetAttribute((const void*)attn_paged_pipe_kernel<HS>, hipFuncAttributeMaxDynamicSharedMemorySize, LDSB);
+        const hipError_t e = hipFuncSetAttribute((const void*)attn_paged_pipe_kernel<HS, CUT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDSB);
         if (e != hipSuccess) return e;
         attr = true;
     }
-    hipLaunchKernelGGL((attn_paged_pipe_kernel<HS>), blocks, 256, LDSB, s, a, w, flags);
+    hipLaunchKernelGGL((attn_paged_pipe_kernel<HS, CUT>), CUT ? pieces_grid<HS>(blocks) : blocks, 256, LDSB, s, a, w, flags, part);
+    if constexpr (CUT) hipLaunchKernelGGL((attn_paged_pieces_kernel<HS>), dim3(blocks, 8), 256, 0, s, a, w, flags, part, redo);
     return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t attn_paged_pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* flags)
+hipError_t attn_paged_pipe_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* redo)
 {
-    return a.c.hs == 64 ? pipe_launch<64>(s, a, w, blocks, flags) : pipe_launch<128>(s, a, w, blocks, flags);
+    return a.c.hs == 64 ? pipe_launch<64>(s, a, w, blocks, redo) : pipe_launch<128>(s, a, w, blocks, redo);
+}
+
+size_t attn_paged_pieces_bytes(const PagedCache& c, int blocks)
+{
+    const int grid = c.hs == 64 ? pieces_grid<64>(blocks) : pieces_grid<128>(blocks);
+    return (size_t)4 * turn_of(c.hs) * 256 * (c.hs + 2) * sizeof(float) + (size_t)grid * sizeof(int);
+}
+hipError_t attn_paged_pieces_launch(hipStream_t s, const PagedAttnArgs& a, const ChunkArgs& w, int blocks, int* redo, void* part)
+{
+    int* flags = (int*)((float*)part + (size_t)4 * turn_of(a.c.hs) * 256 * (a.c.hs + 2));
+    return a.c.hs == 64 ? pipe_launch<64, true>(s, a, w, blocks, flags, redo, (float*)part) : pipe_launch<128, true>(s, a, w, blocks, flags, redo, (float*)part);
 }
 
 }  // namespace mch

@@ -280,9 +280,9 @@ hipError_t k_paged_append(hipStream_t s, DType dt, const PagedCache& c, const vo
                           const float* turns);
 // y (tokens, H, hs) = attention of q (tokens, H, hs) over the pages, every token over the positions up to its own.  maxNew: at most this many new
 // tokens in a sequence, 0 if not known (any value is right).  workspace (may be null: a plain kernel does all), tickets (zero between launches): as much as these say
-size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt);
+size_t attn_paged_workspace_bytes(const PagedCache& c, DType dt, bool pieces = false);   // pieces: 0 where there are none
 size_t attn_paged_tickets();
-hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets);
+hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets, bool pieces = false);
 // The same for `groups` groups of sequences, bounds[g] .. bounds[g + 1] - 1, that have their first shared[g] positions in common: with as much scratch memory as this says (0:
 // the call above is to be taken, which gives the same result)
 size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups);

@@ -2868,10 +2868,14 @@ long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool 
             return 0;
         }
     }
-    size_t wsb = attn_paged_workspace_bytes(c, Q->dt());
-    workspace_or_none(&wsb, &ws);   // without scratch one workgroup a token and head does all of it
+    // long chunks behind a prefix: as over pages, the positions of their tiles in pieces where that fills the chip
+    size_t wsb = prefix ? attn_paged_workspace_bytes(c, Q->dt(), true) : 0;
+    if (wsb) workspace_or_none(&wsb, &ws);
+    const bool pieces = ws != nullptr;
+    if (!pieces) wsb = attn_paged_workspace_bytes(c, Q->dt());
+    if (!pieces) workspace_or_none(&wsb, &ws);   // without scratch one workgroup a token and head does all of it
     ERRCHK(tickets(attn_paged_tickets(), &tk));
-    HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, maxNew, ws, tk));
+    HIPCHK(k_attn_paged(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, maxNew, ws, tk, pieces));
     m_mem.touch((long)pl[14]);
     return 0;
 }
