@@ -360,8 +360,7 @@ def _plain_plan(s):
     result = torch.where(ends[:, None], torch.full_like(result, -1), result)
     left = count - torch.where(granted, need, torch.zeros_like(need)).sum()
     i = torch.arange(pages, device="cuda")
-    # what was taken off the stack still lies there, behind the count
-    s["free_out"][1:] = torch.where(i < count, free[:pages].float(), s["free_out"][1:])
+    s["free_out"][1:] = torch.where(i < left, free[:pages].float(), s["free_out"][1:])
     s["free_out"][0] = left.float()
     i = torch.arange(tokens, device="cuda")
     b = (torch.searchsorted(starts, i, right=True) - 1).clamp(0, B - 1)
@@ -467,8 +466,7 @@ def _exact_plan(c, i, pages, tokens):
             stack += [p for p in old[b, shared[b] // page:-(-lens[b] // page)].tolist() if 0 <= p < pages]
             table[b], after[b], borrowed[b] = -1, 0, 0
     starts, positions, slots, last = [0], [], [], []
-    full, wait, asked = np.zeros(pages + 1), False, 0
-    full[1:1 + len(stack)] = stack
+    wait, asked = False, 0
     for b, n in enumerate(new):
         begin = lens[b]
         lender = source[b] if lens[b] == 0 and n > 0 and 0 <= source[b] < len(new) and source[b] != b and new[source[b]] >= 0 else -1
@@ -491,7 +489,8 @@ def _exact_plan(c, i, pages, tokens):
                 slots.append(np.where(table[b, places // page] >= 0, table[b, places // page] * page + places % page, -1))
         starts.append(starts[-1] + (after[b] - begin if after[b] > lens[b] else 0))
         last.append(starts[-1] - 1 if starts[-1] > starts[-2] else -1)
-    full[0] = len(stack)
+    full = np.zeros(pages + 1)
+    full[0], full[1:1 + len(stack)] = len(stack), stack
     rows = [np.zeros(tokens) for _ in range(2)]
     for r, parts in zip(rows, (positions, slots)):
         if parts:
