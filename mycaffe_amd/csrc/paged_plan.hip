@@ -5,6 +5,7 @@
 //   a sequence without positions that begins behind the prompt of another one takes over that one's first whole pages, up to shared[b] positions;
 //   sequence after sequence takes ceil((len + n) / pageSize) - ceil(len / pageSize) pages from the top of the stack.
 // The first one for which pages or rows do not reach waits, and all behind it: sums over the batch decide, and no sequence overtakes another.
+// Of the stack only what remains is written: a page that comes back and is taken again in the same call goes straight to the row that gets it.
 // Numbers are whole ones in the base type; what is read is brought into its range here, as everywhere in a paged cache.
 #include <algorithm>
 
@@ -35,6 +36,8 @@ template <typename T> struct Plan {
     __device__ const T* in(const void* p) const { return (const T*)p; }
     __device__ int positions() const { return a.maxPages * a.pageSize; }
     __device__ int pages_of(int len) const { return (len + a.pageSize - 1) / a.pageSize; }
+    // free pages that remain whatever the call decides: a sequence takes no more than its rows fill and one that they begin
+    __host__ __device__ int remain(int have) const { return std::max(have - a.tokens / a.pageSize - std::min(a.batch, a.tokens), 0); }
     // -1: ends; else the tokens that it wants
     __device__ int wish(int b) const
     {
@@ -79,7 +82,7 @@ template <typename T> __device__ __forceinline__ Ask ask_of(const Plan<T>& p, in
     return ask_of(p, b, wish, len, take, lender);
 }
 
-// Workgroup 0 decides and writes everything that its decisions change; the others copy what they do not, where the block table and the list of free pages
+// Workgroup 0 decides and writes everything that its decisions change or may change; the others copy what they cannot, where the block table and the list of free pages
 // are not written in place (in place, they all are: a length that changes decides nothing then).
 // What bounds it is one read behind the other in workgroup 0, so whatever it goes through - sequences, pages that come back, pages that are taken, entries that are copied -
 // is one list of items each, a thread an item, whose sequence it finds in the list's sums.  Measured, all memory of its own: 4 sequences of one token 4.5 us (an empty call takes 3.3 - 3.8), 512
@@ -96,14 +99,15 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
     if (blockIdx.x) {
         const int others = gridDim.x - 1, me = blockIdx.x - 1;
         constexpr int EACH = 8;   // reads under way
+        const int remain = p.remain(have);
         if (copyFree)
-            for (long long i0 = (long long)me * EACH * THREADS + tid; i0 < have; i0 += (long long)others * EACH * THREADS) {
+            for (long long i0 = (long long)me * EACH * THREADS + tid; i0 < remain; i0 += (long long)others * EACH * THREADS) {
                 T v[EACH];
 #pragma unroll
-                for (int j = 0; j < EACH; j++) v[j] = free[1 + min(i0 + j * THREADS, (long long)have - 1)];
+                for (int j = 0; j < EACH; j++) v[j] = free[1 + min(i0 + j * THREADS, (long long)remain - 1)];
 #pragma unroll
                 for (int j = 0; j < EACH; j++)
-                    if (i0 + j * THREADS < have) freeOut[1 + i0 + j * THREADS] = v[j];
+                    if (i0 + j * THREADS < remain) freeOut[1 + i0 + j * THREADS] = v[j];
             }
         if (copyTable)
             for (int b = me * WAVES + wave; b < a.batch; b += others * WAVES) {
@@ -129,6 +133,7 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         return;
     }
     __shared__ int sums[3][WAVES], sStart[THREADS + 1], sNeed[THREADS + 1], sCopy[THREADS + 1], sFirst[THREADS], sBegin[THREADS], sTake[THREADS], sRows, sPages;
+    __shared__ int sBack[THREADS + 1], sBackFrom[THREADS], sBackEnd[THREADS];
     // the sequence of item i of a list, by the sums in front of each
     auto whose = [&](const int* starts, int i) __attribute__((always_inline)) -> int {
         int lo = 0;
@@ -157,36 +162,81 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         return q;
     };
     const Asks first = asks_of(tid, false);   // read once, ahead of everything
-    // ---- the pages of the sequences that end, in the order of the sequences ----
-    int count = have;
-    for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
+    // ---- the pages of the sequences that end, in the order of the sequences: places have, have + 1, ... of the stack ----
+    constexpr int EACH = 8;   // entries of a thread, one behind the other, at most
+    // the entries of those of sequences b0 .. b0 + THREADS - 1 as a list
+    auto entries_back = [&](int b0) __attribute__((always_inline)) -> int {
         const int mine = b0 + tid, wish = b0 ? mine < a.batch ? p.wish(mine) : 0 : first.wish;
         const bool ends = wish < 0;
-        if (!__syncthreads_or(ends)) continue;
+        if (!__syncthreads_or(ends)) return 0;
         const int from = !ends ? 0 : b0 ? p.borrowed(mine) : first.shared / a.pageSize, to = !ends ? 0 : p.pages_of(b0 ? p.len(mine) : first.len);
         int items;
-        sStart[tid] = scan<THREADS>(max(to - from, 0), sums[0], &items);
-        sFirst[tid] = from;
+        const int at = scan<THREADS>(max(to - from, 0), sums[0], &items);
+        sBack[tid] = at;
+        sBackFrom[tid] = from - at;
+        sBackEnd[tid] = at + max(to - from, 0);
         __syncthreads();
-        constexpr int EACH = 4;   // entries of a thread, one behind the other
-        for (int i0 = 0; i0 < items; i0 += EACH * THREADS) {
-            int page[EACH], valid = 0;
+        return items;
+    };
+    // the thread's entries of that list, of THREADS EACH from i0 on (-1: no page), and where the first page of them goes behind the `at` that lie in front
+    auto pages_back = [&](int b0, int items, int i0, int (&page)[EACH], int* at) __attribute__((always_inline)) -> int {
+        const int per = min((items - i0 + THREADS - 1) / THREADS, EACH);
+        int valid = 0, all, end = -1, s = 0;
+        T entry[EACH];
 #pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                const int i = i0 + EACH * tid + e, s = whose(sStart, i);
-                page[e] = i < items ? paged_page(table[(size_t)(b0 + s) * a.maxPages + sFirst[s] + i - sStart[s]], a.pages) : -1;
+        for (int e = 0; e < EACH; e++) {
+            const int i = i0 + per * tid + e;
+            entry[e] = (T)-1;
+            if (e >= per || i >= items) continue;
+            if (i >= end) {
+                s = whose(sBack, i);
+                end = sBackEnd[s];
             }
+            entry[e] = table[(size_t)(b0 + s) * a.maxPages + sBackFrom[s] + i];
+        }
 #pragma unroll
-            for (int e = 0; e < EACH; e++) valid += page[e] >= 0;
-            int all;
-            int place = paged_sum(count, scan<THREADS>(valid, sums[1], &all));
+        for (int e = 0; e < EACH; e++) {
+            page[e] = paged_page(entry[e], a.pages);
+            valid += page[e] >= 0;
+        }
+        const int place = paged_sum(*at, scan<THREADS>(valid, sums[1], &all));
+        *at = min(paged_sum(*at, all), a.pages);
+        return place;
+    };
+    int count = have, look[EACH], lookAt = have;
+    bool one = true;   // one look at them is all of them
+#pragma unroll
+    for (int e = 0; e < EACH; e++) look[e] = -1;
+    for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
+        const int items = entries_back(b0);
+        one = one && a.batch <= THREADS && items <= EACH * THREADS;
+        for (int i0 = 0; i0 < items; i0 += EACH * THREADS) lookAt = pages_back(b0, items, i0, look, &count);
+    }
+    // f(place, page) for those at places lo .. hi - 1
+    auto back = [&](int lo, int hi, auto f) __attribute__((always_inline)) {
+        auto each = [&](const int (&page)[EACH], int place) __attribute__((always_inline)) {
 #pragma unroll
             for (int e = 0; e < EACH; e++)
-                if (page[e] >= 0 && place < a.pages) freeOut[1 + place++] = (T)page[e];
-            count = min(paged_sum(count, all), a.pages);
+                if (page[e] >= 0) {
+                    if (place >= lo && place < hi) f(place, page[e]);
+                    place++;
+                }
+        };
+        if (lo >= hi) return;
+        if (one) {
+            each(look, lookAt);
+            return;
         }
-        __syncthreads();
-    }
+        int at = have;
+        for (int b0 = 0; b0 < a.batch && at < hi; b0 += THREADS) {
+            const int items = entries_back(b0);
+            for (int i0 = 0; i0 < items; i0 += EACH * THREADS) {
+                int page[EACH];
+                const int place = pages_back(b0, items, i0, page, &at);
+                each(page, place);
+            }
+        }
+    };
     if (ahead)
         for (int b = tid; b < a.batch; b += THREADS) last[b] = (T)ask_of(p, b).take;
     __syncthreads();
@@ -220,28 +270,32 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         askedPages = paged_sum(askedPages, allPages);
         askedRows = paged_sum(askedRows, allRows);
         if (b < a.batch) {
-            ((T*)a.lensOut)[b] = n < 0 ? (T)0 : granted ? (T)(k.begin + k.rows) : (T)len;
             ((T*)a.starts)[b] = (T)rowAt;
             last[b] = granted ? (T)(rowAt + k.rows - 1) : (T)-1;
-            if (a.sharedOut) ((T*)a.sharedOut)[b] = n < 0 ? (T)0 : granted && len == 0 ? (T)(k.take * a.pageSize) : (T)asks.shared;
+            if (n >= 0) {   // (what those have that end is read until the end)
+                ((T*)a.lensOut)[b] = granted ? (T)(k.begin + k.rows) : (T)len;
+                if (a.sharedOut) ((T*)a.sharedOut)[b] = granted && len == 0 ? (T)(k.take * a.pageSize) : (T)asks.shared;
+            }
         }
         __syncthreads();
-        for (int i = taken + tid; i < pagesUpTo; i += THREADS) {
-            const int s = whose(sNeed, i), at = count - 1 - i;
-            const T page = at < have ? free[1 + at] : freeOut[1 + at];
-            tableOut[(size_t)(b0 + s) * a.maxPages + sFirst[s] + i - sNeed[s]] = (T)paged_page(page, a.pages);
-        }
+        // page `i` of those that are taken is the stack's at place count - 1 - i
+        auto give = [&](int i, int page) __attribute__((always_inline)) {
+            const int s = whose(sNeed, i);
+            tableOut[(size_t)(b0 + s) * a.maxPages + sFirst[s] + i - sNeed[s]] = (T)page;
+        };
+        for (int i = max(taken, count - have) + tid; i < pagesUpTo; i += THREADS) give(i, paged_page(free[count - i], a.pages));
+        // those that come back: to the rows, and what is left of them, behind the last sequences, to the stack
+        const int left = count - pagesUpTo;
+        back(b0 + THREADS < a.batch ? max(have, left) : have, count - taken, [&](int place, int page) __attribute__((always_inline)) {
+            if (place < left) freeOut[1 + place] = (T)page;
+            else give(count - 1 - place, page);
+        });
         for (int i = tid; i < copies; i += THREADS) {
             const int s = whose(sCopy, i), j = i - sCopy[s], lender = sTake[s], row = b0 + s;
             // of a row that waits: its first entries, as many as it would have borrowed, then those that it would have got
             const int e = lender >= 0 || j < -1 - lender ? j : sFirst[s] + j - (-1 - lender);
             tableOut[(size_t)row * a.maxPages + e] = table[(size_t)(lender >= 0 ? lender : row) * a.maxPages + e];
         }
-        if (!copyTable)
-            for (uint64_t m = __ballot(n < 0); m; m &= m - 1) {
-                const size_t row = (size_t)(b0 + 64 * wave + __builtin_ctzll(m)) * a.maxPages;
-                for (int e = lane; e < a.maxPages; e += 64) tableOut[row + e] = (T)-1;
-            }
         __syncthreads();
         if (writeTokens)
             for (int i = rows + tid; i < rowsUpTo; i += THREADS) {
@@ -256,6 +310,28 @@ template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void pa
         taken = pagesUpTo;
         __syncthreads();
     }
+    for (int b0 = 0; b0 < a.batch; b0 += THREADS) {
+        const int b = b0 + tid;
+        const bool ends = b < a.batch && (b0 ? p.wish(b) : first.wish) < 0;
+        if (ends) {
+            ((T*)a.lensOut)[b] = (T)0;
+            if (a.sharedOut) ((T*)a.sharedOut)[b] = (T)0;
+        }
+        if (!copyTable)
+            for (uint64_t m = __ballot(ends); m; m &= m - 1) {
+                const size_t row = (size_t)(b0 + 64 * wave + __builtin_ctzll(m)) * a.maxPages;
+                for (int e = lane; e < a.maxPages; e += 64) tableOut[row + e] = (T)-1;
+            }
+    }
+    if (copyFree)
+        for (int i0 = p.remain(have) + tid, end = min(have, count - taken); i0 < end; i0 += EACH * THREADS) {
+            T v[EACH];
+#pragma unroll
+            for (int j = 0; j < EACH; j++) v[j] = free[1 + min(i0 + j * THREADS, end - 1)];
+#pragma unroll
+            for (int j = 0; j < EACH; j++)
+                if (i0 + j * THREADS < end) freeOut[1 + i0 + j * THREADS] = v[j];
+        }
     if (tid == 0) {
         ((T*)a.starts)[a.batch] = (T)rows;
         freeOut[0] = (T)(count - taken);
@@ -286,7 +362,7 @@ constexpr int BATCH_OF_FEW = 16, ROWS_OF_FEW = 1024;
 template <typename T> hipError_t launch(hipStream_t s, const PagedPlanArgs& a)
 {
     Plan<T> p = {a};
-    const long long entries = (a.table != a.tableOut ? (long long)a.batch * a.maxPages : 0) + (a.free != a.freeOut ? a.pages : 0);
+    const long long entries = (a.table != a.tableOut ? (long long)a.batch * a.maxPages : 0) + (a.free != a.freeOut ? p.remain(a.pages) : 0);
     const bool rows = a.positions || a.slots, own = a.tokens <= ROWS_OF_ONE, few = a.tokens <= ROWS_OF_FEW && a.batch <= BATCH_OF_FEW;
     const int others = (int)std::min<long long>(few ? 1024 : 256, (entries + 4095) / 4096);
     if (few) hipLaunchKernelGGL((paged_plan_kernel<T, 256>), 1 + others, 256, 0, s, p, rows ? 1 : 0);

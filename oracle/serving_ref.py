@@ -11,7 +11,8 @@ def whole(v, lo, hi):
 
 
 def plan(new, lens, table, free, tokens, page, origin=None, shared=None):
-    """PAGED_PLAN: what becomes of lens, table, free, starts, positions, slots, last, shared (positions and slots of the new rows only)."""
+    """PAGED_PLAN: what becomes of lens, table, free, starts, positions, slots, last, shared (positions and slots of the new rows only);
+    listed: how many entries of the stack mean something."""
     table = np.array(table, np.float64)
     B, W = table.shape
     pages = len(free) - 1
@@ -19,8 +20,8 @@ def plan(new, lens, table, free, tokens, page, origin=None, shared=None):
     lens = [whole(n, 0, W * page) for n in lens]
     held = [whole(s, 0, W * page) for s in (shared if shared is not None else [0] * B)]
     valid = lambda p, n: 0 <= p < n  # noqa: E731  (false for what is not a number)
-    free = np.array(free, np.float64)
-    count = whole(free[0], 0, pages)
+    stack = np.array(free, np.float64)
+    count = whole(stack[0], 0, pages)
     old = table.copy()
     after, borrowed = list(lens), list(held)
     for b in range(B):
@@ -28,7 +29,7 @@ def plan(new, lens, table, free, tokens, page, origin=None, shared=None):
             continue
         for e in range(held[b] // page, -(-lens[b] // page)):
             if valid(old[b, e], pages) and count < pages:
-                free[1 + count] = int(old[b, e])
+                stack[1 + count] = int(old[b, e])
                 count += 1
         table[b], after[b], borrowed[b] = -1, 0, 0
     starts, positions, slots, last = [0], [], [], []
@@ -52,7 +53,7 @@ def plan(new, lens, table, free, tokens, page, origin=None, shared=None):
                         table[b, :first] = old[lender, :first]
                     for e in range(first, end):
                         top -= 1
-                        table[b, e] = int(free[1 + top]) if valid(free[1 + top], pages) else -1
+                        table[b, e] = int(stack[1 + top]) if valid(stack[1 + top], pages) else -1
                     if lens[b] == 0:
                         borrowed[b] = begin
                     after[b] = begin + rows
@@ -62,8 +63,9 @@ def plan(new, lens, table, free, tokens, page, origin=None, shared=None):
                         slots.append(int(p) * page + t % page if valid(p, pages) else -1)
         starts.append(starts[-1] + rows)
         last.append(starts[-1] - 1 if rows else -1)
-    free[0] = top
-    return dict(lens=after, table=table, free=free, starts=starts, positions=positions, slots=slots, last=last, shared=borrowed, listed=count)
+    # what lies behind the number that remains is left as it was
+    free = np.concatenate([[top], stack[1:1 + top], np.asarray(free, np.float64)[1 + top:]])
+    return dict(lens=after, table=table, free=free, starts=starts, positions=positions, slots=slots, last=last, shared=borrowed, listed=top)
 
 
 def sample(x, u, temperature=1.0, k=0, p=1.0, m=0.0):
