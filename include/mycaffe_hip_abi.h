@@ -251,6 +251,8 @@ enum {
      *   f{scale}  l{...the 18 of ATTN_PAGED_FWD, groups, hGroups (groups + 1), hShared (groups) [, maxNew]}
      * Group g are the sequences hGroups[g] .. hGroups[g + 1] - 1 (never decreasing; sequences in no group share nothing), which have their first hShared[g] positions
      * in common: as far as these are whole pages, the rows of hTable of those with new tokens name the same ones.  (What counts is what lies in front of every new token of the group.)
+     * Results differ by the order of sums, and by the bits of weights: those of 16-bit rows have sixteen where a prefix is shared; where sharing would not pay, as with long
+     * chunks, it is a call over pages.
      *
      * PAGED_PLAN: room for the next tokens of `batch` sequences.  hNew[b] tokens are wanted behind hLens[b] positions; hNew[b] below 0 ends a sequence.
      *   l{batch, tokens, pages, pageSize, maxPages, hNew, hLens, hTable, hFree, hLensOut, hTableOut, hFreeOut, hStarts, hPositions (0), hSlots (0), hLast

@@ -610,6 +610,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
     typedef FlashTraits<bf16_t> TR;
     typedef ChunkShared<TQ, TC, HSP> S;
     constexpr int NQ = S::NQ, NK = S::NK, KB = S::KB, LD = S::LD;
+    constexpr int NW = NQ == 1 && L::SUMS ? 2 : NQ;                                               // parts of a weight
     constexpr int KJ = KB / 32, KF = HSP / 16, DT = HSP / 32, EPL = 16 / (int)sizeof(TC);
     constexpr int CPR = HSP / EPL, NP = KB * CPR / 256, RPP = 256 / CPR;                          // pieces a row; pieces a thread; rows a round
     constexpr int AHEAD = NK == 3 && HSP == 128 ? 1 : 2;                                          // value fragments under way (1: registers are full)
@@ -882,25 +883,28 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
 #pragma unroll
             for (int v = 0; v < 16; v++) {
                 s[j][v] = __builtin_amdgcn_exp2f(fmaf(s[j][v], c2, ref));
-                if (NQ > 1) l += s[j][v];
+                if (NW > 1) l += s[j][v];
             }
-        // weights in the operand layout: rounded to one bf16 number (eight bits, as the pipe kernel's) and added up as rounded, or in three parts
-        Parts<NQ> p[KJ][2];
+        // weights in the operand layout: of 16-bit rows rounded to one bf16 number (eight bits, as the pipe kernel's) and added up as rounded, or, behind and in shared
+        // prefixes, to two (sixteen bits: most rows of a group are single tokens, which split_run gives as many); of fp32 rows in three parts
+        Parts<NW> p[KJ][2];
 #pragma unroll
         for (int j = 0; j < KJ; j++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 if constexpr (NQ == 1) {
                     p[j][x].p[0] = TR::pack_p(s[j], x);
+                    if constexpr (NW == 2) p[j][x].p[1] = TR::pack_rest(s[j], x, p[j][x].p[0]);
+                    else
 #pragma unroll
-                    for (int e = 0; e < 4; e++) l = pair_sum(p[j][x].p[0][e], l);
+                        for (int e = 0; e < 4; e++) l = pair_sum(p[j][x].p[0][e], l);
                 } else
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        uint32_t out[NQ];
-                        two_parts<NQ>(s[j][8 * x + 2 * e], s[j][8 * x + 2 * e + 1], out);
+                        uint32_t out[NW];
+                        two_parts<NW>(s[j][8 * x + 2 * e], s[j][8 * x + 2 * e + 1], out);
 #pragma unroll
-                        for (int i = 0; i < NQ; i++) p[j][x].p[i][e] = out[i];
+                        for (int i = 0; i < NW; i++) p[j][x].p[i][e] = out[i];
                     }
             }
 #pragma unroll
@@ -909,7 +913,7 @@ __device__ __forceinline__ void chunk_run(const PagedAttnArgs& a, const ChunkArg
 #pragma unroll
             for (int z = NK - 1; z >= 0; z--)
 #pragma unroll
-                for (int y = NQ - 1; y >= 0; y--)
+                for (int y = NW - 1; y >= 0; y--)
                     if (z + y < 3) o[i] = TR::mma(vf[n % AHEAD][z], p[j][x].p[y], o[i]);
             if (n + AHEAD < KJ * 2 * DT) value(n + AHEAD);
         }

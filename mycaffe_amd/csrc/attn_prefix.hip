@@ -363,8 +363,8 @@ PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups)
     p.u.chunk.perTile = 128 / p.u.chunk.tileHeads;
     p.u.chunk.pair = 1;
     // ns a workgroup of two a CU: 2 us and 10 bytes a ns for positions read; 32 positions of 128 rows, or 1 << unit as many, 1.2 us, or 2000 products and sums a ns, six of
-    // them one in fp32 (three over a 16-bit cache)
-    const int parts = dt == BF16 ? 1 : c.ct == BF16 ? 3 : 6;
+    // them one in fp32 (three over a 16-bit cache), and of a weight's two parts two one in 16 bits
+    const float parts = dt == BF16 ? 1.5f : c.ct == BF16 ? 3 : 6;
     p.u.splitCost = 2000.f + p.u.unit * (float)c.hs * 2 * (c.ct == F32 ? 4 : 2) / 10.f;
     // lists are counted in 32 bits; every token is in two entries
     const double positions = c.maxPages * (double)c.pageSize, tokens = c.tokens;
