@@ -340,14 +340,14 @@ struct PrefixPlan {
     double splitUnits, chunkUnits;   // no more than these
 };
 int padded(const PagedCache& c) { return c.hs <= 64 ? 64 : c.hs <= 128 ? 128 : 256; }
-PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups)
+PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups, int maxNew)
 {
     PrefixPlan p = {};
     const int G = c.H / c.kvH, n = groups + c.batch;
     // Single tokens of heads that share no key heads leave little for the matrix cores, and at head sizes up to 64 four workgroups of split_run fit a CU where two of both kinds
     // do: a launch for each.  12 heads of 64, 16 bits, 192 tokens behind 2048 and up to 700 positions 90 us for 97, up to 2000 169 for 209, 96 behind 512 and 700 60 for 82 (the
     // other way 44 for 40 with nothing behind the prefix); 24 heads on 3 the other way, 42 for 34, 12 heads and 8 tokens each 57 for 51.
-    if (padded(c) == 64 && (long long)c.tokens * G <= (long long)c.batch * 5 / 4) p.u.splitGrid = 2 * PREFIX_GRID;
+    if (padded(c) == 64 && prefix_rows(c.tokens, c.batch, maxNew) * G <= (long long)c.batch * 5 / 4) p.u.splitGrid = 2 * PREFIX_GRID;
     p.chunks = c.hs <= 128;
     p.u.kvH = c.kvH;
     p.u.G = G;
@@ -391,33 +391,29 @@ inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
-// What is shared is worth it if the sequences can be long or hold many bytes of keys and values, and have few rows (tokens times the heads that share a key head) each: with many, the
+// When what is shared is worth it (prefix_pays): with many rows a sequence the
 // kernels of attention over pages have whole tiles of one sequence.  us, over pages | shared, 16 bits, heads of 128, single tokens with up to 64 - 300 positions of their own:
 //   32 heads on 8, 16 sequences behind 1024 (71 MB) 20.2 | 25.4, 64 (285 MB) 39.8 | 35.7, 64 behind 256 (84 MB) 17.4 | 29.0; behind 4096, 8 (136 MB) 29.3 | 28.6, 64 125 | 41;
 //   16 on one, 16 behind 1024 (11 MB) 19.1 | 26.6, behind 4096 (36 MB) 41.3 | 29.9; 64 on one, 64 behind 1024 (43 MB) 41.0 | 38.0, behind 4096 80 | 60, behind 12000 189 | 91;
 // in fp32 over 16 bits, 12 heads on 4 of 64, behind 1024, 24 (27 MB) 21.6 | 26.1, 96 (107 MB) 38.9 | 29.4, behind 4096 8 (34 MB) 26.1 | 23.7.
 // By rows a sequence, 16 sequences, 16 bits: 32 heads on 8 behind 2048 and behind 16384, 21 53 | 41, 42 45 | 59 and 178 | 132, 84 53 | 92 and 199 | 248, 167 71 | 125 and 323 | 450; 8 on 8 behind
 // 4096, 42 63 | 58, 83 73 | 92; fp32 behind 2048, 31 43 | 36, 62 38 | 56.
-constexpr int PREFIX_LONG = 3000;   // positions that the sequences can have
-constexpr int PREFIX_ROWS = 32, PREFIX_LONG_ROWS = 64;
 constexpr size_t PREFIX_SCRATCH = 1ull << 30;   // sums of every row on both sides: 4096 tokens of 32 heads of 128 take 138 MB
-constexpr double PREFIX_BYTES = 120e6, PREFIX_BYTES_F32 = 60e6, PREFIX_LONG_BYTES = 32e6;
 
-size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups)
+size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups, int maxNew)
 {
     const int e = dt == BF16 || c.ct == BF16 ? 8 : 4;
     const bool pieces = c.hs % e == 0 && c.sP % e == 0 && c.sH % e == 0 && c.sT % e == 0 && at16(c.k) && at16(c.v) && at16(q) && at16(y);
-    const bool far = c.maxPages * c.pageSize >= PREFIX_LONG;
     const double bytes = (double)c.batch * c.maxPages * c.pageSize * c.kvH * c.hs * 2 * (c.ct == F32 ? 4 : 2);
-    if (!pieces || c.batch < 2 || groups > PREFIX_GROUPS || groups + c.batch > PREFIX_ENTRIES || (long long)c.tokens * (c.H / c.kvH) > (far ? PREFIX_LONG_ROWS : PREFIX_ROWS) * (long long)c.batch ||
-        bytes < (far ? PREFIX_LONG_BYTES : dt == F32 ? PREFIX_BYTES_F32 : PREFIX_BYTES)) return 0;
-    const PrefixPlan p = prefix_plan(c, dt, groups);
+    if (!pieces || groups > PREFIX_GROUPS || groups + c.batch > PREFIX_ENTRIES ||
+        !prefix_pays(prefix_rows(c.tokens, c.batch, maxNew), c.batch, c.H / c.kvH, (long long)c.maxPages * c.pageSize, bytes, dt == F32)) return 0;
+    const PrefixPlan p = prefix_plan(c, dt, groups, maxNew);
     return p.splitUnits < 1e9 && p.chunkUnits <= 1e9 && p.bytes <= PREFIX_SCRATCH ? p.bytes : 0;
 }
 
-hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int groups, const float* bounds, const float* shared, void* workspace)
+hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int groups, const float* bounds, const float* shared, int maxNew, void* workspace)
 {
-    PrefixPlan p = prefix_plan(c, dt, groups);
+    PrefixPlan p = prefix_plan(c, dt, groups, maxNew);
     char* ws = (char*)workspace;
     PrefixWork w = {(PrefixSpan*)(ws + p.spans), (int2*)(ws + p.at), (int2*)(ws + p.splitBegin), (int2*)(ws + p.chunkBegin), (int*)(ws + p.groupOf), (int*)(ws + p.totals),
                     (float*)(ws + p.splitPart), (float*)(ws + p.chunkPart), (float*)(ws + p.sums), bounds, shared, groups, groups + c.batch};
@@ -427,7 +423,7 @@ hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const voi
     p.u.chunk.part = w.chunkPart;
     if (w.n <= 256) hipLaunchKernelGGL((attn_prefix_plan_kernel<256, 256, 256>), 1, 256, 0, s, c, w, p.u);
     else hipLaunchKernelGGL((attn_prefix_plan_kernel<1024, PREFIX_ENTRIES, PREFIX_GROUPS>), 1, 1024, 0, s, c, w, p.u);
-    const dim3 join(c.batch, (c.H + 3) / 4, std::min(64, (c.tokens + c.batch - 1) / c.batch));
+    const dim3 join(c.batch, (c.H + 3) / 4, std::min(64, (int)((prefix_rows(c.tokens, c.batch, maxNew) + c.batch - 1) / c.batch)));
     auto go = [&](auto type, auto ctype) {
         typedef decltype(type) T_;
         typedef decltype(ctype) TC_;

@@ -285,8 +285,8 @@ size_t attn_paged_tickets();
 hipError_t k_attn_paged(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int maxNew, void* workspace, int* tickets, bool pieces = false);
 // The same for `groups` groups of sequences, bounds[g] .. bounds[g + 1] - 1, that have their first shared[g] positions in common: with as much scratch memory as this says (0:
 // the call above is to be taken, which gives the same result)
-size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups);
-hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int groups, const float* bounds, const float* shared, void* workspace);
+size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups, int maxNew);
+hipError_t k_attn_prefix(hipStream_t s, DType dt, const PagedCache& c, const void* q, void* y, float scale, int groups, const float* bounds, const float* shared, int maxNew, void* workspace);
 
 // ---- a step of a server (paged_plan.hip, sample.hip): numbers fp32, or double (`wide`) -----------------------------------------
 // Room for the new tokens of a step.  In: wish (tokens that a sequence wants, below 0: it ends), lens, table (batch, maxPages), free (number of free pages, then

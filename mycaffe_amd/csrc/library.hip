@@ -2860,10 +2860,10 @@ long Kernel::attn_paged_fwd(float* pf, long lf, MCH_LONGLONG* pl, long ll, bool 
     void* ws = nullptr;
     int* tk;
     if (prefix) {
-        size_t wsb = attn_prefix_workspace_bytes(c, Q->dt(), Q->ptr, Y->ptr, (int)pl[18]);
+        size_t wsb = attn_prefix_workspace_bytes(c, Q->dt(), Q->ptr, Y->ptr, (int)pl[18], maxNew);
         workspace_or_none(&wsb, &ws);
         if (ws) {
-            HIPCHK(k_attn_prefix(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)pl[18], (const float*)groups->ptr, (const float*)shared->ptr, ws));
+            HIPCHK(k_attn_prefix(m_stream, Q->dt(), c, Q->ptr, Y->ptr, scale, (int)pl[18], (const float*)groups->ptr, (const float*)shared->ptr, maxNew, ws));
             m_mem.touch((long)pl[14]);
             return 0;
         }

@@ -165,6 +165,19 @@ template <typename F> const char* plan_clash(const long long* l, F at, size_t si
         }
     return nullptr;
 }
+// Attention behind shared prefixes.  Rows of a call that tokens can have: no more than its memory, and than maxNew (0: not known) for each sequence - a server's
+// memory has room for prompts also where a step has single tokens
+PAGED_FN long long prefix_rows(long long tokens, long long batch, long long maxNew) { return maxNew > 0 ? std::min(tokens, batch * maxNew) : tokens; }
+// What is shared is worth it if the sequences can be long (positions, of their tables) or hold many bytes of keys and values, and have few rows (tokens times the `each` heads that share
+// a key head) each; f32: rows of fp32.  Measured beside the kernels.
+constexpr int PREFIX_LONG = 3000;   // positions that the sequences can have
+constexpr int PREFIX_ROWS = 32, PREFIX_LONG_ROWS = 64;
+constexpr double PREFIX_BYTES = 120e6, PREFIX_BYTES_F32 = 60e6, PREFIX_LONG_BYTES = 32e6;
+inline bool prefix_pays(long long rows, long long batch, long long each, long long positions, double bytes, bool f32)
+{
+    const bool far = positions >= PREFIX_LONG;
+    return batch >= 2 && rows * each <= (far ? PREFIX_LONG_ROWS : PREFIX_ROWS) * batch && bytes >= (far ? PREFIX_LONG_BYTES : f32 ? PREFIX_BYTES_F32 : PREFIX_BYTES);
+}
 // SAMPLE_FWD, l{rows, vocab, ..., logitsRows, stride}
 inline bool sample_sizes_ok(long long rows, long long vocab, long long logitsRows, long long stride, long long most)
 {

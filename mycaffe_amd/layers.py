@@ -445,6 +445,7 @@ class PagedBatch(_Paged):
             if new.shape != (self.batch,):
                 raise ValueError("a step has a number for each of its %d places" % self.batch)
             self.new.mutable_cpu_data = new
+        self.max_new = 0 if new is None else max(0, int(new.max()))
         at = lambda *blobs: [b.gpu_data for b in blobs]  # noqa: E731
         state = at(self.lens, self.table, self.free)
         self.cuda.PagedPlan(self.batch, self.tokens, self.pages, self.page_size, self.max_pages, self.new.gpu_data, *state, *state,
