@@ -263,8 +263,9 @@ enum {
      * hFreeOut (entries behind the number that remains mean nothing, and are left as they were) are the three inputs, or all memory of their own.  hStarts (batch + 1) as above; of every new row its position
      * in its sequence and its slot, page * pageSize + place in the page (-1: no page; pages * pageSize is then at most 2^24); hLast (batch): a sequence's last row, or -1.
      * hFrom, hShared, hSharedOut (batch; the last one the second or memory of its own, as the other three): a sequence without positions begins behind
-     * the first hShared[b] positions of sequence hFrom[b], as far as they are whole pages that it has; hSharedOut[b] says how many these are, and of a sequence that
-     * goes on what hShared[b] does: its first pages, up to there, are not its own, and not given back when it ends.
+     * the first hShared[b] positions of sequence hFrom[b], as far as they are whole pages that it has (none of one that ends in the same call); hSharedOut[b] says how many these are, and of a sequence that
+     * goes on what hShared[b] does: its first pages, up to there, are not its own, and not given back when it ends.  Nothing counts who
+     * reads a page: the one that gives it back has to end last.
      *
      * SAMPLE_FWD: the next token of every row of logits (fp32 or 16 bits), drawn with the random number u = hRandom[row]:
      *   l{rows, vocab, hLogits, hRandom, hIds, hTemperature, hTopK, hTopP, hMinP [, hLogProb, hRows, logitsRows, rowStride]}    (from hTemperature on each may be 0)

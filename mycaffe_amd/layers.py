@@ -421,7 +421,7 @@ class PagedBatch(_Paged):
     the blob ``new`` holds.  Places for which pages or rows do not reach wait: ``lens`` does not grow, ``last`` is -1.  ``starts``, ``positions`` and ``last``
     say which rows of the pass are whose; rows behind them are computed from and to whatever their memory holds.
     ``Begin({place: (other, positions)})`` before a Step: an empty place begins behind the first positions of another one, in its pages (whole pages of it; they
-    are the other's, which has to end last).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
+    are the other's, which has to end last, or in the same Step: ``Step(new)`` refuses else, a Step without an argument cannot see it).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
     same pages; attention then reads these once for all of them.  ``Sample(...)`` draws a token for every place that got rows.
     """
 
@@ -433,6 +433,7 @@ class PagedBatch(_Paged):
         self.bounds, self.common = Blob(cuda), Blob(cuda)
         super().__init__(cuda, pages, page_size, max_pages, *(getattr(self, name) for name in shapes), self.bounds, self.common)
         self.batch, self.tokens = batch, tokens
+        self._lenders = {}                              # of places that began behind another one, that one
         for blob in (self.new, self.lens, self.shared):
             blob.mutable_cpu_data = np.zeros(batch, cuda.DTYPE)
         self.table.mutable_cpu_data = np.full((batch, max_pages), -1, cuda.DTYPE)
@@ -444,6 +445,15 @@ class PagedBatch(_Paged):
             new = np.asarray(new, self.cuda.DTYPE)
             if new.shape != (self.batch,):
                 raise ValueError("a step has a number for each of its %d places" % self.batch)
+            ends = set(np.flatnonzero(new <= -1).tolist())
+            early = {b: other for b, other in self._lenders.items() if other in ends and b not in ends}
+            if early:
+                # those that ended in a Step without an argument borrow nothing any more
+                origin, shared = self.origin.mutable_cpu_data, self.shared.mutable_cpu_data
+                for b, other in early.items():
+                    if shared[b] >= self.page_size and origin[b] == other:
+                        raise ValueError("place %d cannot end before place %d, which reads its pages" % (other, b))
+            self._lenders = {b: other for b, other in self._lenders.items() if b not in ends and other not in ends}
             self.new.mutable_cpu_data = new
         self.max_new = 0 if new is None else max(0, int(new.max()))
         at = lambda *blobs: [b.gpu_data for b in blobs]  # noqa: E731
@@ -460,6 +470,7 @@ class PagedBatch(_Paged):
             raise ValueError("only an empty place begins")
         for b, (other, positions) in places.items():
             origin[b], shared[b] = other, positions
+            self._lenders[b] = other
         self.origin.mutable_cpu_data, self.shared.mutable_cpu_data = origin, shared
 
     def Share(self, bounds=(), positions=()):

@@ -1,0 +1,65 @@
+"""Which steps a batch on the device refuses, or shares less in, without a device: places that end while others still read their pages."""
+import numpy as np
+import pytest
+
+from mycaffe_amd.layers import PagedBatch
+from tests.test_layers_batch import Memory
+
+
+def batch_of(*lens, tokens=50):
+    cuda = Memory()
+    batch = PagedBatch(cuda, len(lens), tokens, 64, 4, 16)
+    batch.lens.mutable_cpu_data = np.array(lens, np.float32)
+    return cuda, batch
+
+
+def test_a_lender_ends_last():
+    cuda, batch = batch_of(20, 0, 0)
+    batch.Begin({1: (0, 8)})
+    kept = batch.new.mutable_cpu_data.copy()
+    for new in ([-1, 3, 0], [-1, 0, 0], [-1, 3, 5], [-5, 0, 0]):     # in the step in which the other one begins, before it has, ...
+        with pytest.raises(ValueError, match="place 0 .* place 1"):
+            batch.Step(new)
+        assert cuda.calls.count("PagedPlan") == 0 and np.array_equal(batch.new.mutable_cpu_data, kept)
+    batch.Step([1, 3, 0])
+    with pytest.raises(ValueError, match="place 0 .* place 1"):           # ... and while it lasts
+        batch.Step([-1, 1, 0])
+    assert cuda.calls.count("PagedPlan") == 1
+    batch.Step([1, -1, 0])
+    batch.Step([-1, 1, 0])
+    assert cuda.calls.count("PagedPlan") == 3
+
+
+def test_both_end_at_once():
+    cuda, batch = batch_of(20, 0, 0)
+    batch.Begin({1: (0, 8), 2: (0, 4)})
+    batch.Step([1, 3, 3])
+    with pytest.raises(ValueError, match="place 0 .* place 2"):
+        batch.Step([-1, -1, 1])
+    batch.Step([-1, -1, -1])
+    assert cuda.calls.count("PagedPlan") == 2
+
+
+def test_one_behind_the_other():
+    """The third begins in pages of the second, the first of which are the first's: it keeps the second, which keeps the first."""
+    cuda, batch = batch_of(20, 0, 0)
+    batch.Begin({1: (0, 8)})
+    batch.Step([1, 10, 0])
+    batch.Begin({2: (1, 16)})
+    batch.Step([1, 1, 3])
+    for new in ([-1, 1, 1], [1, -1, 1], [-1, -1, 1]):
+        with pytest.raises(ValueError):
+            batch.Step(new)
+    batch.Step([1, -1, -1])
+    batch.Step([-1, 0, 0])
+
+
+def test_what_a_step_without_an_argument_ended():
+    """Its numbers are the device's, so what is borrowed is looked up there before a step is refused."""
+    cuda, batch = batch_of(20, 0, 0)
+    batch.Begin({1: (0, 8)})
+    batch.Step([1, 3, 0])
+    batch.Step()
+    batch.shared.mutable_cpu_data = np.zeros(3, np.float32)              # what the plan writes of a place that ended
+    batch.Step([-1, 0, 0])
+    assert cuda.calls.count("PagedPlan") == 3
