@@ -422,7 +422,8 @@ class PagedBatch(_Paged):
     say which rows of the pass are whose; rows behind them are computed from and to whatever their memory holds.
     ``Begin({place: (other, positions)})`` before a Step: an empty place begins behind the first positions of another one, in its pages (whole pages of it; they
     are the other's, which has to end last, or in the same Step: ``Step(new)`` refuses else, a Step without an argument cannot see it).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
-    same pages; attention then reads these once for all of them.  ``Sample(...)`` draws a token for every place that got rows.
+    same pages; attention then reads these once for all of them, until a place of the group ends and holds another sequence (as far as ``Step(new)`` says so): then the
+    group shares nothing until ``Share`` is called again.  ``Sample(...)`` draws a token for every place that got rows.
     """
 
     def __init__(self, cuda, batch, tokens, pages, page_size, max_pages):
@@ -434,6 +435,7 @@ class PagedBatch(_Paged):
         super().__init__(cuda, pages, page_size, max_pages, *(getattr(self, name) for name in shapes), self.bounds, self.common)
         self.batch, self.tokens = batch, tokens
         self._lenders = {}                              # of places that began behind another one, that one
+        self._groups, self._ended = [], set()           # [first place, end, positions]; places that ended since these were said
         for blob in (self.new, self.lens, self.shared):
             blob.mutable_cpu_data = np.zeros(batch, cuda.DTYPE)
         self.table.mutable_cpu_data = np.full((batch, max_pages), -1, cuda.DTYPE)
@@ -455,6 +457,10 @@ class PagedBatch(_Paged):
                         raise ValueError("place %d cannot end before place %d, which reads its pages" % (other, b))
             self._lenders = {b: other for b, other in self._lenders.items() if b not in ends and other not in ends}
             self.new.mutable_cpu_data = new
+            self._ended |= ends
+            again = {b for b in self._ended if new[b] > 0}
+            if any(first <= b < end and shared for first, end, shared in self._groups for b in again):
+                self._share([(first, end, 0 if any(first <= b < end for b in again) else shared) for first, end, shared in self._groups])
         self.max_new = 0 if new is None else max(0, int(new.max()))
         at = lambda *blobs: [b.gpu_data for b in blobs]  # noqa: E731
         state = at(self.lens, self.table, self.free)
@@ -477,11 +483,15 @@ class PagedBatch(_Paged):
         bounds, positions = (np.asarray(v, self.cuda.DTYPE) for v in (bounds, positions))
         if len(positions) and (len(bounds) != len(positions) + 1 or (np.diff(bounds) < 0).any() or bounds[0] < 0 or bounds[-1] > self.batch):
             raise ValueError("groups are runs of the %d places, one bound more than groups" % self.batch)
-        self.nGroups = len(positions)
-        if self.nGroups:
-            for blob, values in ((self.bounds, bounds), (self.common, positions)):
-                blob.Reshape(*values.shape)
-                blob.mutable_cpu_data = values
+        self._ended = set()
+        self._share([(int(bounds[g]), int(bounds[g + 1]), positions[g]) for g in range(len(positions))])
+
+    def _share(self, groups):
+        self._groups, self.nGroups = groups, len(groups) if any(shared for _, _, shared in groups) else 0
+        if groups:
+            for blob, values in ((self.bounds, [first for first, _, _ in groups] + [groups[-1][1]]), (self.common, [shared for _, _, shared in groups])):
+                blob.Reshape(len(values))
+                blob.mutable_cpu_data = np.asarray(values, self.cuda.DTYPE)
 
     def Sample(self, logits, random, temperature=None, top_k=None, top_p=None, min_p=None):
         """The next token of every place from logits (1, tokens, vocab) into ``ids`` (-1: a place without rows) with a random number, 0 .. 1, for each place; the

@@ -63,3 +63,36 @@ def test_what_a_step_without_an_argument_ended():
     batch.shared.mutable_cpu_data = np.zeros(3, np.float32)              # what the plan writes of a place that ended
     batch.Step([-1, 0, 0])
     assert cuda.calls.count("PagedPlan") == 3
+
+
+def test_groups_of_places_that_hold_others_now():
+    cuda, batch = batch_of(20, 30, 30, 40, 40)
+    said = lambda: (batch.nGroups, list(batch.bounds.mutable_cpu_data), list(batch.common.mutable_cpu_data))  # noqa: E731
+    batch.Share([0, 3, 5], [16, 8])
+    batch.Step([1, -1, 1, 1, 1])
+    batch.Step([1, 0, 1, 1, 1])
+    assert said() == (2, [0, 3, 5], [16, 8])              # nothing in place 1: what the others share they still do
+    batch.Step([1, 7, 1, 1, 1])
+    assert said() == (2, [0, 3, 5], [0, 8])               # another sequence there: its first positions are its own
+    batch.Step([1, 1, 1, -1, 1])
+    batch.Step([1, 1, 1, 2, 1])
+    assert batch.nGroups == 0                             # nobody shares anything
+    batch.Share([0, 1, 3], [0, 16])
+    batch.Step([-1, 1, 1, 1, 1])
+    batch.Step([4, 1, 1, 1, 1])
+    assert said() == (2, [0, 1, 3], [0, 16])              # place 0 is in no group that shares
+
+
+def test_groups_said_again_count():
+    cuda, batch = batch_of(20, 0, 30)
+    batch.Share([0, 3], [16])
+    batch.Step([1, -1, 1])
+    batch.Begin({1: (0, 16)})
+    batch.Share([0, 3], [16])
+    batch.Step([1, 5, 1])
+    batch.Step([1, 1, 1])
+    assert batch.nGroups == 1 and list(batch.common.mutable_cpu_data) == [16]
+    batch.Share()
+    batch.Step([1, -1, 1])
+    batch.Step([1, 2, 1])
+    assert batch.nGroups == 0

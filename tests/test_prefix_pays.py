@@ -58,8 +58,8 @@ def test_a_step_says_how_many_tokens_it_has_at_most():
 
     cuda = Told()
     batch, layer = PagedBatch(cuda, 4, 7, 6, 4, 4), attention(cuda)
-    batch.Share([0, 4], [4])
     for new, said in (([1, 1, 0, 1], 1), ([1, 5, -1, 0], 5), ([-1, -1, 0, 0], 0), (None, 0), (np.array([2, 2, 2, 1.0]), 2)):
+        batch.Share([0, 4], [4])
         batch.Step(new)
         serve(cuda, [layer], batch)
         assert [c for c in cuda.calls if isinstance(c, tuple)][-1] == ("prefix", said)
