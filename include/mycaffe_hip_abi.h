@@ -259,7 +259,8 @@ enum {
      *     [, hFrom, hShared, hSharedOut]}
      * hFree (pages + 1) is a stack: the number of free pages, then these.  First the pages of sequences that end go on it, in the order of the sequences (their row
      * of the table becomes -1, their length 0); then each sequence in turn takes the pages that it needs off its top.  The first one for which the pages or the `tokens`
-     * rows of the call do not reach waits, unchanged, and so do all behind it; one that is longer than maxPages pages can hold is passed over.  hLensOut, hTableOut and
+     * rows of the call do not reach waits, unchanged, and so do all behind it - for ever, if it wants more than `tokens` rows or than the cache has pages: prompts come in pieces; one that is
+     * longer than maxPages pages can hold is passed over.  hLensOut, hTableOut and
      * hFreeOut (entries behind the number that remains mean nothing, and are left as they were) are the three inputs, or all memory of their own.  hStarts (batch + 1) as above; of every new row its position
      * in its sequence and its slot, page * pageSize + place in the page (-1: no page; pages * pageSize is then at most 2^24); hLast (batch): a sequence's last row, or -1.
      * hFrom, hShared, hSharedOut (batch; the last one the second or memory of its own, as the other three): a sequence without positions begins behind

@@ -418,7 +418,9 @@ class PagedBatch(_Paged):
     with its own length, and passes of up to ``tokens`` rows.  Nothing of a step has to come from the host, so that a loop of steps can be captured.
 
     ``Step(new)`` before a model's pass: place b gets room for ``new[b]`` tokens (below 0: its sequence ends, its pages are free); without an argument what
-    the blob ``new`` holds.  Places for which pages or rows do not reach wait: ``lens`` does not grow, ``last`` is -1.  ``starts``, ``positions`` and ``last``
+    the blob ``new`` holds.  Places for which pages or rows do not reach wait, and all behind them: ``lens`` does not grow, ``last`` is -1.  What no step can have, more tokens
+    than rows or than a sequence's pages hold, ``Step(new)`` refuses: prompts come in pieces.  (A sequence at the end of its table waits, and holds up nobody; one that has all pages of
+    the cache, where ``max_pages`` allows it, everybody behind it.)  ``starts``, ``positions`` and ``last``
     say which rows of the pass are whose; rows behind them are computed from and to whatever their memory holds.
     ``Begin({place: (other, positions)})`` before a Step: an empty place begins behind the first positions of another one, in its pages (whole pages of it; they
     are the other's, which has to end last, or in the same Step: ``Step(new)`` refuses else, a Step without an argument cannot see it).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
@@ -447,6 +449,9 @@ class PagedBatch(_Paged):
             new = np.asarray(new, self.cuda.DTYPE)
             if new.shape != (self.batch,):
                 raise ValueError("a step has a number for each of its %d places" % self.batch)
+            most = min(self.tokens, min(self.max_pages, self.pages) * self.page_size)
+            if not (new == np.floor(new)).all() or (new > most).any():
+                raise ValueError("a place can have whole numbers of new tokens up to %d in a step of %d rows" % (most, self.tokens))
             ends = set(np.flatnonzero(new <= -1).tolist())
             early = {b: other for b, other in self._lenders.items() if other in ends and b not in ends}
             if early:

@@ -96,3 +96,18 @@ def test_groups_said_again_count():
     batch.Step([1, -1, 1])
     batch.Step([1, 2, 1])
     assert batch.nGroups == 0
+
+
+@pytest.mark.parametrize("rows,pages,page,width,most", [(50, 64, 4, 16, 50), (200, 64, 4, 16, 64), (200, 9, 4, 16, 36)])
+def test_wishes_that_no_step_can_grant(rows, pages, page, width, most):
+    """They would wait for ever, and all places behind them."""
+    cuda = Memory()
+    batch = PagedBatch(cuda, 3, rows, pages, page, width)
+    kept = batch.new.mutable_cpu_data.copy()
+    for wish in (most + 1, 1e9, np.inf, np.nan, 0.5, -0.5):
+        with pytest.raises(ValueError, match="up to %d " % most):
+            batch.Step([1, wish, 1])
+        assert cuda.calls.count("PagedPlan") == 0 and np.array_equal(batch.new.mutable_cpu_data, kept)
+    batch.Step([1, most, 1])
+    batch.Step([-1, -3, 0])
+    assert cuda.calls.count("PagedPlan") == 2
