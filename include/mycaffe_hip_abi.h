@@ -275,8 +275,8 @@ enum {
      * largest; above 1: the first.  Drawn is the first token by index at which the sum of the weights left exceeds u times all of it (u below 0 or not a number: 0, from 1 on
      * the last one).  A temperature that is not above 0: the likeliest token.  A logit that is not a number is -inf; of infinite ones each weighs 1.  hLogProb: the
      * logarithm of the token's share of the weights left (0 without a draw).  hRows: which row, of logitsRows (0: rows) at rowStride (0: vocab) values each, a
-     * row's logits are; no such row, or one of -inf alone: id -1.  vocab up to 2^20.  Weights are exact to 2^-50 and sums exact, so the same numbers draw the same tokens
-     * in any batch.
+     * row's logits are; no such row, or one of -inf alone: id -1.  vocab up to 2^20.  Weights are right to 2^-b of the largest, b = min(47, 63 - ceil(log2 vocab)) (46 at 131072 tokens),
+     * and their sums exact, so the same numbers draw the same tokens in any batch.
      */
     MCH_FN_ATTN_DECODE_FWD = 2001,
     MCH_FN_RMSNORM_FWD = 2002,

@@ -5,11 +5,12 @@
 // those that are left exceeds u times all of it.
 //
 // A draw compares u with sums over the whole vocabulary: a sum that is off by e moves every border by e, so with 100000 tokens fp32 sums draw another token every
-// few hundred rows.  Weights are made in 64 bits and held as whole numbers of 2^-FB, which add up to the same in any order; their sums are exact.
+// few hundred rows.  Weights are made in 64 bits, to 2^-48.5 of themselves, and held as whole numbers of 2^-FB of the largest, FB = 50 and less above 2^13 tokens (sample_bits: 46 at
+// 131072), which add up to the same in any order; their sums are exact.
 //
 // A logit takes some 20 instructions of 64 bits where its weight counts, and none where only its place does (top-k): long rows are bound by these, and by their bins, short ones by one
-// pass and one barrier behind the other.  A row is one workgroup's, its logits read two or three times (they stay in the caches); or slices of it are (below).  Measured: top-p
-// of a row of 32000 in fp32 27 us by one workgroup, 21 in slices; 64 rows of 50261 in fp32, top-50, 27 us; 256 rows of 131072 in 16 bits with settings of their own 89 us
+// pass and one barrier behind the other.  A row is one workgroup's, its logits read two or three times (they stay in the caches); or slices of it are (below).  Measured, with
+// rows that no cache of an XCD holds: top-p of a row of 32000 in fp32 24 us; 64 rows of 50261 in fp32, top-50, 27 us; 256 rows of 131072 in 16 bits with settings of their own 86 us
 // (67 MB; largest logits 13, weights 35, borders 8, candidates 17, the rest 17); 48 rows of 200003 in 16 bits by temperature alone 23 us.
 #include <algorithm>
 #include <type_traits>
@@ -1236,13 +1237,13 @@ int sample_bits(int vocab)
 }
 
 // When slices of rows are what workgroups have.  Where every CU has a row or two at most, a row alone takes as long as it is, and five launches some 25 us; more rows than that
-// take turns.  us, a workgroup a row | slices: top-50 in fp32, 1 row of 32000 21.4 | 22.4, of 131072 41.3 | 24.2, 16 of 8000 17.8 | 24.0, 256 of 8000 19.1 | 27.4, of 32000
-// 30.4 | 39.2, 1024 of 4000 63.1 | 49.0; temperature, top-k, top-p and min-p in 16 bits, 1 row of 32000 25.7 | 25.5, 16 47.4 | 36.4, 256 55.5 | 54.7, 4 of 131072 67.0 | 35.3, 16 of 8000
-// 29.1 | 32.5, 1024 of 4000 91.5 | 65.2; top-p in fp32, 1 row of 32000 27.0 | 24.9, 64 38.0 | 39.3, 256 43.6 | 56.1.  (Above CUT_ROWS it is the scratch memory that costs.)
+// take turns.  us, a workgroup a row | slices, the same rows time and again: top-50 in fp32, 1 row of 32000 22.8 | 21.1, of 131072 48.7 | 23.5, 16 of 8000 17.8 | 22.0, 256 of 8000
+// 18.6 | 24.4, of 32000 26.7 | 36.5, 1024 of 4000 62.2 | 48.9; temperature, top-k, top-p and min-p in 16 bits, 1 row of 32000 37.6 | 26.6, 16 46.3 | 32.6, 256 54.5 | 49.9, 4 of 131072 95.5 | 31.4,
+// 16 of 8000 29.0 | 30.0, 1024 of 4000 92.8 | 64.8; top-p in fp32, 1 row of 32000 22.8 | 21.2, 64 36.7 | 33.6, 256 40.1 | 51.8.  (Above CUT_ROWS it is the scratch memory that costs.)
 constexpr int CUT_ROWS = 4096, CUT_FEW = 128, CUT_TURNS = 512;
 static bool cut(const SampleArgs& a) { return a.count <= CUT_ROWS && a.vocab >= (a.count <= CUT_FEW ? 24576 : a.count <= CUT_TURNS ? 49152 : 2048); }
-// Logits a thread of a slice: few where there are few slices.  us, 8 | 32: 64 rows of 32000, the four settings 41.2 | 43.8, temperature alone 15.7 | 18.6, 1024 of 4000 65.2 | 72.0; top-50
-// 256 rows of 32000 47.0 | 39.2, 1024 of 8000 60.2 | 56.6
+// Logits a thread of a slice: few where there are few slices.  us, 8 | 32: 64 rows of 32000, the four settings 35.3 | 40.1, temperature alone 11.6 | 13.0, 1024 of 4000, the four 64.8 | 70.5; top-50,
+// 256 rows of 32000 37.2 | 36.3, 1024 of 8000 59.1 | 58.0
 static int cut_each(const SampleArgs& a)
 {
     const long long slices = (long long)a.count * ((a.vocab + 8 * CUT - 1) / (8 * CUT));

@@ -415,17 +415,19 @@ class PagedSequences(_Paged):
 
 class PagedBatch(_Paged):
     """A batch of sequences whose tables, lengths and free pages live on the device (no counterpart in the reference): ``batch`` places for sequences, each
-    with its own length, and passes of up to ``tokens`` rows.  Nothing of a step has to come from the host, so that a loop of steps can be captured.
+    with its own length, and passes of up to ``tokens`` rows.  A step takes nothing from the host but wishes and random numbers, and writes nothing back to it.
 
     ``Step(new)`` before a model's pass: place b gets room for ``new[b]`` tokens (below 0: its sequence ends, its pages are free); without an argument what
-    the blob ``new`` holds.  Places for which pages or rows do not reach wait, and all behind them: ``lens`` does not grow, ``last`` is -1.  What no step can have, more tokens
-    than rows or than a sequence's pages hold, ``Step(new)`` refuses: prompts come in pieces.  (A sequence at the end of its table waits, and holds up nobody; one that has all pages of
-    the cache, where ``max_pages`` allows it, everybody behind it.)  ``starts``, ``positions`` and ``last``
-    say which rows of the pass are whose; rows behind them are computed from and to whatever their memory holds.
+    the blob ``new`` holds.  Places for which pages or rows do not reach wait, and all behind them: ``lens`` does not grow, ``last`` is -1.  What no step can have,
+    more tokens than rows or than a sequence's pages hold, ``Step(new)`` refuses: prompts come in pieces.  (A sequence at the end of its table waits, and holds up nobody;
+    one that has all pages of the cache, where ``max_pages`` allows it, everybody behind it.)  ``starts``, ``positions`` and ``last`` say which rows of the pass are
+    whose; rows behind them are computed from and to whatever their memory holds.
     ``Begin({place: (other, positions)})`` before a Step: an empty place begins behind the first positions of another one, in its pages (whole pages of it; they
-    are the other's, which has to end last, or in the same Step: ``Step(new)`` refuses else, a Step without an argument cannot see it).  ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the
-    same pages; attention then reads these once for all of them, until a place of the group ends and holds another sequence (as far as ``Step(new)`` says so): then the
-    group shares nothing until ``Share`` is called again.  ``Sample(...)`` draws a token for every place that got rows.
+    are the other's, which has to end last, or in the same Step: ``Step(new)`` refuses else, a Step without an argument cannot see it).
+    ``Share(bounds, positions)``: the places bounds[g] .. bounds[g + 1] - 1 have their first positions[g] positions in the same pages; attention then reads these once
+    for all of them (worth it from about a thousand positions, or 100 MB that are not read again).  When a place of a group ends and holds another sequence, as far as
+    ``Step(new)`` says so, the group shares nothing until ``Share`` is called again.
+    ``Sample(...)`` draws a token for every place that got rows.
     """
 
     def __init__(self, cuda, batch, tokens, pages, page_size, max_pages):
