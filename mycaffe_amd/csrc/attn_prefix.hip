@@ -9,8 +9,8 @@
 //
 // Many rows over a prefix are bound by the matrix cores, few rows behind it by reading the cache, so both kinds of work run side by side, in shares by what they cost.  What
 // remains is the wait for memory at the begin and end of items, and three launches that depend on each other (the list, the work, the sums).  Measured: 64 tokens, 32 heads on 8 of 128 in
-// 16 bits, behind 8192 shared and up to 512 positions of their own, 108 MB and 8.9 GFLOP, 58.5 us (6 + 45 + 7; 248 without sharing); 192 tokens, 12 heads of 64, behind three times 2048 and up to
-// 700, 247 MB, 90 us; 24 sequences of 2 to 5 tokens, 12 heads on 4 of 64 in fp32 over 16 bits, behind 3000 and up to 300, 30.4 us.
+// 16 bits, behind 8192 shared and up to 512 positions of their own, 108 MB and 8.9 GFLOP, 59 us (6 + 45 + 7; 248 without sharing); 192 tokens, 12 heads of 64, behind three times 2048 and up to
+// 700, 247 MB, 90 us; 24 sequences of 2 to 5 tokens, 12 heads on 4 of 64 in fp32 over 16 bits, behind 3000 and up to 300, 30.6 us.
 #include <algorithm>
 
 #include "attn_paged_run.h"
@@ -345,8 +345,8 @@ PrefixPlan prefix_plan(const PagedCache& c, DType dt, int groups, int maxNew)
     PrefixPlan p = {};
     const int G = c.H / c.kvH, n = groups + c.batch;
     // Single tokens of heads that share no key heads leave little for the matrix cores, and at head sizes up to 64 four workgroups of split_run fit a CU where two of both kinds
-    // do: a launch for each.  12 heads of 64, 16 bits, 192 tokens behind 2048 and up to 700 positions 90 us for 97, up to 2000 169 for 209, 96 behind 512 and 700 60 for 82 (the
-    // other way 44 for 40 with nothing behind the prefix); 24 heads on 3 the other way, 42 for 34, 12 heads and 8 tokens each 57 for 51.
+    // do: a launch for each.  12 heads of 64, 16 bits, 192 tokens behind three times 2048 and up to 700 positions 80 us for 87, up to 2000 168 for 220, 96 behind 512 and up to 700 53
+    // for 53 (the other way 45 for 40 with nothing behind the prefix); 24 heads on 3 the other way, 35 for 27, 12 heads and 8 tokens each 51 for 45.
     if (padded(c) == 64 && prefix_rows(c.tokens, c.batch, maxNew) * G <= (long long)c.batch * 5 / 4) p.u.splitGrid = 2 * PREFIX_GRID;
     p.chunks = c.hs <= 128;
     p.u.kvH = c.kvH;
@@ -392,12 +392,13 @@ inline bool at16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 }  // namespace
 
 // When what is shared is worth it (prefix_pays): with many rows a sequence the
-// kernels of attention over pages have whole tiles of one sequence.  us, over pages | shared, 16 bits, heads of 128, single tokens with up to 64 - 300 positions of their own:
-//   32 heads on 8, 16 sequences behind 1024 (71 MB) 20.2 | 25.4, 64 (285 MB) 39.8 | 35.7, 64 behind 256 (84 MB) 17.4 | 29.0; behind 4096, 8 (136 MB) 29.3 | 28.6, 64 125 | 41;
-//   16 on one, 16 behind 1024 (11 MB) 19.1 | 26.6, behind 4096 (36 MB) 41.3 | 29.9; 64 on one, 64 behind 1024 (43 MB) 41.0 | 38.0, behind 4096 80 | 60, behind 12000 189 | 91;
-// in fp32 over 16 bits, 12 heads on 4 of 64, behind 1024, 24 (27 MB) 21.6 | 26.1, 96 (107 MB) 38.9 | 29.4, behind 4096 8 (34 MB) 26.1 | 23.7.
-// By rows a sequence, 16 sequences, 16 bits: 32 heads on 8 behind 2048 and behind 16384, 21 53 | 41, 42 45 | 59 and 178 | 132, 84 53 | 92 and 199 | 248, 167 71 | 125 and 323 | 450; 8 on 8 behind
-// 4096, 42 63 | 58, 83 73 | 92; fp32 behind 2048, 31 43 | 36, 62 38 | 56.
+// kernels of attention over pages have whole tiles of one sequence.  us, over pages | shared, 16 bits, heads of 128, single tokens with up to 300 positions of their own:
+//   32 heads on 8, 16 sequences behind 1024 (88 MB) 21.9 | 25.1, 64 (352 MB) 48.4 | 36.7; behind 4096, 8 (145 MB) 29.1 | 27.7, 64 132 | 44;
+//   16 on one, 16 behind 1024 (11 MB) 18.6 | 27.0, behind 4096 (36 MB) 40.2 | 30.1; 64 on one, 64 behind 1024 (44 MB) 40.9 | 37.7, behind 4096 78 | 62, behind 12000 190 | 97;
+// in fp32 over 16 bits, 12 heads on 4 of 64, behind 1024, 24 (33 MB) 20.3 | 24.7, 96 (132 MB) 41.5 | 31.5, behind 4096 8 (36 MB) 22.2 | 26.0.
+// By rows a sequence, 16 sequences, 16 bits: 32 heads on 8 behind 2048 and behind 16384, 18 52 | 42 and 181 | 100, 39 43 | 60 and 167 | 136, 81 51 | 93 and 182 | 265, 164 67 | 126 and 295 | 481; 8 on
+// 8 behind 4096, 41 61 | 61, 82 71 | 99; fp32 behind 2048, 29 40 | 33, 61 38 | 46.
+// What the host cannot know is what the tables hold: 64 sequences of 32 heads on 8 with 256 shared positions and up to 300 others share too, 44 us for 27.
 constexpr size_t PREFIX_SCRATCH = 1ull << 30;   // sums of every row on both sides: 4096 tokens of 32 heads of 128 take 138 MB
 
 size_t attn_prefix_workspace_bytes(const PagedCache& c, DType dt, const void* q, const void* y, int groups, int maxNew)

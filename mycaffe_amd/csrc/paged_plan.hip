@@ -85,8 +85,9 @@ template <typename T> __device__ __forceinline__ Ask ask_of(const Plan<T>& p, in
 // Workgroup 0 decides and writes everything that its decisions change or may change; the others copy what they cannot, where the block table and the list of free pages
 // are not written in place (in place, they all are: a length that changes decides nothing then).
 // What bounds it is one read behind the other in workgroup 0, so whatever it goes through - sequences, pages that come back, pages that are taken, entries that are copied -
-// is one list of items each, a thread an item, whose sequence it finds in the list's sums.  Measured, all memory of its own: 4 sequences of one token 4.5 us (an empty call takes 3.3 - 3.8), 512
-// with tables of 512 entries, a tenth of which end or begin, 17 - 20 us (13.3 and 5.2 for the rows), 256 prompts 16.6; with loops over the sequences in place of the lists 8.4, 30 and 33.
+// is one list of items each, a thread an item, whose sequence it finds in the list's sums.  Measured, all memory of its own: 4 sequences of one token 4.7 us (an empty call takes 3.3 - 3.8), 512
+// with tables of 512 entries, a tenth of which end or begin, 17 - 20 us (13.2 and 5.6 for the rows), 256 prompts 16 - 17; with loops over the sequences in place of the lists 8.4, 30 and 33.
+// In place, a token for each of 4, 64 and 512 sequences, 4.6, 5.7 and 6.1 us (elsewhere 5.0, 6.0 and 6.6).
 template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void paged_plan_kernel(Plan<T> p, int writeTokens)
 {
     constexpr int WAVES = THREADS / 64;
