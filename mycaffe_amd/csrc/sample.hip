@@ -10,7 +10,7 @@
 //
 // A logit takes some 20 instructions of 64 bits where its weight counts, and none where only its place does (top-k): long rows are bound by these, and by their bins, short ones by one
 // pass and one barrier behind the other.  A row is one workgroup's, its logits read two or three times (they stay in the caches); or slices of it are (below).  Measured, with
-// rows that no cache of an XCD holds: top-p of a row of 32000 in fp32 24 us; 64 rows of 50261 in fp32, top-50, 27 us; 256 rows of 131072 in 16 bits with settings of their own 86 us
+// rows that no cache of an XCD holds: top-p of a row of 32000 in fp32 24 - 25 us; 64 rows of 50261 in fp32, top-50, 27 us; 256 rows of 131072 in 16 bits with settings of their own 86 us
 // (67 MB; largest logits 13, weights 35, borders 8, candidates 17, the rest 17); 48 rows of 200003 in 16 bits by temperature alone 23 us.
 #include <algorithm>
 #include <type_traits>
